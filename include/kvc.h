@@ -418,6 +418,65 @@ int kvc_varlen_decode_cus(int64_t num_decode_rows, int64_t num_prefill_tokens, i
                           int64_t prefill_kq_pairs);
 
 /* ---------------------------------------------------------------------------
+ * Attention with shaped scores, and of drafted token trees, over a bf16 pool.
+ * No reference counterpart (the engine's attention is causal and unshaped).
+ * ------------------------------------------------------------------------- */
+
+/* Bytes of workspace kvc_scored_attention needs. */
+size_t kvc_scored_workspace_bytes(int64_t num_q_tokens, int64_t num_heads, int64_t num_kv_heads,
+                                  int64_t num_decode_rows, int64_t num_prefill,
+                                  int64_t max_seqlen_q);
+
+/* kvc_varlen_attention's rows (decode rows first, then prefill chunks; keys
+ * from the pool through the block tables, or from num_fresh_rows rows of
+ * k_fresh / v_fresh when block_tables is NULL), with other scores and masks.
+ * A query at place p (decode: context - 1; query r of a chunk: sk - sq + r)
+ * sees key j < sk when (j <= p or j < prefix_lens[i], the chunk's two-way
+ * prefix; NULL: none) and (window == 0 or p - j < window), with the score
+ *   s = scale q.k;  s = softcap tanh(s / softcap) when softcap > 0;
+ *   s -= alibi_slopes[h] |p - j| when alibi_slopes (fp32 [num_heads]) is given.
+ * out = softmax(s) . v; a query that sees no key gives 0.  Values at keys a
+ * query does not see never reach it, infinities and NaN included.  A block id
+ * outside the pool reads as zeros.  max_seqlen_q (the longest chunk) chooses
+ * the launch's form; the lengths themselves are read on the device.  Rows of
+ * q / out / k_fresh / v_fresh are 16-byte aligned; at most 256 query heads
+ * per kv head. */
+int kvc_scored_attention(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_q_tokens, int64_t num_heads,
+    const void* k_cache, const void* v_cache, int64_t num_cache_blocks, int64_t page_size,
+    int64_t num_kv_heads, int64_t head_dim, const void* k_fresh, int64_t kf_stride_t,
+    int64_t kf_stride_h, const void* v_fresh, int64_t vf_stride_t, int64_t vf_stride_h,
+    int64_t num_fresh_rows, const int32_t* block_tables, int64_t bt_stride,
+    int64_t max_blocks_per_seq, int64_t num_decode_rows, const int32_t* decode_context_lens,
+    int64_t num_prefill, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+    int64_t max_seqlen_q, const int32_t* prefix_lens, const float* alibi_slopes, float softcap,
+    int64_t window, float scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
+    void* workspace, size_t workspace_bytes, kvc_stream_t stream);
+
+/* Bytes of workspace kvc_tree_attention needs. */
+size_t kvc_tree_workspace_bytes(int64_t num_q_tokens, int64_t num_heads, int64_t num_kv_heads,
+                                int64_t batch, int64_t max_seqlen_q);
+
+/* Attention of drafted token trees: sequence i's tokens are query rows
+ * cu_seqlens_q[i] .. cu_seqlens_q[i+1] - 1 (NULL: max_seqlen_q each), their
+ * keys already in the pool at positions context_lens[i] + t (context_lens
+ * counts what comes before the tree).  Token t sees every context key and the
+ * tree keys u of its mask: bit u % 64 of tree_mask[row][u / 64] (int64
+ * [num_q_tokens, mask_words]; bits at or past the tree's size are ignored).
+ * Its place is context + (bits in its mask) - 1, the depth of a token whose
+ * mask is its path from the root; window, alibi_slopes and softcap are those
+ * of kvc_scored_attention, with the places of queries and tree keys. */
+int kvc_tree_attention(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_q_tokens, int64_t num_heads,
+    const void* k_cache, const void* v_cache, int64_t num_cache_blocks, int64_t page_size,
+    int64_t num_kv_heads, int64_t head_dim, const int32_t* block_tables, int64_t bt_stride,
+    int64_t max_blocks_per_seq, int64_t batch, const int32_t* context_lens,
+    const int32_t* cu_seqlens_q, int64_t max_seqlen_q, const int64_t* tree_mask,
+    int64_t mask_words, const float* alibi_slopes, float softcap, int64_t window, float scale,
+    void* out, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+    size_t workspace_bytes, kvc_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Dequantise gathered int8 rows (the torch-side read path).
  * ------------------------------------------------------------------------- */
 

@@ -1,0 +1,1391 @@
+// Attention of new tokens over the paged cache with shaped scores: decode
+// rows, prefill chunks and drafted token trees, gfx950.
+//
+// For a query token at place p and a visible key at place j, head h:
+//   s = scale q.k;  s = cap tanh(s / cap) (cap > 0);  s -= slope_h |p - j|
+//   out = sum_j softmax_j(s) v_j, 0 for a token that sees no key.
+// Chunk tokens sit at the end of their sequence's keys (p = sk - sq + t) and
+// see keys j <= p or j < prefix, within the window (p - j < window).  Tree
+// token t sees the context j < sk - sq and the tree keys named by its mask
+// bits; its place is sk - sq + popcount(mask_t) - 1, its depth in the tree.
+//
+// Layout of the work.  The G query heads of one kv head and the tokens of a
+// block are the columns of S^T = K Q^T (a lane owns one column, so a row's
+// softmax never leaves its four lane groups), and P, rounded to bf16 as the
+// MFMA takes it, is already the operand of O^T = V^T P^T.  An item is one
+// block of columns of one kv head (or of one column block of several heads,
+// see below) against its visible 32-key tiles; the concatenated tiles of all
+// items are cut into equal shares, one workgroup each, on the device from the
+// device's lengths, so a call needs no lengths on the host and can be
+// captured.  An item cut between shares leaves fp32 partials that a second
+// launch joins.
+//
+// Two forms share the tile arithmetic:
+//   private  few columns (decode rows, small trees): every wave streams its
+//            own tiles through its own LDS slots, without a workgroup
+//            barrier; waves differ in kv head and in tile phase.
+//   shared   many columns (chunks, large trees): the waves split the columns
+//            and read the same tile from a ring of LDS stages.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "kvc_lds.h"
+
+namespace kvc {
+namespace {
+
+constexpr int kD = 128;
+constexpr int kTile = 32;
+constexpr int kTensor = kTile * kD * 2;  // one K or V tile of a head: 8 KiB
+constexpr float kLazyLog2 = 8.f;         // the running reference moves when passed by 2^8
+constexpr float kLowest = -3.402823466e38f;
+
+enum ScoreMode {
+  kPlain = 0,
+  kDistance = 1,
+  kCapFixed = 2,     // cap log2(e) <= kCapFixedMax: 2^x needs no running maximum
+  kCapLazy = 3,
+  kCapDistance = 4,
+};
+// 2^(cap log2 e) stays within 2^80: sums over 2^20 keys and |v| up to 2^27
+// fit fp32 and bf16's range, so exp2 needs no reference.  (With a distance
+// bias the scores have no such floor.)
+constexpr float kCapFixedMax = 80.f;
+
+struct ScoredParams {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t k_row, k_head, v_row, v_head;  // elements per token row and kv head
+  const int32_t* tables;                 // null: fresh rows at cu_k
+  int64_t bt_stride;
+  int max_blocks, num_blocks, page;
+  int64_t fresh_rows;
+  const int32_t* cu_q;  // null: q_per_seq tokens each
+  int q_per_seq;
+  const int32_t* lens;  // keys per sequence (plus the queries, lens_exclude_q), or null
+  const int32_t* cu_k;
+  int lens_exclude_q;
+  const uint32_t* mask;  // tree bits, mask_words 32-bit words a token, or null
+  int mask_words;
+  const int32_t* places;  // tree depths (popcount - 1) per token, or null
+  const int32_t* prefix;
+  const float* slopes;
+  float scale, cap;
+  int window;
+  int batch, num_tokens, heads, kv_heads, group;
+  int heads_per_wg, head_groups;
+  int tokens_per_block;
+  int lane_plan;  // the plan walks sequences across lanes (else blocks)
+  int min_share;
+  int4* rec;  // per item: sequence, block, first and last share
+  int max_items;
+  float* part_o;
+  float2* part_ml;
+};
+
+struct SeqGeo {
+  int q0, sq, sk;
+};
+
+__device__ __forceinline__ SeqGeo seq_geo(const ScoredParams& p, int q0, int q1, int len, int k0,
+                                          int k1) {
+  SeqGeo g;
+  g.q0 = max(0, min(q0, p.num_tokens));
+  g.sq = max(0, min(q1, p.num_tokens) - g.q0);
+  int64_t sk, most;
+  if (p.lens != nullptr) {
+    sk = int64_t(len) + (p.lens_exclude_q ? g.sq : 0);
+  } else {
+    sk = int64_t(k1) - k0;
+  }
+  most = p.tables != nullptr ? int64_t(p.max_blocks) * p.page : p.fresh_rows - max(k0, 0);
+  g.sk = int(max(int64_t(0), min(sk, most)));
+  return g;
+}
+
+// Geometry of sequence i from per-lane (vector) loads or uniform (scalar) ones.
+template <bool kUniform>
+__device__ __forceinline__ SeqGeo load_seq(const ScoredParams& p, int i) {
+  auto at = [&](const int32_t* t, int64_t idx) {
+    if constexpr (kUniform) return table_entry(t, idx);
+    return t[idx];
+  };
+  int q0, q1, len = 0, k0 = 0, k1 = 0;
+  if (p.cu_q != nullptr) {
+    q0 = at(p.cu_q, i);
+    q1 = at(p.cu_q, i + 1);
+  } else {
+    q0 = i * p.q_per_seq;
+    q1 = q0 + p.q_per_seq;
+  }
+  if (p.lens != nullptr) {
+    len = at(p.lens, i);
+  } else {
+    k0 = at(p.cu_k, i);
+    k1 = at(p.cu_k, i + 1);
+  }
+  return seq_geo(p, q0, q1, len, k0, k1);
+}
+
+__device__ __forceinline__ int num_blocks_of(const ScoredParams& p, int sq) {
+  return (sq + p.tokens_per_block - 1) / p.tokens_per_block;
+}
+
+// Key tiles [t0, t1) that block c of a sequence sees.
+struct TileRange {
+  int t0, t1;
+};
+__device__ __forceinline__ TileRange block_tiles(const ScoredParams& p, const SeqGeo& g, int pre,
+                                                 int c) {
+  const int p0 = g.sk - g.sq;
+  const int first = c * p.tokens_per_block;
+  const int last = min(g.sq, first + p.tokens_per_block) - 1;
+  int lo = 0, hi;
+  if (p.mask != nullptr) {
+    hi = g.sk;
+    if (p.window > 0) lo = max(0, p0 - p.window);  // place >= context - 1
+  } else {
+    hi = min(g.sk, max(p0 + last + 1, pre));
+    if (p.window > 0) lo = max(0, p0 + first + 1 - p.window);
+  }
+  TileRange r;
+  r.t0 = lo / kTile;
+  r.t1 = max(r.t0, (max(hi, 0) + kTile - 1) / kTile);
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// One wave's columns and running state.
+// ---------------------------------------------------------------------------
+template <int NCB>
+struct Columns {
+  int token[NCB];         // t, the column's token inside its sequence
+  float place[NCB];       // p, for the distance bias
+  float slope2[NCB];      // slope log2(e)
+  const uint32_t* bits;   // tree: the sequence's masks
+  const int32_t* depths;  // tree: the sequence's depths
+  int pre;                // two-way prefix
+  int p0, sk, sq;         // p0: keys before the sequence's queries
+  int full_lo, full_hi;   // a tile inside these keys needs no mask
+  int any_lo, any_hi;     // a tile outside them is seen by no column
+};
+
+template <int NCB>
+struct State {
+  f32x4_t o[NCB][8];
+  f32x4_t l[NCB];
+  float mu[NCB];
+};
+
+template <int NCB>
+__device__ __forceinline__ void reset(State<NCB>& st, float mu0) {
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+#pragma unroll
+    for (int jj = 0; jj < 8; ++jj) st.o[cb][jj] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    st.l[cb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    st.mu[cb] = mu0;
+  }
+}
+
+__device__ __forceinline__ uint32_t bits_below(int n) {  // bits 0 .. n - 1
+  return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+}
+
+// The visible keys of the lane's column cb in the tile at key j0, as bits.
+template <int NCB>
+__device__ __forceinline__ uint32_t visible_bits(const ScoredParams& p, const Columns<NCB>& c,
+                                                 int cb, int j0) {
+  const int t = c.token[cb];
+  if (p.mask == nullptr) {
+    uint32_t vis = bits_below(min(c.sk, max(c.p0 + t + 1, c.pre)) - j0);
+    if (p.window > 0) vis &= ~bits_below(c.p0 + t + 1 - p.window - j0);
+    return vis;
+  }
+  uint32_t vis = bits_below(c.p0 - j0);
+  const int place = p.window > 0 ? c.p0 + c.depths[t] : 0;
+  if (p.window > 0) vis &= ~bits_below(place + 1 - p.window - j0);
+  const int u0 = j0 - c.p0;  // tree index of the tile's first key
+  if (u0 > -kTile) {
+    const uint32_t* m = c.bits + int64_t(t) * p.mask_words;
+    uint32_t tree;
+    if (u0 >= 0) {
+      const int w = u0 >> 5, sh = u0 & 31;
+      const uint32_t a = w < p.mask_words ? m[w] : 0u;
+      const uint32_t b = w + 1 < p.mask_words ? m[w + 1] : 0u;
+      tree = sh ? (a >> sh) | (b << (32 - sh)) : a;
+    } else {
+      tree = m[0] << (-u0);
+    }
+    tree &= bits_below(c.sk - j0);
+    if (p.window > 0 && p.window < c.sq) {
+      // Only here can two depths of one tree be a window apart.
+      for (int k = max(0, -u0); k < kTile && u0 + k < c.sq; ++k)
+        if (place - c.p0 - c.depths[u0 + k] >= p.window) tree &= ~(1u << k);
+    }
+    vis |= tree;
+  }
+  return vis;
+}
+
+struct Consts {
+  float c2;      // scale log2(e)
+  float zc;      // 2 log2(e) scale / cap
+  float a, a2;   // cap log2(e) and twice that
+};
+
+// The key offset of element e (0 .. 7) of a lane's column inside a tile: the
+// MFMA's C rows 4 lg + i of the two 16-key halves, which is also the K index
+// order of the P operand.
+__device__ __forceinline__ int key_of(int e) { return (e & 3) + 16 * (e >> 2); }
+
+// S^T = K Q^T, the score's shape, the mask, the running softmax, and P^T as
+// the bf16 operand pb.  y holds what the softmax is taken of: the raw logit
+// s (log2-unit score c2 s) for plain scores, the log2-unit score otherwise;
+// -inf at keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} + 1): one
+// exp2 and one reciprocal.  Sums are formed of the rounded P (an MFMA against
+// ones), so the weights add up to the sum that divides them.
+template <int NCB, int MODE>
+__device__ __forceinline__ void score_tile(const ScoredParams& p, const Columns<NCB>& c,
+                                           State<NCB>& st, const u32x4_t (&k)[2][4],
+                                           const u32x4_t (&q)[NCB][4], int j0, int lg,
+                                           const Consts& cs, bool masked, u32x4_t (&pb)[NCB],
+                                           uint32_t (&vis)[NCB]) {
+  constexpr bool kDist = MODE == kDistance || MODE == kCapDistance;
+  constexpr bool kCap = MODE == kCapFixed || MODE == kCapLazy || MODE == kCapDistance;
+  const float unit = MODE == kPlain ? cs.c2 : 1.f;
+  float y[NCB][8];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    f32x4_t lo = {0.f, 0.f, 0.f, 0.f}, hi = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      lo = mfma_bf16(k[0][d], q[cb][d], lo);
+      hi = mfma_bf16(k[1][d], q[cb][d], hi);
+    }
+    // The bias of a key at or before the query's place.
+    const float b0 = kDist ? c.slope2[cb] * (float(j0 + 4 * lg) - c.place[cb]) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float s = e < 4 ? lo[e & 3] : hi[e & 3];
+      float x = s;
+      if constexpr (kCap) {
+        const float w = __builtin_amdgcn_exp2f(s * cs.zc);
+        x = __builtin_fmaf(-cs.a2, __builtin_amdgcn_rcpf(w + 1.f), cs.a);
+      }
+      if constexpr (kDist) {
+        const float bias = __builtin_fmaf(c.slope2[cb], float(key_of(e)), b0);
+        x = kCap ? x + bias : __builtin_fmaf(s, cs.c2, bias);
+      }
+      y[cb][e] = x;
+    }
+  }
+  // (the branch changes y in place: one copy of everything else)
+  if (masked) {
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      vis[cb] = visible_bits<NCB>(p, c, cb, j0);
+      const uint32_t own = vis[cb] >> (4 * lg);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (kDist) {
+          const int j = j0 + 4 * lg + key_of(e);
+          int at = j;
+          if (p.mask != nullptr && j >= c.p0 && j < c.sk) at = c.p0 + c.depths[j - c.p0];
+          y[cb][e] = __builtin_fmaf(
+              -c.slope2[cb], fabsf(c.place[cb] - float(at)) + (float(j) - c.place[cb]), y[cb][e]);
+        }
+        y[cb][e] = ((own >> key_of(e)) & 1u) ? y[cb][e] : -INFINITY;
+      }
+    }
+  }
+  if constexpr (MODE != kCapFixed) {
+    // The reference moves only when a column passes it by 2^8 (or has none).
+    float over = -INFINITY;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      float top = y[cb][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, y[cb][e]);
+      over = fmaxf(over, __builtin_fmaf(top, unit, -st.mu[cb]));
+    }
+    if (__builtin_expect(__any(over > kLazyLog2), 0)) {
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        float top = y[cb][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = fmaxf(top, y[cb][e]);
+        const float mu = fmaxf(st.mu[cb], rows4_max(top) * unit);
+        const float down = __builtin_amdgcn_exp2f(st.mu[cb] - mu);
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) st.o[cb][jj] *= down;
+        st.l[cb] *= down;
+        st.mu[cb] = mu;
+      }
+    }
+  }
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    float pr[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      pr[e] = __builtin_amdgcn_exp2f(MODE == kCapFixed ? y[cb][e]
+                                     : MODE == kPlain ? __builtin_fmaf(y[cb][e], unit, -st.mu[cb])
+                                                      : y[cb][e] - st.mu[cb]);
+    pb[cb] = u32x4_t{pack_bf16x2_fast(pr[0], pr[1]), pack_bf16x2_fast(pr[2], pr[3]),
+                     pack_bf16x2_fast(pr[4], pr[5]), pack_bf16x2_fast(pr[6], pr[7])};
+  }
+}
+
+constexpr uint32_t kOnes2 = 0x3F803F80u;
+
+__device__ __forceinline__ bool not_finite(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a),
+                                                      __builtin_bit_cast(u16x2_t, b)));
+}
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+  return (not_finite(w) ? 0u : w & 0xffffu) | (not_finite(w >> 16) ? 0u : w & 0xffff0000u);
+}
+
+// LDS image of a K or V tile: row r (key) is 256 bytes, its 16-byte chunk ch
+// at chunk ch ^ (r & 15), which keeps both the row-wise K reads (16 rows of
+// one chunk) and the transposed V reads (4 rows x 4 chunks per lane group)
+// on distinct banks without padding, so a tile is eight whole 1 KiB loads.
+// The V operand's rows are dims 32 (m / 4) + 4 jj + m % 4, so that a lane's
+// outputs are 32 consecutive dims of its column.
+struct LdsAddr {
+  int k[4];  // K operand d: row lm, chunk 4 d + lg
+  int v[4];  // V operand pair jj / 2: row 4 lg + lm / 4, chunk 4 (lm % 4) + jj / 2
+};
+__device__ __forceinline__ LdsAddr lds_addrs(int lm, int lg) {
+  LdsAddr a;
+  const int vr = 4 * lg + (lm >> 2);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    a.k[d] = lm * 256 + (((4 * d + lg) ^ lm) << 4);
+    a.v[d] = vr * 256 + (((4 * (lm & 3) + d) ^ vr) << 4);
+  }
+  return a;
+}
+
+__device__ __forceinline__ void read_k(u32x4_t (&k)[2][4], const char* kt, const LdsAddr& a) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      k[h][d] = *reinterpret_cast<const u32x4_t*>(kt + a.k[d] + h * 4096);
+}
+
+__device__ __forceinline__ u32x4_t read_v(const char* vt, const LdsAddr& a, int jj) {
+  const char* s = vt + a.v[jj >> 1] + (jj & 1) * 8;
+  const u32x2_t lo = lds_read_tr16(s), hi = lds_read_tr16(s + 4096);
+  return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// O^T += V^T P^T.  In a masked tile a column's P is 0 at keys it does not see,
+// but 0 times an infinity or NaN held there would still reach its sum: such
+// values are taken out of the operand and added to the columns that do see
+// their key (whose result they decide whatever their weight).
+template <int NCB>
+__device__ __forceinline__ void weigh_tile(State<NCB>& st, const char* vt, u32x4_t (&v)[8],
+                                           const u32x4_t (&pb)[NCB], const uint32_t (&vis)[NCB],
+                                           int lg, bool masked) {
+  bool odd = false;
+  if (masked) {
+    uint32_t most = 0u;
+#pragma unroll
+    for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = max_u16x2(most, v[jj][i] & 0x7fff7fffu);
+    odd = __any(not_finite(most) || not_finite(most >> 16));
+    if (__builtin_expect(odd, 0)) {
+#pragma unroll
+      for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[jj][i] = finite_or_zero(v[jj][i]);
+    }
+  }
+  const u32x4_t ones = {kOnes2, kOnes2, kOnes2, kOnes2};
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) st.l[cb] = mfma_bf16(ones, pb[cb], st.l[cb]);
+#pragma unroll
+  for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) st.o[cb][jj] = mfma_bf16(v[jj], pb[cb], st.o[cb][jj]);
+  {
+    if (__builtin_expect(odd, 0)) {
+      for (int r = 0; r < kTile; ++r) {
+#pragma unroll 1
+        for (int jj = 0; jj < 8; ++jj) {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(
+              vt + r * 256 + (((4 * lg + (jj >> 1)) ^ (r & 15)) << 4) + (jj & 1) * 8);
+          f32x4_t add;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t half = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+            add[i] = not_finite(half) ? bf16_bits_to_f32(half) : 0.f;
+          }
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) {
+            const bool on = ((vis[cb] >> r) & 1u) != 0u;
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+              if (n == jj)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st.o[cb][n][i] += on ? add[i] : 0.f;
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The plan: which item and tile a share starts at.  Every wave works it out
+// for itself from the device's lengths (no barrier before the first load).
+// ---------------------------------------------------------------------------
+// Virtual tiles that every item adds to its cost: its query loads, its pipe's
+// start and its epilogue.
+constexpr int kItemCost = 3;
+
+struct Where {
+  int seq, grp, block, tile;  // tile: offset inside the item
+  int nb;                     // column blocks of the sequences before seq
+  int64_t total;              // cost of the whole call
+  int blocks;                 // column blocks of the whole call
+};
+
+__device__ __forceinline__ int block_cost(const ScoredParams& p, const SeqGeo& g, int pre, int c) {
+  const TileRange r = block_tiles(p, g, pre, c);
+  return r.t1 - r.t0 + kItemCost;
+}
+
+// Cost and column blocks of lane's sequence (lane plan).
+__device__ __forceinline__ void lane_seq(const ScoredParams& p, int i, int& cost, int& nb) {
+  cost = nb = 0;
+  if (i >= p.batch) return;
+  const SeqGeo g = load_seq<false>(p, i);
+  const int pre = p.prefix != nullptr ? p.prefix[i] : 0;
+  nb = num_blocks_of(p, g.sq);
+  for (int c = 0; c < nb; ++c) cost += block_cost(p, g, pre, c);
+  cost *= p.head_groups;
+}
+
+// The same for a wave-uniform sequence, its blocks across the lanes.
+__device__ __forceinline__ int wave_seq(const ScoredParams& p, int i, int lane, int& nb) {
+  const SeqGeo g = load_seq<true>(p, i);
+  const int pre = p.prefix != nullptr ? table_entry(p.prefix, i) : 0;
+  nb = num_blocks_of(p, g.sq);
+  int cost = 0;
+  for (int c = 0; c < nb; c += 64)
+    cost += wave_sum(c + lane < nb ? block_cost(p, g, pre, c + lane) : 0);
+  return cost * p.head_groups;
+}
+
+__device__ __forceinline__ int first_lane(uint64_t m) { return __builtin_ctzll(m); }
+
+// Finds position `at` (share * size, size from the total) in the concatenated
+// items; false when it lies past the end.
+__device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int share, int shares,
+                                           Where& w, int& size) {
+  int total = 0, blocks = 0, cost = 0, nb = 0;
+  if (p.lane_plan) {
+    for (int i = 0; i < p.batch; i += 64) {
+      lane_seq(p, i + lane, cost, nb);
+      total += wave_sum(cost);
+      blocks += wave_sum(nb);
+    }
+  } else {
+    for (int i = 0; i < p.batch; ++i) {
+      total += wave_seq(p, i, lane, nb);
+      blocks += nb;
+    }
+  }
+  w.total = total;
+  w.blocks = blocks;
+  size = max(p.min_share, (total + shares - 1) / shares);
+  const int64_t at64 = int64_t(share) * size;
+  if (at64 >= total) return false;
+  const int at = int(at64);
+  int acc = 0, before = 0, seq = -1, start = 0;
+  if (p.lane_plan) {
+    for (int i = 0; i < p.batch; i += 64) {
+      if (p.batch > 64) lane_seq(p, i + lane, cost, nb);
+      const int upto = wave_scan_add(cost), nbs = wave_scan_add(nb);
+      const uint64_t hit = __ballot(acc + upto > at);
+      if (hit != 0) {
+        const int l = first_lane(hit);
+        seq = i + l;
+        start = acc + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(cost, l);
+        before += __builtin_amdgcn_readlane(nbs, l) - __builtin_amdgcn_readlane(nb, l);
+        break;
+      }
+      acc += __builtin_amdgcn_readlane(upto, 63);
+      before += __builtin_amdgcn_readlane(nbs, 63);
+    }
+  } else {
+    for (int i = 0; i < p.batch; ++i) {
+      cost = wave_seq(p, i, lane, nb);
+      if (acc + cost > at) {
+        seq = i;
+        start = acc;
+        break;
+      }
+      acc += cost;
+      before += nb;
+    }
+  }
+  if (seq < 0) return false;
+  w.seq = seq;
+  w.nb = before;
+  // Inside the sequence: head groups in turn, each over all column blocks.
+  const SeqGeo g = load_seq<true>(p, seq);
+  const int pre = p.prefix != nullptr ? table_entry(p.prefix, seq) : 0;
+  const int n = num_blocks_of(p, g.sq);
+  int each = 0;
+  for (int c = 0; c < n; c += 64)
+    each += wave_sum(c + lane < n ? block_cost(p, g, pre, c + lane) : 0);
+  const int rem = at - start;
+  w.grp = rem / each;
+  int left = rem - w.grp * each;
+  for (int c = 0; c < n; c += 64) {
+    const int one = c + lane < n ? block_cost(p, g, pre, c + lane) : 0;
+    const int upto = wave_scan_add(one);
+    const uint64_t hit = __ballot(upto > left);
+    if (hit != 0) {
+      const int l = first_lane(hit);
+      w.block = c + l;
+      w.tile = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(one, l));
+      return true;
+    }
+    left -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// ---------------------------------------------------------------------------
+// Tile addresses.
+// ---------------------------------------------------------------------------
+struct TileSource {
+  const uint16_t* k;
+  const uint16_t* v;
+  int rows;  // valid rows, 0: reads zeros
+};
+__device__ __forceinline__ TileSource tile_source(const ScoredParams& p, int seq, int64_t fresh0,
+                                                  int sk, int head, int tile) {
+  const int j0 = tile * kTile;
+  int64_t row;
+  int rows = min(kTile, sk - j0);
+  if (p.tables != nullptr) {
+    const int page = j0 / p.page;
+    int blk = 0;
+    if (page < p.max_blocks) {
+      blk = table_entry(p.tables, int64_t(seq) * p.bt_stride + page);
+      if (blk < 0 || blk >= p.num_blocks) rows = 0;
+    } else {
+      rows = 0;
+    }
+    row = rows > 0 ? int64_t(blk) * p.page + (j0 - page * p.page) : 0;
+  } else {
+    row = fresh0 + j0;
+  }
+  TileSource t;
+  t.k = p.k + row * p.k_row + head * p.k_head;
+  t.v = p.v + row * p.v_row + head * p.v_head;
+  t.rows = rows;
+  return t;
+}
+
+// Lane's byte offset of load m (rows 4 m .. 4 m + 3) of a tile.
+struct DmaOffsets {
+  int base[4];  // m = 0 .. 3
+  int step;     // 16 rows
+};
+__device__ __forceinline__ DmaOffsets dma_offsets(int lane, int64_t row_elems) {
+  DmaOffsets o;
+  const int lr = lane >> 4, slot = lane & 15;
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const int r = 4 * m + lr;
+    o.base[m] = r * int(row_elems) * 2 + ((slot ^ r) << 4);
+  }
+  o.step = 16 * int(row_elems) * 2;
+  return o;
+}
+__device__ __forceinline__ int tensor_bytes(int rows, int64_t row_elems) {
+  return rows > 0 ? (rows - 1) * int(row_elems) * 2 + kD * 2 : 0;
+}
+
+template <bool kStream>
+__device__ __forceinline__ void load_rows(const i32x4_t& rsrc, const DmaOffsets& o, int m,
+                                          uint32_t lds) {
+  const int off = o.base[m & 3] + (m >> 2) * o.step;
+  if constexpr (kStream) {
+    dma_to_lds(rsrc, off, lds + m * 1024);
+  } else {
+    dma_to_lds_cached(rsrc, off, lds + m * 1024);
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // all but the newest N
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
+// The kernel.  NW waves; KW of them take different tiles of a segment in the
+// shared form (the others share a tile and split the columns); KW = NW is the
+// private form, where waves split over heads_per_wg kv heads and tile phases.
+// ---------------------------------------------------------------------------
+template <int NW, int NCB, int KW>
+struct Form {
+  static constexpr bool kPrivate = KW == NW;
+  static constexpr int kColWaves = kPrivate ? 1 : NW / KW;
+  static constexpr int kColumns = 16 * NCB * kColWaves;  // per kv head
+  static constexpr int kStage = KW * 2 * kTensor;
+  static constexpr int kStages = kPrivate ? 1 : KW == 4 ? 2 : 4;
+  // waves that hand their state to another: [wave][34 NCB floats][64 lanes]
+  static constexpr int kStateBytes = 34 * NCB * 256;
+  static constexpr int kJoinBytes =
+      kPrivate ? (NW - 1) * kStateBytes : (NW - kColWaves) * kStateBytes;
+  static constexpr int kLds =
+      kStage * kStages > kJoinBytes ? kStage * kStages : kJoinBytes;
+  static_assert(kLds <= 160 * 1024, "one workgroup per CU");
+};
+
+template <int NCB>
+__device__ __forceinline__ void put_state(char* at, const State<NCB>& st, int lane) {
+  float* f = reinterpret_cast<float*>(at) + lane;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+#pragma unroll
+    for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[(cb * 34 + jj * 4 + i) * 64] = st.o[cb][jj][i];
+    f[(cb * 34 + 32) * 64] = st.l[cb][0];
+    f[(cb * 34 + 33) * 64] = st.mu[cb];
+  }
+}
+
+template <int NCB>
+__device__ __forceinline__ void join_state(State<NCB>& st, const char* at, int lane) {
+  const float* f = reinterpret_cast<const float*>(at) + lane;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const float l = f[(cb * 34 + 32) * 64], mu = f[(cb * 34 + 33) * 64];
+    const float top = fmaxf(mu, st.mu[cb]);
+    const float a = __builtin_amdgcn_exp2f(st.mu[cb] - top), b = __builtin_amdgcn_exp2f(mu - top);
+    st.mu[cb] = top;
+    st.l[cb][0] = st.l[cb][0] * a + l * b;
+#pragma unroll
+    for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        st.o[cb][jj][i] = st.o[cb][jj][i] * a + f[(cb * 34 + jj * 4 + i) * 64] * b;
+  }
+}
+
+template <int NW, int NCB, int KW, int MODE>
+__global__ void __launch_bounds__(64 * NW)
+    __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) scored_kernel(ScoredParams p) {
+  using F = Form<NW, NCB, KW>;
+  extern __shared__ __align__(1024) char smem[];
+  const int lane = threadIdx.x & 63, wave = uniform(int(threadIdx.x >> 6));
+  const int lm = lane & 15, lg = lane >> 4;
+  // Consecutive shares on one XCD (workgroup b runs on XCD b mod 8).
+  const int grid = gridDim.x;
+  const int share = grid % 8 == 0 ? (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
+
+  Where w;
+  int size;
+  const bool live = plan_share(p, lane, share, grid, w, size);
+  // Items that this call does not have, up to the bound its merge covers.
+  for (int i = w.blocks * p.head_groups + blockIdx.x * (64 * NW) + threadIdx.x; i < p.max_items;
+       i += grid * 64 * NW)
+    p.rec[i] = int4{0, 0, 0, 0};
+  if (!live) return;
+
+  const int hs = F::kPrivate ? wave % p.heads_per_wg : 0;
+  const int phases = F::kPrivate ? NW / p.heads_per_wg : KW;
+  const int phase = F::kPrivate ? wave / p.heads_per_wg : wave / F::kColWaves;
+  const int cw = F::kPrivate ? 0 : wave % F::kColWaves;
+  const LdsAddr la = lds_addrs(lm, lg);
+  const DmaOffsets ko = dma_offsets(lane, p.k_row), vo = dma_offsets(lane, p.v_row);
+  const uint32_t lds0 = lds_addr(smem);
+  Consts cs;
+  cs.c2 = p.scale * kLog2e;
+  cs.zc = p.cap > 0.f ? 2.f * kLog2e * p.scale / p.cap : 0.f;
+  cs.a = p.cap * kLog2e;
+  cs.a2 = 2.f * cs.a;
+  constexpr float mu0 = MODE == kCapFixed ? 0.f : kLowest;
+
+  int tcol[NCB], gcol[NCB];  // the column's token inside a block, its query head
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const int col = (cw * NCB + cb) * 16 + lm;
+    tcol[cb] = col / p.group;
+    gcol[cb] = col - tcol[cb] * p.group;
+  }
+  const int wave_t0 = cw * NCB * 16 / p.group;
+  const int wave_t1 = min((cw * NCB * 16 + NCB * 16 - 1) / p.group, p.tokens_per_block - 1);
+
+  const int end = int(min(w.total, int64_t(share + 1) * size));
+  int pos = share * size;
+  SeqGeo g = load_seq<true>(p, w.seq);
+  int nblocks = num_blocks_of(p, g.sq);
+  while (true) {
+    const int pre = p.prefix != nullptr ? table_entry(p.prefix, w.seq) : 0;
+    const TileRange range = block_tiles(p, g, pre, w.block);
+    const int tiles = range.t1 - range.t0;
+    const int item = (w.nb + w.block) * p.head_groups + w.grp;
+    const int seg0 = w.tile, seg1 = min(tiles, w.tile + (end - pos));
+    const int last_share = tiles > 0 ? (pos - w.tile + tiles - 1) / size : share;
+    if (w.tile == 0 && threadIdx.x == 0 && item < p.max_items) p.rec[item] = int4{w.seq, w.block, share, last_share};
+
+    if (seg0 < seg1 || (tiles == 0 && w.tile == 0)) {
+      const int head = w.grp * p.heads_per_wg + hs;
+      const int64_t fresh0 =
+          p.tables == nullptr ? max(0, table_entry(p.cu_k, w.seq)) : 0;
+      const int p0 = g.sk - g.sq;
+      const int b0 = w.block * p.tokens_per_block;  // the block's first token
+      const int tmax = min(g.sq, b0 + p.tokens_per_block) - 1;
+
+      Columns<NCB> c;
+      const uint16_t* qp[NCB];
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        // (columns past the block repeat its last token)
+        const int t = min(b0 + tcol[cb], tmax);
+        qp[cb] = p.q + int64_t(g.q0 + t) * p.q_st + int64_t(head * p.group + gcol[cb]) * p.q_sh;
+        c.token[cb] = t;
+        c.place[cb] = float(p0 + (p.mask == nullptr      ? t
+                                  : p.places != nullptr ? p.places[g.q0 + t]
+                                                        : 0));
+        c.slope2[cb] =
+            p.slopes != nullptr ? p.slopes[head * p.group + gcol[cb]] * kLog2e : 0.f;
+      }
+      c.bits = p.mask != nullptr ? p.mask + int64_t(g.q0) * p.mask_words : nullptr;
+      c.depths = p.places != nullptr ? p.places + g.q0 : nullptr;
+      c.pre = pre;
+      c.p0 = p0;
+      c.sk = g.sk;
+      c.sq = g.sq;
+      {
+        const int ta = min(b0 + wave_t0, tmax), tb = min(b0 + wave_t1, tmax);
+        if (p.mask == nullptr) {
+          c.any_lo = p.window > 0 ? p0 + ta + 1 - p.window : 0;
+          c.full_lo = p.window > 0 ? p0 + tb + 1 - p.window : 0;
+          // A two-way prefix makes |p - j| bend inside it.
+          c.full_hi = min(g.sk, MODE == kDistance || MODE == kCapDistance
+                                    ? p0 + ta + 1 : max(p0 + ta + 1, pre));
+          c.any_hi = min(g.sk, max(p0 + tb + 1, pre));
+        } else {
+          c.any_lo = p.window > 0 ? p0 - p.window : 0;
+          c.full_lo = p.window > 0 ? p0 + g.sq - p.window : 0;  // depth < sq
+          c.full_hi = p0;
+          c.any_hi = g.sk;
+        }
+      }
+      u32x4_t q[NCB][4];
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          q[cb][d] = *reinterpret_cast<const u32x4_t*>(qp[cb] + 32 * d + 8 * lg);
+      // Every compiler-tracked load is back before the counted ones start.
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        asm volatile("" : "+v"(c.place[cb]), "+v"(c.slope2[cb]));
+#pragma unroll
+        for (int d = 0; d < 4; ++d) asm volatile("" : "+v"(q[cb][d]));
+      }
+      wait_loads<0>();
+
+      State<NCB> st;
+      reset<NCB>(st, mu0);
+      auto attend = [&](const char* kt, const char* vt, int j0, auto&& k_read, auto&& v_ready,
+                        auto&& v_read) {
+        const bool masked = j0 < c.full_lo || j0 + kTile > c.full_hi;
+        u32x4_t k[2][4], v[8], pb[NCB];
+        uint32_t vis[NCB];
+        read_k(k, kt, la);
+        k_read();
+        score_tile<NCB, MODE>(p, c, st, k, q, j0, lg, cs, masked, pb, vis);
+        v_ready();
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) v[jj] = read_v(vt, la, jj);
+        if (!masked) v_read();
+        weigh_tile<NCB>(st, vt, v, pb, vis, lg, masked);
+        if (masked) v_read();
+      };
+
+      const int t_begin = range.t0 + seg0, t_end = range.t0 + seg1;
+      if constexpr (F::kPrivate) {
+        // Wave-private slots: K 8 KiB, V 8 KiB.  The next tile's K load goes
+        // out as soon as this tile's K is in registers, its V load likewise.
+        const uint32_t kl = lds0 + wave * (2 * kTensor), vl = kl + kTensor;
+        const char* kt = smem + wave * (2 * kTensor);
+        const char* vt = kt + kTensor;
+        auto issue_k = [&](const TileSource& t) {
+          const i32x4_t r = raw_rsrc(t.k, tensor_bytes(t.rows, p.k_row));
+#pragma unroll
+          for (int m = 0; m < 8; ++m) load_rows<true>(r, ko, m, kl);
+        };
+        auto issue_v = [&](const TileSource& t) {
+          const i32x4_t r = raw_rsrc(t.v, tensor_bytes(t.rows, p.v_row));
+#pragma unroll
+          for (int m = 0; m < 8; ++m) load_rows<true>(r, vo, m, vl);
+        };
+        int t = t_begin + phase;
+        if (t < t_end) {
+          TileSource src = tile_source(p, w.seq, fresh0, g.sk, head, t);
+          issue_k(src);
+          issue_v(src);
+        }
+        for (; t < t_end; t += phases) {
+          const bool more = t + phases < t_end;
+          const TileSource next =
+              tile_source(p, w.seq, fresh0, g.sk, head, more ? t + phases : t);
+          wait_loads<8>();
+          attend(
+              kt, vt, t * kTile,
+              [&] {
+                lds_done();
+                if (more) issue_k(next);
+              },
+              [&] {
+                if (more) {
+                  wait_loads<8>();
+                } else {
+                  wait_loads<0>();
+                }
+              },
+              [&] {
+                lds_done();
+                if (more) issue_v(next);
+              });
+        }
+      } else {
+        // Stage s of the ring: KW subtiles, each K then V.  A wave issues
+        // its share of every subtile's 16 loads; three tiles are in flight
+        // under the one that is attended, one barrier a step.
+        constexpr int kPer = 16 * KW / NW;  // loads a wave issues per stage
+        static_assert(16 * KW % NW == 0 && 8 % kPer == 0, "loads split evenly over the waves");
+        const int steps = (t_end - t_begin + KW - 1) / KW;
+        auto issue = [&](int step) {
+          // loads kPer * wave .. + kPer - 1 of the stage: within one tensor
+          const int first = kPer * wave;
+          const int sub = first / 16, tensor = (first / 8) & 1, m0 = first & 7;
+          const int t = t_begin + step * KW + sub;
+          TileSource src{p.k, p.v, 0};
+          if (t < t_end) src = tile_source(p, w.seq, fresh0, g.sk, head, t);
+          const i32x4_t r = tensor ? raw_rsrc(src.v, tensor_bytes(src.rows, p.v_row))
+                                   : raw_rsrc(src.k, tensor_bytes(src.rows, p.k_row));
+          const uint32_t at = lds0 + (step % F::kStages) * F::kStage + (2 * sub + tensor) * kTensor;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            // (m0 is a multiple of kPer: the row offset adds up from it)
+            const int m = m0 + i;
+            const int lr = lane >> 4, r16 = (4 * m + lr) & 15;
+            const int row_bytes = int(tensor ? p.v_row : p.k_row) * 2;
+            dma_to_lds_cached(r, (4 * m + lr) * row_bytes + (((lane & 15) ^ r16) << 4),
+                              at + m * 1024);
+          }
+        };
+#pragma unroll
+        for (int s = 0; s < F::kStages - 1; ++s) issue(s);
+        for (int step = 0; step < steps; ++step) {
+          wait_loads<kPer*(F::kStages - 2)>();
+          pf_barrier();  // this stage is whole, and the one before it free
+          issue(step + F::kStages - 1);
+          const int t = t_begin + step * KW + phase;
+          const int j0 = t * kTile;
+          if (t < t_end && j0 < c.any_hi && j0 + kTile > c.any_lo) {
+            const char* kt = smem + (step % F::kStages) * F::kStage + phase * 2 * kTensor;
+            attend(kt, kt + kTensor, j0, [] {}, [] {}, [] {});
+          }
+        }
+        wait_loads<0>();
+      }
+
+      // Join the tile phases: the waves of phase 0 take in the others' states.
+      if (phases > 1) {
+        const int owners = NW / phases;
+        __syncthreads();
+        if (phase > 0) put_state<NCB>(smem + (wave - owners) * F::kStateBytes, st, lane);
+        __syncthreads();
+        if (phase == 0)
+          for (int f = 1; f < phases; ++f)
+            join_state<NCB>(st, smem + (wave + (f - 1) * owners) * F::kStateBytes, lane);
+        __syncthreads();
+      } else if constexpr (!F::kPrivate) {
+        pf_barrier();  // the ring is free for the next item
+      }
+      if (phase == 0) {
+        if (seg0 == 0 && seg1 == tiles) {
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) {
+            if (tcol[cb] >= p.tokens_per_block || b0 + tcol[cb] > tmax) continue;
+            const float inv = st.l[cb][0] != 0.f ? 1.f / st.l[cb][0] : 0.f;
+            uint32_t o[16];
+#pragma unroll
+            for (int jj = 0; jj < 8; ++jj) {
+              o[2 * jj] = pack_bf16x2_fast(st.o[cb][jj][0] * inv, st.o[cb][jj][1] * inv);
+              o[2 * jj + 1] = pack_bf16x2_fast(st.o[cb][jj][2] * inv, st.o[cb][jj][3] * inv);
+            }
+            uint16_t* dst = p.out + int64_t(g.q0 + b0 + tcol[cb]) * p.o_st +
+                            int64_t(head * p.group + gcol[cb]) * p.o_sh + 32 * lg;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<u32x4_t*>(dst)[i] =
+                  u32x4_t{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+          }
+        } else {
+          // Slot 2 share + 1: the piece that begins its item; else 2 share.
+          const int64_t slot = int64_t(2) * share + (seg0 == 0 ? 1 : 0);
+          const int64_t cols = int64_t(p.heads_per_wg) * F::kColumns;
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) {
+            if (tcol[cb] >= p.tokens_per_block || b0 + tcol[cb] > tmax) continue;
+            const int64_t col = slot * cols + hs * F::kColumns + (cw * NCB + cb) * 16 + lm;
+            float* dst = p.part_o + col * kD + 32 * lg;
+#pragma unroll
+            for (int jj = 0; jj < 8; ++jj) reinterpret_cast<f32x4_t*>(dst)[jj] = st.o[cb][jj];
+            if (lg == 0) p.part_ml[col] = float2{st.mu[cb], st.l[cb][0]};
+          }
+        }
+      }
+    }
+
+    pos += tiles + kItemCost - w.tile;
+    if (pos >= end) break;
+    w.tile = 0;
+    if (++w.block < nblocks) continue;
+    w.block = 0;
+    if (++w.grp < p.head_groups) continue;
+    w.grp = 0;
+    w.nb += nblocks;
+    do {
+      if (++w.seq >= p.batch) return;
+      g = load_seq<true>(p, w.seq);
+      nblocks = num_blocks_of(p, g.sq);
+    } while (nblocks == 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Join the partials of items cut between shares: one workgroup per item and
+// head slot, 32 lanes per column.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) scored_merge_kernel(ScoredParams p, int columns) {
+  const int item = blockIdx.x / p.heads_per_wg, hs = blockIdx.x % p.heads_per_wg;
+  const int4 r = p.rec[item];
+  if (r.w <= r.z) return;  // whole, or not there
+  const SeqGeo g = load_seq<true>(p, r.x);
+  const int head = (item % p.head_groups) * p.heads_per_wg + hs;
+  const int b0 = r.y * p.tokens_per_block;
+  const int tokens = min(g.sq - b0, p.tokens_per_block);
+  const int lane = threadIdx.x & 31;
+  const int64_t cols = int64_t(p.heads_per_wg) * columns;
+  for (int col = threadIdx.x >> 5; col < tokens * p.group; col += 8) {
+    const int64_t at = hs * columns + col;
+    float top = kLowest;
+    for (int s = r.z; s <= r.w; ++s)
+      top = fmaxf(top, p.part_ml[(int64_t(2) * s + (s == r.z)) * cols + at].x);
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int s = r.z; s <= r.w; ++s) {
+      const int64_t c = (int64_t(2) * s + (s == r.z)) * cols + at;
+      const float2 ml = p.part_ml[c];
+      const float a = __builtin_amdgcn_exp2f(ml.x - top);
+      l += ml.y * a;
+      o += reinterpret_cast<const f32x4_t*>(p.part_o + c * kD)[lane] * a;
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const int t = col / p.group;
+    uint16_t* dst = p.out + int64_t(g.q0 + b0 + t) * p.o_st +
+                    int64_t(head * p.group + col - t * p.group) * p.o_sh + 4 * lane;
+    *reinterpret_cast<u32x2_t*>(dst) =
+        u32x2_t{pack_bf16x2_fast(o[0] * inv, o[1] * inv), pack_bf16x2_fast(o[2] * inv, o[3] * inv)};
+  }
+}
+
+// Depth of each tree token: its mask's bits inside the tree but its own.
+__global__ void __launch_bounds__(64) tree_depth_kernel(ScoredParams p, int32_t* depth) {
+  const SeqGeo g = load_seq<true>(p, blockIdx.x);
+  for (int t = threadIdx.x; t < g.sq; t += 64) {
+    const uint32_t* m = p.mask + int64_t(g.q0 + t) * p.mask_words;
+    int n = 0;
+    for (int w = 0; w < p.mask_words && 32 * w < g.sq; ++w) n += __popc(m[w] & bits_below(g.sq - 32 * w));
+    depth[g.q0 + t] = n - 1;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+int cu_count() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        n <= 0)
+      n = 256;
+    cached[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+struct Plan {
+  int form;  // index of the column count below
+  int columns, heads_per_wg, head_groups, tokens_per_block;
+  int grid;
+  int64_t max_items;
+  size_t rec_bytes, ml_bytes, o_bytes;
+  size_t bytes() const { return rec_bytes + ml_bytes + o_bytes; }
+};
+
+constexpr int kFormColumns[] = {16, 32, 64, 128, 256};
+constexpr int kForms = 5;
+
+size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// The form: the narrowest whose columns hold the longest row of the call (its
+// tokens x query heads per kv head), the widest where none does.
+Plan make_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, int64_t max_q) {
+  Plan pl{};
+  const int64_t group = heads / kv_heads;
+  const int64_t want = std::max<int64_t>(1, std::min(max_q, tokens)) * group;
+  pl.form = 0;
+  while (pl.form + 1 < kForms && kFormColumns[pl.form] < want) ++pl.form;
+  pl.columns = kFormColumns[pl.form];
+  int most = pl.form <= 1 ? 4 : 1;
+  while (most > 1 && kv_heads % most != 0) most >>= 1;
+  pl.heads_per_wg = most;
+  pl.head_groups = int(kv_heads / most);
+  pl.tokens_per_block = int(pl.columns / group);
+  pl.grid = cu_count();
+  pl.max_items = (tokens / pl.tokens_per_block + batch) * pl.head_groups;
+  const size_t cols = size_t(2) * pl.grid * pl.heads_per_wg * pl.columns;
+  pl.rec_bytes = up256(size_t(pl.max_items) * sizeof(int4));
+  pl.ml_bytes = up256(cols * sizeof(float2));
+  pl.o_bytes = up256(cols * kD * sizeof(float));
+  return pl;
+}
+
+template <int NW, int NCB, int KW, int MODE>
+int launch_one(const ScoredParams& p, int grid, hipStream_t st) {
+  using F = Form<NW, NCB, KW>;
+  static std::atomic<uint64_t> ready{0};  // devices whose LDS limit is set
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (e == hipSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&scored_kernel<NW, NCB, KW, MODE>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, F::kLds);
+    if (e == hipSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  KVC_REQUIRE(e == hipSuccess, KVC_ERR_RUNTIME, "scored attention: LDS limit: %s",
+              hipGetErrorString(e));
+  scored_kernel<NW, NCB, KW, MODE><<<grid, 64 * NW, F::kLds, st>>>(p);
+  return check_launch("scored attention");
+}
+
+template <int MODE>
+int launch_form(const ScoredParams& p, const Plan& pl, hipStream_t st) {
+  switch (pl.form) {
+    case 0: return launch_one<8, 1, 8, MODE>(p, pl.grid, st);
+    case 1: return launch_one<8, 2, 8, MODE>(p, pl.grid, st);
+    case 2: return launch_one<8, 2, 4, MODE>(p, pl.grid, st);
+    case 3: return launch_one<8, 2, 2, MODE>(p, pl.grid, st);
+    default: return launch_one<8, 2, 1, MODE>(p, pl.grid, st);
+  }
+}
+
+// One launch over `p`'s sequences and its merge.  what: the entry's name.
+int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStream_t st,
+             const char* what) {
+  const Plan pl = make_plan(p.num_tokens, p.heads, p.kv_heads, p.batch, max_q);
+  KVC_REQUIRE(pl.max_items * ((max_keys + kTile - 1) / kTile + kItemCost) < (int64_t(1) << 30),
+              KVC_ERR_VALUE, "%s: too many query blocks x keys for one call", what);
+  p.heads_per_wg = pl.heads_per_wg;
+  p.head_groups = pl.head_groups;
+  p.tokens_per_block = pl.tokens_per_block;
+  const int64_t nb = (std::min<int64_t>(max_q, p.num_tokens) + pl.tokens_per_block - 1) /
+                     pl.tokens_per_block;
+  p.lane_plan = (p.batch + 63) / 64 * nb <= p.batch + p.num_tokens / pl.tokens_per_block / 64;
+  p.min_share = 4;
+  char* w = static_cast<char*>(ws);
+  p.rec = reinterpret_cast<int4*>(w);
+  p.part_ml = reinterpret_cast<float2*>(w + pl.rec_bytes);
+  p.part_o = reinterpret_cast<float*>(w + pl.rec_bytes + pl.ml_bytes);
+  p.max_items = int(pl.max_items);
+  int rc;
+  const bool bias = p.slopes != nullptr;
+  if (p.cap > 0.f) {
+    if (bias) {
+      rc = launch_form<kCapDistance>(p, pl, st);
+    } else if (p.cap * kLog2e <= kCapFixedMax) {
+      rc = launch_form<kCapFixed>(p, pl, st);
+    } else {
+      rc = launch_form<kCapLazy>(p, pl, st);
+    }
+  } else {
+    rc = bias ? launch_form<kDistance>(p, pl, st) : launch_form<kPlain>(p, pl, st);
+  }
+  if (rc != KVC_OK) return rc;
+  scored_merge_kernel<<<unsigned(pl.max_items * pl.heads_per_wg), 256, 0, st>>>(p, pl.columns);
+  return check_launch(what);
+}
+
+bool rows16(const void* p, int64_t st, int64_t sh) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && st % 8 == 0 && sh % 8 == 0;
+}
+
+int check_common(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_t tokens,
+                 int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, float softcap,
+                 int64_t window,
+                 const void* out, int64_t o_st, int64_t o_sh) {
+  KVC_REQUIRE(head_dim == kD, KVC_ERR_VALUE, "%s: head_dim must be 128 (got %lld)", what,
+              (long long)head_dim);
+  KVC_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, KVC_ERR_VALUE,
+              "%s: num_heads must be a multiple of num_kv_heads", what);
+  KVC_REQUIRE(heads / kv_heads <= kFormColumns[kForms - 1], KVC_ERR_VALUE,
+              "%s: at most %d query heads per kv head", what, kFormColumns[kForms - 1]);
+  KVC_REQUIRE(tokens >= 0 && tokens < (int64_t(1) << 30), KVC_ERR_VALUE, "%s: bad token count",
+              what);
+  KVC_REQUIRE(scale > 0.f && std::isfinite(scale), KVC_ERR_VALUE,
+              "%s: scale must be finite and > 0", what);
+  KVC_REQUIRE(softcap >= 0.f && std::isfinite(softcap), KVC_ERR_VALUE,
+              "%s: softcap must be finite and >= 0", what);
+  KVC_REQUIRE(window >= 0 && window < (int64_t(1) << 30), KVC_ERR_VALUE,
+              "%s: window must be >= 0", what);
+  KVC_REQUIRE(tokens == 0 || (q != nullptr && out != nullptr), KVC_ERR_VALUE,
+              "%s: missing q or out", what);
+  KVC_REQUIRE(tokens == 0 || (rows16(q, q_st, q_sh) && rows16(out, o_st, o_sh)), KVC_ERR_ASSERT,
+              "%s: q and out rows must be 16-byte aligned", what);
+  return KVC_OK;
+}
+
+int check_pool(const char* what, const void* k, const void* v, int64_t blocks, int64_t page,
+               int64_t kv_heads, const void* tables, int64_t max_blocks) {
+  KVC_REQUIRE(k != nullptr && v != nullptr && tables != nullptr, KVC_ERR_VALUE,
+              "%s: missing pool or block tables", what);
+  KVC_REQUIRE(page > 0 && page % kTile == 0, KVC_ERR_VALUE,
+              "%s: page_size must be a multiple of 32", what);
+  KVC_REQUIRE(blocks > 0 && blocks < (int64_t(1) << 31) && max_blocks >= 0 &&
+                  max_blocks * page < (int64_t(1) << 30),
+              KVC_ERR_VALUE, "%s: bad pool or table size", what);
+  KVC_REQUIRE(rows16(k, 0, 0) && rows16(v, 0, 0) && kv_heads * kD < (1 << 24), KVC_ERR_ASSERT,
+              "%s: pools must be 16-byte aligned", what);
+  return KVC_OK;
+}
+
+}  // namespace
+}  // namespace kvc
+
+using namespace kvc;
+
+extern "C" size_t kvc_scored_workspace_bytes(int64_t num_q_tokens, int64_t num_heads,
+                                             int64_t num_kv_heads, int64_t num_decode_rows,
+                                             int64_t num_prefill, int64_t max_seqlen_q) {
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || num_q_tokens <= 0 ||
+      num_heads / num_kv_heads > kFormColumns[kForms - 1])
+    return 0;
+  size_t n = 0;
+  if (num_decode_rows > 0)
+    n = make_plan(num_decode_rows, num_heads, num_kv_heads, num_decode_rows, 1).bytes();
+  if (num_prefill > 0 && num_q_tokens > num_decode_rows)
+    n = std::max(n, make_plan(num_q_tokens - num_decode_rows, num_heads, num_kv_heads, num_prefill,
+                              max_seqlen_q)
+                        .bytes());
+  return n;
+}
+
+extern "C" int kvc_scored_attention(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_q_tokens, int64_t num_heads,
+    const void* k_cache, const void* v_cache, int64_t num_cache_blocks, int64_t page_size,
+    int64_t num_kv_heads, int64_t head_dim, const void* k_fresh, int64_t kf_stride_t,
+    int64_t kf_stride_h, const void* v_fresh, int64_t vf_stride_t, int64_t vf_stride_h,
+    int64_t num_fresh_rows, const int32_t* block_tables, int64_t bt_stride,
+    int64_t max_blocks_per_seq, int64_t num_decode_rows, const int32_t* decode_context_lens,
+    int64_t num_prefill, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+    int64_t max_seqlen_q, const int32_t* prefix_lens, const float* alibi_slopes, float softcap,
+    int64_t window, float scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
+    void* workspace, size_t workspace_bytes, kvc_stream_t stream) {
+  clear_error();
+  const char* what = "scored_attention";
+  int rc = check_common(what, q, q_stride_t, q_stride_h, num_q_tokens, num_heads, num_kv_heads,
+                        head_dim, scale, softcap, window, out, out_stride_t, out_stride_h);
+  if (rc != KVC_OK) return rc;
+  KVC_REQUIRE(num_decode_rows >= 0 && num_decode_rows <= num_q_tokens && num_prefill >= 0 &&
+                  max_seqlen_q >= 0,
+              KVC_ERR_VALUE, "%s: bad row counts", what);
+  if (num_q_tokens == 0) return KVC_OK;
+  const bool fresh = block_tables == nullptr;
+  if (fresh) {
+    KVC_REQUIRE(num_decode_rows == 0, KVC_ERR_VALUE, "%s: decode rows need block tables", what);
+    KVC_REQUIRE(num_fresh_rows >= 0 && num_fresh_rows < (int64_t(1) << 30) &&
+                    (num_fresh_rows == 0 || (k_fresh != nullptr && v_fresh != nullptr)),
+                KVC_ERR_VALUE, "%s: without block tables the keys come from k/v", what);
+    KVC_REQUIRE(rows16(k_fresh, kf_stride_t, kf_stride_h) &&
+                    rows16(v_fresh, vf_stride_t, vf_stride_h),
+                KVC_ERR_ASSERT, "%s: k/v rows must be 16-byte aligned", what);
+    KVC_REQUIRE(kf_stride_t >= 0 && vf_stride_t >= 0 && kf_stride_t < (1 << 24) &&
+                    vf_stride_t < (1 << 24),
+                KVC_ERR_VALUE, "%s: k/v row strides must be below 2^24 elements", what);
+  } else {
+    rc = check_pool(what, k_cache, v_cache, num_cache_blocks, page_size, num_kv_heads, block_tables,
+                    max_blocks_per_seq);
+    if (rc != KVC_OK) return rc;
+  }
+  KVC_REQUIRE(num_decode_rows == 0 || decode_context_lens != nullptr, KVC_ERR_VALUE,
+              "%s: missing decode_context_lens", what);
+  KVC_REQUIRE(num_prefill == 0 || (cu_seqlens_q != nullptr && cu_seqlens_k != nullptr),
+              KVC_ERR_VALUE, "%s: missing cu_seqlens", what);
+  const size_t need = kvc_scored_workspace_bytes(num_q_tokens, num_heads, num_kv_heads,
+                                                 num_decode_rows, num_prefill, max_seqlen_q);
+  KVC_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KVC_ERR_WORKSPACE,
+              "%s: workspace of %zu bytes needed", what, need);
+  ScoredParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_st = q_stride_t;
+  p.q_sh = q_stride_h;
+  p.out = static_cast<uint16_t*>(out);
+  p.o_st = out_stride_t;
+  p.o_sh = out_stride_h;
+  p.k = static_cast<const uint16_t*>(fresh ? k_fresh : k_cache);
+  p.v = static_cast<const uint16_t*>(fresh ? v_fresh : v_cache);
+  p.k_row = fresh ? kf_stride_t : num_kv_heads * kD;
+  p.k_head = fresh ? kf_stride_h : kD;
+  p.v_row = fresh ? vf_stride_t : num_kv_heads * kD;
+  p.v_head = fresh ? vf_stride_h : kD;
+  p.tables = block_tables;
+  p.bt_stride = bt_stride;
+  p.max_blocks = int(max_blocks_per_seq);
+  p.num_blocks = int(num_cache_blocks);
+  p.page = int(page_size);
+  p.fresh_rows = num_fresh_rows;
+  p.slopes = alibi_slopes;
+  p.scale = scale;
+  p.cap = softcap;
+  p.window = int(window);
+  p.heads = int(num_heads);
+  p.kv_heads = int(num_kv_heads);
+  p.group = int(num_heads / num_kv_heads);
+  const int64_t max_keys = fresh ? num_fresh_rows : max_blocks_per_seq * page_size;
+  hipStream_t st = as_stream(stream);
+  if (num_decode_rows > 0) {
+    ScoredParams d = p;
+    d.batch = d.num_tokens = int(num_decode_rows);
+    d.q_per_seq = 1;
+    d.lens = decode_context_lens;
+    rc = run_rows(d, 1, max_keys, workspace, st, what);
+    if (rc != KVC_OK) return rc;
+  }
+  if (num_prefill > 0 && num_q_tokens > num_decode_rows) {
+    p.q += num_decode_rows * q_stride_t;
+    p.out += num_decode_rows * out_stride_t;
+    if (!fresh) p.tables += num_decode_rows * bt_stride;
+    p.batch = int(num_prefill);
+    p.num_tokens = int(num_q_tokens - num_decode_rows);
+    p.cu_q = cu_seqlens_q;
+    p.cu_k = cu_seqlens_k;
+    p.prefix = prefix_lens;
+    rc = run_rows(p, max_seqlen_q, max_keys, workspace, st, what);
+  }
+  return rc;
+}
+
+extern "C" size_t kvc_tree_workspace_bytes(int64_t num_q_tokens, int64_t num_heads,
+                                           int64_t num_kv_heads, int64_t batch,
+                                           int64_t max_seqlen_q) {
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || num_q_tokens <= 0 ||
+      num_heads / num_kv_heads > kFormColumns[kForms - 1])
+    return 0;
+  return make_plan(num_q_tokens, num_heads, num_kv_heads, batch, max_seqlen_q).bytes() +
+         up256(size_t(num_q_tokens) * sizeof(int32_t));
+}
+
+extern "C" int kvc_tree_attention(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_q_tokens, int64_t num_heads,
+    const void* k_cache, const void* v_cache, int64_t num_cache_blocks, int64_t page_size,
+    int64_t num_kv_heads, int64_t head_dim, const int32_t* block_tables, int64_t bt_stride,
+    int64_t max_blocks_per_seq, int64_t batch, const int32_t* context_lens,
+    const int32_t* cu_seqlens_q, int64_t max_seqlen_q, const int64_t* tree_mask,
+    int64_t mask_words, const float* alibi_slopes, float softcap, int64_t window, float scale,
+    void* out, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+    size_t workspace_bytes, kvc_stream_t stream) {
+  clear_error();
+  const char* what = "tree_attention";
+  int rc = check_common(what, q, q_stride_t, q_stride_h, num_q_tokens, num_heads, num_kv_heads,
+                        head_dim, scale, softcap, window, out, out_stride_t, out_stride_h);
+  if (rc != KVC_OK) return rc;
+  KVC_REQUIRE(batch >= 0 && max_seqlen_q >= 0, KVC_ERR_VALUE, "%s: bad row counts", what);
+  if (num_q_tokens == 0 || batch == 0) return KVC_OK;
+  rc = check_pool(what, k_cache, v_cache, num_cache_blocks, page_size, num_kv_heads, block_tables,
+                  max_blocks_per_seq);
+  if (rc != KVC_OK) return rc;
+  KVC_REQUIRE(context_lens != nullptr && tree_mask != nullptr, KVC_ERR_VALUE,
+              "%s: missing context_lens or tree_mask", what);
+  KVC_REQUIRE(mask_words > 0 && mask_words < (1 << 20) && mask_words * 64 >= max_seqlen_q,
+              KVC_ERR_VALUE, "%s: tree_mask has too few words for max_seqlen_q", what);
+  KVC_REQUIRE(cu_seqlens_q != nullptr || max_seqlen_q * batch == num_q_tokens, KVC_ERR_VALUE,
+              "%s: without cu_seqlens_q every tree has max_seqlen_q tokens", what);
+  const size_t need =
+      kvc_tree_workspace_bytes(num_q_tokens, num_heads, num_kv_heads, batch, max_seqlen_q);
+  KVC_REQUIRE(workspace != nullptr && workspace_bytes >= need, KVC_ERR_WORKSPACE,
+              "%s: workspace of %zu bytes needed", what, need);
+  ScoredParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_st = q_stride_t;
+  p.q_sh = q_stride_h;
+  p.out = static_cast<uint16_t*>(out);
+  p.o_st = out_stride_t;
+  p.o_sh = out_stride_h;
+  p.k = static_cast<const uint16_t*>(k_cache);
+  p.v = static_cast<const uint16_t*>(v_cache);
+  p.k_row = p.v_row = num_kv_heads * kD;
+  p.k_head = p.v_head = kD;
+  p.tables = block_tables;
+  p.bt_stride = bt_stride;
+  p.max_blocks = int(max_blocks_per_seq);
+  p.num_blocks = int(num_cache_blocks);
+  p.page = int(page_size);
+  p.cu_q = cu_seqlens_q;
+  p.q_per_seq = int(max_seqlen_q);
+  p.lens = context_lens;
+  p.lens_exclude_q = 1;
+  p.mask = reinterpret_cast<const uint32_t*>(tree_mask);
+  p.mask_words = int(2 * mask_words);
+  p.slopes = alibi_slopes;
+  p.scale = scale;
+  p.cap = softcap;
+  p.window = int(window);
+  p.batch = int(batch);
+  p.num_tokens = int(num_q_tokens);
+  p.heads = int(num_heads);
+  p.kv_heads = int(num_kv_heads);
+  p.group = int(num_heads / num_kv_heads);
+  hipStream_t st = as_stream(stream);
+  if (alibi_slopes != nullptr || window > 0) {
+    int32_t* depth = reinterpret_cast<int32_t*>(
+        static_cast<char*>(workspace) + need - up256(size_t(num_q_tokens) * sizeof(int32_t)));
+    tree_depth_kernel<<<unsigned(batch), 64, 0, st>>>(p, depth);
+    rc = check_launch(what);
+    if (rc != KVC_OK) return rc;
+    p.places = depth;
+  }
+  return run_rows(p, max_seqlen_q, max_blocks_per_seq * page_size, workspace, st, what);
+}

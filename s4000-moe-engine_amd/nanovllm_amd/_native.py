@@ -105,6 +105,15 @@ SIGNATURES = {
                                       _I64, _I64, _I64, _I64, _P, _INT, _P, _P, _F32,
                                       _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
                                       _I64, _P, _INT, _P]),
+    "kvc_scored_workspace_bytes": (_SZ, [_I64] * 6),
+    "kvc_scored_attention": (_INT, [_P, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64,
+                                    _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
+                                    _P, _I64, _P, _P, _I64, _P, _P, _F32, _I64, _F32, _P, _I64,
+                                    _I64, _P, _SZ, _P]),
+    "kvc_tree_workspace_bytes": (_SZ, [_I64] * 5),
+    "kvc_tree_attention": (_INT, [_P, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64,
+                                  _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _F32, _I64,
+                                  _F32, _P, _I64, _I64, _P, _SZ, _P]),
     "kvc_stage_decode": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,
                                 _I64, _I64, _I64, _P, _INT, _P, _INT, _P, _I64, _I64, _P, _P, _P,
                                 _P, _P, _P, _I64, _INT, _INT, _P]),
@@ -193,6 +202,15 @@ def call(name: str, *args) -> int:
         msg = _lib.kvc_last_error().decode(errors="replace")
         raise _ERRORS.get(rc, RuntimeError)(msg or f"{name} failed with status {rc}")
     return rc
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> int:
+    """call() with t's device current, so that the launch goes to the device
+    its stream belongs to."""
+    if t.get_device() == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(t.device):
+        return call(name, *args)
 
 
 def query(name: str, *args):
