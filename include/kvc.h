@@ -559,6 +559,23 @@ int kvc_block_copy_ids(void* pool, int64_t planes, int64_t plane_stride, int64_t
                        const int32_t* src_ids, const int32_t* dst_ids, int64_t n,
                        kvc_stream_t stream);
 
+/* Keeps the accepted path of a drafted token tree (no reference counterpart):
+ * for each sequence b and j < path_lens[b] (at most max_path), the row of
+ * row_bytes at position context_lens[b] + paths[b][j] of its block table goes
+ * to position context_lens[b] + j, in every plane (a plane is num_blocks
+ * blocks of page_size rows, planes plane_stride bytes apart), all as one
+ * simultaneous move.  paths is int32 [batch, max_path], rows path_stride
+ * elements apart.  A path is strictly increasing from paths[b][0] >= 0, as the
+ * path from a root of a tree whose parents come before their children is; it
+ * ends at the first entry that is not, or whose position or block lies outside
+ * the table or the pool.  No two sequences may share the rows past their
+ * contexts. */
+int kvc_commit_rows(void* pool, int64_t planes, int64_t plane_stride, int64_t num_blocks,
+                    int64_t page_size, int64_t row_bytes, const int32_t* block_tables,
+                    int64_t bt_stride, int64_t max_blocks_per_seq, const int32_t* context_lens,
+                    const int32_t* paths, int64_t path_stride, int64_t max_path,
+                    const int32_t* path_lens, int64_t batch, kvc_stream_t stream);
+
 /* DMA form of the offload byte moves: one strided 2-D copy per block on the
  * copy engines, block ids read from HOST memory (the block manager's ints).
  * d2h: host_dst + i*host_item_stride <- pool planes of block host_ids[i].
@@ -604,6 +621,28 @@ int kvc_qk_norm_rope_store(const void* q, int64_t q_stride_t, int64_t q_stride_h
                            int64_t k_out_stride_t, int64_t k_out_stride_h, void* k_cache,
                            void* v_cache, int64_t num_slots, const void* slot_mapping,
                            int slot_index_bytes, kvc_stream_t stream);
+
+/* kvc_qk_norm_rope_store for tokens with a position on each of num_axes axes
+ * (1 to 4; time, height and width of images and video; no reference
+ * counterpart): positions is [num_axes, num_tokens], rows position_stride
+ * elements apart, and rotary pair i (dims i and i + 64) turns by the cos and
+ * sin of the position on axis pair_axes_host[i] (64 int32 in HOST memory,
+ * read before the call returns).  Norm and rotation are fp32 throughout and
+ * rounded to bf16 once:
+ *   y = x / sqrt(sum(x^2) / 128 + eps) * w               (no norm when w is NULL)
+ *   out = bf16(y1 * c - y2 * s | y2 * c + y1 * s)
+ * The outputs, the append and the slot and position rules are those of
+ * kvc_qk_norm_rope_store; any number of heads. */
+int kvc_qk_norm_mrope_store(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+    int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+    int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+    const void* positions, int64_t position_stride, int position_index_bytes, int64_t num_axes,
+    const int32_t* pair_axes_host, const void* q_norm_weight, const void* k_norm_weight, float eps,
+    const float* cos_sin_cache, int64_t max_position, void* q_out, int64_t q_out_stride_t,
+    int64_t q_out_stride_h, void* k_out, int64_t k_out_stride_t, int64_t k_out_stride_h,
+    void* k_cache, void* v_cache, int64_t num_slots, const void* slot_mapping,
+    int slot_index_bytes, kvc_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Inputs of a captured decode step.

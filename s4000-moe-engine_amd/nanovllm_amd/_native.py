@@ -114,6 +114,12 @@ SIGNATURES = {
     "kvc_tree_attention": (_INT, [_P, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64,
                                   _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _F32, _I64,
                                   _F32, _P, _I64, _I64, _P, _SZ, _P]),
+    "kvc_qk_norm_mrope_store": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64,
+                                       _I64, _I64, _P, _I64, _INT, _I64, _P, _P, _P, _F32, _P,
+                                       _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P,
+                                       _INT, _P]),
+    "kvc_commit_rows": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64,
+                               _I64, _P, _I64, _P]),
     "kvc_stage_decode": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,
                                 _I64, _I64, _I64, _P, _INT, _P, _INT, _P, _I64, _I64, _P, _P, _P,
                                 _P, _P, _P, _I64, _INT, _INT, _P]),

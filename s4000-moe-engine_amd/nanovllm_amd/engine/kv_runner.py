@@ -381,6 +381,18 @@ class KVCacheRunner:
         self.fence()
         self.mover.copy(src_ids, dst_ids)
 
+    def commit_tree(self, block_tables, context_lens, paths, path_lens) -> None:
+        """commit_tree_path on the pool and, for an int8 pool, on what travels
+        with its rows (per-token-head scales, side rows)."""
+        from ..kernels.tree import commit_tree_path
+        self.fence()
+        rows = [self.kv_cache, self.kv_side]
+        if self.kv_int8 == "tokhead":
+            rows.append(self.kv_scales)
+        for pool in rows:
+            if pool is not None:
+                commit_tree_path(pool, block_tables, context_lens, paths, path_lens)
+
     # -- batch preparation (the Context producer) ----------------------------
     @property
     def device(self) -> torch.device:

@@ -86,3 +86,41 @@ def tree_attention(q, k_cache, v_cache, block_tables, context_lens, tree_mask, s
         tree_mask.size(1), nat.ptr(alibi_slopes), softcap, window, float(scale), out.data_ptr(),
         out.stride(0), out.stride(1), nat.ptr(ws), need, nat.stream_of(q))
     return out
+
+
+def commit_tree_path(kv_cache, block_tables, context_lens, paths, path_lens):
+    """Keeps the accepted path of every sequence's tree, in place: for each
+    sequence b and j < path_lens[b], the token row at position
+    context_lens[b] + paths[b, j] of the pool goes to position
+    context_lens[b] + j, in every layer, K and V, as one simultaneous move
+    (the context then grows by path_lens[b]).  kv_cache is the whole pool
+    [2, L, blocks, page, ...], or a companion of an int8 pool of that shape
+    (scales, side rows); paths int32 [batch, most], a path strictly
+    increasing (tree tokens come after their parents): it ends at the first
+    entry that is not."""
+    if kv_cache.dim() < 4:
+        raise ValueError("pool must be [2, layers, blocks, page, ...]")
+    if not kv_cache.is_contiguous():
+        raise AssertionError("the KV pool must be contiguous")
+    if block_tables.ndim != 2 or paths.ndim != 2 or paths.size(0) != block_tables.size(0):
+        raise ValueError("expected block_tables=[batch,pages] and paths=[batch,most]")
+    dev = kv_cache.device
+    if not (block_tables.device == paths.device == dev):
+        raise ValueError("the pool, block_tables and paths must be on one device")
+    batch = block_tables.size(0)
+    context_lens = _int32(context_lens, batch, "context_lens", dev)
+    path_lens = _int32(path_lens, batch, "path_lens", dev)
+    if block_tables.dtype != torch.int32 or block_tables.stride(1) != 1:
+        block_tables = block_tables.to(torch.int32).contiguous()
+    if paths.dtype != torch.int32 or paths.stride(1) != 1:
+        paths = paths.to(torch.int32).contiguous()
+    nat.require_device(kv_cache)
+    if kv_cache.numel() == 0 or batch == 0:
+        return
+    blocks, page = kv_cache.size(2), kv_cache.size(3)
+    plane = kv_cache[0, 0].numel() * kv_cache.element_size()
+    nat.call_on(
+        kv_cache, "kvc_commit_rows", kv_cache.data_ptr(), kv_cache.size(0) * kv_cache.size(1),
+        plane, blocks, page, plane // (blocks * page), block_tables.data_ptr(),
+        block_tables.stride(0), block_tables.size(1), context_lens.data_ptr(), paths.data_ptr(),
+        paths.stride(0), paths.size(1), path_lens.data_ptr(), batch, nat.stream_of(kv_cache))

@@ -14,6 +14,10 @@ change.  What changes is underneath:
   with the same results and pool bytes as store + decode;
 * prefill and mixed batches are ONE varlen launch instead of a Python loop
   over sequences plus torch.cat (attention.py:146-166, :179-213).
+
+A layer whose scores are shaped (softcap, alibi_slopes, window) or a step with
+a two-way prefix or drafted trees (Context.prefix_lens, Context.tree_mask)
+appends, then attends through scored_attention / tree_attention.
 """
 from __future__ import annotations
 
@@ -27,9 +31,11 @@ from ..kernels.kv_int8 import store_kvcache_int8
 from ..kernels.paged_attention import (paged_decode_append, paged_decode_append_int8_chan,
                                        paged_decode_append_int8_tokhead,
                                        paged_decode_attention)
+from ..kernels.scored import scored_attention
+from ..kernels.tree import tree_attention
 from ..kernels.varlen import varlen_attention, varlen_attention_append
 from ..utils.context import get_context
-from .rotary import qk_norm_rope_store
+from .rotary import qk_norm_mrope_store, qk_norm_rope_store
 
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -65,14 +71,20 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
 
 class Attention(nn.Module):
     """Attention(num_heads, head_dim, scale, num_kv_heads) with the runner-set
-    attributes of attention.py:108-123."""
+    attributes of attention.py:108-123.  softcap, alibi_slopes (fp32
+    [num_heads]) and window shape the layer's scores as in scored_attention
+    (bf16 pools)."""
 
-    def __init__(self, num_heads, head_dim, scale, num_kv_heads):
+    def __init__(self, num_heads, head_dim, scale, num_kv_heads, softcap=0.0, alibi_slopes=None,
+                 window=0):
         super().__init__()
         self.num_heads = num_heads
         self.head_dim = head_dim
         self.scale = scale
         self.num_kv_heads = num_kv_heads
+        self.softcap = softcap
+        self.alibi_slopes = alibi_slopes
+        self.window = window
         self.block_size = None
         self.k_cache = self.v_cache = torch.tensor([])
         self.k_scale = self.v_scale = None      # int8 store scales
@@ -120,16 +132,17 @@ class Attention(nn.Module):
     def forward_fused(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                       v: torch.Tensor, cos_sin_cache: torch.Tensor,
                       q_norm_weight: torch.Tensor | None, k_norm_weight: torch.Tensor | None,
-                      eps: float):
+                      eps: float, rope_sections=None, rope_interleaved: bool = False):
         """Qwen3Attention.forward's q_norm, k_norm and rotary_emb
         (nanovllm/models/qwen3.py:82-85) fused with this layer's append
         (one launch on a bf16 pool), then attention.  q [N, H*D] or
         [N, H, D]; k, v [N, KVH*D] or [N, KVH, D] (views of the qkv
-        projection are fine)."""
+        projection are fine).  With rope_sections, positions are [A, N] on as
+        many axes (qk_norm_mrope_store)."""
         context = get_context()
         if self.kv_fence is not None:
             self.kv_fence(self.kv_layer)
-        N = positions.numel()
+        N = positions.numel() if rope_sections is None else positions.size(-1)
         q3 = q.view(N, self.num_heads, self.head_dim)
         k3 = k.view(N, self.num_kv_heads, self.head_dim)
         v3 = v.view(N, self.num_kv_heads, self.head_dim)
@@ -137,13 +150,55 @@ class Attention(nn.Module):
         bf16_pool = bool(k_cache.numel() and v_cache.numel()) and not self.kv_cache_is_int8
         need_k = not bf16_pool or context.block_tables is None
         with self._profile("attention.qk_norm_rope_store"):
-            q_rot, k_rot = qk_norm_rope_store(
-                q3, k3, v3, positions, cos_sin_cache, q_norm_weight, k_norm_weight, eps,
-                k_cache if bf16_pool else None, v_cache if bf16_pool else None,
-                context.slot_mapping if bf16_pool else None, return_k=need_k)
+            pool = (k_cache, v_cache, context.slot_mapping) if bf16_pool else (None, None, None)
+            if rope_sections is None:
+                q_rot, k_rot = qk_norm_rope_store(
+                    q3, k3, v3, positions, cos_sin_cache, q_norm_weight, k_norm_weight, eps,
+                    *pool, return_k=need_k)
+            else:
+                q_rot, k_rot = qk_norm_mrope_store(
+                    q3, k3, v3, positions, cos_sin_cache, rope_sections, rope_interleaved,
+                    q_norm_weight, k_norm_weight, eps, *pool, return_k=need_k)
         if k_rot is None:
             k_rot = k3  # not read: the rows are in the pool
         return self.forward(q_rot, k_rot, v3, kv_stored=bf16_pool)
+
+    def _shaped(self, context) -> bool:
+        return bool(self.softcap or self.window or self.alibi_slopes is not None
+                    or context.prefix_lens is not None or context.tree_mask is not None)
+
+    def _forward_shaped(self, context, q, k, v, kv_stored):
+        """The append, then attention with shaped scores or masks."""
+        if self.kv_cache_is_int8:
+            raise ValueError("shaped scores, two-way prefixes and drafted trees need a bf16 pool")
+        q = q.view(-1, self.num_heads, self.head_dim)
+        k = k.view(-1, self.num_kv_heads, self.head_dim)
+        v = v.view(-1, self.num_kv_heads, self.head_dim)
+        k_cache, v_cache = self.k_cache, self.v_cache
+        if k_cache.numel() and v_cache.numel() and not kv_stored:
+            with self._profile("attention.kv_store"):
+                store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
+        shape = dict(softcap=self.softcap, alibi_slopes=self.alibi_slopes, window=self.window)
+        if context.tree_mask is not None:
+            with self._profile("attention.tree"):
+                return tree_attention(
+                    q, k_cache, v_cache, context.block_tables, context.context_lens,
+                    context.tree_mask, self.scale, cu_seqlens_q=context.cu_seqlens_q,
+                    max_seqlen_q=context.max_seqlen_q or None, **shape)
+        if context.is_mixed or context.is_prefill:
+            with self._profile("attention.mixed" if context.is_mixed else "attention.prefill"):
+                return scored_attention(
+                    q, k_cache, v_cache, scale=self.scale, block_tables=context.block_tables,
+                    num_decode_rows=context.num_decode_rows if context.is_mixed else 0,
+                    decode_context_lens=context.decode_context_lens if context.is_mixed else None,
+                    cu_seqlens_q=context.cu_seqlens_q, cu_seqlens_k=context.cu_seqlens_k,
+                    cu_seqlens_q_list=context.cu_seqlens_q_list,
+                    cu_seqlens_k_list=context.cu_seqlens_k_list, k=k, v=v,
+                    prefix_lens=context.prefix_lens, **shape)
+        with self._profile("attention.paged_decode"):
+            return scored_attention(
+                q, k_cache, v_cache, scale=self.scale, block_tables=context.block_tables,
+                num_decode_rows=q.size(0), decode_context_lens=context.context_lens, **shape)
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_stored: bool = False):
         """attention.py:130-177.  kv_stored: the step's k/v rows are already
@@ -156,6 +211,8 @@ class Attention(nn.Module):
         k_cache, v_cache = self.k_cache, self.v_cache
         if k_cache.numel() and self.block_size is None:
             self.block_size = k_cache.size(1)
+        if self._shaped(context):
+            return self._forward_shaped(context, q, k, v, kv_stored)
         # A decode step appends inside the decode call (bf16 and per-token-head
         # int8 pools inside the decode launch; per-channel int8 in the same
         # call, as a store launch ahead of the decode).

@@ -6,7 +6,13 @@ All cu_seqlens fields are prefill-only in a mixed batch; decode rows carry
 their own context lengths (nanovllm/utils/context.py:21-28).  One field is
 added at the end: decode_context_lens_list, the decode rows' context lengths
 as host ints (the runner's dec_ctx_lens, nanovllm/engine/model_runner.py:
-597-602), which lets a mixed call size its CU split without a device read.
+597-602), which lets a mixed call size its CU split without a device read.  Two more are
+for what the engine does not do: prefix_lens (int32, one per prefill chunk),
+the keys at a prompt's start that every token of its chunk sees (an image's
+patches see each other both ways), and tree_mask (int64 [tokens, words]), a
+step of drafted token trees: context_lens then counts what comes before each
+tree, slot_mapping places tree token t at position context + t, and
+cu_seqlens_q / max_seqlen_q delimit the trees (absent: all of one size).
 """
 from dataclasses import dataclass
 
@@ -31,6 +37,8 @@ class Context:
     decode_context_lens: torch.Tensor | None = None
     decode_max_context_len: int = 0
     decode_context_lens_list: list | None = None
+    prefix_lens: torch.Tensor | None = None
+    tree_mask: torch.Tensor | None = None
 
 
 _CURRENT = Context()
@@ -45,7 +53,7 @@ def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0
                 cu_seqlens_q_list=None, cu_seqlens_k_list=None,
                 is_mixed=False, num_decode_rows=0,
                 decode_context_lens=None, decode_max_context_len=0,
-                decode_context_lens_list=None):
+                decode_context_lens_list=None, prefix_lens=None, tree_mask=None):
     global _CURRENT
     _CURRENT = Context(
         is_prefill=is_prefill,
@@ -64,6 +72,8 @@ def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0
         decode_context_lens=decode_context_lens,
         decode_max_context_len=decode_max_context_len,
         decode_context_lens_list=decode_context_lens_list,
+        prefix_lens=prefix_lens,
+        tree_mask=tree_mask,
     )
 
 
