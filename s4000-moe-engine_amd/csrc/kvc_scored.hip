@@ -64,6 +64,8 @@ struct ScoredParams {
   const int32_t* tables;                 // null: fresh rows at cu_k
   int64_t bt_stride;
   int max_blocks, num_blocks, page;
+  int page_tiles;  // page / 32
+  float page_rcp;  // 1 / page_tiles
   int64_t fresh_rows;
   const int32_t* cu_q;  // null: q_per_seq tokens each
   int q_per_seq;
@@ -82,8 +84,7 @@ struct ScoredParams {
   int tokens_per_block;
   int lane_plan;  // the plan walks sequences across lanes (else blocks)
   int min_share;
-  int4* rec;  // per item: sequence, block, first and last share
-  int max_items;
+  int4* rec;  // per share: the item it begins and leaves unfinished
   float* part_o;
   float2* part_ml;
 };
@@ -244,35 +245,43 @@ struct Consts {
 // order of the P operand.
 __device__ __forceinline__ int key_of(int e) { return (e & 3) + 16 * (e >> 2); }
 
-// S^T = K Q^T, the score's shape, the mask, the running softmax, and P^T as
-// the bf16 operand pb.  y holds what the softmax is taken of: the raw logit
-// s (log2-unit score c2 s) for plain scores, the log2-unit score otherwise;
-// -inf at keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} + 1): one
-// exp2 and one reciprocal.  Sums are formed of the rounded P (an MFMA against
-// ones), so the weights add up to the sum that divides them.
+// S^T = K Q^T: rows 4 lg + i of the tile's two 16-key halves.
+template <int NCB>
+__device__ __forceinline__ void logits(const u32x4_t (&k)[2][4], const u32x4_t (&q)[NCB][4],
+                                       f32x4_t (&s)[NCB][2]) {
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    s[cb][0] = s[cb][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      s[cb][0] = mfma_bf16(k[0][d], q[cb][d], s[cb][0]);
+      s[cb][1] = mfma_bf16(k[1][d], q[cb][d], s[cb][1]);
+    }
+  }
+}
+
+// The score's shape, the mask, the running softmax, and P^T as the bf16
+// operand pb.  y holds what the softmax is taken of: the raw logit s (log2-
+// unit score c2 s) for plain scores, the log2-unit score otherwise; -inf at
+// keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} + 1): one exp2 and
+// one reciprocal.  Sums are formed of the rounded P (an MFMA against ones),
+// so the weights add up to the sum that divides them.
 template <int NCB, int MODE>
-__device__ __forceinline__ void score_tile(const ScoredParams& p, const Columns<NCB>& c,
-                                           State<NCB>& st, const u32x4_t (&k)[2][4],
-                                           const u32x4_t (&q)[NCB][4], int j0, int lg,
-                                           const Consts& cs, bool masked, u32x4_t (&pb)[NCB],
-                                           uint32_t (&vis)[NCB]) {
+__device__ __forceinline__ void weights(const ScoredParams& p, const Columns<NCB>& c,
+                                        State<NCB>& st, const f32x4_t (&sl)[NCB][2], int j0,
+                                        int lg, const Consts& cs, bool masked,
+                                        u32x4_t (&pb)[NCB]) {
   constexpr bool kDist = MODE == kDistance || MODE == kCapDistance;
   constexpr bool kCap = MODE == kCapFixed || MODE == kCapLazy || MODE == kCapDistance;
   const float unit = MODE == kPlain ? cs.c2 : 1.f;
   float y[NCB][8];
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
-    f32x4_t lo = {0.f, 0.f, 0.f, 0.f}, hi = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      lo = mfma_bf16(k[0][d], q[cb][d], lo);
-      hi = mfma_bf16(k[1][d], q[cb][d], hi);
-    }
     // The bias of a key at or before the query's place.
     const float b0 = kDist ? c.slope2[cb] * (float(j0 + 4 * lg) - c.place[cb]) : 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float s = e < 4 ? lo[e & 3] : hi[e & 3];
+      const float s = sl[cb][e >> 2][e & 3];
       float x = s;
       if constexpr (kCap) {
         const float w = __builtin_amdgcn_exp2f(s * cs.zc);
@@ -289,8 +298,7 @@ __device__ __forceinline__ void score_tile(const ScoredParams& p, const Columns<
   if (masked) {
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
-      vis[cb] = visible_bits<NCB>(p, c, cb, j0);
-      const uint32_t own = vis[cb] >> (4 * lg);
+      const uint32_t own = visible_bits<NCB>(p, c, cb, j0) >> (4 * lg);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if constexpr (kDist) {
@@ -392,21 +400,19 @@ __device__ __forceinline__ u32x4_t read_v(const char* vt, const LdsAddr& a, int 
 
 // O^T += V^T P^T.  In a masked tile a column's P is 0 at keys it does not see,
 // but 0 times an infinity or NaN held there would still reach its sum: such
-// values are taken out of the operand and added to the columns that do see
-// their key (whose result they decide whatever their weight).
+// values are taken out of the operand, and `odd` says so (add_not_finite then
+// gives them to the columns that see them, after the loop).
 template <int NCB>
-__device__ __forceinline__ void weigh_tile(State<NCB>& st, const char* vt, u32x4_t (&v)[8],
-                                           const u32x4_t (&pb)[NCB], const uint32_t (&vis)[NCB],
-                                           int lg, bool masked) {
-  bool odd = false;
+__device__ __forceinline__ void weigh_tile(State<NCB>& st, u32x4_t (&v)[8],
+                                           const u32x4_t (&pb)[NCB], bool masked, bool& odd) {
   if (masked) {
     uint32_t most = 0u;
 #pragma unroll
     for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
       for (int i = 0; i < 4; ++i) most = max_u16x2(most, v[jj][i] & 0x7fff7fffu);
-    odd = __any(not_finite(most) || not_finite(most >> 16));
-    if (__builtin_expect(odd, 0)) {
+    if (__builtin_expect(__any(not_finite(most) || not_finite(most >> 16)), 0)) {
+      odd = true;
 #pragma unroll
       for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
@@ -420,29 +426,30 @@ __device__ __forceinline__ void weigh_tile(State<NCB>& st, const char* vt, u32x4
   for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) st.o[cb][jj] = mfma_bf16(v[jj], pb[cb], st.o[cb][jj]);
-  {
-    if (__builtin_expect(odd, 0)) {
-      for (int r = 0; r < kTile; ++r) {
+}
+
+// Infinities and NaN of one tile's V rows, added to the columns that see their
+// key: they decide its result whatever their weight.  Rare, so plain: each row
+// once, from memory.
+template <int NCB>
+__device__ __forceinline__ void add_not_finite(const ScoredParams& p, const Columns<NCB>& c,
+                                               State<NCB>& st, const uint16_t* v, int rows, int j0,
+                                               int lg) {
+  uint32_t vis[NCB];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) vis[cb] = visible_bits<NCB>(p, c, cb, j0);
 #pragma unroll 1
-        for (int jj = 0; jj < 8; ++jj) {
-          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(
-              vt + r * 256 + (((4 * lg + (jj >> 1)) ^ (r & 15)) << 4) + (jj & 1) * 8);
-          f32x4_t add;
+  for (int r = 0; r < rows; ++r) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t half = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-            add[i] = not_finite(half) ? bf16_bits_to_f32(half) : 0.f;
-          }
+    for (int n = 0; n < 4; ++n) {  // the lane's dims 32 lg + 8 n ..
+      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(v + r * p.v_row + 32 * lg + 8 * n);
 #pragma unroll
-          for (int cb = 0; cb < NCB; ++cb) {
-            const bool on = ((vis[cb] >> r) & 1u) != 0u;
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t half = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+        const float add = not_finite(half) ? bf16_bits_to_f32(half) : 0.f;
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
-              if (n == jj)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) st.o[cb][n][i] += on ? add[i] : 0.f;
-          }
-        }
+        for (int cb = 0; cb < NCB; ++cb)
+          st.o[cb][2 * n + (i >> 2)][i & 3] += ((vis[cb] >> r) & 1u) ? add : 0.f;
       }
     }
   }
@@ -458,9 +465,7 @@ constexpr int kItemCost = 3;
 
 struct Where {
   int seq, grp, block, tile;  // tile: offset inside the item
-  int nb;                     // column blocks of the sequences before seq
   int64_t total;              // cost of the whole call
-  int blocks;                 // column blocks of the whole call
 };
 
 __device__ __forceinline__ int block_cost(const ScoredParams& p, const SeqGeo& g, int pre, int c) {
@@ -496,40 +501,33 @@ __device__ __forceinline__ int first_lane(uint64_t m) { return __builtin_ctzll(m
 // items; false when it lies past the end.
 __device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int share, int shares,
                                            Where& w, int& size) {
-  int total = 0, blocks = 0, cost = 0, nb = 0;
+  int total = 0, cost = 0, nb = 0;
   if (p.lane_plan) {
     for (int i = 0; i < p.batch; i += 64) {
       lane_seq(p, i + lane, cost, nb);
       total += wave_sum(cost);
-      blocks += wave_sum(nb);
     }
   } else {
-    for (int i = 0; i < p.batch; ++i) {
-      total += wave_seq(p, i, lane, nb);
-      blocks += nb;
-    }
+    for (int i = 0; i < p.batch; ++i) total += wave_seq(p, i, lane, nb);
   }
   w.total = total;
-  w.blocks = blocks;
   size = max(p.min_share, (total + shares - 1) / shares);
   const int64_t at64 = int64_t(share) * size;
   if (at64 >= total) return false;
   const int at = int(at64);
-  int acc = 0, before = 0, seq = -1, start = 0;
+  int acc = 0, seq = -1, start = 0;
   if (p.lane_plan) {
     for (int i = 0; i < p.batch; i += 64) {
       if (p.batch > 64) lane_seq(p, i + lane, cost, nb);
-      const int upto = wave_scan_add(cost), nbs = wave_scan_add(nb);
+      const int upto = wave_scan_add(cost);
       const uint64_t hit = __ballot(acc + upto > at);
       if (hit != 0) {
         const int l = first_lane(hit);
         seq = i + l;
         start = acc + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(cost, l);
-        before += __builtin_amdgcn_readlane(nbs, l) - __builtin_amdgcn_readlane(nb, l);
         break;
       }
       acc += __builtin_amdgcn_readlane(upto, 63);
-      before += __builtin_amdgcn_readlane(nbs, 63);
     }
   } else {
     for (int i = 0; i < p.batch; ++i) {
@@ -540,12 +538,10 @@ __device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int 
         break;
       }
       acc += cost;
-      before += nb;
     }
   }
   if (seq < 0) return false;
   w.seq = seq;
-  w.nb = before;
   // Inside the sequence: head groups in turn, each over all column blocks.
   const SeqGeo g = load_seq<true>(p, seq);
   const int pre = p.prefix != nullptr ? table_entry(p.prefix, seq) : 0;
@@ -574,25 +570,27 @@ __device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int 
 // ---------------------------------------------------------------------------
 // Tile addresses.
 // ---------------------------------------------------------------------------
+// The block id of tile's page in a sequence's table (0 for fresh rows), -1
+// past the table.
+__device__ __forceinline__ int page_entry(const ScoredParams& p, int seq, int tile) {
+  if (p.tables == nullptr) return 0;
+  const int page = uniform(div_small(tile, p.page_tiles, p.page_rcp));
+  return page < p.max_blocks ? table_entry(p.tables, int64_t(seq) * p.bt_stride + page) : -1;
+}
+
 struct TileSource {
   const uint16_t* k;
   const uint16_t* v;
   int rows;  // valid rows, 0: reads zeros
 };
-__device__ __forceinline__ TileSource tile_source(const ScoredParams& p, int seq, int64_t fresh0,
-                                                  int sk, int head, int tile) {
+__device__ __forceinline__ TileSource tile_source(const ScoredParams& p, int64_t fresh0, int sk,
+                                                  int head, int tile, int blk) {
   const int j0 = tile * kTile;
   int64_t row;
   int rows = min(kTile, sk - j0);
   if (p.tables != nullptr) {
-    const int page = j0 / p.page;
-    int blk = 0;
-    if (page < p.max_blocks) {
-      blk = table_entry(p.tables, int64_t(seq) * p.bt_stride + page);
-      if (blk < 0 || blk >= p.num_blocks) rows = 0;
-    } else {
-      rows = 0;
-    }
+    if (blk < 0 || blk >= p.num_blocks) rows = 0;
+    const int page = uniform(div_small(tile, p.page_tiles, p.page_rcp));
     row = rows > 0 ? int64_t(blk) * p.page + (j0 - page * p.page) : 0;
   } else {
     row = fresh0 + j0;
@@ -651,8 +649,9 @@ struct Form {
   static constexpr bool kPrivate = KW == NW;
   static constexpr int kColWaves = kPrivate ? 1 : NW / KW;
   static constexpr int kColumns = 16 * NCB * kColWaves;  // per kv head
-  static constexpr int kStage = KW * 2 * kTensor;
-  static constexpr int kStages = kPrivate ? 1 : KW == 4 ? 2 : 4;
+  static constexpr int kSub = kPrivate ? NW : KW == 1 ? 2 : 4;  // tiles per stage
+  static constexpr int kStage = kSub * 2 * kTensor;
+  static constexpr int kStages = kPrivate ? 1 : KW == 1 ? 4 : 2;
   // waves that hand their state to another: [wave][34 NCB floats][64 lanes]
   static constexpr int kStateBytes = 34 * NCB * 256;
   static constexpr int kJoinBytes =
@@ -708,11 +707,10 @@ __global__ void __launch_bounds__(64 * NW)
   Where w;
   int size;
   const bool live = plan_share(p, lane, share, grid, w, size);
-  // Items that this call does not have, up to the bound its merge covers.
-  for (int i = w.blocks * p.head_groups + blockIdx.x * (64 * NW) + threadIdx.x; i < p.max_items;
-       i += grid * 64 * NW)
-    p.rec[i] = int4{0, 0, 0, 0};
-  if (!live) return;
+  if (!live) {
+    if (threadIdx.x == 0) p.rec[share] = int4{0, 0, 0, 0};
+    return;
+  }
 
   const int hs = F::kPrivate ? wave % p.heads_per_wg : 0;
   const int phases = F::kPrivate ? NW / p.heads_per_wg : KW;
@@ -746,11 +744,12 @@ __global__ void __launch_bounds__(64 * NW)
     const int pre = p.prefix != nullptr ? table_entry(p.prefix, w.seq) : 0;
     const TileRange range = block_tiles(p, g, pre, w.block);
     const int tiles = range.t1 - range.t0;
-    const int item = (w.nb + w.block) * p.head_groups + w.grp;
     const int seg0 = w.tile, seg1 = min(tiles, w.tile + (end - pos));
-    const int last_share = tiles > 0 ? (pos - w.tile + tiles - 1) / size : share;
-    if (w.tile == 0 && threadIdx.x == 0 && item < p.max_items) p.rec[item] = int4{w.seq, w.block, share, last_share};
-
+    if (pos + tiles + kItemCost - w.tile >= end && threadIdx.x == 0) {
+      // The share's last item: where it goes on, if it began here.
+      const int last = tiles > 0 ? (pos - w.tile + tiles - 1) / size : share;
+      p.rec[share] = int4{w.seq, w.block, w.grp, w.tile == 0 && last > share ? last : 0};
+    }
     if (seg0 < seg1 || (tiles == 0 && w.tile == 0)) {
       const int head = w.grp * p.heads_per_wg + hs;
       const int64_t fresh0 =
@@ -812,23 +811,9 @@ __global__ void __launch_bounds__(64 * NW)
 
       State<NCB> st;
       reset<NCB>(st, mu0);
-      auto attend = [&](const char* kt, const char* vt, int j0, auto&& k_read, auto&& v_ready,
-                        auto&& v_read) {
-        const bool masked = j0 < c.full_lo || j0 + kTile > c.full_hi;
-        u32x4_t k[2][4], v[8], pb[NCB];
-        uint32_t vis[NCB];
-        read_k(k, kt, la);
-        k_read();
-        score_tile<NCB, MODE>(p, c, st, k, q, j0, lg, cs, masked, pb, vis);
-        v_ready();
-#pragma unroll
-        for (int jj = 0; jj < 8; ++jj) v[jj] = read_v(vt, la, jj);
-        if (!masked) v_read();
-        weigh_tile<NCB>(st, vt, v, pb, vis, lg, masked);
-        if (masked) v_read();
-      };
-
       const int t_begin = range.t0 + seg0, t_end = range.t0 + seg1;
+      u32x4_t k[2][4];
+      bool odd = false;  // a masked tile held infinities or NaN
       if constexpr (F::kPrivate) {
         // Wave-private slots: K 8 KiB, V 8 KiB.  The next tile's K load goes
         // out as soon as this tile's K is in registers, its V load likewise.
@@ -847,76 +832,118 @@ __global__ void __launch_bounds__(64 * NW)
         };
         int t = t_begin + phase;
         if (t < t_end) {
-          TileSource src = tile_source(p, w.seq, fresh0, g.sk, head, t);
+          const TileSource src = tile_source(p, fresh0, g.sk, head, t, page_entry(p, w.seq, t));
           issue_k(src);
           issue_v(src);
         }
         for (; t < t_end; t += phases) {
           const bool more = t + phases < t_end;
-          const TileSource next =
-              tile_source(p, w.seq, fresh0, g.sk, head, more ? t + phases : t);
+          const int tn = more ? t + phases : t;
+          const TileSource next = tile_source(p, fresh0, g.sk, head, tn, page_entry(p, w.seq, tn));
+          const int j0 = t * kTile;
+          const bool masked = j0 < c.full_lo || j0 + kTile > c.full_hi;
           wait_loads<8>();
-          attend(
-              kt, vt, t * kTile,
-              [&] {
-                lds_done();
-                if (more) issue_k(next);
-              },
-              [&] {
-                if (more) {
-                  wait_loads<8>();
-                } else {
-                  wait_loads<0>();
-                }
-              },
-              [&] {
-                lds_done();
-                if (more) issue_v(next);
-              });
+          read_k(k, kt, la);
+          lds_done();
+          if (more) issue_k(next);
+          f32x4_t sl[NCB][2];
+          u32x4_t v[8], pb[NCB];
+          logits<NCB>(k, q, sl);
+          weights<NCB, MODE>(p, c, st, sl, j0, lg, cs, masked, pb);
+          if (more) {
+            wait_loads<8>();
+          } else {
+            wait_loads<0>();
+          }
+#pragma unroll
+          for (int jj = 0; jj < 8; ++jj) v[jj] = read_v(vt, la, jj);
+          lds_done();
+          if (more) issue_v(next);
+          weigh_tile<NCB>(st, v, pb, masked, odd);
         }
       } else {
-        // Stage s of the ring: KW subtiles, each K then V.  A wave issues
-        // its share of every subtile's 16 loads; three tiles are in flight
-        // under the one that is attended, one barrier a step.
-        constexpr int kPer = 16 * KW / NW;  // loads a wave issues per stage
-        static_assert(16 * KW % NW == 0 && 8 % kPer == 0, "loads split evenly over the waves");
-        const int steps = (t_end - t_begin + KW - 1) / KW;
-        auto issue = [&](int step) {
-          // loads kPer * wave .. + kPer - 1 of the stage: within one tensor
-          const int first = kPer * wave;
-          const int sub = first / 16, tensor = (first / 8) & 1, m0 = first & 7;
-          const int t = t_begin + step * KW + sub;
+        // A stage holds kSub tiles, each K then V; every wave issues an equal
+        // part of its loads and attends kSub / KW of its tiles.  One barrier a
+        // step: each wave has its last tile's V in registers (so the stage is
+        // free for the load kStages steps ahead) and its loads of the next
+        // stage are back.  K operands are read a tile ahead, V operands before
+        // the tile's first product, so the LDS latency of both lies under
+        // MFMAs and the softmax.
+        constexpr int kPer = 16 * F::kSub / NW;  // loads a wave issues per stage
+        static_assert(8 % kPer == 0, "a wave's loads lie in one tensor");
+        const int sub = kPer * wave / 16, tensor = (kPer * wave / 8) & 1, m0 = kPer * wave & 7;
+        const int steps = (t_end - t_begin + F::kSub - 1) / F::kSub;
+        auto entry = [&](int step) {
+          const int t = t_begin + step * F::kSub + sub;
+          return t < t_end ? page_entry(p, w.seq, t) : -1;
+        };
+        auto issue = [&](int step, int blk) {
+          const int t = t_begin + step * F::kSub + sub;
           TileSource src{p.k, p.v, 0};
-          if (t < t_end) src = tile_source(p, w.seq, fresh0, g.sk, head, t);
+          if (t < t_end) src = tile_source(p, fresh0, g.sk, head, t, blk);
           const i32x4_t r = tensor ? raw_rsrc(src.v, tensor_bytes(src.rows, p.v_row))
                                    : raw_rsrc(src.k, tensor_bytes(src.rows, p.k_row));
-          const uint32_t at = lds0 + (step % F::kStages) * F::kStage + (2 * sub + tensor) * kTensor;
+          const uint32_t at =
+              lds0 + (step % F::kStages) * F::kStage + (2 * sub + tensor) * kTensor;
+          const int row_bytes = int(tensor ? p.v_row : p.k_row) * 2;
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            // (m0 is a multiple of kPer: the row offset adds up from it)
             const int m = m0 + i;
-            const int lr = lane >> 4, r16 = (4 * m + lr) & 15;
-            const int row_bytes = int(tensor ? p.v_row : p.k_row) * 2;
-            dma_to_lds_cached(r, (4 * m + lr) * row_bytes + (((lane & 15) ^ r16) << 4),
+            const int row = 4 * m + (lane >> 4);
+            dma_to_lds_cached(r, row * row_bytes + (((lane & 15) ^ (row & 15)) << 4),
                               at + m * 1024);
           }
         };
 #pragma unroll
-        for (int s = 0; s < F::kStages - 1; ++s) issue(s);
+        for (int s = 0; s < F::kStages; ++s) issue(s, entry(s));
+        int blk = entry(F::kStages);
+        wait_loads<kPer*(F::kStages - 1)>();
+        pf_barrier();
+        read_k(k, smem + phase * 2 * kTensor, la);
         for (int step = 0; step < steps; ++step) {
-          wait_loads<kPer*(F::kStages - 2)>();
-          pf_barrier();  // this stage is whole, and the one before it free
-          issue(step + F::kStages - 1);
-          const int t = t_begin + step * KW + phase;
-          const int j0 = t * kTile;
-          if (t < t_end && j0 < c.any_hi && j0 + kTile > c.any_lo) {
-            const char* kt = smem + (step % F::kStages) * F::kStage + phase * 2 * kTensor;
-            attend(kt, kt + kTensor, j0, [] {}, [] {}, [] {});
+          const char* stage = smem + (step % F::kStages) * F::kStage;
+#pragma unroll
+          for (int u = 0; u < F::kSub / KW; ++u) {
+            const bool last = u == F::kSub / KW - 1;
+            const char* kt = stage + (u * KW + phase) * 2 * kTensor;
+            const char* vt = kt + kTensor;
+            const int t = t_begin + step * F::kSub + u * KW + phase;
+            const int j0 = t * kTile;
+            const bool active = t < t_end && j0 < c.any_hi && j0 + kTile > c.any_lo;
+            const bool masked = j0 < c.full_lo || j0 + kTile > c.full_hi;
+            f32x4_t sl[NCB][2];
+            u32x4_t v[8], pb[NCB];
+            if (active) {
+#pragma unroll
+              for (int jj = 0; jj < 8; ++jj) v[jj] = read_v(vt, la, jj);
+              logits<NCB>(k, q, sl);
+            }
+            if (last) {
+              wait_loads<kPer*(F::kStages - 2)>();
+              pf_barrier();
+              issue(step + F::kStages, blk);
+              blk = entry(step + F::kStages + 1);
+              read_k(k, smem + ((step + 1) % F::kStages) * F::kStage + phase * 2 * kTensor, la);
+            } else {
+              read_k(k, kt + KW * 2 * kTensor, la);
+            }
+            if (active) {
+              weights<NCB, MODE>(p, c, st, sl, j0, lg, cs, masked, pb);
+              weigh_tile<NCB>(st, v, pb, masked, odd);
+            }
           }
         }
         wait_loads<0>();
       }
 
+      if (__builtin_expect(odd, 0)) {
+        for (int t = t_begin + phase; t < t_end; t += phases) {
+          const int j0 = t * kTile;
+          if (j0 >= c.full_lo && j0 + kTile <= c.full_hi) continue;
+          const TileSource src = tile_source(p, fresh0, g.sk, head, t, page_entry(p, w.seq, t));
+          add_not_finite<NCB>(p, c, st, src.v, src.rows, j0, lg);
+        }
+      }
       // Join the tile phases: the waves of phase 0 take in the others' states.
       if (phases > 1) {
         const int owners = NW / phases;
@@ -973,9 +1000,11 @@ __global__ void __launch_bounds__(64 * NW)
     w.block = 0;
     if (++w.grp < p.head_groups) continue;
     w.grp = 0;
-    w.nb += nblocks;
     do {
-      if (++w.seq >= p.batch) return;
+      if (++w.seq >= p.batch) {
+        if (threadIdx.x == 0) p.rec[share] = int4{0, 0, 0, 0};
+        return;
+      }
       g = load_seq<true>(p, w.seq);
       nblocks = num_blocks_of(p, g.sq);
     } while (nblocks == 0);
@@ -983,40 +1012,56 @@ __global__ void __launch_bounds__(64 * NW)
 }
 
 // ---------------------------------------------------------------------------
-// Join the partials of items cut between shares: one workgroup per item and
-// head slot, 32 lanes per column.
+// Join the partials of items cut between shares: workgroup (share, eight
+// columns) takes the item that begins in the share and ends in another, 32
+// lanes per column.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) scored_merge_kernel(ScoredParams p, int columns) {
-  const int item = blockIdx.x / p.heads_per_wg, hs = blockIdx.x % p.heads_per_wg;
-  const int4 r = p.rec[item];
-  if (r.w <= r.z) return;  // whole, or not there
+constexpr int kMergeColumns = 8;
+constexpr int kMergeAhead = 4;  // pieces whose loads are in flight together
+__global__ void __launch_bounds__(32 * kMergeColumns)
+    scored_merge_kernel(ScoredParams p, int columns) {
+  const int share = blockIdx.x;
+  const int4 r = p.rec[share];
+  if (r.w <= share) return;
+  const int per_head = columns / kMergeColumns;
+  const int hs = blockIdx.y / per_head;
+  const int col = (blockIdx.y - hs * per_head) * kMergeColumns + int(threadIdx.x >> 5);
   const SeqGeo g = load_seq<true>(p, r.x);
-  const int head = (item % p.head_groups) * p.heads_per_wg + hs;
+  const int head = r.z * p.heads_per_wg + hs;
   const int b0 = r.y * p.tokens_per_block;
   const int tokens = min(g.sq - b0, p.tokens_per_block);
+  if (col >= tokens * p.group) return;
   const int lane = threadIdx.x & 31;
-  const int64_t cols = int64_t(p.heads_per_wg) * columns;
-  for (int col = threadIdx.x >> 5; col < tokens * p.group; col += 8) {
-    const int64_t at = hs * columns + col;
-    float top = kLowest;
-    for (int s = r.z; s <= r.w; ++s)
-      top = fmaxf(top, p.part_ml[(int64_t(2) * s + (s == r.z)) * cols + at].x);
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int s = r.z; s <= r.w; ++s) {
-      const int64_t c = (int64_t(2) * s + (s == r.z)) * cols + at;
-      const float2 ml = p.part_ml[c];
-      const float a = __builtin_amdgcn_exp2f(ml.x - top);
-      l += ml.y * a;
-      o += reinterpret_cast<const f32x4_t*>(p.part_o + c * kD)[lane] * a;
+  const int64_t cols = int64_t(p.heads_per_wg) * columns, at = hs * columns + col;
+  float top = kLowest, l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = share; s0 <= r.w; s0 += kMergeAhead) {
+    float2 ml[kMergeAhead];
+    f32x4_t part[kMergeAhead];
+#pragma unroll
+    for (int i = 0; i < kMergeAhead; ++i) {
+      const int s = min(s0 + i, r.w);
+      const int64_t c = (int64_t(2) * s + (s == share)) * cols + at;
+      ml[i] = p.part_ml[c];
+      part[i] = reinterpret_cast<const f32x4_t*>(p.part_o + c * kD)[lane];
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int t = col / p.group;
-    uint16_t* dst = p.out + int64_t(g.q0 + b0 + t) * p.o_st +
-                    int64_t(head * p.group + col - t * p.group) * p.o_sh + 4 * lane;
-    *reinterpret_cast<u32x2_t*>(dst) =
-        u32x2_t{pack_bf16x2_fast(o[0] * inv, o[1] * inv), pack_bf16x2_fast(o[2] * inv, o[3] * inv)};
+#pragma unroll
+    for (int i = 0; i < kMergeAhead; ++i) {
+      if (s0 + i > r.w) continue;
+      const float next = fmaxf(top, ml[i].x);
+      const float a = __builtin_amdgcn_exp2f(top - next);
+      const float b = __builtin_amdgcn_exp2f(ml[i].x - next);
+      top = next;
+      l = l * a + ml[i].y * b;
+      o = o * a + part[i] * b;
+    }
   }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int t = col / p.group;
+  uint16_t* dst = p.out + int64_t(g.q0 + b0 + t) * p.o_st +
+                  int64_t(head * p.group + col - t * p.group) * p.o_sh + 4 * lane;
+  *reinterpret_cast<u32x2_t*>(dst) =
+      u32x2_t{pack_bf16x2_fast(o[0] * inv, o[1] * inv), pack_bf16x2_fast(o[2] * inv, o[3] * inv)};
 }
 
 // Depth of each tree token: its mask's bits inside the tree but its own.
@@ -1078,7 +1123,7 @@ Plan make_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, i
   pl.grid = cu_count();
   pl.max_items = (tokens / pl.tokens_per_block + batch) * pl.head_groups;
   const size_t cols = size_t(2) * pl.grid * pl.heads_per_wg * pl.columns;
-  pl.rec_bytes = up256(size_t(pl.max_items) * sizeof(int4));
+  pl.rec_bytes = up256(size_t(pl.grid) * sizeof(int4));
   pl.ml_bytes = up256(cols * sizeof(float2));
   pl.o_bytes = up256(cols * kD * sizeof(float));
   return pl;
@@ -1130,7 +1175,6 @@ int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStrea
   p.rec = reinterpret_cast<int4*>(w);
   p.part_ml = reinterpret_cast<float2*>(w + pl.rec_bytes);
   p.part_o = reinterpret_cast<float*>(w + pl.rec_bytes + pl.ml_bytes);
-  p.max_items = int(pl.max_items);
   int rc;
   const bool bias = p.slopes != nullptr;
   if (p.cap > 0.f) {
@@ -1145,7 +1189,8 @@ int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStrea
     rc = bias ? launch_form<kDistance>(p, pl, st) : launch_form<kPlain>(p, pl, st);
   }
   if (rc != KVC_OK) return rc;
-  scored_merge_kernel<<<unsigned(pl.max_items * pl.heads_per_wg), 256, 0, st>>>(p, pl.columns);
+  const dim3 mg{unsigned(pl.grid), unsigned(pl.heads_per_wg * pl.columns / kMergeColumns)};
+  scored_merge_kernel<<<mg, 32 * kMergeColumns, 0, st>>>(p, pl.columns);
   return check_launch(what);
 }
 
@@ -1185,7 +1230,7 @@ int check_pool(const char* what, const void* k, const void* v, int64_t blocks, i
   KVC_REQUIRE(page > 0 && page % kTile == 0, KVC_ERR_VALUE,
               "%s: page_size must be a multiple of 32", what);
   KVC_REQUIRE(blocks > 0 && blocks < (int64_t(1) << 31) && max_blocks >= 0 &&
-                  max_blocks * page < (int64_t(1) << 30),
+                  max_blocks * page < (int64_t(1) << 29),
               KVC_ERR_VALUE, "%s: bad pool or table size", what);
   KVC_REQUIRE(rows16(k, 0, 0) && rows16(v, 0, 0) && kv_heads * kD < (1 << 24), KVC_ERR_ASSERT,
               "%s: pools must be 16-byte aligned", what);
@@ -1236,7 +1281,7 @@ extern "C" int kvc_scored_attention(
   const bool fresh = block_tables == nullptr;
   if (fresh) {
     KVC_REQUIRE(num_decode_rows == 0, KVC_ERR_VALUE, "%s: decode rows need block tables", what);
-    KVC_REQUIRE(num_fresh_rows >= 0 && num_fresh_rows < (int64_t(1) << 30) &&
+    KVC_REQUIRE(num_fresh_rows >= 0 && num_fresh_rows < (int64_t(1) << 29) &&
                     (num_fresh_rows == 0 || (k_fresh != nullptr && v_fresh != nullptr)),
                 KVC_ERR_VALUE, "%s: without block tables the keys come from k/v", what);
     KVC_REQUIRE(rows16(k_fresh, kf_stride_t, kf_stride_h) &&
@@ -1276,6 +1321,8 @@ extern "C" int kvc_scored_attention(
   p.max_blocks = int(max_blocks_per_seq);
   p.num_blocks = int(num_cache_blocks);
   p.page = int(page_size);
+  p.page_tiles = int(page_size / kTile);
+  p.page_rcp = page_size > 0 ? 1.f / float(page_size / kTile) : 0.f;
   p.fresh_rows = num_fresh_rows;
   p.slopes = alibi_slopes;
   p.scale = scale;
@@ -1363,6 +1410,8 @@ extern "C" int kvc_tree_attention(
   p.max_blocks = int(max_blocks_per_seq);
   p.num_blocks = int(num_cache_blocks);
   p.page = int(page_size);
+  p.page_tiles = int(page_size / kTile);
+  p.page_rcp = page_size > 0 ? 1.f / float(page_size / kTile) : 0.f;
   p.cu_q = cu_seqlens_q;
   p.q_per_seq = int(max_seqlen_q);
   p.lens = context_lens;
