@@ -38,8 +38,9 @@ namespace {
 constexpr int kD = 128;
 constexpr int kTile = 32;
 constexpr int kTensor = kTile * kD * 2;  // one K or V tile of a head: 8 KiB
-constexpr float kLazyLog2 = 8.f;         // the running reference moves when passed by 2^8
+constexpr uint32_t kLazyBits = 0x4380u;  // bf16 2^8: a weight past it moves the running reference
 constexpr float kLowest = -3.402823466e38f;
+constexpr uint32_t kOnes2 = 0x3F803F80u;  // two bf16 ones
 
 enum ScoreMode {
   kPlain = 0,
@@ -80,6 +81,7 @@ struct ScoredParams {
   float scale, cap;
   int window;
   int batch, num_tokens, heads, kv_heads, group;
+  float group_rcp;  // 1 / group
   int heads_per_wg, head_groups;
   int tokens_per_block;
   int lane_plan;  // the plan walks sequences across lanes (else blocks)
@@ -165,7 +167,8 @@ __device__ __forceinline__ TileRange block_tiles(const ScoredParams& p, const Se
 // ---------------------------------------------------------------------------
 template <int NCB>
 struct Columns {
-  int token[NCB];         // t, the column's token inside its sequence
+  int first, last;        // the block's tokens
+  int col0;               // the wave's first column in the block
   float place[NCB];       // p, for the distance bias
   float slope2[NCB];      // slope log2(e)
   const uint32_t* bits;   // tree: the sequence's masks
@@ -176,10 +179,26 @@ struct Columns {
   int any_lo, any_hi;     // a tile outside them is seen by no column
 };
 
+// The token, inside its block, and the query head of column col0 + 16 cb + lm.
+// (Worked out where it is needed, which is rarely: kept, it would take
+// registers from the loop.)
+struct ColumnOf {
+  int token, head;
+};
+__device__ __forceinline__ ColumnOf column_of(const ScoredParams& p, int col0, int cb) {
+  int lane = int(threadIdx.x);
+  asm volatile("" : "+v"(lane));
+  const int col = col0 + 16 * cb + (lane & 15);
+  ColumnOf c;
+  c.token = div_small(col, p.group, p.group_rcp);
+  c.head = col - c.token * p.group;
+  return c;
+}
+
 template <int NCB>
 struct State {
   f32x4_t o[NCB][8];
-  f32x4_t l[NCB];
+  float l[NCB];  // over the lane's own keys; of the column once the loop is done
   float mu[NCB];
 };
 
@@ -189,7 +208,7 @@ __device__ __forceinline__ void reset(State<NCB>& st, float mu0) {
   for (int cb = 0; cb < NCB; ++cb) {
 #pragma unroll
     for (int jj = 0; jj < 8; ++jj) st.o[cb][jj] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    st.l[cb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    st.l[cb] = 0.f;
     st.mu[cb] = mu0;
   }
 }
@@ -202,7 +221,7 @@ __device__ __forceinline__ uint32_t bits_below(int n) {  // bits 0 .. n - 1
 template <int NCB>
 __device__ __forceinline__ uint32_t visible_bits(const ScoredParams& p, const Columns<NCB>& c,
                                                  int cb, int j0) {
-  const int t = c.token[cb];
+  const int t = min(c.first + column_of(p, c.col0, cb).token, c.last);
   if (p.mask == nullptr) {
     uint32_t vis = bits_below(min(c.sk, max(c.p0 + t + 1, c.pre)) - j0);
     if (p.window > 0) vis &= ~bits_below(c.p0 + t + 1 - p.window - j0);
@@ -261,27 +280,24 @@ __device__ __forceinline__ void logits(const u32x4_t (&k)[2][4], const u32x4_t (
 }
 
 // The score's shape, the mask, the running softmax, and P^T as the bf16
-// operand pb.  y holds what the softmax is taken of: the raw logit s (log2-
-// unit score c2 s) for plain scores, the log2-unit score otherwise; -inf at
-// keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} + 1): one exp2 and
+// operand pb.  y comes in as the logits and becomes what the softmax is taken
+// of: the raw logit s (log2-unit score c2 s) for plain scores, the log2-unit
+// score otherwise; -inf at keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} + 1): one exp2 and
 // one reciprocal.  Sums are formed of the rounded P (an MFMA against ones),
 // so the weights add up to the sum that divides them.
 template <int NCB, int MODE>
-__device__ __forceinline__ void weights(const ScoredParams& p, const Columns<NCB>& c,
-                                        State<NCB>& st, const f32x4_t (&sl)[NCB][2], int j0,
-                                        int lg, const Consts& cs, bool masked,
-                                        u32x4_t (&pb)[NCB]) {
+__device__ __forceinline__ void shape_scores(const Columns<NCB>& c, f32x4_t (&y)[NCB][2], int j0,
+                                             int lg, const Consts& cs) {
   constexpr bool kDist = MODE == kDistance || MODE == kCapDistance;
   constexpr bool kCap = MODE == kCapFixed || MODE == kCapLazy || MODE == kCapDistance;
-  const float unit = MODE == kPlain ? cs.c2 : 1.f;
-  float y[NCB][8];
+  if constexpr (!kDist && !kCap) return;
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
     // The bias of a key at or before the query's place.
     const float b0 = kDist ? c.slope2[cb] * (float(j0 + 4 * lg) - c.place[cb]) : 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float s = sl[cb][e >> 2][e & 3];
+      const float s = y[cb][e >> 2][e & 3];
       float x = s;
       if constexpr (kCap) {
         const float w = __builtin_amdgcn_exp2f(s * cs.zc);
@@ -291,137 +307,186 @@ __device__ __forceinline__ void weights(const ScoredParams& p, const Columns<NCB
         const float bias = __builtin_fmaf(c.slope2[cb], float(key_of(e)), b0);
         x = kCap ? x + bias : __builtin_fmaf(s, cs.c2, bias);
       }
-      y[cb][e] = x;
+      y[cb][e >> 2][e & 3] = x;
     }
-  }
-  // (the branch changes y in place: one copy of everything else)
-  if (masked) {
-#pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) {
-      const uint32_t own = visible_bits<NCB>(p, c, cb, j0) >> (4 * lg);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (kDist) {
-          const int j = j0 + 4 * lg + key_of(e);
-          int at = j;
-          if (p.mask != nullptr && j >= c.p0 && j < c.sk) at = c.p0 + c.depths[j - c.p0];
-          y[cb][e] = __builtin_fmaf(
-              -c.slope2[cb], fabsf(c.place[cb] - float(at)) + (float(j) - c.place[cb]), y[cb][e]);
-        }
-        y[cb][e] = ((own >> key_of(e)) & 1u) ? y[cb][e] : -INFINITY;
-      }
-    }
-  }
-  if constexpr (MODE != kCapFixed) {
-    // The reference moves only when a column passes it by 2^8 (or has none).
-    float over = -INFINITY;
-#pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) {
-      float top = y[cb][0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, y[cb][e]);
-      over = fmaxf(over, __builtin_fmaf(top, unit, -st.mu[cb]));
-    }
-    if (__builtin_expect(__any(over > kLazyLog2), 0)) {
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        float top = y[cb][0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) top = fmaxf(top, y[cb][e]);
-        const float mu = fmaxf(st.mu[cb], rows4_max(top) * unit);
-        const float down = __builtin_amdgcn_exp2f(st.mu[cb] - mu);
-#pragma unroll
-        for (int jj = 0; jj < 8; ++jj) st.o[cb][jj] *= down;
-        st.l[cb] *= down;
-        st.mu[cb] = mu;
-      }
-    }
-  }
-#pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) {
-    float pr[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      pr[e] = __builtin_amdgcn_exp2f(MODE == kCapFixed ? y[cb][e]
-                                     : MODE == kPlain ? __builtin_fmaf(y[cb][e], unit, -st.mu[cb])
-                                                      : y[cb][e] - st.mu[cb]);
-    pb[cb] = u32x4_t{pack_bf16x2_fast(pr[0], pr[1]), pack_bf16x2_fast(pr[2], pr[3]),
-                     pack_bf16x2_fast(pr[4], pr[5]), pack_bf16x2_fast(pr[6], pr[7])};
   }
 }
 
-constexpr uint32_t kOnes2 = 0x3F803F80u;
+// (in place: one copy of everything around it)
+template <int NCB, int MODE>
+__device__ __forceinline__ void mask_scores(const ScoredParams& p, const Columns<NCB>& c,
+                                            f32x4_t (&y)[NCB][2], int j0, int lg) {
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    const uint32_t own = visible_bits<NCB>(p, c, cb, j0) >> (4 * lg);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x = y[cb][e >> 2][e & 3];
+      if constexpr (MODE == kDistance || MODE == kCapDistance) {
+        const int j = j0 + 4 * lg + key_of(e);
+        int at = j;
+        if (p.mask != nullptr && j >= c.p0 && j < c.sk) at = c.p0 + c.depths[j - c.p0];
+        x = __builtin_fmaf(-c.slope2[cb],
+                           fabsf(c.place[cb] - float(at)) + (float(j) - c.place[cb]), x);
+      }
+      y[cb][e >> 2][e & 3] = ((own >> key_of(e)) & 1u) ? x : -INFINITY;
+    }
+  }
+}
 
-__device__ __forceinline__ bool not_finite(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t,
                             __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a),
                                                       __builtin_bit_cast(u16x2_t, b)));
 }
+
+// P^T of the tile, relative to each column's reference.
+template <int NCB, int MODE>
+__device__ __forceinline__ void exponentials(const State<NCB>& st, const f32x4_t (&y)[NCB][2],
+                                             const Consts& cs, u32x4_t (&pb)[NCB]) {
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    float pr[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = y[cb][e >> 2][e & 3];
+      pr[e] = __builtin_amdgcn_exp2f(MODE == kCapFixed ? x
+                                     : MODE == kPlain  ? __builtin_fmaf(x, cs.c2, -st.mu[cb])
+                                                       : x - st.mu[cb]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t two = pack_bf16x2_fast(pr[2 * i], pr[2 * i + 1]);
+      asm volatile("" : "+v"(two));  // (else it is packed anew for every use)
+      pb[cb][i] = two;
+    }
+  }
+}
+
+// The reference moves only when a weight passes 2^8 (or a column has none
+// yet), which the packed weights themselves say; the tile's are then formed
+// again.
+template <int NCB, int MODE>
+__device__ __forceinline__ void follow_reference(State<NCB>& st, const f32x4_t (&y)[NCB][2],
+                                                 const Consts& cs, u32x4_t (&pb)[NCB]) {
+  if constexpr (MODE == kCapFixed) return;
+  const float unit = MODE == kPlain ? cs.c2 : 1.f;
+  uint32_t most = 0u;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = max_u16x2(most, pb[cb][i]);
+  const bool past = (most >> 16) > kLazyBits || (most & 0xffffu) > kLazyBits;
+  if (__builtin_expect(__any(past), 0)) {
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      float top = y[cb][0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, y[cb][e >> 2][e & 3]);
+      const float mu = fmaxf(st.mu[cb], rows4_max(top) * unit);
+      const float down = __builtin_amdgcn_exp2f(st.mu[cb] - mu);
+#pragma unroll
+      for (int jj = 0; jj < 8; ++jj) st.o[cb][jj] *= down;
+      st.l[cb] *= down;
+      st.mu[cb] = mu;
+    }
+    exponentials<NCB, MODE>(st, y, cs, pb);
+  }
+}
+
+template <int NCB>
+__device__ __forceinline__ void sum_weights(State<NCB>& st, const u32x4_t (&pb)[NCB]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      const uint32_t two = pb[cb][i];
+      st.l[cb] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two),
+                                                 __builtin_bit_cast(bf16x2_t, kOnes2), st.l[cb],
+                                                 false);
+    }
+}
+
+template <int NCB, int MODE>
+__device__ __forceinline__ void weights(const ScoredParams& p, const Columns<NCB>& c,
+                                        State<NCB>& st, f32x4_t (&y)[NCB][2], int j0, int lg,
+                                        const Consts& cs, bool masked, u32x4_t (&pb)[NCB]) {
+  shape_scores<NCB, MODE>(c, y, j0, lg, cs);
+  if (__builtin_expect(masked, 0)) mask_scores<NCB, MODE>(p, c, y, j0, lg);
+  exponentials<NCB, MODE>(st, y, cs, pb);
+  follow_reference<NCB, MODE>(st, y, cs, pb);
+  sum_weights<NCB>(st, pb);
+}
+
+__device__ __forceinline__ bool not_finite(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
 __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
   return (not_finite(w) ? 0u : w & 0xffffu) | (not_finite(w >> 16) ? 0u : w & 0xffff0000u);
 }
 
-// LDS image of a K or V tile: row r (key) is 256 bytes, its 16-byte chunk ch
-// at chunk ch ^ (r & 15), which keeps both the row-wise K reads (16 rows of
-// one chunk) and the transposed V reads (4 rows x 4 chunks per lane group)
-// on distinct banks without padding, so a tile is eight whole 1 KiB loads.
-// The V operand's rows are dims 32 (m / 4) + 4 jj + m % 4, so that a lane's
-// outputs are 32 consecutive dims of its column.
+// LDS image of a K or V tile: row r (key) is 256 bytes; K's 16-byte chunk ch
+// lies at chunk ch ^ (r & 15), V's at ch ^ 2 (r & 7).  A K operand read takes
+// one chunk of 16 rows per lane group, a V operand read (transposed, 8 bytes a
+// lane) 32 bytes of four rows per lane group: either way the lanes served
+// together lie on distinct banks without padding, so a tile is eight whole
+// 1 KiB loads.  (V rows permuted so that a lane's outputs are 32 consecutive
+// dims read two lane groups from the same banks: 2 extra cycles per V read.)
 struct LdsAddr {
-  int k[4];  // K operand d: row lm, chunk 4 d + lg
-  int v[4];  // V operand pair jj / 2: row 4 lg + lm / 4, chunk 4 (lm % 4) + jj / 2
+  int k;  // K operand d: row lm, chunk 4 d + lg, at k ^ (d << 6)
+  int v;  // V operand jj: row 4 lg + lm / 4, dims 16 jj + 4 (lm % 4) .., at v ^ (jj << 5)
 };
 __device__ __forceinline__ LdsAddr lds_addrs(int lm, int lg) {
   LdsAddr a;
-  const int vr = 4 * lg + (lm >> 2);
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    a.k[d] = lm * 256 + (((4 * d + lg) ^ lm) << 4);
-    a.v[d] = vr * 256 + (((4 * (lm & 3) + d) ^ vr) << 4);
-  }
+  const int vr = 4 * lg + (lm >> 2), piece = lm & 3;
+  a.k = lm * 256 + ((lg ^ lm) << 4);
+  a.v = vr * 256 + (((piece >> 1) ^ ((vr & 7) << 1)) << 4) + (piece & 1) * 8;
   return a;
 }
+__device__ __forceinline__ int k_swizzle(int row) { return row & 15; }
+__device__ __forceinline__ int v_swizzle(int row) { return (row & 7) << 1; }
 
+__device__ __forceinline__ u32x4_t read_k1(const char* kt, const LdsAddr& a, int h, int d) {
+  return *reinterpret_cast<const u32x4_t*>(kt + (a.k ^ (d << 6)) + h * 4096);
+}
 __device__ __forceinline__ void read_k(u32x4_t (&k)[2][4], const char* kt, const LdsAddr& a) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
-      k[h][d] = *reinterpret_cast<const u32x4_t*>(kt + a.k[d] + h * 4096);
+    for (int h = 0; h < 2; ++h) k[h][d] = read_k1(kt, a, h, d);
 }
 
-__device__ __forceinline__ u32x4_t read_v(const char* vt, const LdsAddr& a, int jj) {
-  const char* s = vt + a.v[jj >> 1] + (jj & 1) * 8;
+__device__ __forceinline__ u32x4_t read_v1(const char* vt, const LdsAddr& a, int jj) {
+  const char* s = vt + (a.v ^ (jj << 5));
   const u32x2_t lo = lds_read_tr16(s), hi = lds_read_tr16(s + 4096);
   return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
 }
+__device__ __forceinline__ void read_v(u32x4_t (&v)[8], const char* vt, const LdsAddr& a) {
+#pragma unroll
+  for (int jj = 0; jj < 8; ++jj) v[jj] = read_v1(vt, a, jj);
+}
 
-// O^T += V^T P^T.  In a masked tile a column's P is 0 at keys it does not see,
-// but 0 times an infinity or NaN held there would still reach its sum: such
-// values are taken out of the operand, and `odd` says so (add_not_finite then
-// gives them to the columns that see them, after the loop).
+// In a masked tile a column's P is 0 at keys it does not see, but 0 times an
+// infinity or NaN held there would still reach its sum: such values are taken
+// out of the operand, and the answer says so (add_not_finite then gives them
+// to the columns that see them, after the loop).
+__device__ __forceinline__ bool take_out_not_finite(u32x4_t (&v)[8]) {
+  uint32_t most = 0u;
+#pragma unroll
+  for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = max_u16x2(most, v[jj][i] & 0x7fff7fffu);
+  if (__builtin_expect(!__any(not_finite(most) || not_finite(most >> 16)), 1)) return false;
+#pragma unroll
+  for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[jj][i] = finite_or_zero(v[jj][i]);
+  return true;
+}
+
+// O^T += V^T P^T.
 template <int NCB>
-__device__ __forceinline__ void weigh_tile(State<NCB>& st, u32x4_t (&v)[8],
-                                           const u32x4_t (&pb)[NCB], bool masked, bool& odd) {
-  if (masked) {
-    uint32_t most = 0u;
-#pragma unroll
-    for (int jj = 0; jj < 8; ++jj)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) most = max_u16x2(most, v[jj][i] & 0x7fff7fffu);
-    if (__builtin_expect(__any(not_finite(most) || not_finite(most >> 16)), 0)) {
-      odd = true;
-#pragma unroll
-      for (int jj = 0; jj < 8; ++jj)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[jj][i] = finite_or_zero(v[jj][i]);
-    }
-  }
-  const u32x4_t ones = {kOnes2, kOnes2, kOnes2, kOnes2};
-#pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) st.l[cb] = mfma_bf16(ones, pb[cb], st.l[cb]);
+__device__ __forceinline__ void weigh(State<NCB>& st, const u32x4_t (&v)[8],
+                                      const u32x4_t (&pb)[NCB]) {
 #pragma unroll
   for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
@@ -441,15 +506,15 @@ __device__ __forceinline__ void add_not_finite(const ScoredParams& p, const Colu
 #pragma unroll 1
   for (int r = 0; r < rows; ++r) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {  // the lane's dims 32 lg + 8 n ..
-      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(v + r * p.v_row + 32 * lg + 8 * n);
+    for (int jj = 0; jj < 8; ++jj) {
+      const u32x2_t w = *reinterpret_cast<const u32x2_t*>(v + r * p.v_row + 16 * jj + 4 * lg);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const uint32_t half = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
         const float add = not_finite(half) ? bf16_bits_to_f32(half) : 0.f;
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb)
-          st.o[cb][2 * n + (i >> 2)][i & 3] += ((vis[cb] >> r) & 1u) ? add : 0.f;
+          st.o[cb][jj][i] += ((vis[cb] >> r) & 1u) ? add : 0.f;
       }
     }
   }
@@ -607,13 +672,14 @@ struct DmaOffsets {
   int base[4];  // m = 0 .. 3
   int step;     // 16 rows
 };
+template <bool kV>
 __device__ __forceinline__ DmaOffsets dma_offsets(int lane, int64_t row_elems) {
   DmaOffsets o;
   const int lr = lane >> 4, slot = lane & 15;
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     const int r = 4 * m + lr;
-    o.base[m] = r * int(row_elems) * 2 + ((slot ^ r) << 4);
+    o.base[m] = r * int(row_elems) * 2 + ((slot ^ (kV ? v_swizzle(r) : k_swizzle(r))) << 4);
   }
   o.step = 16 * int(row_elems) * 2;
   return o;
@@ -649,9 +715,11 @@ struct Form {
   static constexpr bool kPrivate = KW == NW;
   static constexpr int kColWaves = kPrivate ? 1 : NW / KW;
   static constexpr int kColumns = 16 * NCB * kColWaves;  // per kv head
-  static constexpr int kSub = kPrivate ? NW : KW == 1 ? 2 : 4;  // tiles per stage
+  static constexpr int kSub = kPrivate ? NW : KW == 1 ? 8 : 4;  // tiles per stage
   static constexpr int kStage = kSub * 2 * kTensor;
-  static constexpr int kStages = kPrivate ? 1 : KW == 1 ? 4 : 2;
+  static constexpr int kStages = kPrivate || KW == 1 ? 1 : 2;
+  static constexpr bool kTurns = KW == 1;
+  static constexpr int kRing = 8;  // tiles, taking turns
   // waves that hand their state to another: [wave][34 NCB floats][64 lanes]
   static constexpr int kStateBytes = 34 * NCB * 256;
   static constexpr int kJoinBytes =
@@ -670,7 +738,7 @@ __device__ __forceinline__ void put_state(char* at, const State<NCB>& st, int la
     for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[(cb * 34 + jj * 4 + i) * 64] = st.o[cb][jj][i];
-    f[(cb * 34 + 32) * 64] = st.l[cb][0];
+    f[(cb * 34 + 32) * 64] = st.l[cb];
     f[(cb * 34 + 33) * 64] = st.mu[cb];
   }
 }
@@ -684,7 +752,7 @@ __device__ __forceinline__ void join_state(State<NCB>& st, const char* at, int l
     const float top = fmaxf(mu, st.mu[cb]);
     const float a = __builtin_amdgcn_exp2f(st.mu[cb] - top), b = __builtin_amdgcn_exp2f(mu - top);
     st.mu[cb] = top;
-    st.l[cb][0] = st.l[cb][0] * a + l * b;
+    st.l[cb] = st.l[cb] * a + l * b;
 #pragma unroll
     for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
@@ -717,7 +785,6 @@ __global__ void __launch_bounds__(64 * NW)
   const int phase = F::kPrivate ? wave / p.heads_per_wg : wave / F::kColWaves;
   const int cw = F::kPrivate ? 0 : wave % F::kColWaves;
   const LdsAddr la = lds_addrs(lm, lg);
-  const DmaOffsets ko = dma_offsets(lane, p.k_row), vo = dma_offsets(lane, p.v_row);
   const uint32_t lds0 = lds_addr(smem);
   Consts cs;
   cs.c2 = p.scale * kLog2e;
@@ -726,15 +793,9 @@ __global__ void __launch_bounds__(64 * NW)
   cs.a2 = 2.f * cs.a;
   constexpr float mu0 = MODE == kCapFixed ? 0.f : kLowest;
 
-  int tcol[NCB], gcol[NCB];  // the column's token inside a block, its query head
-#pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) {
-    const int col = (cw * NCB + cb) * 16 + lm;
-    tcol[cb] = col / p.group;
-    gcol[cb] = col - tcol[cb] * p.group;
-  }
-  const int wave_t0 = cw * NCB * 16 / p.group;
-  const int wave_t1 = min((cw * NCB * 16 + NCB * 16 - 1) / p.group, p.tokens_per_block - 1);
+  const int col0 = cw * NCB * 16;
+  const int wave_t0 = col0 / p.group;
+  const int wave_t1 = min((col0 + NCB * 16 - 1) / p.group, p.tokens_per_block - 1);
 
   const int end = int(min(w.total, int64_t(share + 1) * size));
   int pos = share * size;
@@ -763,15 +824,18 @@ __global__ void __launch_bounds__(64 * NW)
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) {
         // (columns past the block repeat its last token)
-        const int t = min(b0 + tcol[cb], tmax);
-        qp[cb] = p.q + int64_t(g.q0 + t) * p.q_st + int64_t(head * p.group + gcol[cb]) * p.q_sh;
-        c.token[cb] = t;
-        c.place[cb] = float(p0 + (p.mask == nullptr      ? t
-                                  : p.places != nullptr ? p.places[g.q0 + t]
-                                                        : 0));
-        c.slope2[cb] =
-            p.slopes != nullptr ? p.slopes[head * p.group + gcol[cb]] * kLog2e : 0.f;
+        const ColumnOf col = column_of(p, col0, cb);
+        const int t = min(b0 + col.token, tmax);
+        qp[cb] = p.q + int64_t(g.q0 + t) * p.q_st + int64_t(head * p.group + col.head) * p.q_sh;
+        c.place[cb] = c.slope2[cb] = 0.f;
+        if constexpr (MODE == kDistance || MODE == kCapDistance) {
+          c.place[cb] = float(p0 + (p.mask == nullptr ? t : p.places[g.q0 + t]));
+          c.slope2[cb] = p.slopes[head * p.group + col.head] * kLog2e;
+        }
       }
+      c.first = b0;
+      c.last = tmax;
+      c.col0 = col0;
       c.bits = p.mask != nullptr ? p.mask + int64_t(g.q0) * p.mask_words : nullptr;
       c.depths = p.places != nullptr ? p.places + g.q0 : nullptr;
       c.pre = pre;
@@ -803,7 +867,8 @@ __global__ void __launch_bounds__(64 * NW)
       // Every compiler-tracked load is back before the counted ones start.
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) {
-        asm volatile("" : "+v"(c.place[cb]), "+v"(c.slope2[cb]));
+        if constexpr (MODE == kDistance || MODE == kCapDistance)
+          asm volatile("" : "+v"(c.place[cb]), "+v"(c.slope2[cb]));
 #pragma unroll
         for (int d = 0; d < 4; ++d) asm volatile("" : "+v"(q[cb][d]));
       }
@@ -817,6 +882,8 @@ __global__ void __launch_bounds__(64 * NW)
       if constexpr (F::kPrivate) {
         // Wave-private slots: K 8 KiB, V 8 KiB.  The next tile's K load goes
         // out as soon as this tile's K is in registers, its V load likewise.
+        const DmaOffsets ko = dma_offsets<false>(lane, p.k_row);
+        const DmaOffsets vo = dma_offsets<true>(lane, p.v_row);
         const uint32_t kl = lds0 + wave * (2 * kTensor), vl = kl + kTensor;
         const char* kt = smem + wave * (2 * kTensor);
         const char* vt = kt + kTensor;
@@ -855,12 +922,169 @@ __global__ void __launch_bounds__(64 * NW)
           } else {
             wait_loads<0>();
           }
-#pragma unroll
-          for (int jj = 0; jj < 8; ++jj) v[jj] = read_v(vt, la, jj);
+          read_v(v, vt, la);
           lds_done();
           if (more) issue_v(next);
-          weigh_tile<NCB>(st, v, pb, masked, odd);
+          if (masked) odd |= take_out_not_finite(v);
+          weigh<NCB>(st, v, pb);
         }
+      } else if constexpr (F::kTurns) {
+        // The waves take turns: while the first four (one on each SIMD) run
+        // their products and read operands, the other four run a softmax, and
+        // a barrier swaps them, so that matrix and vector units work side by
+        // side.  Products of a turn: S of tile i and O of tile i - 1.  Tile u
+        // is last read in the later half's turn u, so that its slot is loaded
+        // again a turn on, kRing - 1 tiles ahead.
+        const bool later = wave >= NW / 2;
+        const int n = t_end - t_begin;
+        // A wave's part of a tile: rows 4 wave .. + 3 of K and of V.
+        const int drow = 4 * wave + (lane >> 4);
+        const int kvoff = drow * int(p.k_row) * 2 + (((lane & 15) ^ k_swizzle(drow)) << 4);
+        const int vvoff = drow * int(p.v_row) * 2 + (((lane & 15) ^ v_swizzle(drow)) << 4);
+        // The loads' resources move along a page by adds; a page's block (the
+        // next one's entry is read a page ahead), and a ragged last tile, are
+        // set apart, once each.
+        const bool paged = p.tables != nullptr;
+        const int32_t* table = p.tables + int64_t(w.seq) * p.bt_stride;
+        int page = paged ? uniform(div_small(t_begin, p.page_tiles, p.page_rcp)) : 0;
+        auto entry = [&](int pg) { return paged && pg < p.max_blocks ? table_entry(table, pg) : -1; };
+        int ahead = entry(page + 1);
+        int to_load = n;  // tiles not yet asked for
+        int to_stop;      // of them, before the next special one
+        uint32_t at = lds0 + wave * 1024;
+        const uint32_t at_end = lds0 + F::kRing * 2 * kTensor;
+        i32x4_t kr, vr;
+        const int kstep = kTile * int(p.k_row) * 2, vstep = kTile * int(p.v_row) * 2;
+        const int whole = min(n, g.sk / kTile - t_begin);  // tiles with all 32 keys
+        auto aim = [&](int blk, int first) {  // resources of the tile `first` tiles into the page
+          const bool there = !paged || (blk >= 0 && blk < p.num_blocks);
+          const int done = n - to_load;
+          const int64_t row = paged ? int64_t(there ? blk : 0) * p.page + first * kTile
+                                    : fresh0 + int64_t(t_begin + done) * kTile;
+          const int rows = !there || to_load <= 0 ? 0
+                           : done < whole         ? kTile
+                                                  : g.sk - (t_begin + done) * kTile;
+          kr = raw_rsrc(p.k + row * p.k_row + head * p.k_head, tensor_bytes(rows, p.k_row));
+          vr = raw_rsrc(p.v + row * p.v_row + head * p.v_head, tensor_bytes(rows, p.v_row));
+          to_stop = paged ? p.page_tiles - first : 1 << 30;
+          to_stop = to_load <= 0 ? 1 << 30 : min(to_stop, done < whole ? whole - done : to_load);
+        };
+        int in_page = t_begin - page * p.page_tiles, blk = entry(page);
+        aim(blk, in_page);
+        auto load = [&] {  // the next tile's two loads, and where the one after lies
+          uint32_t m0;
+          asm volatile(
+              "s_mov_b32 %0, m0\n\t"
+              "s_mov_b32 m0, %3\n\t"
+              "s_nop 0\n\t"
+              "buffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
+              "s_add_u32 m0, m0, %6\n\t"
+              "s_nop 0\n\t"
+              "buffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
+              "s_mov_b32 m0, %0"
+              : "=&s"(m0)
+              : "v"(kvoff), "v"(vvoff), "s"(at), "s"(kr), "s"(vr), "n"(kTensor)
+              : "memory", "scc");
+          at += 2 * kTensor;
+          if (at >= at_end) at -= F::kRing * 2 * kTensor;
+          --to_load;
+          --to_stop;
+          const uint64_t ka = (uint64_t(uint32_t(kr[1])) << 32 | uint32_t(kr[0])) + uint32_t(kstep);
+          const uint64_t va = (uint64_t(uint32_t(vr[1])) << 32 | uint32_t(vr[0])) + uint32_t(vstep);
+          kr[0] = int(uint32_t(ka));
+          kr[1] = int(uint32_t(ka >> 32));
+          vr[0] = int(uint32_t(va));
+          vr[1] = int(uint32_t(va >> 32));
+        };
+        auto steer = [&] {  // a new page, the ragged tile, or the end (rows 0: zeros)
+          if (__builtin_expect(to_stop > 0, 1)) return;
+          in_page = t_begin + (n - to_load) - page * p.page_tiles;
+          if (paged && in_page >= p.page_tiles) {
+            in_page -= p.page_tiles;
+            ++page;
+            blk = ahead;
+            ahead = entry(page + 1);
+            smem_drain();
+          }
+          aim(blk, in_page);
+        };
+        constexpr int kNewer = 2 * (F::kRing - 4);  // loads of the tiles past the next three
+#pragma unroll 1
+        for (int i = 0; i < F::kRing - 1; ++i) {
+          load();
+          steer();
+        }
+        wait_loads<kNewer>();
+        pf_barrier();
+        read_k(k, smem, la);
+        lds_done();
+        if (later) pf_barrier();
+        f32x4_t sl[NCB][2];
+        u32x4_t v[8] = {}, pb[NCB] = {};  // (nothing to weigh in the first turn)
+        // Tiles that every column sees whole, as i.  (Tiles that none of a
+        // wave's columns sees are attended with every weight 0.)
+        const int full0 = (max(c.full_lo, 0) + kTile - 1) / kTile - t_begin;
+        const int full1 = c.full_hi / kTile - t_begin;
+        int always = 1;
+        asm volatile("" : "+s"(always));
+        for (int i = 0; i <= n; ++i) {
+          // The next tile's K and this one's V operands come in under the two
+          // products, as these let go of the ones before.
+          const char* vt = smem + (i & (F::kRing - 1)) * (2 * kTensor) + kTensor;
+          const char* next = smem + ((i + 1) & (F::kRing - 1)) * (2 * kTensor);
+          __builtin_amdgcn_s_setprio(1);
+          // (the opaque test, always true, only keeps the two products apart:
+          // one block would be scheduled as a single chain)
+          if (always) {
+            load();
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int cb = 0; cb < NCB; ++cb)
+                  sl[cb][h] = mfma_bf16(k[h][d], q[cb][d],
+                                        d == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sl[cb][h]);
+                k[h][d] = read_k1(next, la, h, d);
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              __builtin_amdgcn_sched_group_barrier(0x008, NCB, 0);  // MFMA
+              __builtin_amdgcn_sched_group_barrier(0x004, 2, 0);    // SALU
+              __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);    // LDS read
+            }
+          }
+#pragma unroll
+          for (int jj = 0; jj < 8; ++jj) {
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb)
+              st.o[cb][jj] = mfma_bf16(v[jj], pb[cb], st.o[cb][jj]);
+            v[jj] = read_v1(vt, la, jj);
+          }
+#pragma unroll
+          for (int jj = 0; jj < 8; ++jj) {
+            __builtin_amdgcn_sched_group_barrier(0x008, NCB, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);    // VALU: addresses
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);    // LDS reads
+          }
+          __builtin_amdgcn_s_setprio(0);
+          __builtin_amdgcn_sched_barrier(0);
+          pf_barrier();
+          __builtin_amdgcn_sched_barrier(0);
+          if (__builtin_expect(i < n, 1)) {
+            steer();
+            const bool masked = i < full0 || i >= full1;
+            if (__builtin_expect(masked, 0)) odd |= take_out_not_finite(v);
+            weights<NCB, MODE>(p, c, st, sl, (t_begin + i) * kTile, lg, cs, masked, pb);
+            wait_loads<kNewer>();
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          pf_barrier();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (!later) pf_barrier();
+        wait_loads<0>();
       } else {
         // A stage holds kSub tiles, each K then V; every wave issues an equal
         // part of its loads and attends kSub / KW of its tiles.  One barrier a
@@ -890,8 +1114,8 @@ __global__ void __launch_bounds__(64 * NW)
           for (int i = 0; i < kPer; ++i) {
             const int m = m0 + i;
             const int row = 4 * m + (lane >> 4);
-            dma_to_lds_cached(r, row * row_bytes + (((lane & 15) ^ (row & 15)) << 4),
-                              at + m * 1024);
+            const int swz = tensor ? v_swizzle(row) : k_swizzle(row);
+            dma_to_lds_cached(r, row * row_bytes + (((lane & 15) ^ swz) << 4), at + m * 1024);
           }
         };
 #pragma unroll
@@ -914,8 +1138,7 @@ __global__ void __launch_bounds__(64 * NW)
             f32x4_t sl[NCB][2];
             u32x4_t v[8], pb[NCB];
             if (active) {
-#pragma unroll
-              for (int jj = 0; jj < 8; ++jj) v[jj] = read_v(vt, la, jj);
+              read_v(v, vt, la);
               logits<NCB>(k, q, sl);
             }
             if (last) {
@@ -929,7 +1152,8 @@ __global__ void __launch_bounds__(64 * NW)
             }
             if (active) {
               weights<NCB, MODE>(p, c, st, sl, j0, lg, cs, masked, pb);
-              weigh_tile<NCB>(st, v, pb, masked, odd);
+              if (masked) odd |= take_out_not_finite(v);
+              weigh<NCB>(st, v, pb);
             }
           }
         }
@@ -944,6 +1168,8 @@ __global__ void __launch_bounds__(64 * NW)
           add_not_finite<NCB>(p, c, st, src.v, src.rows, j0, lg);
         }
       }
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) st.l[cb] = rows4_sum(st.l[cb]);
       // Join the tile phases: the waves of phase 0 take in the others' states.
       if (phases > 1) {
         const int owners = NW / phases;
@@ -961,20 +1187,17 @@ __global__ void __launch_bounds__(64 * NW)
         if (seg0 == 0 && seg1 == tiles) {
 #pragma unroll
           for (int cb = 0; cb < NCB; ++cb) {
-            if (tcol[cb] >= p.tokens_per_block || b0 + tcol[cb] > tmax) continue;
-            const float inv = st.l[cb][0] != 0.f ? 1.f / st.l[cb][0] : 0.f;
-            uint32_t o[16];
+            const ColumnOf co = column_of(p, col0, cb);
+            if (co.token >= p.tokens_per_block || b0 + co.token > tmax) continue;
+            const float inv = st.l[cb] != 0.f ? 1.f / st.l[cb] : 0.f;
+            uint16_t* dst = p.out + int64_t(g.q0 + b0 + co.token) * p.o_st +
+                            int64_t(head * p.group + co.head) * p.o_sh + 4 * lg;
 #pragma unroll
             for (int jj = 0; jj < 8; ++jj) {
-              o[2 * jj] = pack_bf16x2_fast(st.o[cb][jj][0] * inv, st.o[cb][jj][1] * inv);
-              o[2 * jj + 1] = pack_bf16x2_fast(st.o[cb][jj][2] * inv, st.o[cb][jj][3] * inv);
+              const f32x4_t o = st.o[cb][jj] * inv;
+              *reinterpret_cast<u32x2_t*>(dst + 16 * jj) =
+                  u32x2_t{pack_bf16x2_fast(o[0], o[1]), pack_bf16x2_fast(o[2], o[3])};
             }
-            uint16_t* dst = p.out + int64_t(g.q0 + b0 + tcol[cb]) * p.o_st +
-                            int64_t(head * p.group + gcol[cb]) * p.o_sh + 32 * lg;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              reinterpret_cast<u32x4_t*>(dst)[i] =
-                  u32x4_t{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
           }
         } else {
           // Slot 2 share + 1: the piece that begins its item; else 2 share.
@@ -982,12 +1205,14 @@ __global__ void __launch_bounds__(64 * NW)
           const int64_t cols = int64_t(p.heads_per_wg) * F::kColumns;
 #pragma unroll
           for (int cb = 0; cb < NCB; ++cb) {
-            if (tcol[cb] >= p.tokens_per_block || b0 + tcol[cb] > tmax) continue;
+            const ColumnOf co = column_of(p, col0, cb);
+            if (co.token >= p.tokens_per_block || b0 + co.token > tmax) continue;
             const int64_t col = slot * cols + hs * F::kColumns + (cw * NCB + cb) * 16 + lm;
-            float* dst = p.part_o + col * kD + 32 * lg;
+            float* dst = p.part_o + col * kD + 4 * lg;
 #pragma unroll
-            for (int jj = 0; jj < 8; ++jj) reinterpret_cast<f32x4_t*>(dst)[jj] = st.o[cb][jj];
-            if (lg == 0) p.part_ml[col] = float2{st.mu[cb], st.l[cb][0]};
+            for (int jj = 0; jj < 8; ++jj)
+              *reinterpret_cast<f32x4_t*>(dst + 16 * jj) = st.o[cb][jj];
+            if (lg == 0) p.part_ml[col] = float2{st.mu[cb], st.l[cb]};
           }
         }
       }
@@ -1331,6 +1556,7 @@ extern "C" int kvc_scored_attention(
   p.heads = int(num_heads);
   p.kv_heads = int(num_kv_heads);
   p.group = int(num_heads / num_kv_heads);
+  p.group_rcp = 1.f / float(p.group);
   const int64_t max_keys = fresh ? num_fresh_rows : max_blocks_per_seq * page_size;
   hipStream_t st = as_stream(stream);
   if (num_decode_rows > 0) {
@@ -1427,6 +1653,7 @@ extern "C" int kvc_tree_attention(
   p.heads = int(num_heads);
   p.kv_heads = int(num_kv_heads);
   p.group = int(num_heads / num_kv_heads);
+  p.group_rcp = 1.f / float(p.group);
   hipStream_t st = as_stream(stream);
   if (alibi_slopes != nullptr || window > 0) {
     int32_t* depth = reinterpret_cast<int32_t*>(
