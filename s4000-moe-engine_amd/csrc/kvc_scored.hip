@@ -39,6 +39,7 @@ constexpr int kD = 128;
 constexpr int kTile = 32;
 constexpr int kTensor = kTile * kD * 2;  // one K or V tile of a head: 8 KiB
 constexpr uint32_t kLazyBits = 0x4380u;  // bf16 2^8: a weight past it moves the running reference
+constexpr int kNoKey = 1 << 30;  // a key position that no column sees
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint32_t kOnes2 = 0x3F803F80u;  // two bf16 ones
 
@@ -176,7 +177,6 @@ struct Columns {
   int pre;                // two-way prefix
   int p0, sk, sq;         // p0: keys before the sequence's queries
   int full_lo, full_hi;   // a tile inside these keys needs no mask
-  int any_lo, any_hi;     // a tile outside them is seen by no column
 };
 
 // The token, inside its block, and the query head of column col0 + 16 cb + lm.
@@ -715,17 +715,14 @@ struct Form {
   static constexpr bool kPrivate = KW == NW;
   static constexpr int kColWaves = kPrivate ? 1 : NW / KW;
   static constexpr int kColumns = 16 * NCB * kColWaves;  // per kv head
-  static constexpr int kSub = kPrivate ? NW : KW == 1 ? 8 : 4;  // tiles per stage
-  static constexpr int kStage = kSub * 2 * kTensor;
-  static constexpr int kStages = kPrivate || KW == 1 ? 1 : 2;
-  static constexpr bool kTurns = KW == 1;
-  static constexpr int kRing = 8;  // tiles, taking turns
+  static constexpr int kSlots = 8;  // tiles held: one a wave, or a ring
+  static constexpr int kSlotBytes = kSlots * 2 * kTensor;
   // waves that hand their state to another: [wave][34 NCB floats][64 lanes]
   static constexpr int kStateBytes = 34 * NCB * 256;
   static constexpr int kJoinBytes =
       kPrivate ? (NW - 1) * kStateBytes : (NW - kColWaves) * kStateBytes;
-  static constexpr int kLds =
-      kStage * kStages > kJoinBytes ? kStage * kStages : kJoinBytes;
+  static constexpr int kLds = kSlotBytes > kJoinBytes ? kSlotBytes : kJoinBytes;
+  static_assert(NW == kSlots && (kPrivate || KW <= 2));
   static_assert(kLds <= 160 * 1024, "one workgroup per CU");
 };
 
@@ -845,17 +842,13 @@ __global__ void __launch_bounds__(64 * NW)
       {
         const int ta = min(b0 + wave_t0, tmax), tb = min(b0 + wave_t1, tmax);
         if (p.mask == nullptr) {
-          c.any_lo = p.window > 0 ? p0 + ta + 1 - p.window : 0;
           c.full_lo = p.window > 0 ? p0 + tb + 1 - p.window : 0;
           // A two-way prefix makes |p - j| bend inside it.
           c.full_hi = min(g.sk, MODE == kDistance || MODE == kCapDistance
                                     ? p0 + ta + 1 : max(p0 + ta + 1, pre));
-          c.any_hi = min(g.sk, max(p0 + tb + 1, pre));
         } else {
-          c.any_lo = p.window > 0 ? p0 - p.window : 0;
           c.full_lo = p.window > 0 ? p0 + g.sq - p.window : 0;  // depth < sq
           c.full_hi = p0;
-          c.any_hi = g.sk;
         }
       }
       u32x4_t q[NCB][4];
@@ -864,20 +857,20 @@ __global__ void __launch_bounds__(64 * NW)
 #pragma unroll
         for (int d = 0; d < 4; ++d)
           q[cb][d] = *reinterpret_cast<const u32x4_t*>(qp[cb] + 32 * d + 8 * lg);
-      // Every compiler-tracked load is back before the counted ones start.
+      // The queries are waited for once the first tiles are on their way: the
+      // compiler's wait for them covers those too.
+      auto settle = [&] {
 #pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        if constexpr (MODE == kDistance || MODE == kCapDistance)
-          asm volatile("" : "+v"(c.place[cb]), "+v"(c.slope2[cb]));
+        for (int cb = 0; cb < NCB; ++cb) {
+          if constexpr (MODE == kDistance || MODE == kCapDistance)
+            asm volatile("" : "+v"(c.place[cb]), "+v"(c.slope2[cb]));
 #pragma unroll
-        for (int d = 0; d < 4; ++d) asm volatile("" : "+v"(q[cb][d]));
-      }
-      wait_loads<0>();
-
+          for (int d = 0; d < 4; ++d) asm volatile("" : "+v"(q[cb][d]));
+        }
+      };
       State<NCB> st;
       reset<NCB>(st, mu0);
       const int t_begin = range.t0 + seg0, t_end = range.t0 + seg1;
-      u32x4_t k[2][4];
       bool odd = false;  // a masked tile held infinities or NaN
       if constexpr (F::kPrivate) {
         // Wave-private slots: K 8 KiB, V 8 KiB.  The next tile's K load goes
@@ -903,6 +896,8 @@ __global__ void __launch_bounds__(64 * NW)
           issue_k(src);
           issue_v(src);
         }
+        settle();
+        u32x4_t k[2][4];
         for (; t < t_end; t += phases) {
           const bool more = t + phases < t_end;
           const int tn = more ? t + phases : t;
@@ -928,15 +923,19 @@ __global__ void __launch_bounds__(64 * NW)
           if (masked) odd |= take_out_not_finite(v);
           weigh<NCB>(st, v, pb);
         }
-      } else if constexpr (F::kTurns) {
+      } else {
         // The waves take turns: while the first four (one on each SIMD) run
         // their products and read operands, the other four run a softmax, and
         // a barrier swaps them, so that matrix and vector units work side by
-        // side.  Products of a turn: S of tile i and O of tile i - 1.  Tile u
-        // is last read in the later half's turn u, so that its slot is loaded
-        // again a turn on, kRing - 1 tiles ahead.
+        // side.  Products of a turn: S of the wave's tile of step i and O of
+        // its tile of step i - 1.  A step has KW tiles: one that all waves
+        // attend, or one for each half.  Step s is last read in the later
+        // half's turn s, so its slots are loaded again a turn on, kRing - 1
+        // steps ahead.
+        constexpr int kRing = F::kSlots / KW;
         const bool later = wave >= NW / 2;
-        const int n = t_end - t_begin;
+        const int n = t_end - t_begin, steps = (n + KW - 1) / KW;
+        const int own = KW == 2 && later ? 1 : 0;  // the wave's tile of a step
         // A wave's part of a tile: rows 4 wave .. + 3 of K and of V.
         const int drow = 4 * wave + (lane >> 4);
         const int kvoff = drow * int(p.k_row) * 2 + (((lane & 15) ^ k_swizzle(drow)) << 4);
@@ -948,15 +947,15 @@ __global__ void __launch_bounds__(64 * NW)
         const int32_t* table = p.tables + int64_t(w.seq) * p.bt_stride;
         int page = paged ? uniform(div_small(t_begin, p.page_tiles, p.page_rcp)) : 0;
         auto entry = [&](int pg) { return paged && pg < p.max_blocks ? table_entry(table, pg) : -1; };
-        int ahead = entry(page + 1);
+        int blk = entry(page), ahead = entry(page + 1);
         int to_load = n;  // tiles not yet asked for
         int to_stop;      // of them, before the next special one
         uint32_t at = lds0 + wave * 1024;
-        const uint32_t at_end = lds0 + F::kRing * 2 * kTensor;
+        const uint32_t at_end = lds0 + F::kSlots * 2 * kTensor;
         i32x4_t kr, vr;
         const int kstep = kTile * int(p.k_row) * 2, vstep = kTile * int(p.v_row) * 2;
         const int whole = min(n, g.sk / kTile - t_begin);  // tiles with all 32 keys
-        auto aim = [&](int blk, int first) {  // resources of the tile `first` tiles into the page
+        auto aim = [&](int first) {  // resources of the tile `first` tiles into the page
           const bool there = !paged || (blk >= 0 && blk < p.num_blocks);
           const int done = n - to_load;
           const int64_t row = paged ? int64_t(there ? blk : 0) * p.page + first * kTile
@@ -969,8 +968,7 @@ __global__ void __launch_bounds__(64 * NW)
           to_stop = paged ? p.page_tiles - first : 1 << 30;
           to_stop = to_load <= 0 ? 1 << 30 : min(to_stop, done < whole ? whole - done : to_load);
         };
-        int in_page = t_begin - page * p.page_tiles, blk = entry(page);
-        aim(blk, in_page);
+        aim(t_begin - page * p.page_tiles);
         auto load = [&] {  // the next tile's two loads, and where the one after lies
           uint32_t m0;
           asm volatile(
@@ -986,7 +984,7 @@ __global__ void __launch_bounds__(64 * NW)
               : "v"(kvoff), "v"(vvoff), "s"(at), "s"(kr), "s"(vr), "n"(kTensor)
               : "memory", "scc");
           at += 2 * kTensor;
-          if (at >= at_end) at -= F::kRing * 2 * kTensor;
+          if (at >= at_end) at -= F::kSlots * 2 * kTensor;
           --to_load;
           --to_stop;
           const uint64_t ka = (uint64_t(uint32_t(kr[1])) << 32 | uint32_t(kr[0])) + uint32_t(kstep);
@@ -998,45 +996,58 @@ __global__ void __launch_bounds__(64 * NW)
         };
         auto steer = [&] {  // a new page, the ragged tile, or the end (rows 0: zeros)
           if (__builtin_expect(to_stop > 0, 1)) return;
-          in_page = t_begin + (n - to_load) - page * p.page_tiles;
-          if (paged && in_page >= p.page_tiles) {
-            in_page -= p.page_tiles;
+          int first = t_begin + (n - to_load) - page * p.page_tiles;
+          if (paged && first >= p.page_tiles) {
+            first -= p.page_tiles;
             ++page;
             blk = ahead;
             ahead = entry(page + 1);
             smem_drain();
           }
-          aim(blk, in_page);
+          aim(first);
         };
-        constexpr int kNewer = 2 * (F::kRing - 4);  // loads of the tiles past the next three
+        // Loads a wave may still have on the way when what the next turns read
+        // (V of step i + 1, K of step i + 2) has to be in place: waited for
+        // ahead of the barrier before the first half's turn.  The later half
+        // does so after its softmax, a turn early, where the ring is deep
+        // enough for that.
+        constexpr bool kEarly = KW == 1;
+        constexpr int kNewer = 2 * KW * (kRing - (kEarly ? 4 : 3));
 #pragma unroll 1
-        for (int i = 0; i < F::kRing - 1; ++i) {
+        for (int i = 0; i < KW * (kRing - 1); ++i) {
           load();
           steer();
         }
+        settle();
         wait_loads<kNewer>();
         pf_barrier();
-        read_k(k, smem, la);
+        u32x4_t k[2][4];
+        read_k(k, smem + own * 2 * kTensor, la);
         lds_done();
         if (later) pf_barrier();
         f32x4_t sl[NCB][2];
         u32x4_t v[8] = {}, pb[NCB] = {};  // (nothing to weigh in the first turn)
-        // Tiles that every column sees whole, as i.  (Tiles that none of a
-        // wave's columns sees are attended with every weight 0.)
+        // Tiles that every column sees whole, counted from t_begin.  (Tiles
+        // that none of a wave's columns sees are attended with every weight 0.)
         const int full0 = (max(c.full_lo, 0) + kTile - 1) / kTile - t_begin;
         const int full1 = c.full_hi / kTile - t_begin;
         int always = 1;
         asm volatile("" : "+s"(always));
-        for (int i = 0; i <= n; ++i) {
+        for (int i = 0; i <= steps; ++i) {
           // The next tile's K and this one's V operands come in under the two
           // products, as these let go of the ones before.
-          const char* vt = smem + (i & (F::kRing - 1)) * (2 * kTensor) + kTensor;
-          const char* next = smem + ((i + 1) & (F::kRing - 1)) * (2 * kTensor);
+          const int u = KW * i + own;
+          const char* vt = smem + (u & (F::kSlots - 1)) * (2 * kTensor) + kTensor;
+          const char* next = smem + ((u + KW) & (F::kSlots - 1)) * (2 * kTensor);
           __builtin_amdgcn_s_setprio(1);
           // (the opaque test, always true, only keeps the two products apart:
           // one block would be scheduled as a single chain)
           if (always) {
             load();
+            if constexpr (KW == 2) {
+              steer();
+              load();
+            }
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
 #pragma unroll
@@ -1070,93 +1081,25 @@ __global__ void __launch_bounds__(64 * NW)
           }
           __builtin_amdgcn_s_setprio(0);
           __builtin_amdgcn_sched_barrier(0);
+          if constexpr (!kEarly)
+            if (later) wait_loads<kNewer>();
           pf_barrier();
           __builtin_amdgcn_sched_barrier(0);
-          if (__builtin_expect(i < n, 1)) {
+          if (__builtin_expect(i < steps, 1)) {
             steer();
-            const bool masked = i < full0 || i >= full1;
+            const bool masked = u < full0 || u >= full1;
             if (__builtin_expect(masked, 0)) odd |= take_out_not_finite(v);
-            weights<NCB, MODE>(p, c, st, sl, (t_begin + i) * kTile, lg, cs, masked, pb);
-            wait_loads<kNewer>();
+            // (a step's second tile may lie past the segment)
+            const bool gone = KW == 2 && u >= n;
+            weights<NCB, MODE>(p, c, st, sl, gone ? kNoKey : (t_begin + u) * kTile, lg, cs,
+                               masked || gone, pb);
+            if (kEarly || !later) wait_loads<kNewer>();
           }
           __builtin_amdgcn_sched_barrier(0);
           pf_barrier();
           __builtin_amdgcn_sched_barrier(0);
         }
         if (!later) pf_barrier();
-        wait_loads<0>();
-      } else {
-        // A stage holds kSub tiles, each K then V; every wave issues an equal
-        // part of its loads and attends kSub / KW of its tiles.  One barrier a
-        // step: each wave has its last tile's V in registers (so the stage is
-        // free for the load kStages steps ahead) and its loads of the next
-        // stage are back.  K operands are read a tile ahead, V operands before
-        // the tile's first product, so the LDS latency of both lies under
-        // MFMAs and the softmax.
-        constexpr int kPer = 16 * F::kSub / NW;  // loads a wave issues per stage
-        static_assert(8 % kPer == 0, "a wave's loads lie in one tensor");
-        const int sub = kPer * wave / 16, tensor = (kPer * wave / 8) & 1, m0 = kPer * wave & 7;
-        const int steps = (t_end - t_begin + F::kSub - 1) / F::kSub;
-        auto entry = [&](int step) {
-          const int t = t_begin + step * F::kSub + sub;
-          return t < t_end ? page_entry(p, w.seq, t) : -1;
-        };
-        auto issue = [&](int step, int blk) {
-          const int t = t_begin + step * F::kSub + sub;
-          TileSource src{p.k, p.v, 0};
-          if (t < t_end) src = tile_source(p, fresh0, g.sk, head, t, blk);
-          const i32x4_t r = tensor ? raw_rsrc(src.v, tensor_bytes(src.rows, p.v_row))
-                                   : raw_rsrc(src.k, tensor_bytes(src.rows, p.k_row));
-          const uint32_t at =
-              lds0 + (step % F::kStages) * F::kStage + (2 * sub + tensor) * kTensor;
-          const int row_bytes = int(tensor ? p.v_row : p.k_row) * 2;
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const int m = m0 + i;
-            const int row = 4 * m + (lane >> 4);
-            const int swz = tensor ? v_swizzle(row) : k_swizzle(row);
-            dma_to_lds_cached(r, row * row_bytes + (((lane & 15) ^ swz) << 4), at + m * 1024);
-          }
-        };
-#pragma unroll
-        for (int s = 0; s < F::kStages; ++s) issue(s, entry(s));
-        int blk = entry(F::kStages);
-        wait_loads<kPer*(F::kStages - 1)>();
-        pf_barrier();
-        read_k(k, smem + phase * 2 * kTensor, la);
-        for (int step = 0; step < steps; ++step) {
-          const char* stage = smem + (step % F::kStages) * F::kStage;
-#pragma unroll
-          for (int u = 0; u < F::kSub / KW; ++u) {
-            const bool last = u == F::kSub / KW - 1;
-            const char* kt = stage + (u * KW + phase) * 2 * kTensor;
-            const char* vt = kt + kTensor;
-            const int t = t_begin + step * F::kSub + u * KW + phase;
-            const int j0 = t * kTile;
-            const bool active = t < t_end && j0 < c.any_hi && j0 + kTile > c.any_lo;
-            const bool masked = j0 < c.full_lo || j0 + kTile > c.full_hi;
-            f32x4_t sl[NCB][2];
-            u32x4_t v[8], pb[NCB];
-            if (active) {
-              read_v(v, vt, la);
-              logits<NCB>(k, q, sl);
-            }
-            if (last) {
-              wait_loads<kPer*(F::kStages - 2)>();
-              pf_barrier();
-              issue(step + F::kStages, blk);
-              blk = entry(step + F::kStages + 1);
-              read_k(k, smem + ((step + 1) % F::kStages) * F::kStage + phase * 2 * kTensor, la);
-            } else {
-              read_k(k, kt + KW * 2 * kTensor, la);
-            }
-            if (active) {
-              weights<NCB, MODE>(p, c, st, sl, j0, lg, cs, masked, pb);
-              if (masked) odd |= take_out_not_finite(v);
-              weigh<NCB>(st, v, pb);
-            }
-          }
-        }
         wait_loads<0>();
       }
 
@@ -1377,7 +1320,7 @@ int launch_form(const ScoredParams& p, const Plan& pl, hipStream_t st) {
   switch (pl.form) {
     case 0: return launch_one<8, 1, 8, MODE>(p, pl.grid, st);
     case 1: return launch_one<8, 2, 8, MODE>(p, pl.grid, st);
-    case 2: return launch_one<8, 2, 4, MODE>(p, pl.grid, st);
+    case 2: return launch_one<8, 1, 2, MODE>(p, pl.grid, st);
     case 3: return launch_one<8, 2, 2, MODE>(p, pl.grid, st);
     default: return launch_one<8, 2, 1, MODE>(p, pl.grid, st);
   }
