@@ -157,6 +157,10 @@ class _NoHostPath:
     time a decode step)."""
     decode = staticmethod(lambda *_: None)
     rope = staticmethod(lambda *_: None)
+    scored = staticmethod(lambda *_: None)
+    tree = staticmethod(lambda *_: None)
+    mrope = staticmethod(lambda *_: None)
+    commit = staticmethod(lambda *_: None)
 
 
 _host = None
@@ -208,6 +212,13 @@ def call(name: str, *args) -> int:
         msg = _lib.kvc_last_error().decode(errors="replace")
         raise _ERRORS.get(rc, RuntimeError)(msg or f"{name} failed with status {rc}")
     return rc
+
+
+def is_current(t) -> bool:
+    """t is a tensor on the current GPU (the native host path makes its
+    launches there)."""
+    return isinstance(t, torch.Tensor) and t.is_cuda \
+        and t.get_device() == torch.cuda.current_device()
 
 
 def call_on(t: torch.Tensor, name: str, *args) -> int:

@@ -92,6 +92,13 @@ def scored_attention(q, k_cache, v_cache, *, scale, block_tables=None, num_decod
     softcap * tanh(score / softcap) if softcap > 0, then minus
     alibi_slopes[h] * |p - j| (fp32 [H]) if given.  Returns out [T, H, 128]
     bf16; a query that sees no key gives 0."""
+    if nat.is_current(q):
+        done = nat.host().scored(q, k_cache, v_cache, block_tables, num_decode_rows,
+                                 decode_context_lens, cu_seqlens_q, cu_seqlens_k,
+                                 cu_seqlens_q_list, cu_seqlens_k_list, k, v, softcap,
+                                 alibi_slopes, window, prefix_lens, scale, nat.stream_of(q))
+        if done is not None:
+            return done
     fresh = block_tables is None
     if fresh and (k is None or v is None):
         raise ValueError("without block_tables the keys come from k/v")

@@ -49,6 +49,12 @@ def tree_attention(q, k_cache, v_cache, block_tables, context_lens, tree_mask, s
     window as in scored_attention, with the token's depth (bits in its mask,
     less one) for its distance from the context.  Returns out [T, H, 128];
     a token that sees no key gives 0."""
+    if nat.is_current(q):
+        done = nat.host().tree(q, k_cache, v_cache, block_tables, context_lens, tree_mask, scale,
+                               cu_seqlens_q, max_seqlen_q, softcap, alibi_slopes, window,
+                               nat.stream_of(q))
+        if done is not None:
+            return done
     q = check_queries(q, k_cache.size(2), "tree attention")
     T, num_heads, head_dim = q.shape
     block_tables = check_pool(q, k_cache, v_cache, block_tables)
@@ -98,6 +104,9 @@ def commit_tree_path(kv_cache, block_tables, context_lens, paths, path_lens):
     (scales, side rows); paths int32 [batch, most], a path strictly
     increasing (tree tokens come after their parents): it ends at the first
     entry that is not."""
+    if nat.is_current(kv_cache) and nat.host().commit(kv_cache, block_tables, context_lens, paths,
+                                                      path_lens, nat.stream_of(kv_cache)):
+        return
     if kv_cache.dim() < 4:
         raise ValueError("pool must be [2, layers, blocks, page, ...]")
     if not kv_cache.is_contiguous():

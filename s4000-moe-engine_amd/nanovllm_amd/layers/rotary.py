@@ -119,6 +119,12 @@ def pair_axes(sections: tuple, interleaved: bool, half: int = 64) -> np.ndarray:
     return axes
 
 
+@functools.lru_cache(maxsize=64)
+def _pair_axes_at(sections: tuple, interleaved: bool) -> tuple[np.ndarray, int]:
+    axes = pair_axes(sections, interleaved)
+    return axes, axes.ctypes.data
+
+
 def qk_norm_mrope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None,
                         positions: torch.Tensor, cos_sin_cache: torch.Tensor, sections,
                         interleaved: bool = False, q_norm_weight: torch.Tensor | None = None,
@@ -130,13 +136,19 @@ def qk_norm_mrope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None
     (`kvc_qk_norm_mrope_store`; time, height and width of images and video):
     positions [A, N], sections the rotary pairs of each axis (64 in all), in
     runs or interleaved (pair_axes).  fp32 throughout, rounded to bf16 once."""
+    _, axes_at = _pair_axes_at(tuple(sections), bool(interleaved))
+    if q_out is None and nat.is_current(q):
+        done = nat.host().mrope(q, k, v, positions, cos_sin_cache, axes_at, len(sections),
+                                q_norm_weight, k_norm_weight, eps, k_cache, v_cache, slot_mapping,
+                                return_k, nat.stream_of(q))
+        if done is not None:
+            return done
     N, H, D = q.shape
     KVH = k.size(1)
     if D != 128 or k.size(2) != D:
         raise ValueError("qk_norm_mrope_store requires head_dim=128")
     if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16:
         raise ValueError("q and k must be bf16")
-    axes = pair_axes(tuple(sections), bool(interleaved))
     if positions.ndim != 2 or positions.size(0) != len(sections) or positions.size(1) != N:
         raise ValueError(f"positions must be [{len(sections)}, {N}], one row per axis")
     if k.size(0) != N:
@@ -182,7 +194,7 @@ def qk_norm_mrope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None
         q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
         nat.ptr(v), v.stride(0) if v is not None else 0, v.stride(1) if v is not None else 0,
         N, H, KVH, D, positions.data_ptr(), positions.stride(0), positions.element_size(),
-        len(sections), axes.ctypes.data, nat.ptr(qw), nat.ptr(kw), float(eps),
+        len(sections), axes_at, nat.ptr(qw), nat.ptr(kw), float(eps),
         cos_sin_cache.data_ptr(), cos_sin_cache.size(0),
         q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
         nat.ptr(k_out), k_out.stride(0) if k_out is not None else 0,
