@@ -87,6 +87,7 @@ struct ScoredParams {
   int tokens_per_block;
   int lane_plan;  // the plan walks sequences across lanes (else blocks)
   int min_share;
+  int whole;  // items are not cut: a share counts items
   int4* rec;  // per share: the item it begins and leaves unfinished
   float* part_o;
   float2* part_ml;
@@ -534,26 +535,30 @@ struct Where {
 };
 
 __device__ __forceinline__ int block_cost(const ScoredParams& p, const SeqGeo& g, int pre, int c) {
+  if (p.whole) return 1;
   const TileRange r = block_tiles(p, g, pre, c);
   return r.t1 - r.t0 + kItemCost;
 }
 
 // Cost and column blocks of lane's sequence (lane plan).
-__device__ __forceinline__ void lane_seq(const ScoredParams& p, int i, int& cost, int& nb) {
-  cost = nb = 0;
-  if (i >= p.batch) return;
-  const SeqGeo g = load_seq<false>(p, i);
-  const int pre = p.prefix != nullptr ? p.prefix[i] : 0;
-  nb = num_blocks_of(p, g.sq);
+__device__ __forceinline__ int lane_seq(const ScoredParams& p, int i, SeqGeo& g, int& pre) {
+  g = SeqGeo{0, 0, 0};
+  pre = 0;
+  if (i >= p.batch) return 0;
+  g = load_seq<false>(p, i);
+  pre = p.prefix != nullptr ? p.prefix[i] : 0;
+  const int nb = num_blocks_of(p, g.sq);
+  int cost = 0;
   for (int c = 0; c < nb; ++c) cost += block_cost(p, g, pre, c);
-  cost *= p.head_groups;
+  return cost * p.head_groups;
 }
 
 // The same for a wave-uniform sequence, its blocks across the lanes.
-__device__ __forceinline__ int wave_seq(const ScoredParams& p, int i, int lane, int& nb) {
-  const SeqGeo g = load_seq<true>(p, i);
-  const int pre = p.prefix != nullptr ? table_entry(p.prefix, i) : 0;
-  nb = num_blocks_of(p, g.sq);
+__device__ __forceinline__ int wave_seq(const ScoredParams& p, int i, int lane, SeqGeo& g,
+                                        int& pre) {
+  g = load_seq<true>(p, i);
+  pre = p.prefix != nullptr ? table_entry(p.prefix, i) : 0;
+  const int nb = num_blocks_of(p, g.sq);
   int cost = 0;
   for (int c = 0; c < nb; c += 64)
     cost += wave_sum(c + lane < nb ? block_cost(p, g, pre, c + lane) : 0);
@@ -565,38 +570,63 @@ __device__ __forceinline__ int first_lane(uint64_t m) { return __builtin_ctzll(m
 // Finds position `at` (share * size, size from the total) in the concatenated
 // items; false when it lies past the end.
 __device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int share, int shares,
-                                           Where& w, int& size) {
-  int total = 0, cost = 0, nb = 0;
+                                           Where& w, SeqGeo& g, int& pre, int& size) {
+  int total = 0, cost = 0;
+  SeqGeo mine = {0, 0, 0};  // lane_plan: this lane's sequence
+  int mine_pre = 0;
+  g = SeqGeo{0, 0, 0};
+  pre = 0;
+  if (p.whole && (p.batch == 1 || p.cu_q == nullptr)) {  // as many items in each sequence
+    g = load_seq<true>(p, 0);
+    const int n = num_blocks_of(p, g.sq);
+    const int each = n * p.head_groups;
+    w.total = each * p.batch;
+    size = (w.total + shares - 1) / shares;
+    const int64_t at = int64_t(share) * size;
+    if (at >= w.total) return false;
+    w.seq = p.batch == 1 ? 0 : int(at) / each;
+    if (w.seq != 0) g = load_seq<true>(p, w.seq);
+    if (p.prefix != nullptr) pre = table_entry(p.prefix, w.seq);
+    const int rem = int(at) - w.seq * each;
+    w.grp = rem / n;
+    w.block = rem - w.grp * n;
+    w.tile = 0;
+    return true;
+  }
   if (p.lane_plan) {
     for (int i = 0; i < p.batch; i += 64) {
-      lane_seq(p, i + lane, cost, nb);
+      cost = lane_seq(p, i + lane, mine, mine_pre);
       total += wave_sum(cost);
     }
   } else {
-    for (int i = 0; i < p.batch; ++i) total += wave_seq(p, i, lane, nb);
+    for (int i = 0; i < p.batch; ++i) total += wave_seq(p, i, lane, g, pre);
   }
   w.total = total;
-  size = max(p.min_share, (total + shares - 1) / shares);
+  size = max(p.whole ? 1 : p.min_share, (total + shares - 1) / shares);
   const int64_t at64 = int64_t(share) * size;
   if (at64 >= total) return false;
   const int at = int(at64);
   int acc = 0, seq = -1, start = 0;
   if (p.lane_plan) {
     for (int i = 0; i < p.batch; i += 64) {
-      if (p.batch > 64) lane_seq(p, i + lane, cost, nb);
+      if (p.batch > 64) cost = lane_seq(p, i + lane, mine, mine_pre);
       const int upto = wave_scan_add(cost);
       const uint64_t hit = __ballot(acc + upto > at);
       if (hit != 0) {
         const int l = first_lane(hit);
         seq = i + l;
         start = acc + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(cost, l);
+        g.q0 = __builtin_amdgcn_readlane(mine.q0, l);
+        g.sq = __builtin_amdgcn_readlane(mine.sq, l);
+        g.sk = __builtin_amdgcn_readlane(mine.sk, l);
+        pre = __builtin_amdgcn_readlane(mine_pre, l);
         break;
       }
       acc += __builtin_amdgcn_readlane(upto, 63);
     }
   } else {
     for (int i = 0; i < p.batch; ++i) {
-      cost = wave_seq(p, i, lane, nb);
+      cost = wave_seq(p, i, lane, g, pre);
       if (acc + cost > at) {
         seq = i;
         start = acc;
@@ -608,13 +638,18 @@ __device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int 
   if (seq < 0) return false;
   w.seq = seq;
   // Inside the sequence: head groups in turn, each over all column blocks.
-  const SeqGeo g = load_seq<true>(p, seq);
-  const int pre = p.prefix != nullptr ? table_entry(p.prefix, seq) : 0;
   const int n = num_blocks_of(p, g.sq);
+  const int rem = at - start;
+  if (n == 1) {
+    const int each = block_cost(p, g, pre, 0);
+    w.grp = rem / each;
+    w.block = 0;
+    w.tile = rem - w.grp * each;
+    return true;
+  }
   int each = 0;
   for (int c = 0; c < n; c += 64)
     each += wave_sum(c + lane < n ? block_cost(p, g, pre, c + lane) : 0);
-  const int rem = at - start;
   w.grp = rem / each;
   int left = rem - w.grp * each;
   for (int c = 0; c < n; c += 64) {
@@ -717,10 +752,10 @@ struct Form {
   static constexpr int kColumns = 16 * NCB * kColWaves;  // per kv head
   static constexpr int kSlots = 8;  // tiles held: one a wave, or a ring
   static constexpr int kSlotBytes = kSlots * 2 * kTensor;
-  // waves that hand their state to another: [wave][34 NCB floats][64 lanes]
-  static constexpr int kStateBytes = 34 * NCB * 256;
-  static constexpr int kJoinBytes =
-      kPrivate ? (NW - 1) * kStateBytes : (NW - kColWaves) * kStateBytes;
+  // A wave's state while tile phases are joined: [cb][8][64 lanes] of O, then
+  // [cb][64] of (reference, sum).
+  static constexpr int kStateBytes = NCB * (8 * 64 * 16 + 64 * 8);
+  static constexpr int kJoinBytes = KW > 1 ? NW * kStateBytes : 0;
   static constexpr int kLds = kSlotBytes > kJoinBytes ? kSlotBytes : kJoinBytes;
   static_assert(NW == kSlots && (kPrivate || KW <= 2));
   static_assert(kLds <= 160 * 1024, "one workgroup per CU");
@@ -728,33 +763,50 @@ struct Form {
 
 template <int NCB>
 __device__ __forceinline__ void put_state(char* at, const State<NCB>& st, int lane) {
-  float* f = reinterpret_cast<float*>(at) + lane;
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
 #pragma unroll
     for (int jj = 0; jj < 8; ++jj)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[(cb * 34 + jj * 4 + i) * 64] = st.o[cb][jj][i];
-    f[(cb * 34 + 32) * 64] = st.l[cb];
-    f[(cb * 34 + 33) * 64] = st.mu[cb];
+      *reinterpret_cast<f32x4_t*>(at + (cb * 8 + jj) * 1024 + lane * 16) = st.o[cb][jj];
+    *reinterpret_cast<float2*>(at + NCB * 8192 + cb * 512 + lane * 8) =
+        float2{st.mu[cb], st.l[cb]};
   }
 }
 
-template <int NCB>
-__device__ __forceinline__ void join_state(State<NCB>& st, const char* at, int lane) {
-  const float* f = reinterpret_cast<const float*>(at) + lane;
+// Join the states of kPhases waves, kept `step` apart: the wave of phase f
+// makes a kPhases-th of the rows of O^T and hands them on.
+template <int NCB, int kPhases, class Emit>
+__device__ __forceinline__ void join_states(const char* at, int step, int f, int lane,
+                                            const Emit& emit) {
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
-    const float l = f[(cb * 34 + 32) * 64], mu = f[(cb * 34 + 33) * 64];
-    const float top = fmaxf(mu, st.mu[cb]);
-    const float a = __builtin_amdgcn_exp2f(st.mu[cb] - top), b = __builtin_amdgcn_exp2f(mu - top);
-    st.mu[cb] = top;
-    st.l[cb] = st.l[cb] * a + l * b;
+    float2 ml[kPhases];
+    float b[kPhases];
+    f32x4_t part[8];
 #pragma unroll
-    for (int jj = 0; jj < 8; ++jj)
+    for (int i = 0; i < kPhases; ++i)
+      ml[i] = *reinterpret_cast<const float2*>(at + i * step + NCB * 8192 + cb * 512 + lane * 8);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        st.o[cb][jj][i] = st.o[cb][jj][i] * a + f[(cb * 34 + jj * 4 + i) * 64] * b;
+    for (int i = 0; i < 8; ++i)
+      part[i] = *reinterpret_cast<const f32x4_t*>(
+          at + (i % kPhases) * step + (cb * 8 + f * (8 / kPhases) + i / kPhases) * 1024 +
+          lane * 16);
+    float top = ml[0].x, l = 0.f;
+#pragma unroll
+    for (int i = 1; i < kPhases; ++i) top = fmaxf(top, ml[i].x);
+#pragma unroll
+    for (int i = 0; i < kPhases; ++i) {
+      b[i] = __builtin_amdgcn_exp2f(ml[i].x - top);
+      l += ml[i].y * b[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i += kPhases) {
+      f32x4_t o = part[i] * b[0];
+#pragma unroll
+      for (int j = 1; j < kPhases; ++j) o += part[i + j] * b[j];
+      part[i / kPhases] = o;
+    }
+    emit(cb, f * (8 / kPhases), 8 / kPhases, part, top, l);
   }
 }
 
@@ -769,11 +821,13 @@ __global__ void __launch_bounds__(64 * NW)
   const int grid = gridDim.x;
   const int share = grid % 8 == 0 ? (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
 
+  touch_kernel_args(int(sizeof(ScoredParams)));
   Where w;
-  int size;
-  const bool live = plan_share(p, lane, share, grid, w, size);
+  SeqGeo g;
+  int size, pre;
+  const bool live = plan_share(p, lane, share, grid, w, g, pre, size);
   if (!live) {
-    if (threadIdx.x == 0) p.rec[share] = int4{0, 0, 0, 0};
+    if (threadIdx.x == 0 && !p.whole) p.rec[share] = int4{0, 0, 0, 0};
     return;
   }
 
@@ -796,14 +850,12 @@ __global__ void __launch_bounds__(64 * NW)
 
   const int end = int(min(w.total, int64_t(share + 1) * size));
   int pos = share * size;
-  SeqGeo g = load_seq<true>(p, w.seq);
   int nblocks = num_blocks_of(p, g.sq);
   while (true) {
-    const int pre = p.prefix != nullptr ? table_entry(p.prefix, w.seq) : 0;
     const TileRange range = block_tiles(p, g, pre, w.block);
     const int tiles = range.t1 - range.t0;
-    const int seg0 = w.tile, seg1 = min(tiles, w.tile + (end - pos));
-    if (pos + tiles + kItemCost - w.tile >= end && threadIdx.x == 0) {
+    const int seg0 = w.tile, seg1 = p.whole ? tiles : min(tiles, w.tile + (end - pos));
+    if (!p.whole && pos + tiles + kItemCost - w.tile >= end && threadIdx.x == 0) {
       // The share's last item: where it goes on, if it began here.
       const int last = tiles > 0 ? (pos - w.tile + tiles - 1) / size : share;
       p.rec[share] = int4{w.seq, w.block, w.grp, w.tile == 0 && last > share ? last : 0};
@@ -1113,55 +1165,57 @@ __global__ void __launch_bounds__(64 * NW)
       }
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) st.l[cb] = rows4_sum(st.l[cb]);
-      // Join the tile phases: the waves of phase 0 take in the others' states.
-      if (phases > 1) {
-        const int owners = NW / phases;
-        __syncthreads();
-        if (phase > 0) put_state<NCB>(smem + (wave - owners) * F::kStateBytes, st, lane);
-        __syncthreads();
-        if (phase == 0)
-          for (int f = 1; f < phases; ++f)
-            join_state<NCB>(st, smem + (wave + (f - 1) * owners) * F::kStateBytes, lane);
-        __syncthreads();
-      } else if constexpr (!F::kPrivate) {
-        pf_barrier();  // the ring is free for the next item
-      }
-      if (phase == 0) {
+      // Rows 16 jj .. 16 (jj + n) of a column block of O^T: the item's result,
+      // or a partial in slot 2 share + 1 (the piece that begins its item), else
+      // 2 share.
+      auto emit = [&](int cb, int jj0, int n, const f32x4_t* o, float mu, float l) {
+        const ColumnOf co = column_of(p, col0, cb);
+        if (co.token >= p.tokens_per_block || b0 + co.token > tmax) return;
         if (seg0 == 0 && seg1 == tiles) {
+          const float inv = l != 0.f ? 1.f / l : 0.f;
+          uint16_t* dst = p.out + int64_t(g.q0 + b0 + co.token) * p.o_st +
+                          int64_t(head * p.group + co.head) * p.o_sh + 4 * lg + 16 * jj0;
 #pragma unroll
-          for (int cb = 0; cb < NCB; ++cb) {
-            const ColumnOf co = column_of(p, col0, cb);
-            if (co.token >= p.tokens_per_block || b0 + co.token > tmax) continue;
-            const float inv = st.l[cb] != 0.f ? 1.f / st.l[cb] : 0.f;
-            uint16_t* dst = p.out + int64_t(g.q0 + b0 + co.token) * p.o_st +
-                            int64_t(head * p.group + co.head) * p.o_sh + 4 * lg;
-#pragma unroll
-            for (int jj = 0; jj < 8; ++jj) {
-              const f32x4_t o = st.o[cb][jj] * inv;
-              *reinterpret_cast<u32x2_t*>(dst + 16 * jj) =
-                  u32x2_t{pack_bf16x2_fast(o[0], o[1]), pack_bf16x2_fast(o[2], o[3])};
-            }
+          for (int i = 0; i < n; ++i) {
+            const f32x4_t r = o[i] * inv;
+            *reinterpret_cast<u32x2_t*>(dst + 16 * i) =
+                u32x2_t{pack_bf16x2_fast(r[0], r[1]), pack_bf16x2_fast(r[2], r[3])};
           }
         } else {
-          // Slot 2 share + 1: the piece that begins its item; else 2 share.
           const int64_t slot = int64_t(2) * share + (seg0 == 0 ? 1 : 0);
-          const int64_t cols = int64_t(p.heads_per_wg) * F::kColumns;
+          const int64_t col = (slot * p.heads_per_wg + hs) * F::kColumns +
+                              (cw * NCB + cb) * 16 + lm;
+          float* dst = p.part_o + col * kD + 4 * lg + 16 * jj0;
 #pragma unroll
-          for (int cb = 0; cb < NCB; ++cb) {
-            const ColumnOf co = column_of(p, col0, cb);
-            if (co.token >= p.tokens_per_block || b0 + co.token > tmax) continue;
-            const int64_t col = slot * cols + hs * F::kColumns + (cw * NCB + cb) * 16 + lm;
-            float* dst = p.part_o + col * kD + 4 * lg;
-#pragma unroll
-            for (int jj = 0; jj < 8; ++jj)
-              *reinterpret_cast<f32x4_t*>(dst + 16 * jj) = st.o[cb][jj];
-            if (lg == 0) p.part_ml[col] = float2{st.mu[cb], st.l[cb]};
+          for (int i = 0; i < n; ++i) *reinterpret_cast<f32x4_t*>(dst + 16 * i) = o[i];
+          if (lg == 0 && jj0 == 0) p.part_ml[col] = float2{mu, l};
+        }
+      };
+      if constexpr (KW > 1) {
+        const int owners = NW / phases;
+        const char* first = smem + (wave % owners) * F::kStateBytes;
+        const int step = owners * F::kStateBytes;
+        __syncthreads();
+        put_state<NCB>(smem + wave * F::kStateBytes, st, lane);
+        __syncthreads();
+        if (phases == 2) {
+          join_states<NCB, 2>(first, step, phase, lane, emit);
+        } else if constexpr (F::kPrivate) {
+          if (phases == 4) {
+            join_states<NCB, 4>(first, step, phase, lane, emit);
+          } else {
+            join_states<NCB, 8>(first, step, phase, lane, emit);
           }
         }
+        __syncthreads();
+      } else {
+        pf_barrier();  // the ring is free for the next item
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) emit(cb, 0, 8, st.o[cb], st.mu[cb], st.l[cb]);
       }
     }
 
-    pos += tiles + kItemCost - w.tile;
+    pos += p.whole ? 1 : tiles + kItemCost - w.tile;
     if (pos >= end) break;
     w.tile = 0;
     if (++w.block < nblocks) continue;
@@ -1170,10 +1224,11 @@ __global__ void __launch_bounds__(64 * NW)
     w.grp = 0;
     do {
       if (++w.seq >= p.batch) {
-        if (threadIdx.x == 0) p.rec[share] = int4{0, 0, 0, 0};
+        if (threadIdx.x == 0 && !p.whole) p.rec[share] = int4{0, 0, 0, 0};
         return;
       }
       g = load_seq<true>(p, w.seq);
+      pre = p.prefix != nullptr ? table_entry(p.prefix, w.seq) : 0;
       nblocks = num_blocks_of(p, g.sq);
     } while (nblocks == 0);
   }
@@ -1264,6 +1319,7 @@ struct Plan {
   int form;  // index of the column count below
   int columns, heads_per_wg, head_groups, tokens_per_block;
   int grid;
+  bool whole;
   int64_t max_items;
   size_t rec_bytes, ml_bytes, o_bytes;
   size_t bytes() const { return rec_bytes + ml_bytes + o_bytes; }
@@ -1274,16 +1330,23 @@ constexpr int kForms = 5;
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Up to this many keys a row of few columns is one workgroup's, head by head
+// (its waves take tiles in turn), while there are workgroups for all: nothing
+// is cut, and the merge is not launched.
+constexpr int64_t kWholeKeys = 1024;
+
 // The form: the narrowest whose columns hold the longest row of the call (its
 // tokens x query heads per kv head), the widest where none does.
-Plan make_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, int64_t max_q) {
+Plan make_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, int64_t max_q,
+               int64_t max_keys) {
   Plan pl{};
   const int64_t group = heads / kv_heads;
   const int64_t want = std::max<int64_t>(1, std::min(max_q, tokens)) * group;
   pl.form = 0;
   while (pl.form + 1 < kForms && kFormColumns[pl.form] < want) ++pl.form;
   pl.columns = kFormColumns[pl.form];
-  int most = pl.form <= 1 ? 4 : 1;
+  pl.whole = pl.form <= 1 && max_keys <= kWholeKeys && batch * kv_heads <= cu_count();
+  int most = pl.form <= 1 && !pl.whole ? 4 : 1;
   while (most > 1 && kv_heads % most != 0) most >>= 1;
   pl.heads_per_wg = most;
   pl.head_groups = int(kv_heads / most);
@@ -1329,7 +1392,7 @@ int launch_form(const ScoredParams& p, const Plan& pl, hipStream_t st) {
 // One launch over `p`'s sequences and its merge.  what: the entry's name.
 int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStream_t st,
              const char* what) {
-  const Plan pl = make_plan(p.num_tokens, p.heads, p.kv_heads, p.batch, max_q);
+  const Plan pl = make_plan(p.num_tokens, p.heads, p.kv_heads, p.batch, max_q, max_keys);
   KVC_REQUIRE(pl.max_items * ((max_keys + kTile - 1) / kTile + kItemCost) < (int64_t(1) << 30),
               KVC_ERR_VALUE, "%s: too many query blocks x keys for one call", what);
   p.heads_per_wg = pl.heads_per_wg;
@@ -1339,6 +1402,7 @@ int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStrea
                      pl.tokens_per_block;
   p.lane_plan = (p.batch + 63) / 64 * nb <= p.batch + p.num_tokens / pl.tokens_per_block / 64;
   p.min_share = 4;
+  p.whole = pl.whole;
   char* w = static_cast<char*>(ws);
   p.rec = reinterpret_cast<int4*>(w);
   p.part_ml = reinterpret_cast<float2*>(w + pl.rec_bytes);
@@ -1356,7 +1420,7 @@ int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStrea
   } else {
     rc = bias ? launch_form<kDistance>(p, pl, st) : launch_form<kPlain>(p, pl, st);
   }
-  if (rc != KVC_OK) return rc;
+  if (rc != KVC_OK || pl.whole) return rc;
   const dim3 mg{unsigned(pl.grid), unsigned(pl.heads_per_wg * pl.columns / kMergeColumns)};
   scored_merge_kernel<<<mg, 32 * kMergeColumns, 0, st>>>(p, pl.columns);
   return check_launch(what);
@@ -1418,10 +1482,10 @@ extern "C" size_t kvc_scored_workspace_bytes(int64_t num_q_tokens, int64_t num_h
     return 0;
   size_t n = 0;
   if (num_decode_rows > 0)
-    n = make_plan(num_decode_rows, num_heads, num_kv_heads, num_decode_rows, 1).bytes();
+    n = make_plan(num_decode_rows, num_heads, num_kv_heads, num_decode_rows, 1, kWholeKeys + 1).bytes();
   if (num_prefill > 0 && num_q_tokens > num_decode_rows)
     n = std::max(n, make_plan(num_q_tokens - num_decode_rows, num_heads, num_kv_heads, num_prefill,
-                              max_seqlen_q)
+                              max_seqlen_q, kWholeKeys + 1)
                         .bytes());
   return n;
 }
@@ -1530,7 +1594,8 @@ extern "C" size_t kvc_tree_workspace_bytes(int64_t num_q_tokens, int64_t num_hea
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || num_q_tokens <= 0 ||
       num_heads / num_kv_heads > kFormColumns[kForms - 1])
     return 0;
-  return make_plan(num_q_tokens, num_heads, num_kv_heads, batch, max_seqlen_q).bytes() +
+  return make_plan(num_q_tokens, num_heads, num_kv_heads, batch, max_seqlen_q, kWholeKeys + 1)
+             .bytes() +
          up256(size_t(num_q_tokens) * sizeof(int32_t));
 }
 
