@@ -1320,6 +1320,7 @@ struct Plan {
   int columns, heads_per_wg, head_groups, tokens_per_block;
   int grid;
   bool whole;
+  int64_t max_blocks;  // of all sequences, if none has more than max_q tokens
   int64_t max_items;
   size_t rec_bytes, ml_bytes, o_bytes;
   size_t bytes() const { return rec_bytes + ml_bytes + o_bytes; }
@@ -1330,10 +1331,14 @@ constexpr int kForms = 5;
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Up to this many keys a row of few columns is one workgroup's, head by head
-// (its waves take tiles in turn), while there are workgroups for all: nothing
-// is cut, and the merge is not launched.
-constexpr int64_t kWholeKeys = 1024;
+// Tables of few keys: an item is one workgroup's, nothing is cut and the merge
+// is not launched, while there is a workgroup for each.  Measured, whole
+// against cut: one decode row of 8 kv heads 10.3 / 14.7 us over 512 keys, 17.4
+// / 15.0 over 1024; prompts (a workgroup takes a tile a turn there, not eight)
+// of 256 tokens 24.3 / 28.5 us, of 512 tokens 34.3 / 31.2 for one and 37.6 /
+// 43.6 for four of them, whose items fill the card as they are.
+constexpr int64_t kWholeKeys = 768;
+constexpr int64_t kWholeKeysFewItems = 384;
 
 // The form: the narrowest whose columns hold the longest row of the call (its
 // tokens x query heads per kv head), the widest where none does.
@@ -1345,12 +1350,17 @@ Plan make_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, i
   pl.form = 0;
   while (pl.form + 1 < kForms && kFormColumns[pl.form] < want) ++pl.form;
   pl.columns = kFormColumns[pl.form];
-  pl.whole = pl.form <= 1 && max_keys <= kWholeKeys && batch * kv_heads <= cu_count();
+  pl.tokens_per_block = int(pl.columns / group);
+  pl.max_blocks = std::min(tokens / pl.tokens_per_block + batch,
+                           batch * ((want / group + pl.tokens_per_block - 1) / pl.tokens_per_block));
+  const int64_t items = pl.max_blocks * kv_heads;
+  pl.whole = items <= cu_count() &&
+             max_keys <= (pl.form <= 1 || items >= cu_count() / 4 ? kWholeKeys
+                                                                   : kWholeKeysFewItems);
   int most = pl.form <= 1 && !pl.whole ? 4 : 1;
   while (most > 1 && kv_heads % most != 0) most >>= 1;
   pl.heads_per_wg = most;
   pl.head_groups = int(kv_heads / most);
-  pl.tokens_per_block = int(pl.columns / group);
   pl.grid = cu_count();
   pl.max_items = (tokens / pl.tokens_per_block + batch) * pl.head_groups;
   const size_t cols = size_t(2) * pl.grid * pl.heads_per_wg * pl.columns;
@@ -1392,7 +1402,14 @@ int launch_form(const ScoredParams& p, const Plan& pl, hipStream_t st) {
 // One launch over `p`'s sequences and its merge.  what: the entry's name.
 int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStream_t st,
              const char* what) {
-  const Plan pl = make_plan(p.num_tokens, p.heads, p.kv_heads, p.batch, max_q, max_keys);
+  // Keys that one sequence's tokens see, as far as the host knows (this only
+  // steers the plan): fresh rows hold every sequence's, each as many keys as
+  // queries or more.
+  int64_t seen = max_keys;
+  if (p.tables == nullptr)
+    seen = std::min(seen, std::max<int64_t>(0, max_keys - p.num_tokens) + max_q);
+  if (p.window > 0 && p.prefix == nullptr) seen = std::min<int64_t>(seen, p.window + max_q);
+  const Plan pl = make_plan(p.num_tokens, p.heads, p.kv_heads, p.batch, max_q, seen);
   KVC_REQUIRE(pl.max_items * ((max_keys + kTile - 1) / kTile + kItemCost) < (int64_t(1) << 30),
               KVC_ERR_VALUE, "%s: too many query blocks x keys for one call", what);
   p.heads_per_wg = pl.heads_per_wg;
