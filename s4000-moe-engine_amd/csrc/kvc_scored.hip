@@ -258,7 +258,12 @@ struct Consts {
   float c2;      // scale log2(e)
   float zc;      // 2 log2(e) scale / cap
   float a, a2;   // cap log2(e) and twice that
+  float z;       // scale / cap
 };
+// Caps that kCapFixed does not take: 1 - 2 / (e^{2z} + 1) is off by 2^-22 of
+// the cap, so below |z| = 1/16 tanh comes from its series, z (1 - z^2 / 3 + 2
+// z^4 / 15), off by 17 / 315 z^6 < 2^-28 relative.
+constexpr float kSeriesBelow = 1.f / 256;  // z^2
 
 // The key offset of element e (0 .. 7) of a lane's column inside a tile: the
 // MFMA's C rows 4 lg + i of the two 16-key halves, which is also the K index
@@ -283,9 +288,9 @@ __device__ __forceinline__ void logits(const u32x4_t (&k)[2][4], const u32x4_t (
 // The score's shape, the mask, the running softmax, and P^T as the bf16
 // operand pb.  y comes in as the logits and becomes what the softmax is taken
 // of: the raw logit s (log2-unit score c2 s) for plain scores, the log2-unit
-// score otherwise; -inf at keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} + 1): one exp2 and
-// one reciprocal.  Sums are formed of the rounded P (an MFMA against ones),
-// so the weights add up to the sum that divides them.
+// score otherwise; -inf at keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} +
+// 1): one exp2 and one reciprocal.  Sums are formed of the rounded P, so the
+// weights add up to the sum that divides them.
 template <int NCB, int MODE>
 __device__ __forceinline__ void shape_scores(const Columns<NCB>& c, f32x4_t (&y)[NCB][2], int j0,
                                              int lg, const Consts& cs) {
@@ -303,6 +308,11 @@ __device__ __forceinline__ void shape_scores(const Columns<NCB>& c, f32x4_t (&y)
       if constexpr (kCap) {
         const float w = __builtin_amdgcn_exp2f(s * cs.zc);
         x = __builtin_fmaf(-cs.a2, __builtin_amdgcn_rcpf(w + 1.f), cs.a);
+        if constexpr (MODE != kCapFixed) {
+          const float z = s * cs.z, z2 = z * z;
+          const float series = __builtin_fmaf(z2, __builtin_fmaf(z2, 2.f / 15, -1.f / 3), 1.f);
+          x = z2 < kSeriesBelow ? s * cs.c2 * series : x;
+        }
       }
       if constexpr (kDist) {
         const float bias = __builtin_fmaf(c.slope2[cb], float(key_of(e)), b0);
@@ -842,6 +852,7 @@ __global__ void __launch_bounds__(64 * NW)
   cs.zc = p.cap > 0.f ? 2.f * kLog2e * p.scale / p.cap : 0.f;
   cs.a = p.cap * kLog2e;
   cs.a2 = 2.f * cs.a;
+  cs.z = p.cap > 0.f ? p.scale / p.cap : 0.f;
   constexpr float mu0 = MODE == kCapFixed ? 0.f : kLowest;
 
   const int col0 = cw * NCB * 16;
@@ -1459,10 +1470,12 @@ int check_common(const char* what, const void* q, int64_t q_st, int64_t q_sh, in
               "%s: at most %d query heads per kv head", what, kFormColumns[kForms - 1]);
   KVC_REQUIRE(tokens >= 0 && tokens < (int64_t(1) << 30), KVC_ERR_VALUE, "%s: bad token count",
               what);
-  KVC_REQUIRE(scale > 0.f && std::isfinite(scale), KVC_ERR_VALUE,
+  KVC_REQUIRE(scale > 0.f && std::isfinite(4.f * scale), KVC_ERR_VALUE,
               "%s: scale must be finite and > 0", what);
   KVC_REQUIRE(softcap >= 0.f && std::isfinite(softcap), KVC_ERR_VALUE,
               "%s: softcap must be finite and >= 0", what);
+  KVC_REQUIRE(softcap == 0.f || std::isfinite(4.f * scale / softcap), KVC_ERR_VALUE,
+              "%s: scale / softcap is too large", what);
   KVC_REQUIRE(window >= 0 && window < (int64_t(1) << 30), KVC_ERR_VALUE,
               "%s: window must be >= 0", what);
   KVC_REQUIRE(tokens == 0 || (q != nullptr && out != nullptr), KVC_ERR_VALUE,
@@ -1524,7 +1537,7 @@ extern "C" int kvc_scored_attention(
                         head_dim, scale, softcap, window, out, out_stride_t, out_stride_h);
   if (rc != KVC_OK) return rc;
   KVC_REQUIRE(num_decode_rows >= 0 && num_decode_rows <= num_q_tokens && num_prefill >= 0 &&
-                  max_seqlen_q >= 0,
+                  num_prefill < (int64_t(1) << 30) && max_seqlen_q >= 0,
               KVC_ERR_VALUE, "%s: bad row counts", what);
   if (num_q_tokens == 0) return KVC_OK;
   const bool fresh = block_tables == nullptr;
@@ -1630,7 +1643,8 @@ extern "C" int kvc_tree_attention(
   int rc = check_common(what, q, q_stride_t, q_stride_h, num_q_tokens, num_heads, num_kv_heads,
                         head_dim, scale, softcap, window, out, out_stride_t, out_stride_h);
   if (rc != KVC_OK) return rc;
-  KVC_REQUIRE(batch >= 0 && max_seqlen_q >= 0, KVC_ERR_VALUE, "%s: bad row counts", what);
+  KVC_REQUIRE(batch >= 0 && batch < (int64_t(1) << 30) && max_seqlen_q >= 0, KVC_ERR_VALUE,
+              "%s: bad row counts", what);
   if (num_q_tokens == 0 || batch == 0) return KVC_OK;
   rc = check_pool(what, k_cache, v_cache, num_cache_blocks, page_size, num_kv_heads, block_tables,
                   max_blocks_per_seq);

@@ -1,0 +1,180 @@
+"""Shaped-score attention on both sides of every choice that the launch makes
+from sizes: tables short enough to stay uncut or not, one batch entry or
+several, uniform rows or offsets, more blocks than workgroups, and caps of any
+size."""
+import pytest
+import torch
+
+from nanovllm_amd.kernels.scored import scored_attention
+from nanovllm_amd.kernels.tree import tree_attention
+from scored_oracle import attend, check, chunk_mask, paged, slopes_of, tree_mask
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SCALE = 128 ** -0.5
+
+
+def _normal(n, heads, seed, wide=2.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, heads, 128, generator=gen) * wide).to(torch.bfloat16)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _chunks(q, ks, vs, chunks, label, pool=None, cap=0.0, window=0, prefix=None, most=None):
+    """One call over chunks (queries, keys), from the pool or fresh."""
+    cu_q, cu_k = [0], [0]
+    for n, m in chunks:
+        cu_q.append(cu_q[-1] + n)
+        cu_k.append(cu_k[-1] + m)
+    kw = dict(scale=SCALE, softcap=cap, window=window, cu_seqlens_q=_i32(cu_q),
+              cu_seqlens_k=_i32(cu_k), cu_seqlens_q_list=cu_q, cu_seqlens_k_list=cu_k,
+              prefix_lens=None if prefix is None else _i32(prefix))
+    if pool is None:
+        out = scored_attention(q.to(DEV), None, None, k=torch.cat(ks).to(DEV),
+                               v=torch.cat(vs).to(DEV), **kw)
+    else:
+        kc, vc, bt = pool
+        out = scored_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), block_tables=bt.to(DEV), **kw)
+    wants, bounds = [], []
+    for i, (n, m) in enumerate(chunks):
+        if n == 0:
+            continue
+        sees, away = chunk_mask(n, m, window, prefix[i] if prefix else 0)
+        w, b = attend(q[cu_q[i]:cu_q[i + 1]], ks[i], vs[i], sees, away, scale=SCALE, cap=cap)
+        wants.append(w)
+        bounds.append(b)
+    check(out, torch.cat(wants), torch.cat(bounds), label)
+
+
+@pytest.mark.parametrize("pages", [1, 11, 12, 13, 23, 24, 25])
+@pytest.mark.parametrize("heads,kvh", [(16, 8), (8, 1), (40, 2)])
+@pytest.mark.parametrize("batch", [1, 3])
+def test_decode_tables_around_the_cut(pages, heads, kvh, batch):
+    lens = [32 * pages - i * 7 for i in range(batch)]
+    kc, vc, bt, ks, vs = paged(lens, 32, kvh, pages)
+    q = _normal(batch, heads, 1)
+    out = scored_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), scale=SCALE,
+                           block_tables=bt.to(DEV), num_decode_rows=batch,
+                           decode_context_lens=_i32(lens), softcap=50.0)
+    wb = [attend(q[i:i + 1], ks[i], vs[i], *chunk_mask(1, lens[i], 0, 0), scale=SCALE, cap=50.0)
+          for i in range(batch)]
+    check(out, torch.cat([w for w, _ in wb]), torch.cat([b for _, b in wb]),
+          f"decode of {batch}, {pages} pages, {heads}/{kvh}")
+
+
+@pytest.mark.parametrize("keys", [64, 383, 385, 767, 769])
+@pytest.mark.parametrize("heads,kvh", [(4, 2), (16, 2)])
+def test_prompts_around_the_cut(keys, heads, kvh):
+    """Fresh prompts: one, and one with an empty neighbour on either side."""
+    for chunks in ([(keys, keys)], [(0, 0), (keys // 2, keys // 2), (0, 0), (1, keys - keys // 2)]):
+        ks = [_normal(m, kvh, 3 + i, 1.0) for i, (_, m) in enumerate(chunks)]
+        vs = [_normal(m, kvh, 9 + i, 1.0) for i, (_, m) in enumerate(chunks)]
+        _chunks(_normal(sum(n for n, _ in chunks), heads, 4), ks, vs, chunks,
+                f"fresh {chunks} {heads}/{kvh}")
+
+
+@pytest.mark.parametrize("batch", [2, 64, 65, 130])
+def test_many_short_sequences(batch):
+    """As many rows as fit the card's workgroups and more, uneven chunks, an
+    image prefix in some."""
+    chunks = [((i * 5) % 7, 40 + (i * 13) % 57) for i in range(batch)]
+    kc, vc, bt, ks, vs = paged([m for _, m in chunks], 32, 2, 5)
+    prefix = [(i % 3) * 33 for i in range(batch)]
+    _chunks(_normal(sum(n for n, _ in chunks), 4, 6), ks, vs, chunks, f"{batch} short chunks",
+            pool=(kc, vc, bt), prefix=prefix)
+
+
+@pytest.mark.parametrize("window", [1, 100, 700, 1 << 20])
+def test_windows_make_long_tables_short(window):
+    chunks = [(9, 2000), (17, 1400)]
+    kc, vc, bt, ks, vs = paged([m for _, m in chunks], 64, 2, 7)
+    _chunks(_normal(26, 8, 8), ks, vs, chunks, f"window {window}", pool=(kc, vc, bt),
+            window=window, cap=30.0)
+
+
+@pytest.mark.parametrize("uniform", [False, True])
+@pytest.mark.parametrize("trees,tokens,ctx", [(1, 8, 300), (1, 40, 340), (3, 16, 500), (5, 64, 100),
+                                              (70, 3, 60)])
+def test_short_trees(uniform, trees, tokens, ctx):
+    gen = torch.Generator().manual_seed(11)
+    sizes = [tokens if uniform else max(1, tokens - i % 3) for i in range(trees)]
+    lens = [max(0, ctx - 41 * i) for i in range(trees)]
+    kc, vc, bt, ks, vs = paged([c + n for c, n in zip(lens, sizes)], 32, 2, 13)
+    bits, at = [], 0
+    for n in sizes:
+        b = torch.eye(n, dtype=torch.bool)
+        for t in range(1, n):
+            b[t] |= b[int(torch.randint(0, t, (1,), generator=gen))]
+        bits.append(b)
+    mask = torch.zeros(sum(sizes), 1, dtype=torch.int64)
+    for b in bits:
+        for row in b:
+            word = sum(1 << u for u in range(len(row)) if row[u])
+            mask[at, 0] = word - (1 << 64) if word >> 63 else word
+            at += 1
+    q = _normal(sum(sizes), 8, 12)
+    cu = [0]
+    for n in sizes:
+        cu.append(cu[-1] + n)
+    kw = {} if uniform else dict(cu_seqlens_q=_i32(cu), max_seqlen_q=tokens)
+    out = tree_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), bt.to(DEV), _i32(lens), mask.to(DEV),
+                         SCALE, **kw)
+    wb = [attend(q[cu[i]:cu[i + 1]], ks[i], vs[i], *tree_mask(bits[i], lens[i], 0), scale=SCALE)
+          for i in range(trees)]
+    check(out, torch.cat([w for w, _ in wb]), torch.cat([b for _, b in wb]),
+          f"{trees} trees of {tokens} over {ctx}")
+
+
+def test_more_tokens_than_announced():
+    """max_seqlen_q steers the launch only: trees longer than it, in a table
+    short enough to stay uncut, are attended all the same."""
+    sizes, lens = [40, 150], [100, 20]
+    kc, vc, bt, ks, vs = paged([c + n for c, n in zip(lens, sizes)], 32, 2, 17)
+    bits = [torch.tril(torch.ones(n, n, dtype=torch.bool)) for n in sizes]
+    mask = torch.zeros(190, 3, dtype=torch.int64)
+    for base, b in ((0, bits[0]), (40, bits[1])):
+        for t, row in enumerate(b):
+            for w in range(3):
+                word = sum(1 << u for u, x in enumerate(row[64 * w:64 * w + 64].tolist()) if x)
+                mask[base + t, w] = word - (1 << 64) if word >> 63 else word
+    q = _normal(190, 32, 18)
+    for most in (1, 8, 64):
+        out = tree_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), bt.to(DEV), _i32(lens),
+                             mask.to(DEV), SCALE, cu_seqlens_q=_i32([0, 40, 190]),
+                             max_seqlen_q=most)
+        wb = [attend(q[a:b], ks[i], vs[i], *tree_mask(bits[i], lens[i], 0), scale=SCALE)
+              for i, (a, b) in enumerate(((0, 40), (40, 190)))]
+        check(out, torch.cat([w for w, _ in wb]), torch.cat([b for _, b in wb]),
+              f"announced {most}")
+
+
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("cap", [1e6, 1e30])
+def test_caps_far_above_the_scores(cap, slopes):
+    """Such a cap changes a score by less than 2^-30 of it (z^2 / 3 with |z| <
+    1e-4): the result is the uncapped one, to its bound.  Rows of one tile, of
+    a few and of cut items."""
+    lens = [20, 300, 2000]
+    kc, vc, bt, ks, vs = paged(lens, 64, 2, 19)
+    q = _normal(3, 8, 20)
+    sl = slopes_of(8) if slopes else None
+    out = scored_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), scale=SCALE,
+                           block_tables=bt.to(DEV), num_decode_rows=3,
+                           decode_context_lens=_i32(lens), softcap=cap,
+                           alibi_slopes=None if sl is None else sl.to(DEV))
+    wb = [attend(q[i:i + 1], ks[i], vs[i], *chunk_mask(1, lens[i], 0, 0), scale=SCALE, slopes=sl)
+          for i in range(3)]
+    check(out, torch.cat([w for w, _ in wb]), torch.cat([b for _, b in wb]), f"cap {cap}")
+
+
+@pytest.mark.parametrize("cap", [60.0, 1000.0])
+def test_caps_where_series_and_exponentials_meet(cap):
+    """Scores on both sides of |score| = cap / 16."""
+    chunks = [(40, 70)]
+    kc, vc, bt, ks, vs = paged([70], 32, 2, 21)
+    for wide in (0.5, 4.0, 20.0):
+        _chunks(_normal(40, 8, 22, wide), ks, vs, chunks, f"cap {cap} width {wide}",
+                pool=(kc, vc, bt), cap=cap)

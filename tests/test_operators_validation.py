@@ -216,3 +216,14 @@ def test_entry_points_refuse_before_any_launch():
                    (dict(planes=0), 0)):
         got, msg = commit(**kw)
         assert got == rc, (kw, got, msg)
+
+
+def test_caps_and_scales_that_fp32_cannot_divide():
+    """scale / softcap past fp32 would make 0 x inf of a zero logit."""
+    buf = ctypes.create_string_buffer(4096)
+    at = (ctypes.addressof(buf) + 255) // 256 * 256
+    for cap, scale, rc in ((1e-38, 100.0, -1), (0.0, 3e38, -1), (1e-30, 0.1, -4), (1e30, 0.1, -4)):
+        got, msg = _c("kvc_scored_attention", at, 1024, 128, 1, 8, at, at, 4, 32, 2, 128, None, 0,
+                      0, None, 0, 0, 0, at, 1, 1, 1, at, 0, None, None, 1, None, None, cap, 0,
+                      scale, at, 1024, 128, at, 0, None)
+        assert got == rc and msg, (cap, scale, got, msg)
