@@ -536,8 +536,11 @@ __device__ __forceinline__ void add_not_finite(const ScoredParams& p, const Colu
 // for itself from the device's lengths (no barrier before the first load).
 // ---------------------------------------------------------------------------
 // Virtual tiles that every item adds to its cost: its query loads, its pipe's
-// start and its epilogue.
-constexpr int kItemCost = 3;
+// start, its masked tiles (two to three times an ordinary one) and its
+// epilogue.  Measured with 3, 7, 12, 19, 26 of them: four prompts with images
+// 267, 252, 239, 248, 259 us, four windowed chunks 60, 55, 52, 55, 57 us, 37
+// trees 74, 71, 69, 71, 74 us; long items do not care.
+constexpr int kItemCost = 12;
 
 struct Where {
   int seq, grp, block, tile;  // tile: offset inside the item
