@@ -1329,52 +1329,32 @@ int cu_count() {
   return n;
 }
 
+constexpr int kFormColumns[] = {16, 32, 64, 128, 256};
+constexpr int kForms = 5;
+
 struct Plan {
-  int form;  // index of the column count below
+  int form;  // index of the column count
   int columns, heads_per_wg, head_groups, tokens_per_block;
   int grid;
   bool whole;
-  int64_t max_blocks;  // of all sequences, if none has more than max_q tokens
   int64_t max_items;
   size_t rec_bytes, ml_bytes, o_bytes;
   size_t bytes() const { return rec_bytes + ml_bytes + o_bytes; }
 };
 
-constexpr int kFormColumns[] = {16, 32, 64, 128, 256};
-constexpr int kForms = 5;
-
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Tables of few keys: an item is one workgroup's, nothing is cut and the merge
-// is not launched, while there is a workgroup for each.  Measured, whole
-// against cut: one decode row of 8 kv heads 10.3 / 14.7 us over 512 keys, 17.4
-// / 15.0 over 1024; prompts (a workgroup takes a tile a turn there, not eight)
-// of 256 tokens 24.3 / 28.5 us, of 512 tokens 34.3 / 31.2 for one and 37.6 /
-// 43.6 for four of them, whose items fill the card as they are.
-constexpr int64_t kWholeKeys = 768;
-constexpr int64_t kWholeKeysFewItems = 384;
-
-// The form: the narrowest whose columns hold the longest row of the call (its
-// tokens x query heads per kv head), the widest where none does.
-Plan make_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, int64_t max_q,
-               int64_t max_keys) {
+Plan lay_out(int form, bool whole, int64_t tokens, int64_t group, int64_t kv_heads,
+             int64_t batch) {
   Plan pl{};
-  const int64_t group = heads / kv_heads;
-  const int64_t want = std::max<int64_t>(1, std::min(max_q, tokens)) * group;
-  pl.form = 0;
-  while (pl.form + 1 < kForms && kFormColumns[pl.form] < want) ++pl.form;
-  pl.columns = kFormColumns[pl.form];
-  pl.tokens_per_block = int(pl.columns / group);
-  pl.max_blocks = std::min(tokens / pl.tokens_per_block + batch,
-                           batch * ((want / group + pl.tokens_per_block - 1) / pl.tokens_per_block));
-  const int64_t items = pl.max_blocks * kv_heads;
-  pl.whole = items <= cu_count() &&
-             max_keys <= (pl.form <= 1 || items >= cu_count() / 4 ? kWholeKeys
-                                                                   : kWholeKeysFewItems);
-  int most = pl.form <= 1 && !pl.whole ? 4 : 1;
+  pl.form = form;
+  pl.whole = whole;
+  pl.columns = kFormColumns[form];
+  int most = form <= 1 && !whole ? 4 : 1;
   while (most > 1 && kv_heads % most != 0) most >>= 1;
   pl.heads_per_wg = most;
   pl.head_groups = int(kv_heads / most);
+  pl.tokens_per_block = int(pl.columns / group);
   pl.grid = cu_count();
   pl.max_items = (tokens / pl.tokens_per_block + batch) * pl.head_groups;
   const size_t cols = size_t(2) * pl.grid * pl.heads_per_wg * pl.columns;
@@ -1382,6 +1362,94 @@ Plan make_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, i
   pl.ml_bytes = up256(cols * sizeof(float2));
   pl.o_bytes = up256(cols * kD * sizeof(float));
   return pl;
+}
+
+// The narrowest form that holds the longest row, or the last.
+int holding_form(int64_t longest, int64_t group) {
+  int f = 0;
+  while (f + 1 < kForms && kFormColumns[f] < longest * group) ++f;
+  return f;
+}
+
+// The form and whether items are cut.
+//
+// Up to 32 columns (the longest row's tokens x query heads per kv head) the
+// private forms serve, the narrowest that holds them.  Over at most kWholeKeys
+// keys, and with a workgroup for each, their items stay whole: nothing is cut
+// and the merge is not launched.  One decode row of 8 kv heads, whole against
+// cut: 10.3 / 14.7 us over 512 keys, 17.4 / 15.0 over 1024 (one CU's loads
+// bound it then).
+//
+// Wider rows take any turns form up to the narrowest that holds them, whole or
+// cut, whichever these estimates call cheapest, in tenths of a 256-column
+// tile.  A narrower form makes more items of less work each: that spares a
+// ragged batch empty columns and lets a short call stay whole on more CUs, but
+// every tile is read more often.  Measured, the narrowest form that holds the
+// longest row and is cut, against this choice: a prompt of 512 tokens (16 / 8
+// heads) 30.2 / 16.6 us, four of 256 (32 / 4) 27.5 / 22.0; four windowed chunks
+// 52.4 / 40.3; one tree of 31 tokens over 333 keys (32 / 4) 26.3 / 15.3; 37
+// ragged trees 69 / 66.  Over 195 calls of 1 to 64 sequences the times fall by
+// a fifth (geometric mean); the worst, four trees of 8 tokens over 1000 keys,
+// goes from 21.2 to 23.5.
+constexpr int64_t kWholeKeys = 768;
+constexpr int kTileCost[] = {0, 0, 4, 6, 10};  // of a form's tile
+constexpr int kPieceCost = 80;   // an item's, or a piece's, setup, pipe fill and epilogue
+constexpr int kMergeCost[] = {0, 0, 140, 180, 240};  // its launch, partials both ways
+
+// Column blocks of all sequences, of which the host knows the tokens and the
+// longest: a sequence fills half of its last one.
+int64_t likely_blocks(int64_t tokens, int64_t batch, int64_t longest, int64_t per_block) {
+  const int64_t most = batch * ((longest + per_block - 1) / per_block);
+  return batch * longest == tokens ? most : std::min(most, (tokens + batch * per_block / 2) / per_block);
+}
+
+// max_keys: keys of the longest sequence as far as the host knows; window: a
+// window's keys, 0 without one (or where a two-way prefix reaches past it).
+// These two decide the form and `whole` alone, never what is computed.
+Plan make_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, int64_t max_q,
+               int64_t max_keys, int64_t window) {
+  const int64_t group = heads / kv_heads;
+  const int64_t longest = std::max<int64_t>(1, std::min(max_q, tokens));
+  const int widest = holding_form(longest, group);
+  if (widest <= 1) {
+    const int64_t per_block = kFormColumns[widest] / group;
+    const int64_t keys = window > 0 ? std::min(max_keys, window + per_block) : max_keys;
+    const bool whole = keys <= kWholeKeys &&
+                       likely_blocks(tokens, batch, longest, per_block) * kv_heads <= cu_count();
+    return lay_out(widest, whole, tokens, group, kv_heads, batch);
+  }
+  const int64_t grid = cu_count();
+  int form = widest;
+  bool uncut = false;
+  int64_t least = INT64_MAX;
+  for (int f = widest; f >= 2 && kFormColumns[f] >= group; --f) {
+    const int64_t per_block = kFormColumns[f] / group;
+    const int64_t items = likely_blocks(tokens, batch, longest, per_block) * kv_heads;
+    const bool windowed = window > 0 && window + per_block < max_keys;
+    const int64_t tiles = (windowed ? window + per_block : max_keys) / kTile + 1;
+    // (a prompt's rows see from few keys to all, and lengths differ, if less
+    // where a window bounds them: cut, the mean counts, not the longest)
+    const int64_t mean = (tiles * (windowed ? 75 : 60) + 99) / 100;
+    const int64_t rounds = (items + grid - 1) / grid;
+    const int64_t whole = rounds > 1 && !windowed
+                              ? INT64_MAX
+                              : rounds * (tiles * kTileCost[f] + kPieceCost);
+    const int64_t cut = items * (mean * kTileCost[f] + kPieceCost) / grid + kPieceCost +
+                        kMergeCost[f];
+    if (std::min(whole, cut) < least) {
+      least = std::min(whole, cut);
+      form = f;
+      uncut = whole <= cut;
+    }
+  }
+  return lay_out(form, uncut, tokens, group, kv_heads, batch);
+}
+
+// Workspace that holds for whatever make_plan chooses once it knows the keys.
+size_t plan_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t batch, int64_t max_q) {
+  const int64_t group = heads / kv_heads;
+  const int form = holding_form(std::max<int64_t>(1, std::min(max_q, tokens)), group);
+  return lay_out(form, false, tokens, group, kv_heads, batch).bytes();
 }
 
 template <int NW, int NCB, int KW, int MODE>
@@ -1422,8 +1490,8 @@ int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStrea
   int64_t seen = max_keys;
   if (p.tables == nullptr)
     seen = std::min(seen, std::max<int64_t>(0, max_keys - p.num_tokens) + max_q);
-  if (p.window > 0 && p.prefix == nullptr) seen = std::min<int64_t>(seen, p.window + max_q);
-  const Plan pl = make_plan(p.num_tokens, p.heads, p.kv_heads, p.batch, max_q, seen);
+  const Plan pl = make_plan(p.num_tokens, p.heads, p.kv_heads, p.batch, max_q, seen,
+                            p.prefix == nullptr ? p.window : 0);
   KVC_REQUIRE(pl.max_items * ((max_keys + kTile - 1) / kTile + kItemCost) < (int64_t(1) << 30),
               KVC_ERR_VALUE, "%s: too many query blocks x keys for one call", what);
   p.heads_per_wg = pl.heads_per_wg;
@@ -1515,11 +1583,10 @@ extern "C" size_t kvc_scored_workspace_bytes(int64_t num_q_tokens, int64_t num_h
     return 0;
   size_t n = 0;
   if (num_decode_rows > 0)
-    n = make_plan(num_decode_rows, num_heads, num_kv_heads, num_decode_rows, 1, kWholeKeys + 1).bytes();
+    n = plan_bytes(num_decode_rows, num_heads, num_kv_heads, num_decode_rows, 1);
   if (num_prefill > 0 && num_q_tokens > num_decode_rows)
-    n = std::max(n, make_plan(num_q_tokens - num_decode_rows, num_heads, num_kv_heads, num_prefill,
-                              max_seqlen_q, kWholeKeys + 1)
-                        .bytes());
+    n = std::max(n, plan_bytes(num_q_tokens - num_decode_rows, num_heads, num_kv_heads,
+                               num_prefill, max_seqlen_q));
   return n;
 }
 
@@ -1627,8 +1694,7 @@ extern "C" size_t kvc_tree_workspace_bytes(int64_t num_q_tokens, int64_t num_hea
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || num_q_tokens <= 0 ||
       num_heads / num_kv_heads > kFormColumns[kForms - 1])
     return 0;
-  return make_plan(num_q_tokens, num_heads, num_kv_heads, batch, max_seqlen_q, kWholeKeys + 1)
-             .bytes() +
+  return plan_bytes(num_q_tokens, num_heads, num_kv_heads, batch, max_seqlen_q) +
          up256(size_t(num_q_tokens) * sizeof(int32_t));
 }
 

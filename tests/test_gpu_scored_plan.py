@@ -178,3 +178,38 @@ def test_caps_where_series_and_exponentials_meet(cap):
     for wide in (0.5, 4.0, 20.0):
         _chunks(_normal(40, 8, 22, wide), ks, vs, chunks, f"cap {cap} width {wide}",
                 pool=(kc, vc, bt), cap=cap)
+
+
+@pytest.mark.parametrize("form", [dict(), dict(softcap=50.0), dict(softcap=200.0),
+                                  dict(alibi_slopes=True), dict(softcap=50.0, alibi_slopes=True)])
+@pytest.mark.parametrize("batch,most,ctx", [(8, 8, 2500), (80, 16, 2500), (80, 31, 4000)])
+def test_long_trees_of_every_width(batch, most, ctx, form):
+    """64, 128 and 256 columns of one kv head, contexts long enough that items
+    are cut between workgroups.  A few of the sequences against 64 bits."""
+    heads = 8
+    gen = torch.Generator().manual_seed(23)
+    sizes = [max(1, most - i % 4) for i in range(batch)]
+    lens = [ctx - (97 * i) % 400 for i in range(batch)]
+    kc, vc, bt, ks, vs = paged([c + n for c, n in zip(lens, sizes)], 64, 1, 24)
+    mask, bits = torch.zeros(sum(sizes), 1, dtype=torch.int64), []
+    cu = [0]
+    for n in sizes:
+        b = torch.eye(n, dtype=torch.bool)
+        for t in range(1, n):
+            b[t] |= b[int(torch.randint(0, t, (1,), generator=gen))]
+            mask[cu[-1] + t, 0] = sum(1 << u for u in range(n) if b[t, u])
+        mask[cu[-1], 0] = 1
+        bits.append(b)
+        cu.append(cu[-1] + n)
+    q = _normal(sum(sizes), heads, 25)
+    kw = dict(form)
+    sl = slopes_of(heads) if kw.pop("alibi_slopes", False) else None
+    out = tree_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), bt.to(DEV), _i32(lens), mask.to(DEV),
+                         SCALE, cu_seqlens_q=_i32(cu), max_seqlen_q=most,
+                         alibi_slopes=None if sl is None else sl.to(DEV), **kw)
+    for i in range(0, batch, max(1, batch // 3)):
+        sees, away = tree_mask(bits[i], lens[i], 0)
+        w, b = attend(q[cu[i]:cu[i + 1]], ks[i], vs[i], sees, away, scale=SCALE,
+                      cap=kw.get("softcap", 0.0), slopes=sl)
+        check(out[cu[i]:cu[i + 1]], w, b, f"{batch} trees of {most} over {ctx}, sequence {i} {form}")
+    assert bool(torch.isfinite(out).all())
