@@ -11,7 +11,9 @@
 // order holds whatever the device holds.
 //
 // Bound by latency (lengths, path, table, row: four dependent reads) for one
-// user, by HBM for a batch: each moved row is read and written once.
+// user (4 us), by HBM for a batch: each moved row is read and written once (64
+// sequences, K and V of 28 layers, 29 MB both ways: 7.5 us, of which the four
+// reads are half).
 #include "kvc_internal.h"
 
 namespace kvc {

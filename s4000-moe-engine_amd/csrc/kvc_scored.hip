@@ -12,20 +12,32 @@
 // Layout of the work.  The G query heads of one kv head and the tokens of a
 // block are the columns of S^T = K Q^T (a lane owns one column, so a row's
 // softmax never leaves its four lane groups), and P, rounded to bf16 as the
-// MFMA takes it, is already the operand of O^T = V^T P^T.  An item is one
-// block of columns of one kv head (or of one column block of several heads,
-// see below) against its visible 32-key tiles; the concatenated tiles of all
-// items are cut into equal shares, one workgroup each, on the device from the
-// device's lengths, so a call needs no lengths on the host and can be
-// captured.  An item cut between shares leaves fp32 partials that a second
-// launch joins.
+// MFMA takes it, is already the operand of O^T = V^T P^T; logits, sums and O
+// are fp32.  An item is one block of columns against the 32-key tiles it sees;
+// the tiles of all items, in one row, are cut into equal shares, one workgroup
+// each, on the device from the device's lengths, so a call needs no lengths on
+// the host and can be captured.  An item cut between shares leaves fp32
+// partials that a second launch joins.  Short calls are not cut and have no
+// second launch (make_plan).
 //
-// Two forms share the tile arithmetic:
-//   private  few columns (decode rows, small trees): every wave streams its
-//            own tiles through its own LDS slots, without a workgroup
-//            barrier; waves differ in kv head and in tile phase.
-//   shared   many columns (chunks, large trees): the waves split the columns
-//            and read the same tile from a ring of LDS stages.
+// Two kinds of form share the tile arithmetic:
+//   private  up to 32 columns (decode rows, small trees): every wave streams
+//            its own tiles through its own LDS slots, without a workgroup
+//            barrier; waves differ in kv head and in tile phase.  Bound by HBM
+//            in a batch (48 ragged decode rows with a distance bias: 447 MB in
+//            71 us, 6.3 TB/s, of about 6.9 that reading alone reaches), by
+//            latency for one user (333 keys, 8 us: launch, lengths, table,
+//            queries, two rounds of tiles and the join in turn).
+//   turns    64 to 256 columns (chunks, larger trees): the waves split the
+//            columns and read the same tile from a ring of LDS slots; one half
+//            multiplies while the other takes its softmax.  Bound by the issue
+//            of both: 2100 cycles a 256-column tile for plain scores, 2550 for
+//            capped ones, of which the matrix unit is busy 1024 (64 trees of
+//            64 tokens over 4096 keys: 838 TFLOP/s; a chunk of 2048 over 14336
+//            keys, capped: 880).
+// Tried and not kept in the turns form: V operands read under the softmax
+// instead of under the products (chunk 570 -> 620 us), half of the caps taken
+// between the products of O (no change).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -754,9 +766,9 @@ __device__ __forceinline__ void wait_loads() {  // all but the newest N
 __device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// The kernel.  NW waves; KW of them take different tiles of a segment in the
-// shared form (the others share a tile and split the columns); KW = NW is the
-// private form, where waves split over heads_per_wg kv heads and tile phases.
+// The kernel.  NW waves.  Turns forms: a step has KW tiles, and NW / KW waves
+// attend each, 16 NCB columns a wave.  KW = NW is the private form, where waves
+// split over heads_per_wg kv heads and tile phases.
 // ---------------------------------------------------------------------------
 template <int NW, int NCB, int KW>
 struct Form {
@@ -1350,7 +1362,13 @@ Plan lay_out(int form, bool whole, int64_t tokens, int64_t group, int64_t kv_hea
   pl.form = form;
   pl.whole = whole;
   pl.columns = kFormColumns[form];
-  int most = form <= 1 && !whole ? 4 : 1;
+  // kv heads a private workgroup takes together (neighbours in a token's row,
+  // read together): that suits HBM when the items fill the card, more and
+  // smaller pieces when they do not.  Measured with 1 / 2 / 4: 16 decode rows of
+  // 4 kv heads over 2048 keys 19.8 / 20.7 / 23.8 us, 16 of 8 heads 30.3 / 28.0 /
+  // 29.7, 48 ragged rows of 4 heads 80.2 / 78.4 / 77.3.
+  const int64_t items = batch * kv_heads;
+  int most = form > 1 || whole || items <= cu_count() / 4 ? 1 : items <= cu_count() / 2 ? 2 : 4;
   while (most > 1 && kv_heads % most != 0) most >>= 1;
   pl.heads_per_wg = most;
   pl.head_groups = int(kv_heads / most);
@@ -1377,8 +1395,8 @@ int holding_form(int64_t longest, int64_t group) {
 // private forms serve, the narrowest that holds them.  Over at most kWholeKeys
 // keys, and with a workgroup for each, their items stay whole: nothing is cut
 // and the merge is not launched.  One decode row of 8 kv heads, whole against
-// cut: 10.3 / 14.7 us over 512 keys, 17.4 / 15.0 over 1024 (one CU's loads
-// bound it then).
+// cut: 10.3 / 13 us over 512 keys, 17.4 / 13.6 over 1024 (one CU's loads bound
+// it then).
 //
 // Wider rows take any turns form up to the narrowest that holds them, whole or
 // cut, whichever these estimates call cheapest, in tenths of a 256-column
@@ -1500,6 +1518,9 @@ int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStrea
   const int64_t nb = (std::min<int64_t>(max_q, p.num_tokens) + pl.tokens_per_block - 1) /
                      pl.tokens_per_block;
   p.lane_plan = (p.batch + 63) / 64 * nb <= p.batch + p.num_tokens / pl.tokens_per_block / 64;
+  // A share has four tiles at least: with 2 / 4 / 8, one decode row over 2048
+  // keys took 20.2 / 17.9 / 20.4 us (8 kv heads, 4 a workgroup), 16.0 / 14.5 /
+  // 15.2 (2 kv heads, both in one).
   p.min_share = 4;
   p.whole = pl.whole;
   char* w = static_cast<char*>(ws);
