@@ -437,10 +437,10 @@ size_t kvc_scored_workspace_bytes(int64_t num_q_tokens, int64_t num_heads, int64
  *   s -= alibi_slopes[h] |p - j| when alibi_slopes (fp32 [num_heads]) is given.
  * out = softmax(s) . v; a query that sees no key gives 0.  Values at keys a
  * query does not see never reach it, infinities and NaN included.  A block id
- * outside the pool reads as zeros.  max_seqlen_q (the longest chunk) chooses
- * the launch's form; the lengths themselves are read on the device.  Rows of
- * q / out / k_fresh / v_fresh are 16-byte aligned; at most 256 query heads
- * per kv head. */
+ * outside the pool reads as zeros.  max_seqlen_q (the longest chunk) and the
+ * table's width steer the launch; the lengths themselves are read on the
+ * device.  Rows of q / out / k_fresh / v_fresh are 16-byte aligned; at most 256
+ * query heads per kv head; scale > 0, and scale / softcap must be finite. */
 int kvc_scored_attention(
     const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_q_tokens, int64_t num_heads,
     const void* k_cache, const void* v_cache, int64_t num_cache_blocks, int64_t page_size,

@@ -47,8 +47,8 @@ def tree_attention(q, k_cache, v_cache, block_tables, context_lens, tree_mask, s
     Token t sees every context key and the tree keys of its mask (tree_mask
     int64 [T, words], bit u % 64 of word u / 64).  softcap, alibi_slopes and
     window as in scored_attention, with the token's depth (bits in its mask,
-    less one) for its distance from the context.  Returns out [T, H, 128];
-    a token that sees no key gives 0."""
+    less one) for its distance from the context.  Returns out [T, H, 128]; a
+    token that sees no key gives 0, rows past the last tree are not written."""
     if nat.is_current(q):
         done = nat.host().tree(q, k_cache, v_cache, block_tables, context_lens, tree_mask, scale,
                                cu_seqlens_q, max_seqlen_q, softcap, alibi_slopes, window,
@@ -103,7 +103,8 @@ def commit_tree_path(kv_cache, block_tables, context_lens, paths, path_lens):
     [2, L, blocks, page, ...], or a companion of an int8 pool of that shape
     (scales, side rows); paths int32 [batch, most], a path strictly
     increasing (tree tokens come after their parents): it ends at the first
-    entry that is not."""
+    entry that is not.  No two sequences may share the pages behind their
+    contexts."""
     if nat.is_current(kv_cache) and nat.host().commit(kv_cache, block_tables, context_lens, paths,
                                                       path_lens, nat.stream_of(kv_cache)):
         return

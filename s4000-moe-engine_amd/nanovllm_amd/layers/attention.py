@@ -83,7 +83,7 @@ class Attention(nn.Module):
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.softcap = softcap
-        self.alibi_slopes = alibi_slopes
+        self.register_buffer("alibi_slopes", alibi_slopes, persistent=False)
         self.window = window
         self.block_size = None
         self.k_cache = self.v_cache = torch.tensor([])

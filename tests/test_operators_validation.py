@@ -227,3 +227,12 @@ def test_caps_and_scales_that_fp32_cannot_divide():
                       0, None, 0, 0, 0, at, 1, 1, 1, at, 0, None, None, 1, None, None, cap, 0,
                       scale, at, 1024, 128, at, 0, None)
         assert got == rc and msg, (cap, scale, got, msg)
+
+
+def test_a_layers_slopes_move_with_it():
+    from nanovllm_amd.layers.attention import Attention
+    layer = Attention(8, 128, 0.1, 2, alibi_slopes=torch.ones(8))
+    assert dict(layer.named_buffers())["alibi_slopes"] is layer.alibi_slopes
+    assert not layer.state_dict()
+    assert layer.to("meta").alibi_slopes.device.type == "meta"
+    assert Attention(8, 128, 0.1, 2).alibi_slopes is None
