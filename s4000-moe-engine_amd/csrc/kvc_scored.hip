@@ -601,19 +601,21 @@ __device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int 
   int mine_pre = 0;
   g = SeqGeo{0, 0, 0};
   pre = 0;
-  if (p.whole && (p.batch == 1 || p.cu_q == nullptr)) {  // as many items in each sequence
+  if (p.whole && (p.batch == 1 || p.cu_q == nullptr)) {
+    // As many items in each sequence: no walk, and (small calls are all
+    // latency) no division where the quotient is plain.
     g = load_seq<true>(p, 0);
-    const int n = num_blocks_of(p, g.sq);
+    const int n = g.sq <= p.tokens_per_block ? min(g.sq, 1) : num_blocks_of(p, g.sq);
     const int each = n * p.head_groups;
     w.total = each * p.batch;
-    size = (w.total + shares - 1) / shares;
+    size = w.total <= shares ? 1 : (w.total + shares - 1) / shares;
     const int64_t at = int64_t(share) * size;
     if (at >= w.total) return false;
     w.seq = p.batch == 1 ? 0 : int(at) / each;
     if (w.seq != 0) g = load_seq<true>(p, w.seq);
     if (p.prefix != nullptr) pre = table_entry(p.prefix, w.seq);
     const int rem = int(at) - w.seq * each;
-    w.grp = rem / n;
+    w.grp = n == 1 ? rem : rem / n;
     w.block = rem - w.grp * n;
     w.tile = 0;
     return true;
@@ -847,6 +849,8 @@ __global__ void __launch_bounds__(64 * NW)
   const int share = grid % 8 == 0 ? (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
 
   touch_kernel_args(int(sizeof(ScoredParams)));
+  // The tables' first line on its way beside the lengths'.
+  int warm = p.whole && p.tables != nullptr && p.max_blocks > 0 ? table_entry(p.tables, 0) : 0;
   Where w;
   SeqGeo g;
   int size, pre;
@@ -856,6 +860,7 @@ __global__ void __launch_bounds__(64 * NW)
     return;
   }
 
+  asm volatile("" ::"s"(warm));
   const int hs = F::kPrivate ? wave % p.heads_per_wg : 0;
   const int phases = F::kPrivate ? NW / p.heads_per_wg : KW;
   const int phase = F::kPrivate ? wave / p.heads_per_wg : wave / F::kColWaves;
@@ -871,12 +876,13 @@ __global__ void __launch_bounds__(64 * NW)
   constexpr float mu0 = MODE == kCapFixed ? 0.f : kLowest;
 
   const int col0 = cw * NCB * 16;
-  const int wave_t0 = col0 / p.group;
-  const int wave_t1 = min((col0 + NCB * 16 - 1) / p.group, p.tokens_per_block - 1);
+  const int wave_t0 = uniform(div_small(col0, p.group, p.group_rcp));
+  const int wave_t1 = min(uniform(div_small(col0 + NCB * 16 - 1, p.group, p.group_rcp)),
+                          p.tokens_per_block - 1);
 
   const int end = int(min(w.total, int64_t(share + 1) * size));
   int pos = share * size;
-  int nblocks = num_blocks_of(p, g.sq);
+  int nblocks = g.sq <= p.tokens_per_block ? 1 : num_blocks_of(p, g.sq);
   while (true) {
     const TileRange range = block_tiles(p, g, pre, w.block);
     const int tiles = range.t1 - range.t0;
@@ -978,8 +984,10 @@ __global__ void __launch_bounds__(64 * NW)
         u32x4_t k[2][4];
         for (; t < t_end; t += phases) {
           const bool more = t + phases < t_end;
-          const int tn = more ? t + phases : t;
-          const TileSource next = tile_source(p, fresh0, g.sk, head, tn, page_entry(p, w.seq, tn));
+          TileSource next = {};
+          if (more)
+            next = tile_source(p, fresh0, g.sk, head, t + phases,
+                               page_entry(p, w.seq, t + phases));
           const int j0 = t * kTile;
           const bool masked = j0 < c.full_lo || j0 + kTile > c.full_hi;
           wait_loads<8>();
@@ -1221,9 +1229,9 @@ __global__ void __launch_bounds__(64 * NW)
         const int owners = NW / phases;
         const char* first = smem + (wave % owners) * F::kStateBytes;
         const int step = owners * F::kStateBytes;
-        __syncthreads();
+        pf_barrier();
         put_state<NCB>(smem + wave * F::kStateBytes, st, lane);
-        __syncthreads();
+        pf_barrier();
         if (phases == 2) {
           join_states<NCB, 2>(first, step, phase, lane, emit);
         } else if constexpr (F::kPrivate) {
@@ -1233,7 +1241,7 @@ __global__ void __launch_bounds__(64 * NW)
             join_states<NCB, 8>(first, step, phase, lane, emit);
           }
         }
-        __syncthreads();
+        pf_barrier();
       } else {
         pf_barrier();  // the ring is free for the next item
 #pragma unroll

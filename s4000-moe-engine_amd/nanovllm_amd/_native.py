@@ -214,11 +214,15 @@ def call(name: str, *args) -> int:
     return rc
 
 
+# (torch.cuda.current_device without its initialisation check: a tensor on the
+# GPU has passed that)
+_current_gpu = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def is_current(t) -> bool:
     """t is a tensor on the current GPU (the native host path makes its
     launches there)."""
-    return isinstance(t, torch.Tensor) and t.is_cuda \
-        and t.get_device() == torch.cuda.current_device()
+    return isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == _current_gpu()
 
 
 def call_on(t: torch.Tensor, name: str, *args) -> int:
