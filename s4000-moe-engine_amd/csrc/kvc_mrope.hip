@@ -16,8 +16,8 @@
 // the token's head rows: lane j holds dims 8 j .. 8 j + 7 and 64 + 8 j ..,
 // 16 bytes each, so a rotation pair never leaves its lane and the sum of
 // squares is three DPP moves.  Bound by HBM: each row is read and written
-// once; 16384 tokens of 32 / 4 heads, 344 MB, take 72 us (4.8 TB/s, a large
-// copy's rate).  A decode step of 64 tokens takes 4 us, the launch and three
+// once; 16384 tokens of 32 / 4 heads, 344 MB, take 67 us (5.1 TB/s; torch's
+// copy of 2 GiB 4.9), 58 where a part of them is cached still.  A decode step of 64 tokens takes 4 us, the launch and three
 // dependent reads (position, table, row).
 #include "kvc_lds.h"
 
@@ -176,16 +176,23 @@ __global__ void __launch_bounds__(kThreads) qk_norm_mrope_store_kernel(MropeArgs
         o2[i / 2] = pack_bf16x2_fast(x2[i] * c[i] + x1[i] * s[i],
                                      x2[i + 1] * c[i + 1] + x1[i + 1] * s[i + 1]);
       }
+      if (kr < 0) {
+        // Past the caches: q_out is most of what is written, and pushed out of
+        // them by itself before attention reads it.  Measured, 16384 tokens of
+        // 32 / 4 heads, the same call again: 58 us so, 73 through the caches, 57
+        // with the pool's rows past them too; with inputs from HBM 67 so, 72
+        // through the caches.  Attention after it takes as long in all three.
+        uint16_t* row = a.q_out + n * a.qo_st + r * a.qo_sh;
+        __builtin_nontemporal_store(o1, reinterpret_cast<u32x4_t*>(row + 8 * j));
+        __builtin_nontemporal_store(o2, reinterpret_cast<u32x4_t*>(row + kPairs + 8 * j));
+        continue;
+      }
       auto put = [&](uint16_t* row) {
         *reinterpret_cast<u32x4_t*>(row + 8 * j) = o1;
         *reinterpret_cast<u32x4_t*>(row + kPairs + 8 * j) = o2;
       };
-      if (kr < 0) {
-        put(a.q_out + n * a.qo_st + r * a.qo_sh);
-      } else {
-        if (a.k_out != nullptr) put(a.k_out + n * a.ko_st + kr * a.ko_sh);
-        if (sl >= 0) put(a.k_cache + (sl * a.num_kv_heads + kr) * kD);
-      }
+      if (a.k_out != nullptr) put(a.k_out + n * a.ko_st + kr * a.ko_sh);
+      if (sl >= 0) put(a.k_cache + (sl * a.num_kv_heads + kr) * kD);
     }
   }
 }
@@ -300,8 +307,8 @@ extern "C" int kvc_qk_norm_mrope_store(
   const int sb = cache ? slot_index_bytes : 4;
   // Four tokens a workgroup share its position and table loads; up to 1024
   // tokens one each keeps every CU busy.  Measured, 1 / 4 a workgroup (32 / 4
-  // heads): 64 tokens 5.5 / 6.4 us, 1024 6.1 / 7.6, 2048 11.6 / 10.7, 16384
-  // 94.9 / 72.7.
+  // heads, q_out through the caches): 64 tokens 5.5 / 6.4 us, 1024 6.1 / 7.6,
+  // 2048 11.6 / 10.7, 16384 94.9 / 72.7.
   if (num_tokens > 1024) {
     launch<4, 5>(a, position_index_bytes, sb, st);
   } else {
