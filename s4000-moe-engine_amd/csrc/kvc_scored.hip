@@ -100,7 +100,8 @@ struct ScoredParams {
   int lane_plan;  // the plan walks sequences across lanes (else blocks)
   int min_share;
   int whole;  // items are not cut: a share counts items
-  int4* rec;  // per share: the item it begins and leaves unfinished
+  int4* rec;  // per share, of the item it begins and leaves unfinished: first
+              // token, tokens, head group, last share (0: none)
   float* part_o;
   float2* part_ml;
 };
@@ -890,7 +891,9 @@ __global__ void __launch_bounds__(64 * NW)
     if (!p.whole && pos + tiles + kItemCost - w.tile >= end && threadIdx.x == 0) {
       // The share's last item: where it goes on, if it began here.
       const int last = tiles > 0 ? (pos - w.tile + tiles - 1) / size : share;
-      p.rec[share] = int4{w.seq, w.block, w.grp, w.tile == 0 && last > share ? last : 0};
+      const int b0 = w.block * p.tokens_per_block;
+      p.rec[share] = int4{g.q0 + b0, min(g.sq - b0, p.tokens_per_block), w.grp,
+                          w.tile == 0 && last > share ? last : 0};
     }
     if (seg0 < seg1 || (tiles == 0 && w.tile == 0)) {
       const int head = w.grp * p.heads_per_wg + hs;
@@ -1283,11 +1286,8 @@ __global__ void __launch_bounds__(32 * kMergeColumns)
   const int per_head = columns / kMergeColumns;
   const int hs = blockIdx.y / per_head;
   const int col = (blockIdx.y - hs * per_head) * kMergeColumns + int(threadIdx.x >> 5);
-  const SeqGeo g = load_seq<true>(p, r.x);
   const int head = r.z * p.heads_per_wg + hs;
-  const int b0 = r.y * p.tokens_per_block;
-  const int tokens = min(g.sq - b0, p.tokens_per_block);
-  if (col >= tokens * p.group) return;
+  if (col >= r.y * p.group) return;
   const int lane = threadIdx.x & 31;
   const int64_t cols = int64_t(p.heads_per_wg) * columns, at = hs * columns + col;
   float top = kLowest, l = 0.f;
@@ -1315,7 +1315,7 @@ __global__ void __launch_bounds__(32 * kMergeColumns)
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
   const int t = col / p.group;
-  uint16_t* dst = p.out + int64_t(g.q0 + b0 + t) * p.o_st +
+  uint16_t* dst = p.out + int64_t(r.x + t) * p.o_st +
                   int64_t(head * p.group + col - t * p.group) * p.o_sh + 4 * lane;
   *reinterpret_cast<u32x2_t*>(dst) =
       u32x2_t{pack_bf16x2_fast(o[0] * inv, o[1] * inv), pack_bf16x2_fast(o[2] * inv, o[3] * inv)};
