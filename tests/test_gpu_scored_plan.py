@@ -213,3 +213,42 @@ def test_long_trees_of_every_width(batch, most, ctx, form):
                       cap=kw.get("softcap", 0.0), slopes=sl)
         check(out[cu[i]:cu[i + 1]], w, b, f"{batch} trees of {most} over {ctx}, sequence {i} {form}")
     assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("batch", [40, 100])
+def test_uncut_items_in_several_rounds(batch):
+    """Windowed chunks: several whole items a workgroup, among them sequences
+    without queries.  A few of the sequences against 64 bits."""
+    heads = kvh = 8
+    chunks = [(0 if i % 13 == 5 else 40 - i % 9, 300 - i) for i in range(batch)]
+    kc, vc, bt, ks, vs = paged([m for _, m in chunks], 32, kvh, 27)
+    cu_q, cu_k = [0], [0]
+    for n, m in chunks:
+        cu_q.append(cu_q[-1] + n)
+        cu_k.append(cu_k[-1] + m)
+    q = _normal(cu_q[-1], heads, 28)
+    out = scored_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), scale=SCALE, window=20, softcap=50.0,
+                           block_tables=bt.to(DEV), cu_seqlens_q=_i32(cu_q),
+                           cu_seqlens_k=_i32(cu_k), cu_seqlens_q_list=cu_q, cu_seqlens_k_list=cu_k)
+    for i in range(0, batch, 7):
+        n, m = chunks[i]
+        if n == 0:
+            continue
+        w, b = attend(q[cu_q[i]:cu_q[i + 1]], ks[i], vs[i], *chunk_mask(n, m, 20, 0), scale=SCALE,
+                      cap=50.0)
+        check(out[cu_q[i]:cu_q[i + 1]], w, b, f"{batch} windowed chunks, sequence {i}")
+    assert bool(torch.isfinite(out).all())
+
+
+def test_tables_without_pages():
+    """Rows whose table holds no page at all see no key."""
+    kc = torch.randn(2, 32, 2, 128).to(torch.bfloat16).to(DEV)
+    tables = torch.zeros(3, 5, dtype=torch.int32, device=DEV)
+    q = _normal(3, 8, 29).to(DEV)
+    with pytest.raises(ValueError):
+        scored_attention(q, kc, kc, scale=SCALE, block_tables=torch.zeros(
+            3, 0, dtype=torch.int32, device=DEV), num_decode_rows=3,
+            decode_context_lens=_i32([1, 2, 3]))
+    out = scored_attention(q, kc, kc, scale=SCALE, block_tables=tables, num_decode_rows=3,
+                           decode_context_lens=_i32([0, 0, 0]))
+    assert not out.any()
