@@ -19,7 +19,9 @@ store_kvcache(k, v, k_cache, v_cache, slot_mapping) then the paged decode,
 as one paged_decode_append call (the append rides in the decode launch; a
 padded row's slot is position 0 of its scratch-block table row, as the fused
 append requires), which writes the runner's output buffer itself: a copy
-node per layer cost 4-5 us each on the replay's critical path.  Nothing
+node per layer cost 4-5 us each on the replay's critical path.  A layer with
+shaped scores (a cap, a bias by distance, a window) appends in a launch of its
+own, then attends through scored_attention into the same buffer.  Nothing
 records a host synchronisation or a memset: loop
 bounds come from the device context_lens, and the split-K workspace is taken
 from torch's caching allocator (the graph's private pool during capture).
@@ -30,6 +32,8 @@ import torch
 
 from .. import _native as nat
 from ..kernels.paged_attention import decode_append_into
+from ..kernels.scored import scored_attention
+from ..layers.attention import store_kvcache
 
 
 def default_buckets(max_bs: int) -> list[int]:
@@ -65,10 +69,13 @@ class DecodeGraphRunner:
     offload, a put may still be reading a block that the replay appends
     into after the block manager reallocated it, and a replayed graph holds
     none of the eager per-layer waits).  from_kv_runner binds it; a runner
-    built without one is for pools that no asynchronous move touches."""
+    built without one is for pools that no asynchronous move touches.
+
+    score_shapes: scored_attention's softcap, alibi_slopes and window as a dict,
+    for all layers or one per layer (None or an empty dict: plain scores)."""
 
     def __init__(self, k_caches, v_caches, num_heads: int, max_bs: int, max_blocks_per_seq: int,
-                 scale: float, buckets: list[int] | None = None, fence=None):
+                 scale: float, buckets: list[int] | None = None, fence=None, score_shapes=None):
         assert len(k_caches) == len(v_caches) and len(k_caches) > 0
         self.fence = fence
         self.k_caches, self.v_caches = list(k_caches), list(v_caches)
@@ -96,10 +103,19 @@ class DecodeGraphRunner:
                                        dtype=torch.int32, device=dev)
         self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self.pool = None
+        if score_shapes is None or isinstance(score_shapes, dict):
+            score_shapes = [score_shapes] * L
+        if len(score_shapes) != L:
+            raise ValueError(f"{len(score_shapes)} score shapes for {L} layers")
+        self.score_shapes = [dict(s) if s else {} for s in score_shapes]
+        for s in self.score_shapes:
+            if not set(s) <= {"softcap", "alibi_slopes", "window"}:
+                raise ValueError(f"a score shape has softcap, alibi_slopes and window (got {set(s)})")
 
     @classmethod
     def from_kv_runner(cls, kv_runner, num_heads: int, max_bs: int, max_blocks_per_seq: int,
-                       scale: float, buckets: list[int] | None = None) -> "DecodeGraphRunner":
+                       scale: float, buckets: list[int] | None = None,
+                       score_shapes=None) -> "DecodeGraphRunner":
         """A runner over every layer of a KVCacheRunner's bf16 pool, fenced by
         that runner (its asynchronous offload copies, if any, are ordered
         before each capture and replay)."""
@@ -108,12 +124,19 @@ class DecodeGraphRunner:
         k_caches = [kv_runner.kv_cache[0, i] for i in range(kv_runner.num_layers)]
         v_caches = [kv_runner.kv_cache[1, i] for i in range(kv_runner.num_layers)]
         return cls(k_caches, v_caches, num_heads, max_bs, max_blocks_per_seq, scale, buckets,
-                   fence=kv_runner.fence)
+                   fence=kv_runner.fence, score_shapes=score_shapes)
 
     def _step(self, bs: int) -> None:
         sm, cl, bt = self.slot_mapping[:bs], self.context_lens[:bs], self.block_tables[:bs]
         for layer in range(self.num_layers):
             kc, vc = self.k_caches[layer], self.v_caches[layer]
+            shape = self.score_shapes[layer]
+            if shape:
+                store_kvcache(self.k[layer, :bs], self.v[layer, :bs], kc, vc, sm)
+                scored_attention(self.q[layer, :bs], kc, vc, scale=self.scale, block_tables=bt,
+                                 num_decode_rows=bs, decode_context_lens=cl,
+                                 out=self.out[layer, :bs], **shape)
+                continue
             decode_append_into(
                 self.out[layer, :bs], self.q[layer, :bs], self.k[layer, :bs], self.v[layer, :bs],
                 kc, vc, sm, bt, cl, self.scale)

@@ -83,7 +83,7 @@ def _int32(t, n, what, device):
 def scored_attention(q, k_cache, v_cache, *, scale, block_tables=None, num_decode_rows=0,
                      decode_context_lens=None, cu_seqlens_q=None, cu_seqlens_k=None,
                      cu_seqlens_q_list=None, cu_seqlens_k_list=None, k=None, v=None,
-                     softcap=0.0, alibi_slopes=None, window=0, prefix_lens=None):
+                     softcap=0.0, alibi_slopes=None, window=0, prefix_lens=None, out=None):
     """q: [T, H, 128] bf16 with T = num_decode_rows + prefill tokens, rows and
     keys as in varlen_attention (a bf16 pool through block_tables, or the
     step's fresh k / v when block_tables is None).  A query at place p sees
@@ -91,8 +91,8 @@ def scored_attention(q, k_cache, v_cache, *, scale, block_tables=None, num_decod
     and, with a window, p - j < window; its score is scale q.k, then
     softcap * tanh(score / softcap) if softcap > 0, then minus
     alibi_slopes[h] * |p - j| (fp32 [H]) if given.  Returns out [T, H, 128]
-    bf16; a query that sees no key gives 0."""
-    if nat.is_current(q):
+    bf16 (the given one, or a new one); a query that sees no key gives 0."""
+    if out is None and nat.is_current(q):
         done = nat.host().scored(q, k_cache, v_cache, block_tables, num_decode_rows,
                                  decode_context_lens, cu_seqlens_q, cu_seqlens_k,
                                  cu_seqlens_q_list, cu_seqlens_k_list, k, v, softcap,
@@ -159,8 +159,13 @@ def scored_attention(q, k_cache, v_cache, *, scale, block_tables=None, num_decod
         max_blocks = block_tables.size(1)
         pool = (k_cache.data_ptr(), v_cache.data_ptr(), blocks, page, kvh, head_dim, None, 0, 0,
                 None, 0, 0, 0, block_tables.data_ptr(), block_tables.stride(0), max_blocks)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype
+                            or out.device != q.device or not _rows_ok(out)):
+        raise ValueError("out must be bf16 [tokens,heads,128] on q's device, its rows 16-byte "
+                         "aligned")
     nat.require_device(q)
-    out = torch.empty((T, num_heads, head_dim), dtype=q.dtype, device=q.device)
+    if out is None:
+        out = torch.empty((T, num_heads, head_dim), dtype=q.dtype, device=q.device)
     if T == 0:
         return out
     need = nat.query("kvc_scored_workspace_bytes", T, num_heads, kvh, num_decode_rows, num_prefill,

@@ -236,3 +236,23 @@ def test_a_layers_slopes_move_with_it():
     assert not layer.state_dict()
     assert layer.to("meta").alibi_slopes.device.type == "meta"
     assert Attention(8, 128, 0.1, 2).alibi_slopes is None
+
+
+@pytest.mark.parametrize("out", [torch.zeros(2, 8, 128, dtype=torch.bfloat16),
+                                 torch.zeros(3, 8, 128),
+                                 torch.zeros(3, 8, 132, dtype=torch.bfloat16)[..., 4:]])
+def test_scored_attention_refuses_other_outputs(out):
+    with pytest.raises(ValueError, match="out must be"):
+        _scored(out=out)
+
+
+def test_graph_runner_checks_score_shapes():
+    from nanovllm_amd.engine.graph_runner import DecodeGraphRunner
+    caches = [torch.zeros(3, 32, 2, 128, dtype=torch.bfloat16) for _ in range(2)]
+    for bad in ([dict(window=3)], dict(cap=50.0), [dict(), dict(prefix_lens=None)]):
+        with pytest.raises(ValueError, match="score shape"):
+            DecodeGraphRunner(caches, caches, 8, 2, 2, 0.1, score_shapes=bad)
+    one = dict(window=3)
+    runner = DecodeGraphRunner(caches, caches, 8, 2, 2, 0.1, score_shapes=[None, one])
+    assert runner.score_shapes == [{}, one]
+    assert DecodeGraphRunner(caches, caches, 8, 2, 2, 0.1, score_shapes=one).score_shapes == [one] * 2
