@@ -13,7 +13,9 @@ constexpr int kBufWord3 = 0x00020000;  // gfx9 raw buffer: 32-bit data format
 // the compiler's wait-count pass does not treat it as a pending LDS write
 // (it would then drain every load in flight before each barrier and LDS read,
 // serialising the prefetch); the caller waits with explicit vmcnt counts.
-// M0 carries the LDS address and is restored afterwards.
+// M0 carries the LDS address and is restored afterwards; a load may not read
+// it in the cycle after a scalar write (one wait state, which the compiler
+// does not insert inside inline asm).
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i32x4_t raw_rsrc(const void* base, int bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
@@ -27,6 +29,7 @@ __device__ __forceinline__ void dma_to_lds(const i32x4_t& rsrc, int voff, uint32
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
       "buffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
@@ -41,6 +44,7 @@ __device__ __forceinline__ void dma_to_lds_cached(const i32x4_t& rsrc, int voff,
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
       "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
