@@ -86,7 +86,8 @@ def scored_attention(q, k_cache, v_cache, *, scale, block_tables=None, num_decod
                      softcap=0.0, alibi_slopes=None, window=0, prefix_lens=None, out=None):
     """q: [T, H, 128] bf16 with T = num_decode_rows + prefill tokens, rows and
     keys as in varlen_attention (a bf16 pool through block_tables, or the
-    step's fresh k / v when block_tables is None).  A query at place p sees
+    step's fresh k / v when block_tables is None; cu_seqlens_q starts at 0,
+    the first row after the decode rows).  A query at place p sees
     key j when j <= p or j < prefix_lens[i] (int32, one per prefill chunk),
     and, with a window, p - j < window; its score is scale q.k, then
     softcap * tanh(score / softcap) if softcap > 0, then minus
@@ -111,15 +112,18 @@ def scored_attention(q, k_cache, v_cache, *, scale, block_tables=None, num_decod
         cu_q = cu_seqlens_q_list if cu_seqlens_q_list is not None else cu_seqlens_q.tolist()
         cu_k = cu_seqlens_k_list if cu_seqlens_k_list is not None else cu_seqlens_k.tolist()
         num_prefill = len(cu_q) - 1
-        if len(cu_k) != len(cu_q):
-            raise ValueError("cu_seqlens_q and cu_seqlens_k differ in length")
+        if len(cu_k) != len(cu_q) or not cu_q:
+            raise ValueError("cu_seqlens_q and cu_seqlens_k differ in length or are empty")
+        if cu_q[0] != 0 or cu_k[0] < 0:
+            raise ValueError("cu_seqlens_q must start at 0, cu_seqlens_k at 0 or later (got "
+                             f"{cu_q[0]}, {cu_k[0]})")
         for i in range(num_prefill):
             n, m = cu_q[i + 1] - cu_q[i], cu_k[i + 1] - cu_k[i]
             if n < 0 or m < 0 or (n > 0 and m < n):
                 raise ValueError("a prefill chunk has fewer keys than queries")
             max_q = max(max_q, n)
         keys = cu_k[-1]
-        tokens = cu_q[-1] - cu_q[0]
+        tokens = cu_q[-1]
     else:
         tokens = 0
     if num_decode_rows + tokens != T:

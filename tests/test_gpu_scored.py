@@ -294,3 +294,15 @@ def test_two_streams_at_once():
     for i in range(2):
         for got in outs[i]:
             assert torch.equal(got, want[i])
+
+
+def test_fresh_keys_from_a_later_row():
+    """cu_seqlens_k are rows of k / v and may start past the first."""
+    gen = torch.Generator().manual_seed(36)
+    k, v = (torch.randn(60, 2, 128, generator=gen).to(torch.bfloat16) for _ in range(2))
+    q = _queries(45, 8, 37)
+    out = scored_attention(q.to(DEV), None, None, scale=SCALE, k=k.to(DEV), v=v.to(DEV),
+                           cu_seqlens_q_list=[0, 15, 45], cu_seqlens_k_list=[7, 25, 60])
+    for a, b, c, d in ((0, 15, 7, 25), (15, 45, 25, 60)):
+        w, bound = attend(q[a:b], k[c:d], v[c:d], *chunk_mask(b - a, d - c, 0, 0), scale=SCALE)
+        check(out[a:b], w, bound, f"keys {c}..{d}")

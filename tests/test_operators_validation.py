@@ -256,3 +256,21 @@ def test_graph_runner_checks_score_shapes():
     runner = DecodeGraphRunner(caches, caches, 8, 2, 2, 0.1, score_shapes=[None, one])
     assert runner.score_shapes == [{}, one]
     assert DecodeGraphRunner(caches, caches, 8, 2, 2, 0.1, score_shapes=one).score_shapes == [one] * 2
+
+
+@pytest.mark.parametrize("bad", [
+    dict(cu_seqlens_q_list=[5, 8], cu_seqlens_k_list=[0, 3]),     # a slice of a larger batch
+    dict(cu_seqlens_q_list=[2, 5], cu_seqlens_k_list=[2, 5]),
+    dict(cu_seqlens_q_list=[-1, 2], cu_seqlens_k_list=[0, 3]),
+    dict(cu_seqlens_q=torch.tensor([5, 8]), cu_seqlens_k=torch.tensor([0, 3])),
+    dict(cu_seqlens_q_list=[0, 3], cu_seqlens_k_list=[-3, 0]),
+    dict(cu_seqlens_q_list=[0, 3], cu_seqlens_k_list=[-1, 2], block_tables=None,
+         k=torch.zeros(2, 2, 128, dtype=torch.bfloat16),
+         v=torch.zeros(2, 2, 128, dtype=torch.bfloat16)),
+    dict(cu_seqlens_q_list=[], cu_seqlens_k_list=[]),
+])
+def test_offsets_that_do_not_start_at_the_first_row(bad):
+    """cu_seqlens_q are rows of this q: the kernel would leave those before the
+    first offset unwritten and cut the last sequence."""
+    with pytest.raises(ValueError):
+        _scored(num_decode_rows=0, **bad)
