@@ -569,6 +569,8 @@ PyObject* mrope(PyObject*, PyObject* const* a, Py_ssize_t n) {
           !kc->is_contiguous() || !vc->is_contiguous() || !is_index(slots, tokens, *q, &sb))
         Py_RETURN_NONE;
       num_slots = kc->numel() / (kvh * 128);
+    } else if (a[11] != Py_None) {
+      Py_RETURN_NONE;  // a v pool alone is refused
     }
     axes_p = PyLong_AsVoidPtr(a[5]);
     stream = PyLong_AsVoidPtr(a[14]);

@@ -173,3 +173,9 @@ def test_other_forms_go_to_the_python_path(monkeypatch, case):
 def test_refusals_are_the_same(monkeypatch, case):
     (a, b), _ = _both(monkeypatch, REFUSED[case])
     assert isinstance(a, type) and a is b
+
+
+def test_mrope_refuses_a_v_pool_alone(monkeypatch):
+    """Without the k pool nothing would be appended."""
+    (a, b), served = _both(monkeypatch, lambda: _mrope(k_cache=None))
+    assert not served and a is b is ValueError
