@@ -83,6 +83,8 @@ class Attention(nn.Module):
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.softcap = softcap
+        if alibi_slopes is not None:
+            alibi_slopes = alibi_slopes.to(torch.float32)
         self.register_buffer("alibi_slopes", alibi_slopes, persistent=False)
         self.window = window
         self.block_size = None
@@ -104,6 +106,15 @@ class Attention(nn.Module):
         # (kv_layer, k, v) on every forward; it records calibration
         # statistics between kv_calibrate_begin and kv_calibrate_freeze.
         self.kv_observe = None
+
+    def _apply(self, fn, recurse=True):
+        """Slopes follow the layer's device and stay fp32: rounded by a cast of
+        the model to bf16, a bias of 20 would be off by up to 0.08."""
+        slopes = self.alibi_slopes
+        super()._apply(fn, recurse)
+        if slopes is not None and self.alibi_slopes.dtype != torch.float32:
+            self.alibi_slopes = slopes.to(self.alibi_slopes.device)
+        return self
 
     def _profile(self, name):
         if self.profiler is None:

@@ -274,3 +274,25 @@ def test_offsets_that_do_not_start_at_the_first_row(bad):
     first offset unwritten and cut the last sequence."""
     with pytest.raises(ValueError):
         _scored(num_decode_rows=0, **bad)
+
+
+def test_a_layers_slopes_stay_fp32():
+    """Casting the model does not round them, whichever way it is cast; moved
+    and cast at once, they move."""
+    from nanovllm_amd.layers.attention import Attention
+    slopes = torch.tensor([2.0 ** (-8.0 * (i + 1) / 12) for i in range(12)])
+    for cast in (lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(),
+                 lambda m: m.bfloat16().float(), lambda m: m.to("cpu", torch.bfloat16)):
+        model = torch.nn.Sequential(torch.nn.Linear(2, 2),
+                                    Attention(12, 128, 0.1, 2, alibi_slopes=slopes.clone()))
+        assert cast(model) is model
+        layer = model[1]
+        assert layer.alibi_slopes.dtype == torch.float32
+        assert torch.equal(layer.alibi_slopes, slopes)
+        assert dict(layer.named_buffers())["alibi_slopes"] is layer.alibi_slopes
+    moved = Attention(12, 128, 0.1, 2, alibi_slopes=slopes).to("meta", torch.bfloat16)
+    assert moved.alibi_slopes.device.type == "meta"
+    assert moved.alibi_slopes.dtype == torch.float32
+    given = Attention(12, 128, 0.1, 2, alibi_slopes=slopes.double()).alibi_slopes
+    assert given.dtype == torch.float32 and torch.equal(given, slopes)
+    assert Attention(12, 128, 0.1, 2).to(torch.bfloat16).alibi_slopes is None
