@@ -257,8 +257,9 @@ __device__ __forceinline__ uint32_t visible_bits(const ScoredParams& p, const Co
       tree = m[0] << (-u0);
     }
     tree &= bits_below(c.sk - j0);
-    if (p.window > 0 && p.window < c.sq) {
-      // Only here can two depths of one tree be a window apart.
+    if (p.window > 0 && p.window <= c.sq) {
+      // Only here can two depths of one tree, -1 (no bits) to sq - 1, be a
+      // window apart.
       for (int k = max(0, -u0); k < kTile && u0 + k < c.sq; ++k)
         if (place - c.p0 - c.depths[u0 + k] >= p.window) tree &= ~(1u << k);
     }

@@ -187,3 +187,24 @@ def test_captured_step(form):
             check(got[i * n:(i + 1) * n],
                   *attend(q[i * n:(i + 1) * n], ks[i][:c + n], vs[i][:c + n], sees, away,
                           scale=SCALE, slopes=sl), f"replay {step}")
+
+
+def _some_bits(size, seed):
+    return random.Random(seed).getrandbits(size)
+
+
+@pytest.mark.parametrize("size", [1, 3, 5, 33, 64])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_windows_as_wide_as_the_tree(size, slopes):
+    """A token that sees the whole tree is `size` places past a key whose own
+    mask is empty: outside a window of `size`, inside one of `size` + 1."""
+    sizes, ctx = [size] * 3, [0, 40, 31]
+    mask = torch.zeros(3 * size, 1, dtype=torch.int64)
+    for i in range(3):
+        for t in range(1, size):
+            word = (1 << size) - 1 if t == size - 1 else _some_bits(size, t + i)
+            mask[i * size + t, 0] = word - (1 << 64) if word >> 63 else word
+    for window in (max(1, size - 1), size, size + 1):
+        out = _run(ctx, sizes, mask, 8, 2, 32, 110 + size, window=window, slopes=slopes,
+                   label=f"window {window} of {size}")
+        assert bool(torch.isfinite(out.float()).all())
