@@ -32,7 +32,7 @@ import torch
 
 from .. import _native as nat
 from ..kernels.paged_attention import decode_append_into
-from ..kernels.scored import scored_attention
+from ..kernels.scored import check_scores, scored_attention
 from ..layers.attention import store_kvcache
 
 
@@ -72,7 +72,8 @@ class DecodeGraphRunner:
     built without one is for pools that no asynchronous move touches.
 
     score_shapes: scored_attention's softcap, alibi_slopes and window as a dict,
-    for all layers or one per layer (None or an empty dict: plain scores)."""
+    for all layers or one per layer (None or an empty dict: plain scores).
+    from_kv_runner takes the bound layers' own unless it is given some."""
 
     def __init__(self, k_caches, v_caches, num_heads: int, max_bs: int, max_blocks_per_seq: int,
                  scale: float, buckets: list[int] | None = None, fence=None, score_shapes=None):
@@ -111,6 +112,9 @@ class DecodeGraphRunner:
         for s in self.score_shapes:
             if not set(s) <= {"softcap", "alibi_slopes", "window"}:
                 raise ValueError(f"a score shape has softcap, alibi_slopes and window (got {set(s)})")
+            if s:
+                check_scores(scale, s.get("softcap"), s.get("alibi_slopes"), s.get("window"),
+                             num_heads, dev)
 
     @classmethod
     def from_kv_runner(cls, kv_runner, num_heads: int, max_bs: int, max_blocks_per_seq: int,
@@ -118,9 +122,13 @@ class DecodeGraphRunner:
                        score_shapes=None) -> "DecodeGraphRunner":
         """A runner over every layer of a KVCacheRunner's bf16 pool, fenced by
         that runner (its asynchronous offload copies, if any, are ordered
-        before each capture and replay)."""
+        before each capture and replay).  score_shapes: None for what the
+        layers bound to that runner shape their scores with (bind them
+        first), else as in the constructor ({}: plain scores)."""
         if kv_runner.kv_int8 is not None:
             raise ValueError("the captured decode step runs on a bf16 pool")
+        if score_shapes is None:
+            score_shapes = kv_runner.score_shapes()
         k_caches = [kv_runner.kv_cache[0, i] for i in range(kv_runner.num_layers)]
         v_caches = [kv_runner.kv_cache[1, i] for i in range(kv_runner.num_layers)]
         return cls(k_caches, v_caches, num_heads, max_bs, max_blocks_per_seq, scale, buckets,

@@ -247,14 +247,17 @@ class KVCacheRunner:
         self.async_copy_engine = async_copy_engine
         self.kv_async = None
         self._calib = None     # (amax [L, 2, KVH, D], abs_sum, token counts) while calibrating
+        self._layers = []      # the modules of the last bind()
 
     def bind(self, modules) -> int:
         """Hand per-layer views to every module that has k_cache/v_cache
         (model_runner.py:494-508); returns the number of layers bound."""
         layer = 0
+        self._layers = []
         for m in modules:
             if not (hasattr(m, "k_cache") and hasattr(m, "v_cache")):
                 continue
+            self._layers.append(m)
             m.k_cache = self.kv_cache[0, layer]
             m.v_cache = self.kv_cache[1, layer]
             if self.kv_int8 == "tokhead":
@@ -275,6 +278,17 @@ class KVCacheRunner:
             m.kv_observe = self._observe if self.kv_int8 == "chan" else None
             layer += 1
         return layer
+
+    def score_shapes(self) -> list:
+        """What the bound layers make of their scores, one entry per pool
+        layer: their softcap, alibi_slopes and window, or None for plain ones
+        (and for layers not bound)."""
+        shapes = [None] * self.num_layers
+        for m in self._layers:
+            shape = {name: getattr(m, name, None) for name in ("softcap", "alibi_slopes", "window")}
+            if shape["softcap"] or shape["window"] or shape["alibi_slopes"] is not None:
+                shapes[m.kv_layer] = shape
+        return shapes
 
     # -- per-channel int8 calibration (model_runner.py:510-577) ---------------
     def kv_calibrate_begin(self) -> None:

@@ -5,8 +5,10 @@ import pytest
 import torch
 
 from nanovllm_amd.engine.graph_runner import DecodeGraphRunner, pad_decode_inputs
+from nanovllm_amd.engine.kv_runner import KVCacheRunner
 from nanovllm_amd.kernels.scored import scored_attention
-from nanovllm_amd.layers.attention import store_kvcache
+from nanovllm_amd.layers.attention import Attention, store_kvcache
+from nanovllm_amd.utils.context import reset_context, set_context
 from scored_oracle import attend, check, chunk_mask, slopes_of
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +88,40 @@ def test_out_is_written_in_place():
     assert scored_attention(q, kc, kc, out=out, **kw) is out
     assert torch.equal(out, want)
     assert bool((wide[:, 0] == 7).all()) and bool((wide[:, 2] == 7).all())
+
+
+def test_bound_layers_replay_as_they_run():
+    """The captured step of a runner's bound layers, shaped or not, gives what
+    the layers give eagerly, without their shapes being passed."""
+    gen = torch.Generator().manual_seed(7)
+    layers = [Attention(HEADS, 128, SCALE, KVH, softcap=30.0), Attention(HEADS, 128, SCALE, KVH),
+              Attention(HEADS, 128, SCALE, KVH, alibi_slopes=slopes_of(HEADS), window=40).to(DEV)]
+    kv = KVCacheRunner(LAYERS, BLOCKS, PAGE, KVH, 128, device=DEV)
+    kv.kv_cache.copy_(torch.randn(kv.kv_cache.shape, generator=gen))
+    kv.bind(layers)
+    runner = DecodeGraphRunner.from_kv_runner(kv, HEADS, max_bs=4, max_blocks_per_seq=WIDTH,
+                                              scale=SCALE)
+    before = kv.kv_cache.clone()
+    runner.capture()
+    kv.kv_cache.copy_(before)
+    for rnd in range(3):
+        q, k, v, slots, lens, tables, host_lens = _batch(4, 70 + rnd)
+        q, k, v, slots, lens, tables = (x.to(DEV) for x in (q, k, v, slots, lens, tables))
+        got = runner.run(q, k, v, slots, lens, tables).clone()
+        set_context(False, slot_mapping=slots, context_lens=lens, block_tables=tables,
+                    max_context_len=max(host_lens))
+        want = [layer(q[i], k[i], v[i]) for i, layer in enumerate(layers)]
+        torch.cuda.synchronize()
+        for i in (0, 2):
+            # (a full bucket and tables of the same width: the same launches,
+            # whose sums no timing orders)
+            pages = [tables[r, :(n + PAGE - 1) // PAGE].long() for r, n in enumerate(host_lens)]
+            for r, n in enumerate(host_lens):
+                ks, vs = (kv.kv_cache[x, i][pages[r]].flatten(0, 1)[:n].cpu() for x in range(2))
+                cap, window = layers[i].softcap, layers[i].window
+                sl = layers[i].alibi_slopes
+                w, b = attend(q[i, r:r + 1].cpu(), ks, vs, *chunk_mask(1, n, window, 0),
+                              scale=SCALE, cap=cap, slopes=None if sl is None else sl.cpu())
+                check(got[i, r:r + 1], w, b, f"round {rnd} layer {i} row {r}")
+            assert torch.equal(got[i].view(torch.int16), want[i].view(torch.int16))
+    reset_context()

@@ -296,3 +296,41 @@ def test_a_layers_slopes_stay_fp32():
     given = Attention(12, 128, 0.1, 2, alibi_slopes=slopes.double()).alibi_slopes
     assert given.dtype == torch.float32 and torch.equal(given, slopes)
     assert Attention(12, 128, 0.1, 2).to(torch.bfloat16).alibi_slopes is None
+
+
+def _bound(monkeypatch, *layers):
+    from nanovllm_amd.engine import kv_runner
+    monkeypatch.setattr(kv_runner, "BlockMover", lambda pool: None)     # (needs a GPU pool)
+    kv = kv_runner.KVCacheRunner(len(layers), 2, 32, 2, 128, device="cpu")
+    assert kv.bind(layers) == len(layers)
+    return kv
+
+
+def test_graph_runner_takes_the_bound_layers_shapes(monkeypatch):
+    """A shaped layer is captured shaped without being named again."""
+    from nanovllm_amd.engine.graph_runner import DecodeGraphRunner
+    from nanovllm_amd.layers.attention import Attention
+    slopes = torch.ones(8)
+    layers = [Attention(8, 128, 0.1, 2), Attention(8, 128, 0.1, 2, softcap=50.0, window=7),
+              Attention(8, 128, 0.1, 2, alibi_slopes=slopes)]
+    kv = _bound(monkeypatch, *layers)
+    got = DecodeGraphRunner.from_kv_runner(kv, 8, 2, 2, 0.1).score_shapes
+    assert got[0] == {}
+    assert got[1] == dict(softcap=50.0, alibi_slopes=None, window=7)
+    assert got[2]["alibi_slopes"] is layers[2].alibi_slopes and not got[2]["softcap"]
+    plain = DecodeGraphRunner.from_kv_runner(kv, 8, 2, 2, 0.1, score_shapes={})
+    assert plain.score_shapes == [{}] * 3
+    one = dict(window=3)
+    assert DecodeGraphRunner.from_kv_runner(kv, 8, 2, 2, 0.1,
+                                            score_shapes=one).score_shapes == [one] * 3
+    assert _bound(monkeypatch, Attention(8, 128, 0.1, 2)).score_shapes() == [None]
+
+
+@pytest.mark.parametrize("bad", [dict(softcap=-1.0), dict(window=-2),
+                                 dict(alibi_slopes=torch.ones(7)),
+                                 dict(alibi_slopes=torch.ones(8, device="meta"))])
+def test_graph_runner_checks_values_before_a_capture(bad):
+    from nanovllm_amd.engine.graph_runner import DecodeGraphRunner
+    caches = [torch.zeros(3, 32, 2, 128, dtype=torch.bfloat16)]
+    with pytest.raises(ValueError):
+        DecodeGraphRunner(caches, caches, 8, 2, 2, 0.1, score_shapes=bad)
