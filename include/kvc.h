@@ -436,8 +436,10 @@ size_t kvc_scored_workspace_bytes(int64_t num_q_tokens, int64_t num_heads, int64
  *   s = scale q.k;  s = softcap tanh(s / softcap) when softcap > 0;
  *   s -= alibi_slopes[h] |p - j| when alibi_slopes (fp32 [num_heads]) is given.
  * out = softmax(s) . v; a query that sees no key gives 0.  Values at keys a
- * query does not see never reach it, infinities and NaN included.  A block id
- * outside the pool reads as zeros.  max_seqlen_q (the longest chunk) and the
+ * query does not see never reach it, infinities and NaN included.  Values from
+ * 2^-64 to 2^64 in magnitude keep their precision whatever the scores and
+ * lengths (sums of weights and values are fp32; far larger ones may overflow
+ * them, far smaller ones vanish).  A block id outside the pool reads as zeros.  max_seqlen_q (the longest chunk) and the
  * table's width steer the launch; the lengths themselves are read on the
  * device.  Rows of q / out / k_fresh / v_fresh are 16-byte aligned; at most 256
  * query heads per kv head; scale > 0, and scale / softcap must be finite. */

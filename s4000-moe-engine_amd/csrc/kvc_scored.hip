@@ -51,6 +51,12 @@ constexpr int kD = 128;
 constexpr int kTile = 32;
 constexpr int kTensor = kTile * kD * 2;  // one K or V tile of a head: 8 KiB
 constexpr uint32_t kLazyBits = 0x4380u;  // bf16 2^8: a weight past it moves the running reference
+// Under a near cap scores lie within 2 cap log2(e) <= 160 binades, so a reference
+// kNearAbove over a column's largest score so far mostly serves for good: once
+// it is no more than kNearRoom below the cap, no weight can pass 2^30 whatever
+// follows, and the reference is not looked at again.  Weights are 2^-54 of what
+// they would be, far from fp32's ends: values from 2^-64 to 2^64 are served.
+constexpr float kNearAbove = 54.f, kNearRoom = 30.f;
 constexpr int kNoKey = 1 << 30;  // a key position that no column sees
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint32_t kOnes2 = 0x3F803F80u;  // two bf16 ones
@@ -58,14 +64,14 @@ constexpr uint32_t kOnes2 = 0x3F803F80u;  // two bf16 ones
 enum ScoreMode {
   kPlain = 0,
   kDistance = 1,
-  kCapFixed = 2,     // cap log2(e) <= kCapFixedMax: 2^x needs no running maximum
-  kCapLazy = 3,
+  kCapNear = 2,      // cap log2(e) <= kCapNearMax
+  kCapFar = 3,
   kCapDistance = 4,
 };
-// 2^(cap log2 e) stays within 2^80: sums over 2^20 keys and |v| up to 2^27
-// fit fp32 and bf16's range, so exp2 needs no reference.  (With a distance
-// bias the scores have no such floor.)
-constexpr float kCapFixedMax = 80.f;
+// Up to this cap (55) tanh by exp2 and a reciprocal, off by 2^-22 of the cap,
+// serves scores of any size: 2^-22 x 55 is 2^-16.  The cap's last product and
+// the reference then fold into one fma in front of exp2.
+constexpr float kCapNearMax = 80.f;
 
 struct ScoredParams {
   const uint16_t* q;
@@ -214,17 +220,19 @@ struct State {
   f32x4_t o[NCB][8];
   float l[NCB];  // over the lane's own keys; of the column once the loop is done
   float mu[NCB];
+  int settled;   // a near cap's references serve for good
 };
 
 template <int NCB>
-__device__ __forceinline__ void reset(State<NCB>& st, float mu0) {
+__device__ __forceinline__ void reset(State<NCB>& st) {
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
 #pragma unroll
     for (int jj = 0; jj < 8; ++jj) st.o[cb][jj] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     st.l[cb] = 0.f;
-    st.mu[cb] = mu0;
+    st.mu[cb] = kLowest;
   }
+  st.settled = 0;
 }
 
 __device__ __forceinline__ uint32_t bits_below(int n) {  // bits 0 .. n - 1
@@ -274,7 +282,7 @@ struct Consts {
   float a, a2;   // cap log2(e) and twice that
   float z;       // scale / cap
 };
-// Caps that kCapFixed does not take: 1 - 2 / (e^{2z} + 1) is off by 2^-22 of
+// Caps that kCapNear does not take: 1 - 2 / (e^{2z} + 1) is off by 2^-22 of
 // the cap, so below |z| = 1/16 tanh comes from its series, z (1 - z^2 / 3 + 2
 // z^4 / 15), off by 17 / 315 z^6 < 2^-28 relative.
 constexpr float kSeriesBelow = 1.f / 256;  // z^2
@@ -301,15 +309,16 @@ __device__ __forceinline__ void logits(const u32x4_t (&k)[2][4], const u32x4_t (
 
 // The score's shape, the mask, the running softmax, and P^T as the bf16
 // operand pb.  y comes in as the logits and becomes what the softmax is taken
-// of: the raw logit s (log2-unit score c2 s) for plain scores, the log2-unit
-// score otherwise; -inf at keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} +
+// of: the raw logit s (log2-unit score c2 s) for plain scores, r = -1 / (e^{2z}
+// + 1) (log2-unit score a + 2 a r) under a near cap, the log2-unit score
+// otherwise; -inf at keys the column does not see.  tanh(z) = 1 - 2 / (e^{2z} +
 // 1): one exp2 and one reciprocal.  Sums are formed of the rounded P, so the
 // weights add up to the sum that divides them.
 template <int NCB, int MODE>
 __device__ __forceinline__ void shape_scores(const Columns<NCB>& c, f32x4_t (&y)[NCB][2], int j0,
                                              int lg, const Consts& cs) {
   constexpr bool kDist = MODE == kDistance || MODE == kCapDistance;
-  constexpr bool kCap = MODE == kCapFixed || MODE == kCapLazy || MODE == kCapDistance;
+  constexpr bool kCap = MODE == kCapNear || MODE == kCapFar || MODE == kCapDistance;
   if constexpr (!kDist && !kCap) return;
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
@@ -321,8 +330,9 @@ __device__ __forceinline__ void shape_scores(const Columns<NCB>& c, f32x4_t (&y)
       float x = s;
       if constexpr (kCap) {
         const float w = __builtin_amdgcn_exp2f(s * cs.zc);
-        x = __builtin_fmaf(-cs.a2, __builtin_amdgcn_rcpf(w + 1.f), cs.a);
-        if constexpr (MODE != kCapFixed) {
+        x = __builtin_amdgcn_rcpf(-1.f - w);
+        if constexpr (MODE != kCapNear) {
+          x = __builtin_fmaf(cs.a2, x, cs.a);
           const float z = s * cs.z, z2 = z * z;
           const float series = __builtin_fmaf(z2, __builtin_fmaf(z2, 2.f / 15, -1.f / 3), 1.f);
           x = z2 < kSeriesBelow ? s * cs.c2 * series : x;
@@ -366,6 +376,16 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
                                                       __builtin_bit_cast(u16x2_t, b)));
 }
 
+// The log2-unit score of y: unit y + base.
+template <int MODE>
+__device__ __forceinline__ float unit_of(const Consts& cs) {
+  return MODE == kPlain ? cs.c2 : MODE == kCapNear ? cs.a2 : 1.f;
+}
+template <int MODE>
+__device__ __forceinline__ float base_of(const Consts& cs) {
+  return MODE == kCapNear ? cs.a : 0.f;
+}
+
 // P^T of the tile, relative to each column's reference.
 template <int NCB, int MODE>
 __device__ __forceinline__ void exponentials(const State<NCB>& st, const f32x4_t (&y)[NCB][2],
@@ -373,12 +393,13 @@ __device__ __forceinline__ void exponentials(const State<NCB>& st, const f32x4_t
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) {
     float pr[8];
+    const float base = base_of<MODE>(cs) - st.mu[cb];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = y[cb][e >> 2][e & 3];
-      pr[e] = __builtin_amdgcn_exp2f(MODE == kCapFixed ? x
-                                     : MODE == kPlain  ? __builtin_fmaf(x, cs.c2, -st.mu[cb])
-                                                       : x - st.mu[cb]);
+      pr[e] = __builtin_amdgcn_exp2f(MODE == kPlain || MODE == kCapNear
+                                         ? __builtin_fmaf(x, unit_of<MODE>(cs), base)
+                                         : x + base);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -389,14 +410,43 @@ __device__ __forceinline__ void exponentials(const State<NCB>& st, const f32x4_t
   }
 }
 
-// The reference moves only when a weight passes 2^8 (or a column has none
-// yet), which the packed weights themselves say; the tile's are then formed
-// again.
+// The columns' references up to the tile's largest scores.
+template <int NCB, int MODE>
+__device__ __forceinline__ void raise_reference(State<NCB>& st, const f32x4_t (&y)[NCB][2],
+                                                const Consts& cs) {
+  constexpr float kAbove = MODE == kCapNear ? kNearAbove : 0.f;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+    float top = y[cb][0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, y[cb][e >> 2][e & 3]);
+    const float mu = fmaxf(st.mu[cb], __builtin_fmaf(rows4_max(top), unit_of<MODE>(cs),
+                                                     base_of<MODE>(cs) + kAbove));
+    const float down = __builtin_amdgcn_exp2f(st.mu[cb] - mu);
+#pragma unroll
+    for (int jj = 0; jj < 8; ++jj) st.o[cb][jj] *= down;
+    st.l[cb] *= down;
+    st.mu[cb] = mu;
+  }
+}
+
+// A near cap's, ahead of the weights, until it serves for good.
+template <int NCB>
+__device__ __forceinline__ void settle_reference(State<NCB>& st, const f32x4_t (&y)[NCB][2],
+                                                 const Consts& cs) {
+  raise_reference<NCB, kCapNear>(st, y, cs);
+  bool serves = true;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) serves &= st.mu[cb] >= cs.a - kNearRoom;
+  st.settled = uniform(int(__all(serves)));
+}
+
+// Otherwise the reference moves only when a weight passes 2^8 (or a column has
+// none yet), which the packed weights themselves say; the tile's are then
+// formed again.
 template <int NCB, int MODE>
 __device__ __forceinline__ void follow_reference(State<NCB>& st, const f32x4_t (&y)[NCB][2],
                                                  const Consts& cs, u32x4_t (&pb)[NCB]) {
-  if constexpr (MODE == kCapFixed) return;
-  const float unit = MODE == kPlain ? cs.c2 : 1.f;
   uint32_t most = 0u;
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb)
@@ -404,18 +454,7 @@ __device__ __forceinline__ void follow_reference(State<NCB>& st, const f32x4_t (
     for (int i = 0; i < 4; ++i) most = max_u16x2(most, pb[cb][i]);
   const bool past = (most >> 16) > kLazyBits || (most & 0xffffu) > kLazyBits;
   if (__builtin_expect(__any(past), 0)) {
-#pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) {
-      float top = y[cb][0][0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, y[cb][e >> 2][e & 3]);
-      const float mu = fmaxf(st.mu[cb], rows4_max(top) * unit);
-      const float down = __builtin_amdgcn_exp2f(st.mu[cb] - mu);
-#pragma unroll
-      for (int jj = 0; jj < 8; ++jj) st.o[cb][jj] *= down;
-      st.l[cb] *= down;
-      st.mu[cb] = mu;
-    }
+    raise_reference<NCB, MODE>(st, y, cs);
     exponentials<NCB, MODE>(st, y, cs, pb);
   }
 }
@@ -438,9 +477,17 @@ __device__ __forceinline__ void weights(const ScoredParams& p, const Columns<NCB
                                         State<NCB>& st, f32x4_t (&y)[NCB][2], int j0, int lg,
                                         const Consts& cs, bool masked, u32x4_t (&pb)[NCB]) {
   shape_scores<NCB, MODE>(c, y, j0, lg, cs);
-  if (__builtin_expect(masked, 0)) mask_scores<NCB, MODE>(p, c, y, j0, lg);
-  exponentials<NCB, MODE>(st, y, cs, pb);
-  follow_reference<NCB, MODE>(st, y, cs, pb);
+  if constexpr (MODE == kCapNear) {
+    if (__builtin_expect(masked || !st.settled, 0)) {
+      if (masked) mask_scores<NCB, MODE>(p, c, y, j0, lg);
+      if (!st.settled) settle_reference<NCB>(st, y, cs);
+    }
+    exponentials<NCB, MODE>(st, y, cs, pb);
+  } else {
+    if (__builtin_expect(masked, 0)) mask_scores<NCB, MODE>(p, c, y, j0, lg);
+    exponentials<NCB, MODE>(st, y, cs, pb);
+    follow_reference<NCB, MODE>(st, y, cs, pb);
+  }
   sum_weights<NCB>(st, pb);
 }
 
@@ -875,7 +922,6 @@ __global__ void __launch_bounds__(64 * NW)
   cs.a = p.cap * kLog2e;
   cs.a2 = 2.f * cs.a;
   cs.z = p.cap > 0.f ? p.scale / p.cap : 0.f;
-  constexpr float mu0 = MODE == kCapFixed ? 0.f : kLowest;
 
   const int col0 = cw * NCB * 16;
   const int wave_t0 = uniform(div_small(col0, p.group, p.group_rcp));
@@ -957,7 +1003,7 @@ __global__ void __launch_bounds__(64 * NW)
         }
       };
       State<NCB> st;
-      reset<NCB>(st, mu0);
+      reset<NCB>(st);
       const int t_begin = range.t0 + seg0, t_end = range.t0 + seg1;
       bool odd = false;  // a masked tile held infinities or NaN
       if constexpr (F::kPrivate) {
@@ -1541,10 +1587,10 @@ int run_rows(ScoredParams p, int64_t max_q, int64_t max_keys, void* ws, hipStrea
   if (p.cap > 0.f) {
     if (bias) {
       rc = launch_form<kCapDistance>(p, pl, st);
-    } else if (p.cap * kLog2e <= kCapFixedMax) {
-      rc = launch_form<kCapFixed>(p, pl, st);
+    } else if (p.cap * kLog2e <= kCapNearMax) {
+      rc = launch_form<kCapNear>(p, pl, st);
     } else {
-      rc = launch_form<kCapLazy>(p, pl, st);
+      rc = launch_form<kCapFar>(p, pl, st);
     }
   } else {
     rc = bias ? launch_form<kDistance>(p, pl, st) : launch_form<kPlain>(p, pl, st);

@@ -252,3 +252,24 @@ def test_tables_without_pages():
     out = scored_attention(q, kc, kc, scale=SCALE, block_tables=tables, num_decode_rows=3,
                            decode_context_lens=_i32([0, 0, 0]))
     assert not out.any()
+
+
+@pytest.mark.parametrize("tokens", [1, 8, 16, 32, 64])
+@pytest.mark.parametrize("cap", [20.0, 50.0, 55.0, 60.0])
+@pytest.mark.parametrize("ends", ["low", "high", "rise", "fall"])
+@pytest.mark.parametrize("power", [-60, 60])
+def test_values_far_from_one_under_a_cap(tokens, cap, ends, power):
+    """Every score at one end of the cap, or half of the keys at either: the
+    weights' sums stay within fp32's range, whichever end comes first."""
+    chunks = [(tokens, 300), (tokens, 1500)]
+    gen = torch.Generator().manual_seed(31)
+    ks, vs = [], []
+    for i, (_, m) in enumerate(chunks):
+        k = 1 + 0.1 * torch.randn(m, 2, 128, generator=gen)
+        low = {"low": slice(0, m), "high": slice(0, 0), "rise": slice(0, m // 2),
+               "fall": slice(m // 2, m)}[ends]
+        k[low] *= -1
+        ks.append(k.to(torch.bfloat16))
+        vs.append(_normal(m, 2, 32 + i, 1.0) * 2.0 ** power)
+    q = (30 * (1 + 0.1 * torch.randn(2 * tokens, 8, 128, generator=gen))).to(torch.bfloat16)
+    _chunks(q, ks, vs, chunks, f"{tokens} tokens, cap {cap}, {ends}, values 2^{power}", cap=cap)
