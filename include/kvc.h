@@ -439,10 +439,12 @@ size_t kvc_scored_workspace_bytes(int64_t num_q_tokens, int64_t num_heads, int64
  * query does not see never reach it, infinities and NaN included.  Values from
  * 2^-64 to 2^64 in magnitude keep their precision whatever the scores and
  * lengths (sums of weights and values are fp32; far larger ones may overflow
- * them, far smaller ones vanish).  A block id outside the pool reads as zeros.  max_seqlen_q (the longest chunk) and the
- * table's width steer the launch; the lengths themselves are read on the
- * device.  Rows of q / out / k_fresh / v_fresh are 16-byte aligned; at most 256
- * query heads per kv head; scale > 0, and scale / softcap must be finite. */
+ * them, far smaller ones vanish).  A block id outside
+ * the pool reads as zeros; keys past the block table (or num_fresh_rows) are not
+ * seen, places stay those of the given lengths.  max_seqlen_q (the longest
+ * chunk) and the table's width steer the launch; the lengths themselves are read
+ * on the device.  Rows of q / out / k_fresh / v_fresh are 16-byte aligned; at
+ * most 256 query heads per kv head; scale > 0, and scale / softcap must be finite. */
 int kvc_scored_attention(
     const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_q_tokens, int64_t num_heads,
     const void* k_cache, const void* v_cache, int64_t num_cache_blocks, int64_t page_size,

@@ -4,10 +4,10 @@
 // For a query token at place p and a visible key at place j, head h:
 //   s = scale q.k;  s = cap tanh(s / cap) (cap > 0);  s -= slope_h |p - j|
 //   out = sum_j softmax_j(s) v_j, 0 for a token that sees no key.
-// Chunk tokens sit at the end of their sequence's keys (p = sk - sq + t) and
-// see keys j <= p or j < prefix, within the window (p - j < window).  Tree
-// token t sees the context j < sk - sq and the tree keys named by its mask
-// bits; its place is sk - sq + popcount(mask_t) - 1, its depth in the tree.
+// Chunk tokens sit at the end of their sequence's keys (p = p0 + t, p0 the keys
+// before the chunk) and see keys j <= p or j < prefix, within the window (p - j
+// < window).  Tree token t sees the context j < p0 and the tree keys named by
+// its mask bits; its place is p0 + popcount(mask_t) - 1, its depth in the tree.
 //
 // Layout of the work.  The G query heads of one kv head and the tokens of a
 // block are the columns of S^T = K Q^T (a lane owns one column, so a row's
@@ -113,22 +113,22 @@ struct ScoredParams {
 };
 
 struct SeqGeo {
-  int q0, sq, sk;
+  int q0, sq;
+  int sk;  // keys that there are: no more than the table's pages or the fresh rows hold
+  int p0;  // place of the first query: by the given lengths, cut or not
 };
+constexpr int64_t kLongest = int64_t(1) << 29;  // of a length (tables hold fewer keys)
 
 __device__ __forceinline__ SeqGeo seq_geo(const ScoredParams& p, int q0, int q1, int len, int k0,
                                           int k1) {
   SeqGeo g;
   g.q0 = max(0, min(q0, p.num_tokens));
   g.sq = max(0, min(q1, p.num_tokens) - g.q0);
-  int64_t sk, most;
-  if (p.lens != nullptr) {
-    sk = int64_t(len) + (p.lens_exclude_q ? g.sq : 0);
-  } else {
-    sk = int64_t(k1) - k0;
-  }
-  most = p.tables != nullptr ? int64_t(p.max_blocks) * p.page : p.fresh_rows - max(k0, 0);
-  g.sk = int(max(int64_t(0), min(sk, most)));
+  int64_t keys = p.lens != nullptr ? len : int64_t(k1) - k0;
+  keys = max(int64_t(0), min(keys, kLongest)) + (p.lens_exclude_q ? g.sq : 0);
+  const int64_t most = p.tables != nullptr ? int64_t(p.max_blocks) * p.page : p.fresh_rows - max(k0, 0);
+  g.sk = int(max(int64_t(0), min(keys, most)));
+  g.p0 = int(keys) - g.sq;
   return g;
 }
 
@@ -166,7 +166,7 @@ struct TileRange {
 };
 __device__ __forceinline__ TileRange block_tiles(const ScoredParams& p, const SeqGeo& g, int pre,
                                                  int c) {
-  const int p0 = g.sk - g.sq;
+  const int p0 = g.p0;
   const int first = c * p.tokens_per_block;
   const int last = min(g.sq, first + p.tokens_per_block) - 1;
   int lo = 0, hi;
@@ -249,7 +249,7 @@ __device__ __forceinline__ uint32_t visible_bits(const ScoredParams& p, const Co
     if (p.window > 0) vis &= ~bits_below(c.p0 + t + 1 - p.window - j0);
     return vis;
   }
-  uint32_t vis = bits_below(c.p0 - j0);
+  uint32_t vis = bits_below(min(c.p0, c.sk) - j0);
   const int place = p.window > 0 ? c.p0 + c.depths[t] : 0;
   if (p.window > 0) vis &= ~bits_below(place + 1 - p.window - j0);
   const int u0 = j0 - c.p0;  // tree index of the tile's first key
@@ -616,7 +616,7 @@ __device__ __forceinline__ int block_cost(const ScoredParams& p, const SeqGeo& g
 
 // Cost and column blocks of lane's sequence (lane plan).
 __device__ __forceinline__ int lane_seq(const ScoredParams& p, int i, SeqGeo& g, int& pre) {
-  g = SeqGeo{0, 0, 0};
+  g = SeqGeo{};
   pre = 0;
   if (i >= p.batch) return 0;
   g = load_seq<false>(p, i);
@@ -646,9 +646,9 @@ __device__ __forceinline__ int first_lane(uint64_t m) { return __builtin_ctzll(m
 __device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int share, int shares,
                                            Where& w, SeqGeo& g, int& pre, int& size) {
   int total = 0, cost = 0;
-  SeqGeo mine = {0, 0, 0};  // lane_plan: this lane's sequence
+  SeqGeo mine = {};  // lane_plan: this lane's sequence
   int mine_pre = 0;
-  g = SeqGeo{0, 0, 0};
+  g = SeqGeo{};
   pre = 0;
   if (p.whole && (p.batch == 1 || p.cu_q == nullptr)) {
     // As many items in each sequence: no walk, and (small calls are all
@@ -695,6 +695,7 @@ __device__ __forceinline__ bool plan_share(const ScoredParams& p, int lane, int 
         g.q0 = __builtin_amdgcn_readlane(mine.q0, l);
         g.sq = __builtin_amdgcn_readlane(mine.sq, l);
         g.sk = __builtin_amdgcn_readlane(mine.sk, l);
+        g.p0 = __builtin_amdgcn_readlane(mine.p0, l);
         pre = __builtin_amdgcn_readlane(mine_pre, l);
         break;
       }
@@ -946,7 +947,7 @@ __global__ void __launch_bounds__(64 * NW)
       const int head = w.grp * p.heads_per_wg + hs;
       const int64_t fresh0 =
           p.tables == nullptr ? max(0, table_entry(p.cu_k, w.seq)) : 0;
-      const int p0 = g.sk - g.sq;
+      const int p0 = g.p0;
       const int b0 = w.block * p.tokens_per_block;  // the block's first token
       const int tmax = min(g.sq, b0 + p.tokens_per_block) - 1;
 
@@ -982,7 +983,7 @@ __global__ void __launch_bounds__(64 * NW)
                                     ? p0 + ta + 1 : max(p0 + ta + 1, pre));
         } else {
           c.full_lo = p.window > 0 ? p0 + g.sq - p.window : 0;  // depth < sq
-          c.full_hi = p0;
+          c.full_hi = min(p0, g.sk);
         }
       }
       u32x4_t q[NCB][4];

@@ -306,3 +306,29 @@ def test_fresh_keys_from_a_later_row():
     for a, b, c, d in ((0, 15, 7, 25), (15, 45, 25, 60)):
         w, bound = attend(q[a:b], k[c:d], v[c:d], *chunk_mask(b - a, d - c, 0, 0), scale=SCALE)
         check(out[a:b], w, bound, f"keys {c}..{d}")
+
+
+@pytest.mark.parametrize("form", [dict(), dict(cap=30.0), dict(slopes=True), dict(window=40),
+                                  dict(window=90, slopes=True)])
+@pytest.mark.parametrize("pages", [1, 2, 4])
+def test_places_past_a_short_table(form, pages):
+    """Lengths beyond the block table: the keys it holds, at the places that the
+    lengths give (a window may then see none of them)."""
+    dec, chunks, page = [70, 128, 200], [(5, 70), (40, 129), (90, 200)], 32
+    kc, vc, bt, ks, vs = paged(dec + [m for _, m in chunks], page, 2, 38)
+    most = pages * page
+    q = _queries(3 + 135, 8, 39)
+    sl = slopes_of(8) if form.get("slopes") else None
+    cap, window = form.get("cap", 0.0), form.get("window", 0)
+    out = scored_attention(
+        q.to(DEV), kc.to(DEV), vc.to(DEV), scale=SCALE, block_tables=bt[:, :pages].to(DEV),
+        num_decode_rows=3, decode_context_lens=torch.tensor(dec, dtype=torch.int32, device=DEV),
+        cu_seqlens_q_list=[0, 5, 45, 135], cu_seqlens_k_list=[0, 70, 199, 399], softcap=cap,
+        alibi_slopes=None if sl is None else sl.to(DEV), window=window)
+    at = 0
+    for i, (n, m) in enumerate([(1, c) for c in dec] + chunks):
+        sees, away = chunk_mask(n, m, window, 0)
+        w, b = attend(q[at:at + n], ks[i][:most], vs[i][:most], sees[:, :most], away[:, :most],
+                      scale=SCALE, cap=cap, slopes=sl)
+        check(out[at:at + n], w, b, f"{pages} pages {form} sequence {i}")
+        at += n

@@ -208,3 +208,27 @@ def test_windows_as_wide_as_the_tree(size, slopes):
         out = _run(ctx, sizes, mask, 8, 2, 32, 110 + size, window=window, slopes=slopes,
                    label=f"window {window} of {size}")
         assert bool(torch.isfinite(out.float()).all())
+
+
+@pytest.mark.parametrize("form", [dict(), dict(window=9), dict(slopes=True),
+                                  dict(window=30, slopes=True)])
+@pytest.mark.parametrize("heads,most", [(16, 7), (16, 40)])
+def test_trees_past_a_short_table(form, heads, most):
+    """A table that ends inside the tree, or inside its context: tokens see what
+    it holds of their own paths, and nothing of another's."""
+    rng = random.Random(9)
+    ctx, sizes = [30, 60, 64, 100], [most] * 4
+    mask = tree_mask_from_parents([_parents(rng, t) for t in sizes])
+    kc, vc, bt, ks, vs = paged([c + t for c, t in zip(ctx, sizes)], 32, 2, 120)
+    q = _queries(4 * most, heads, 121)
+    sl = slopes_of(heads) if form.get("slopes") else None
+    window = form.get("window", 0)
+    out = tree_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), bt[:, :2].contiguous().to(DEV),
+                         torch.tensor(ctx, dtype=torch.int32, device=DEV), mask.to(DEV), SCALE,
+                         alibi_slopes=None if sl is None else sl.to(DEV), window=window)
+    for i, c in enumerate(ctx):
+        rows = slice(i * most, (i + 1) * most)
+        sees, away = tree_mask(_dense(mask[rows], most), c, window)
+        w, b = attend(q[rows], ks[i][:64], vs[i][:64], sees[:, :64], away[:, :64], scale=SCALE,
+                      slopes=sl)
+        check(out[rows], w, b, f"short table {form} sequence {i}")
