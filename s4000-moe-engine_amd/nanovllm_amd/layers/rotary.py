@@ -116,6 +116,7 @@ def pair_axes(sections: tuple, interleaved: bool, half: int = 64) -> np.ndarray:
             axes[a:step * sections[a]:step] = a
     else:
         axes[:] = np.repeat(np.arange(len(sections)), sections)
+    axes.flags.writeable = False    # every later call reads this array
     return axes
 
 

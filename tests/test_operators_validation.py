@@ -334,3 +334,11 @@ def test_graph_runner_checks_values_before_a_capture(bad):
     caches = [torch.zeros(3, 32, 2, 128, dtype=torch.bfloat16)]
     with pytest.raises(ValueError):
         DecodeGraphRunner(caches, caches, 8, 2, 2, 0.1, score_shapes=bad)
+
+
+def test_pair_axes_cannot_be_written():
+    """One array serves every call with the same sections."""
+    axes = pair_axes((16, 24, 24), False)
+    with pytest.raises(ValueError):
+        axes[0] = 2
+    assert pair_axes((16, 24, 24), False)[0] == 0
