@@ -48,7 +48,7 @@ def tree_attention(q, k_cache, v_cache, block_tables, context_lens, tree_mask, s
     int64 [T, words], bit u % 64 of word u / 64).  softcap, alibi_slopes and
     window as in scored_attention, with the token's depth (bits in its mask,
     less one) for its distance from the context.  Returns out [T, H, 128]; a
-    token that sees no key gives 0, rows past the last tree are not written."""
+    token that sees no key gives 0, rows of no tree are not written."""
     if nat.is_current(q):
         done = nat.host().tree(q, k_cache, v_cache, block_tables, context_lens, tree_mask, scale,
                                cu_seqlens_q, max_seqlen_q, softcap, alibi_slopes, window,
