@@ -17,8 +17,9 @@
 // 16 bytes each, so a rotation pair never leaves its lane and the sum of
 // squares is three DPP moves.  Bound by HBM: each row is read and written
 // once; 16384 tokens of 32 / 4 heads, 344 MB, take 67 us (5.1 TB/s; torch's
-// copy of 2 GiB 4.9), 58 where a part of them is cached still.  A decode step of 64 tokens takes 4 us, the launch and three
-// dependent reads (position, table, row).
+// copy of 2 GiB 4.9), 58 where a part of them is cached still.  A decode step of
+// 64 tokens takes 4 us, the launch and three dependent reads (position, table,
+// row).
 #include "kvc_lds.h"
 
 namespace kvc {

@@ -31,7 +31,7 @@
 //   turns    64 to 256 columns (chunks, larger trees): the waves split the
 //            columns and read the same tile from a ring of LDS slots; one half
 //            multiplies while the other takes its softmax.  Bound by the issue
-//            of both: 2100 cycles a 256-column tile for plain scores, 2550 for
+//            of both: 2100 cycles a 256-column tile for plain scores, 2600 for
 //            capped ones, of which the matrix unit is busy 1024 (64 trees of
 //            64 tokens over 4096 keys: 838 TFLOP/s; a chunk of 2048 over 14336
 //            keys, capped: 880).
