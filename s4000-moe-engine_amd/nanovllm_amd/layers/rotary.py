@@ -98,7 +98,6 @@ def qk_norm_rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None,
     return q_out, k_out
 
 
-@functools.lru_cache(maxsize=64)
 def pair_axes(sections: tuple, interleaved: bool, half: int = 64) -> np.ndarray:
     """The axis of each of a head's rotary pairs, int32 [half].  sections[a] is
     the number of pairs of axis a: in runs, axis 0 first; interleaved, axis a
@@ -116,7 +115,6 @@ def pair_axes(sections: tuple, interleaved: bool, half: int = 64) -> np.ndarray:
             axes[a:step * sections[a]:step] = a
     else:
         axes[:] = np.repeat(np.arange(len(sections)), sections)
-    axes.flags.writeable = False    # every later call reads this array
     return axes
 
 

@@ -336,9 +336,12 @@ def test_graph_runner_checks_values_before_a_capture(bad):
         DecodeGraphRunner(caches, caches, 8, 2, 2, 0.1, score_shapes=bad)
 
 
-def test_pair_axes_cannot_be_written():
-    """One array serves every call with the same sections."""
+def test_pair_axes_belong_to_the_caller():
+    """Writing to them changes no later call's."""
+    from nanovllm_amd.layers.rotary import _pair_axes_at
+    held, at = _pair_axes_at((16, 24, 24), False)
     axes = pair_axes((16, 24, 24), False)
-    with pytest.raises(ValueError):
-        axes[0] = 2
-    assert pair_axes((16, 24, 24), False)[0] == 0
+    assert axes.ctypes.data != at and axes.tolist() == held.tolist()
+    axes[0] = 2
+    assert pair_axes((16, 24, 24), False)[0] == 0 and held[0] == 0
+    assert _pair_axes_at((16, 24, 24), False)[1] == at
