@@ -15,7 +15,7 @@ COMMENT = re.compile(r"//[^\n]*|/\*.*?\*/", re.S)
 ASM = re.compile(r"\basm\s+(?:volatile\s*)?\(")
 STRING = re.compile(r'\s*"((?:[^"\\]|\\.)*)"')
 WRITES_M0 = re.compile(r"s_\w+\s+m0\b")
-LOADS_LDS = re.compile(r"(?:buffer|global)_load_\w+\b.*(?:\blds\b|_lds_)")
+LOADS_LDS = re.compile(r"buffer_load_\w+\b.*\blds\b|(?:global|scratch)_load_lds_\w+")
 
 
 def _statements(text):
@@ -52,3 +52,5 @@ def test_the_scan_finds_such_loads():
     bad = 'asm volatile("s_mov_b32 m0, %0\\n\\t"\n "buffer_load_dwordx4 %1, %2, 0 offen lds");'
     (lines,) = _statements(bad)
     assert _unwaited(lines)
+    assert _unwaited(["s_add_u32 m0, m0, s3", "global_load_lds_dwordx4 v[0:1], off"])
+    assert not _unwaited(["s_mov_b32 m0, s3", "s_nop 0", "global_load_lds_dwordx4 v[0:1], off"])
