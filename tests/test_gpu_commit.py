@@ -116,3 +116,40 @@ def test_runner_moves_everything_that_travels_with_a_row(mode):
     torch.cuda.synchronize()
     for p, was in zip(pools, before):
         assert torch.equal(p.cpu(), _want(was, 32, tables, ctx, paths, lens))
+
+
+def test_captured_and_replayed():
+    """One captured move serves other contexts, tables and paths, with eager
+    moves between the replays."""
+    page, room, most = 32, 40, 12
+    tables, blocks = _case((2, 128), page, [60, 60], room, 7)
+    gen = torch.Generator().manual_seed(8)
+    pool = torch.randint(-100, 100, (2, 2, blocks, page, 2, 128), generator=gen).to(torch.int16)
+    pool_d, table_d = torch.empty_like(pool, device=DEV), tables.to(DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    ctx_d, path_d, len_d = torch.zeros(2, **i32), torch.zeros(2, most, **i32), torch.zeros(2, **i32)
+
+    def call():
+        commit_tree_path(pool_d, table_d, ctx_d, path_d, len_d)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    rng = random.Random(9)
+    for ctx in ([60, 3], [0, 31], [33, 64], [60, 3]):
+        lens = [rng.randint(0, most) for _ in ctx]
+        paths = torch.tensor([sorted(rng.sample(range(room - 8), n)) + [0] * (most - n)
+                              for n in lens], dtype=torch.int32)
+        table = tables.flip(0) if ctx[0] == 0 else tables
+        ctx_d.copy_(torch.tensor(ctx, dtype=torch.int32))
+        path_d.copy_(paths)
+        len_d.copy_(torch.tensor(lens, dtype=torch.int32))
+        table_d.copy_(table)
+        want = _want(pool, page, table, ctx, paths, lens)
+        for run in (graph.replay, call):
+            pool_d.copy_(pool)
+            run()
+            torch.cuda.synchronize()
+            assert torch.equal(pool_d.cpu(), want)
