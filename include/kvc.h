@@ -25,6 +25,12 @@
  *                          [num_blocks, page_size, num_kv_heads, n_out_max],
  *                          out_idx2d int32 [num_kv_heads, n_out_max],
  *                          head_n_out int32 [num_kv_heads].
+ *   4-bit floats           codes uint8 [num_blocks, page_size, num_kv_heads,
+ *                          64] (dim 2j in the low half of byte j: bit 3 the
+ *                          sign, 0 .. 7 = 0, 0.5, 1, 1.5, 2, 3, 4, 6), scales
+ *                          uint8 [num_blocks, page_size, num_kv_heads, 4]:
+ *                          byte g is the exponent + 127 of the power of two
+ *                          that scales dims 32g .. 32g + 31 (255: NaN).
  *   whole-block slabs      a block of a multi-layer pool
  *                          [planes, num_blocks, block_bytes] (planes =
  *                          2 * layers for the engine's [2, L, ...] pool) is
@@ -673,6 +679,97 @@ int kvc_stage_decode(const void* q, int64_t q_layer_stride, int64_t q_row_stride
                      int64_t bt_stride, int64_t bt_cols, void* q_dst, void* k_dst, void* v_dst,
                      int32_t* slots_dst, int32_t* lens_dst, int32_t* tables_dst, int64_t dst_cols,
                      int32_t scratch_slot, int32_t scratch_block, kvc_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * The KV cache in 4-bit floats (no reference counterpart).
+ * ------------------------------------------------------------------------- */
+
+/* kvc_store_kv into a 4-bit pool: bf16 key/value rows [num_tokens, KVH, 128],
+ * 16-byte aligned, quantised as they are stored.  A run of 32 dims takes the
+ * smallest power of two that brings its largest magnitude to 6 or less (2^-126
+ * at least, 2^125 at most: finite values stay finite); values round to the
+ * nearest code, ties to the even mantissa.  A run that holds an infinity or a
+ * NaN is NaN (scale 255, codes 0).  Slots as for kvc_store_kv. */
+int kvc_store_fp4(const void* key, int64_t key_stride_n, int64_t key_stride_h, const void* value,
+                  int64_t value_stride_n, int64_t value_stride_h, uint8_t* k_cache,
+                  uint8_t* v_cache, uint8_t* k_scale, uint8_t* v_scale, int64_t num_slots,
+                  const void* slot_mapping, int slot_index_bytes, int64_t num_tokens,
+                  int64_t num_kv_heads, int64_t head_dim, kvc_stream_t stream);
+
+/* rows x 128 values of codes [rows, 64] and scales [rows, 4] as bf16 (exact but
+ * for magnitudes under 2^-126, which bf16 holds with fewer bits). */
+int kvc_dequant_fp4(const uint8_t* codes, const uint8_t* scale, int64_t rows, int64_t head_dim,
+                    void* out, kvc_stream_t stream);
+
+/* kvc_gather_kv over a 4-bit pool: chunk i's keys and values (block table row
+ * block_table_row0 + i), as bf16, at rows cu_seqlens_k[i] .. of out_k / out_v
+ * [total_keys, KVH, 128].  Keys whose table entry is bad are zeros. */
+int kvc_gather_kv_fp4(const uint8_t* k_cache, const uint8_t* v_cache, const uint8_t* k_scale,
+                      const uint8_t* v_scale, int64_t num_cache_blocks, int64_t page_size,
+                      int64_t num_kv_heads, int64_t head_dim, const int32_t* block_tables,
+                      int64_t bt_stride, int64_t max_blocks_per_seq, int64_t block_table_row0,
+                      int64_t num_prefill, const int32_t* cu_seqlens_k, int64_t total_keys,
+                      void* out_k, void* out_v, kvc_stream_t stream);
+
+/* Bytes of workspace kvc_paged_decode_fp4 needs for this launch shape (0 for
+ * short tables); sized from the table width, never from context lengths. */
+size_t kvc_paged_decode_fp4_workspace_bytes(int64_t batch, int64_t num_heads,
+                                            int64_t num_kv_heads, int64_t page_size,
+                                            int64_t max_blocks_per_seq);
+
+/* kvc_paged_decode over a 4-bit pool: q/out bf16 [batch, num_heads, 128], any
+ * number of query heads per kv head, page_size a multiple of 32, tables of up to
+ * 2^26 keys.  Scores, sums and outputs are fp32 until the one rounding to bf16;
+ * weights are rounded to bf16 for the product with V.  A row with
+ * context_lens[b] <= 0 gives zeros; a length past its table counts the table's
+ * keys; keys whose table entry is bad read as zeros. */
+int kvc_paged_decode_fp4(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                         const uint8_t* k_cache, const uint8_t* v_cache, const uint8_t* k_scale,
+                         const uint8_t* v_scale, int64_t num_cache_blocks, int64_t page_size,
+                         int64_t num_kv_heads, int64_t head_dim, const int32_t* block_tables,
+                         int64_t bt_stride, int64_t max_blocks_per_seq,
+                         const int32_t* context_lens, int64_t batch, int64_t num_heads,
+                         float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                         void* workspace, size_t workspace_bytes, kvc_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * A step's tables from its requests' lengths, on the device.
+ * ------------------------------------------------------------------------- */
+
+/* What KVCacheRunner's host code builds for a step (nanovllm/engine/
+ * model_runner.py:579-699 with the block manager's allocation), for callers
+ * whose lengths live on the device.  Row b holds num_blocks[b] pages (the first
+ * entries of its row of block_tables) for context_lens[b] tokens and asks for
+ * query_lens[b] new ones; free_blocks[0 .. num_free[0]) is a stack of free
+ * pages (free_size entries at most).
+ *   1. Rows with finished[b] != 0 (finished may be NULL) give their pages back,
+ *      pushed in row and table order, and are empty from then on.
+ *   2. Every row with query_lens[b] > 0 needs ceil((context + query) / page) -
+ *      held pages.  It is granted its tokens if its table row is wide enough,
+ *      if it needs no page or the pages needed by all rows up to it are there,
+ *      and if the tokens wanted by the rows up to it fit into max_tokens
+ *      (tokens_per_row 0) or its own into tokens_per_row.  A row that is not
+ *      granted keeps what it holds and takes no page.
+ *   3. Granted rows take pages from the top of the stack, in row order, into
+ *      their table rows behind those they hold.
+ * Outputs: query_lens_out (granted tokens), seq_lens_out (keys that the step
+ * attends: context + granted, 0 for a row without tokens), context_lens_out
+ * (context + granted), num_blocks_out, num_free_out, cu_seqlens_q / cu_seqlens_k
+ * [batch + 1] (sums of query_lens_out and seq_lens_out), and for the tokens
+ * slot_mapping and positions [max_tokens]: packed in row order (tokens_per_row
+ * 0), else row b's at b * tokens_per_row; tokens that there are not get pad_slot
+ * and position 0.  block_tables and free_blocks change in place; context_lens,
+ * num_blocks, num_free and query_lens may be their own outputs (context_lens_out
+ * over context_lens and so on).  Lengths count up to 2^29. */
+int kvc_step_tables(const int32_t* context_lens, const int32_t* query_lens,
+                    const uint8_t* finished, int32_t* block_tables, int64_t bt_stride,
+                    int64_t max_blocks_per_seq, int64_t batch, const int32_t* num_blocks,
+                    int32_t* free_blocks, int64_t free_size, const int32_t* num_free,
+                    int64_t page_size, int64_t max_tokens, int64_t tokens_per_row,
+                    int32_t pad_slot, int32_t* slot_mapping, int64_t* positions,
+                    int32_t* query_lens_out, int32_t* seq_lens_out, int32_t* context_lens_out,
+                    int32_t* num_blocks_out, int32_t* num_free_out, int32_t* cu_seqlens_q,
+                    int32_t* cu_seqlens_k, kvc_stream_t stream);
 
 #ifdef __cplusplus
 }

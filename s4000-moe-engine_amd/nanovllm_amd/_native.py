@@ -25,6 +25,7 @@ LIB_PATH = pathlib.Path(os.environ.get("KVC_LIBRARY", PKG_ROOT / "lib" / "libkvc
 KVC_KV_BF16 = 0
 KVC_KV_INT8_TOKHEAD = 1
 KVC_KV_INT8_CHAN = 2
+KVC_KV_FP4 = 3  # of this package alone: the 4-bit entry points are their own
 # include/kvc.h KVC_STATIC_SCRATCH_BYTES
 STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -38,6 +39,7 @@ _ERRORS = {
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
+_I32 = ctypes.c_int32
 _F32 = ctypes.c_float
 _SZ = ctypes.c_size_t
 
@@ -120,6 +122,17 @@ SIGNATURES = {
                                        _INT, _P]),
     "kvc_commit_rows": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64,
                                _I64, _P, _I64, _P]),
+    "kvc_store_fp4": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _INT, _I64,
+                             _I64, _I64, _P]),
+    "kvc_dequant_fp4": (_INT, [_P, _P, _I64, _I64, _P, _P]),
+    "kvc_gather_kv_fp4": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64,
+                                 _I64, _P, _I64, _P, _P, _P]),
+    "kvc_paged_decode_fp4_workspace_bytes": (_SZ, [_I64] * 5),
+    "kvc_paged_decode_fp4": (_INT, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P,
+                                    _I64, _I64, _P, _I64, _I64, _F32, _P, _I64, _I64, _P, _SZ,
+                                    _P]),
+    "kvc_step_tables": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I64,
+                               _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "kvc_stage_decode": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,
                                 _I64, _I64, _I64, _P, _INT, _P, _INT, _P, _I64, _I64, _P, _P, _P,
                                 _P, _P, _P, _I64, _INT, _INT, _P]),

@@ -10,6 +10,7 @@ Differences that only widen what is accepted:
   * int8 pools in either encoding: per-channel read scales [KVH, D] with the
     bf16 outlier side pool (the engine's current layout), or per-token-head
     scales [blocks, page, KVH] (k_scale.dim() == 3);
+  * pools of 4-bit floats with their scales (kernels/kv_fp4.py);
   * the side pool is used without the reference's host sync on
     int(head_n_out.max()) (paged_attention.py:218): the kernel reads
     head_n_out on the device.
@@ -22,6 +23,7 @@ import numpy as np
 import torch
 
 from .. import _native as nat
+from .kv_fp4 import paged_decode_fp4
 
 
 def _check_append_enabled() -> bool:
@@ -43,8 +45,13 @@ def _kv_encoding(k_cache: torch.Tensor, k_scale: torch.Tensor | None) -> int:
         if k_scale is None:
             raise ValueError("an int8 KV pool needs k_scale/v_scale")
         return nat.KVC_KV_INT8_TOKHEAD if k_scale.dim() == 3 else nat.KVC_KV_INT8_CHAN
+    if k_cache.dtype == torch.uint8:
+        if k_scale is None:
+            raise ValueError("a 4-bit KV pool needs k_scale/v_scale")
+        return nat.KVC_KV_FP4
     if k_cache.dtype != torch.bfloat16:
-        raise ValueError(f"KV pool dtype {k_cache.dtype} is not supported (bf16 or int8)")
+        raise ValueError(f"KV pool dtype {k_cache.dtype} is not supported (bf16, int8 or 4-bit "
+                         "floats in uint8)")
     if k_scale is not None:
         raise ValueError("k_scale given for a bf16 KV pool")
     return nat.KVC_KV_BF16
@@ -55,6 +62,9 @@ def paged_decode_attention(
     k_scale=None, v_scale=None, side_k=None, side_v=None,
     out_idx2d=None, head_n_out=None,
 ):
+    if k_cache.dtype == torch.uint8:
+        return paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
+                                scale)
     if q.is_cuda and k_scale is None:
         done = nat.host().decode(None, q, k_cache, v_cache, block_tables, context_lens, scale,
                                  nat.stream_of(q), None, None, None)

@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from .. import _native as nat
+from .kv_fp4 import check_fp4_pool, gather_kv_fp4, paged_decode_fp4
 from .paged_attention import _kv_encoding
 
 
@@ -132,11 +133,18 @@ def gather_kv(k_cache, v_cache, block_tables, cu_seqlens_k, cu_seqlens_k_list, *
     """_gather_kv (nanovllm/layers/attention.py:33-51) for every prefill chunk
     of a step in one launch (kvc_gather_kv): chunk i's keys, read through
     block table row block_table_row0 + i and dequantised as the reference
-    does for an int8 pool, at rows cu_seqlens_k[i] .. of the returned bf16
-    (K, V), each [cu_seqlens_k[-1], KVH, D]."""
+    does for an int8 pool (or from a 4-bit one), at rows cu_seqlens_k[i] .. of
+    the returned bf16 (K, V), each [cu_seqlens_k[-1], KVH, D]."""
     enc = _kv_encoding(k_cache, k_scale)
     cu_k = list(cu_seqlens_k_list)
     total = cu_k[-1]
+    if enc == nat.KVC_KV_FP4:
+        tables = block_tables.to(torch.int32)
+        if tables.stride(1) != 1:
+            tables = tables.contiguous()
+        return gather_kv_fp4(k_cache, v_cache, k_scale, v_scale, tables,
+                             cu_seqlens_k.to(torch.int32).contiguous(), total, block_table_row0,
+                             len(cu_k) - 1)
     kvh, page = k_cache.size(2), k_cache.size(1)
     out_k = torch.empty((total, kvh, k_cache.size(3)), dtype=torch.bfloat16, device=k_cache.device)
     out_v = torch.empty_like(out_k)
@@ -169,7 +177,7 @@ def gather_kv(k_cache, v_cache, block_tables, cu_seqlens_k, cu_seqlens_k_list, *
 def _gathered_prefill(c, q, nd, k_cache, v_cache, scale, k_scale, v_scale, side_k, side_v,
                       out_idx2d, head_n_out):
     """Prefill rows (query rows nd ..) over an int8 pool as the reference reads
-    them: the chunks' keys gathered and dequantised to bf16 (gather_kv,
+    them, or over a 4-bit one: the chunks' keys gathered and dequantised to bf16 (gather_kv,
     block table rows nd + i), then the bf16 stream-K prefill over those rows,
     whose outlier dims (a per-channel pool) take the residue product."""
     kg, vg = gather_kv(k_cache, v_cache, c.block_tables, c.cu_seqlens_k, c.cu_k_list,
@@ -195,6 +203,10 @@ def _gathered_prefill(c, q, nd, k_cache, v_cache, scale, k_scale, v_scale, side_
 def _paged_rows(c, q, nd, k_cache, v_cache, scale, k_scale, v_scale, side_k, side_v, out_idx2d,
                 head_n_out, has_side):
     """The decode rows 0 .. nd - 1 of a mixed call alone (no prefill chunks)."""
+    if c.enc == nat.KVC_KV_FP4:
+        paged_decode_fp4(q[:nd], k_cache, v_cache, k_scale, v_scale, c.block_tables[:nd],
+                         c.decode_context_lens, scale, c.out[:nd])
+        return
     nat.call(
         "kvc_varlen_attention",
         q.data_ptr(), q.stride(0), q.stride(1), nd, c.num_heads,
@@ -232,8 +244,10 @@ def varlen_attention(q, k_cache, v_cache, *, scale, block_tables=None,
     if c.T == 0:
         return c.out
     enc, fresh, q = c.enc, c.fresh, c.q
+    if enc == nat.KVC_KV_FP4:
+        check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
     gathered = (enc != nat.KVC_KV_BF16 and not fresh and c.num_prefill
-                and os.environ.get("KVC_PREFILL_SK", "1") != "0")
+                and (enc == nat.KVC_KV_FP4 or os.environ.get("KVC_PREFILL_SK", "1") != "0"))
     has_side = enc == nat.KVC_KV_INT8_CHAN and side_k is not None and head_n_out is not None
     # fresh rows gathered from a per-channel pool name its outlier dims
     fresh_out = fresh and out_idx2d is not None and head_n_out is not None
@@ -243,13 +257,17 @@ def varlen_attention(q, k_cache, v_cache, *, scale, block_tables=None,
         k_scale = k_scale.to(torch.float32).contiguous()
         v_scale = v_scale.to(torch.float32).contiguous()
     if gathered:
-        # Int8 pool: the decode rows (if any) through the paged decode alone,
+        # Int8 or 4-bit pool: the decode rows (if any) through the paged decode alone,
         # then the prefill rows over their gathered, dequantised keys.
         if num_decode_rows:
             _paged_rows(c, q, num_decode_rows, k_cache, v_cache, scale, k_scale, v_scale,
                         side_k, side_v, out_idx2d, head_n_out, has_side)
         return _gathered_prefill(c, q, num_decode_rows, k_cache, v_cache, scale, k_scale, v_scale,
                                  side_k, side_v, out_idx2d, head_n_out)
+    if enc == nat.KVC_KV_FP4:
+        _paged_rows(c, q, num_decode_rows, k_cache, v_cache, scale, k_scale, v_scale, None, None,
+                    None, None, False)
+        return c.out
     nat.call(
         "kvc_varlen_attention",
         q.data_ptr(), q.stride(0), q.stride(1), c.T, c.num_heads,
