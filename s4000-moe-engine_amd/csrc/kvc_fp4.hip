@@ -21,6 +21,7 @@
 // lengths, table, tiles and merge for single rows.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "kvc_fp4.h"
 #include "kvc_lds.h"
@@ -128,17 +129,18 @@ gather_fp4_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
 // Paged decode.
 // ---------------------------------------------------------------------------
 constexpr int kWaves = 8;
-constexpr int kTile = 64;                       // keys
-constexpr int kCodeBytes = kTile * kFp4RowBytes;  // of K or V, 4 KiB
-constexpr int kPowerBytes = kTile * kFp4Powers;   // 256
-constexpr int kVAt = kCodeBytes, kKsAt = 2 * kCodeBytes, kVsAt = kKsAt + kPowerBytes;
-constexpr int kSlotBytes = kVsAt + kPowerBytes;  // 8.5 KiB
+constexpr int kTileRows = 64;                         // (key, head) rows of a wave's tile
+constexpr int kCodeBytes = kTileRows * kFp4RowBytes;  // of K or V, 4 KiB
+constexpr int kPowerBytes = kTileRows * kFp4Powers;   // 256
+constexpr int kVAt = kCodeBytes, kKpAt = 2 * kCodeBytes, kVpAt = kKpAt + kPowerBytes;
+constexpr int kSlotBytes = kVpAt + kPowerBytes;  // 8.5 KiB
 constexpr int kSlots = 2;
-constexpr int kLoads = 12;  // of a tile: K and V in four each, powers in two each
 constexpr float kLowest = -3.402823466e38f;
-constexpr float kSlack = 8.f;  // binades that a score may pass the running reference by
+// Binades that a score may pass the running reference by: a weight of up to 4
+// times the largest power, 2^125, is still finite.
+constexpr float kSlack = 2.f;
 constexpr int kStateBytes = 8 * 64 * 16 + 64 * 8;  // a wave's O and (reference, sum)
-static_assert(kStateBytes <= kSlots * kSlotBytes);
+static_assert(kStateBytes <= kSlotBytes);  // (one a head, a slot each)
 
 struct Fp4Params {
   const uint16_t* q;
@@ -158,37 +160,35 @@ struct Fp4Params {
   int batch, kv_heads, group;
   int col_blocks;          // of 16 query heads, of a kv head's
   int heads_per_wg;        // kv heads of a workgroup
+  int tile_shift;          // log2 of the keys of a wave's tile
   int groups;              // workgroup items of a row: kv head groups x col_blocks
   int cols;                // columns kept of a partial: min(16, group)
   int min_share;
+  float grid_rcp;
   int whole;               // one workgroup an item, no partials
-  float c2;                // scale log2(e)
+  float c2;                // |scale| log2(e)
+  uint32_t flip;           // sign bits of a bf16 pair where scale is negative
   int2* rec;               // of each item: first and last share
   float* part_o;
   float2* part_ml;
 };
 
-// Keys of row b that the tables can hold; steps of a row (a step is one tile of
-// every phase), 1 for a row without keys: it writes zeros.
+// Keys of row b that the tables can hold; tiles of a row, 1 for a row without
+// keys: it writes zeros.
 __device__ __forceinline__ int keys_of(const Fp4Params& p, int len) {
   const int64_t most = int64_t(p.max_blocks) * p.page;
   return int(min(int64_t(max(len, 0)), most));
 }
-__device__ __forceinline__ int steps_of(int keys, int step_keys) {
-  return max(1, (keys + step_keys - 1) / step_keys);
+__device__ __forceinline__ int tiles_of(const Fp4Params& p, int keys) {
+  return max(1, (keys + (1 << p.tile_shift) - 1) >> p.tile_shift);
 }
 
-__device__ __forceinline__ void dma_dword(const i32x4_t& rsrc, int voff, uint32_t lds) {
-  uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dword %1, %3, 0 offen nt lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "v"(voff), "s"(lds), "s"(rsrc)
-      : "memory");
+// floor(x / d), given rcp, 1 / d to within a few ulp, for quotients below 2^20.
+__device__ __forceinline__ int div_steps(int64_t x, int64_t d, float rcp) {
+  int q = int(float(x) * rcp);
+  q += int64_t(q + 1) * d <= x ? 1 : 0;
+  q -= int64_t(q) * d > x ? 1 : 0;
+  return uniform(q);
 }
 
 template <int N>
@@ -196,50 +196,188 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+typedef int v2i_t __attribute__((ext_vector_type(2)));
+typedef int v8i_t __attribute__((ext_vector_type(8)));
+typedef float f32x2v_t __attribute__((ext_vector_type(2)));
+typedef short s16x2v_t __attribute__((ext_vector_type(2)));
+
+// A column's query as the two 8-bit operands (e4m3) of the scaled MFMA: x = hi +
+// lo, hi = x rounded to four significant bits, lo the rest, which four bits hold
+// as well.  Both count in one power of two for the row, lo 16 times finer.  x is
+// met to 2^-21 of the row's largest magnitude (lo's last place), exactly from
+// 2^-13 of it up.
+struct Query {
+  v8i_t hi, lo;     // dims 16 lg .. + 15, then 64 + 16 lg .. + 15
+  int hi_power, lo_power;
+};
+struct QueryRow {  // bf16, dims 16 lg .., 16 lg + 8 .., 64 + 16 lg .., 64 + 16 lg + 8 ..
+  u32x4_t x[4];
+};
+__device__ __forceinline__ QueryRow load_query(const uint16_t* row, int lg) {
+  QueryRow r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r.x[i] = *reinterpret_cast<const u32x4_t*>(row + 64 * (i >> 1) + 16 * lg + 8 * (i & 1));
+  return r;
+}
+__device__ __forceinline__ Query split_query(const QueryRow& r, uint32_t flip) {
+  const u32x4_t(&x)[4] = r.x;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, top_bits(x[i]));
+  top = __float_as_uint(rows4_max(__uint_as_float(top << 16))) >> 16;
+  Query q;
+  // (a magnitude of 2^e counts 2^7; the low end leaves room for lo's power)
+  q.hi_power = max(int(top >> 7) - 7, 5);
+  q.lo_power = q.hi_power - 4;
+  const float hp = __uint_as_float(uint32_t(q.hi_power) << 23);
+  const float lp = __uint_as_float(uint32_t(q.lo_power) << 23);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {  // four dims
+    const uint32_t a = x[w >> 1][2 * (w & 1)] ^ flip, b = x[w >> 1][2 * (w & 1) + 1] ^ flip;
+    typedef short s16x2_t __attribute__((ext_vector_type(2)));
+    s16x2_t h = {0, 0}, l = {0, 0};
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, a), hp, false);
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, b), hp, true);
+    const int hw = __builtin_bit_cast(int, h);
+    const f32x2v_t back0 = __builtin_bit_cast(f32x2v_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, hp, false));
+    const f32x2v_t back1 = __builtin_bit_cast(f32x2v_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, hp, true));
+    l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_bits_to_f32(a & 0xffffu) - back0[0],
+                                                 bf16_bits_to_f32(a >> 16) - back0[1], lp, false);
+    l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_bits_to_f32(b & 0xffffu) - back1[0],
+                                                 bf16_bits_to_f32(b >> 16) - back1[1], lp, true);
+    q.hi[w] = hw;
+    q.lo[w] = __builtin_bit_cast(int, l);
+  }
+  return q;
+}
+
+typedef const __attribute__((address_space(4))) Fp4Params KernelArgs;
+__device__ __forceinline__ KernelArgs* kernel_args() {
+  KernelArgs* a = (KernelArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return a;
+}
+
 struct Carry {  // a wave's running softmax and output, column lane & 15
   f32x4_t o[8];  // channels 16 cb + 4 (lane >> 4) ..
-  float m, l;
+  f32x4_t l;     // the column's sum, in every element
+  float m;
 };
 
-// One tile in `slot`: keys j0 .. j0 + 63 of a row of n keys.
-__device__ __forceinline__ void attend_tile(const char* slot, const u32x4_t (&q)[4], Carry& c,
-                                            int j0, int n, int lm, int lg, float c2) {
-  f32x4_t s[4];
+// S^T += K Q^T: 16 rows of 128 codes with their powers (run lane >> 4).
+__device__ __forceinline__ f32x4_t mfma_fp4(const u32x4_t& k, const v8i_t& q, const f32x4_t& c,
+                                            int k_power, int q_power) {
+  const v8i_t a = {int(k[0]), int(k[1]), int(k[2]), int(k[3]), 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, c, 4, 0, 0, k_power, 0, q_power);
+}
+
+// A wave's tile is 64 rows of codes: 64 keys of one kv head (NH = 1) or 32 keys of
+// two (NH = 2), in two halves h of 32 keys.  Two heads next to each other are a
+// whole 128-byte line of the pool, and a wave that reads half lines gets 5.1 TB/s
+// of HBM where whole ones give 6.1 (loads alone, 16 rows of 32768 keys, 4 heads).
+//
+// In LDS: NH = 1, 64-byte rows, K's in the order of the MFMA's rows (16-row part
+// 2 h + t: key 8 (r >> 2) + 4 t + (r & 3) of the half), V's in key order.  NH = 2,
+// 128-byte rows in key order.  A row's 16-byte parts are turned (by xor) so that
+// neither kind of operand read meets a bank twice.
+template <int NH>
+struct TileLayout;
+template <>
+struct TileLayout<1> {
+  static __device__ int key(int x, int lm, int lg) {  // of 16-row part x = 2 h + t
+    return 1024 * x + 64 * lm + 16 * (lg ^ (lm >> 2));
+  }
+  static __device__ int value(int cb, int lm, int lg) {
+    const int h = lm >> 3, k = 8 * lg + (lm & 7);
+    return 2048 * h + 64 * k + 16 * ((cb >> 1) ^ (((k >> 2) & 1) + 2 * h)) + 8 * (cb & 1);
+  }
+  // Offsets of a lane's 16 bytes in the pool, of load m (of 4): K, V.
+  static __device__ int load_key(int m, int lane, int row_bytes) {
+    const int r = lane >> 2;
+    return (8 * (r >> 2) + 4 * (m & 1) + (r & 3)) * row_bytes + 16 * ((lane & 3) ^ (r >> 2));
+  }
+  static __device__ int load_value(int m, int lane, int row_bytes) {
+    return (16 * (m & 1) + (lane >> 2)) * row_bytes +
+           16 * ((lane & 3) ^ (((lane >> 4) & 1) + 2 * (m >> 1)));
+  }
+};
+template <>
+struct TileLayout<2> {
+  static __device__ int key(int x, int lm, int lg) {
+    return 1024 * (lm >> 2) + 128 * (4 * (x & 1) + (lm & 3)) +
+           16 * ((4 * (x >> 1) + lg) ^ (lm >> 1));
+  }
+  static __device__ int value(int cb, int lm, int lg) {
+    return 1024 * lg + 128 * (lm & 7) + 16 * ((4 * (lm >> 3) + (cb >> 1)) ^ ((lm >> 1) & 3)) +
+           8 * (cb & 1);
+  }
+  static __device__ int load_key(int m, int lane, int row_bytes) {
+    return (8 * m + (lane >> 3)) * row_bytes + 16 * ((lane & 7) ^ (2 * m + ((lane >> 4) & 1)));
+  }
+  static __device__ int load_value(int m, int lane, int row_bytes) {
+    return (8 * m + (lane >> 3)) * row_bytes + 16 * ((lane & 7) ^ ((lane >> 4) & 3));
+  }
+};
+
+// A tile in registers.  K: four operands of 16 rows and the lane's run's power of
+// each.  V: of each 16 channels, the lane's 8 keys 8 lg + j of both halves, channel
+// lm, and those keys' powers; mine: the powers of key lane & 31 of half lane >> 5.
+struct Tile {
+  u32x4_t k[4];
+  int k_power[4];
+  v2i_t v[8];
+  u32x4_t v_power[2][2];
+  uint32_t mine;
+};
+template <int NH>
+__device__ __forceinline__ void read_tile(Tile& t, const char* at, int lane, int lm, int lg) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    const u32x4_t w =
-        *reinterpret_cast<const u32x4_t*>(slot + 1024 * x + 64 * lm + 16 * (lg ^ (lm >> 2)));
+    t.k[x] = *reinterpret_cast<const u32x4_t*>(at + TileLayout<NH>::key(x, lm, lg));
     const int key = 32 * (x >> 1) + 8 * (lm >> 2) + 4 * (x & 1) + (lm & 3);
-    const float power =
-        power_f32(*reinterpret_cast<const uint8_t*>(slot + kKsAt + 4 * key + lg));
-    s[x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < 4; ++d) s[x] = mfma_bf16(dequant_fp4x8(w[d], power), q[d], s[x]);
+    t.k_power[x] = *reinterpret_cast<const uint8_t*>(at + kKpAt + 4 * key + lg);
   }
-  // The lane's keys: 32 h + 8 lg + j for h = 0, 1 and j = 0 .. 7.
-  u32x4_t pw[2][2];
+#pragma unroll
+  for (int cb = 0; cb < 8; ++cb)
+    t.v[cb] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+        (__attribute__((address_space(3))) v2i_t*)((__attribute__((address_space(3))) char*)(
+            at + kVAt + TileLayout<NH>::value(cb, lm, lg))));
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      pw[h][i] = *reinterpret_cast<const u32x4_t*>(slot + kVsAt + 4 * (32 * h + 8 * lg + 4 * i));
-  float y[16];
+      t.v_power[h][i] =
+          *reinterpret_cast<const u32x4_t*>(at + kVpAt + 4 * (32 * h + 8 * lg + 4 * i));
+  t.mine = *reinterpret_cast<const uint32_t*>(at + kVpAt + 4 * lane);
+}
+
+// The keys of a tile past its row's `left`: scores -infinity, no power (what lies
+// there may hold anything).
+template <int NH>
+__device__ __forceinline__ void mask_tile(Tile& t, f32x4_t (&s)[4], int left, int lane, int lg) {
+  int first = 8 * lg;  // (opaque: nothing of this is worked out for every tile)
+  asm volatile("" : "+v"(first));
 #pragma unroll
-  for (int e = 0; e < 16; ++e) y[e] = s[e >> 2][e & 3] * c2;
-  if (j0 + kTile > n) {
-    // (what lies behind the row's keys may hold anything: weight 0, power 1)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const bool seen = j0 + 32 * (e >> 3) + 8 * lg + (e & 7) < n;
-      y[e] = seen ? y[e] : -INFINITY;
-      const uint32_t word = pw[e >> 3][(e >> 2) & 1][e & 3];
-      pw[e >> 3][(e >> 2) & 1][e & 3] = seen ? word : 0x7f7f7f7fu;
+    for (int j = 0; j < 8; ++j) {
+      const bool seen = (NH == 1 ? 32 * h : 0) + first + j < left;
+      s[2 * h + (j >> 2)][j & 3] = seen ? s[2 * h + (j >> 2)][j & 3] : -INFINITY;
+      const uint32_t word = t.v_power[h][j >> 2][j & 3];
+      t.v_power[h][j >> 2][j & 3] = seen ? word : 0u;
     }
-  }
-  float top = y[0];
+  if ((NH == 1 ? lane : lane & 31) >= left) t.mine = 0;
+}
+
+// The weights of N scores of a column (bf16 pairs), the reference and the sum.
+template <int N>
+__device__ __forceinline__ void weights(const f32x4_t* s, Carry& c, float c2, u32x4_t* w) {
+  float top = s[0][0];
 #pragma unroll
-  for (int e = 1; e < 16; ++e) top = fmaxf(top, y[e]);
-  // The reference moves only when a score passes it by 2^kSlack.
+  for (int e = 1; e < N; ++e) top = fmaxf(top, s[e >> 2][e & 3]);
+  top *= c2;
+  // The reference moves only when a score passes it by kSlack.
   if (__builtin_amdgcn_ballot_w64(top > c.m + kSlack) != 0) {
     const float next = fmaxf(c.m, rows4_max(top));
     const float a = __builtin_amdgcn_exp2f(c.m - next);
@@ -248,46 +386,133 @@ __device__ __forceinline__ void attend_tile(const char* slot, const u32x4_t (&q)
 #pragma unroll
     for (int cb = 0; cb < 8; ++cb) c.o[cb] *= a;
   }
-  float w[16];
+  const u32x4_t ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 #pragma unroll
-  for (int e = 0; e < 16; e += 2) {
-    const uint32_t r = pack_bf16x2_fast(__builtin_amdgcn_exp2f(y[e] - c.m),
-                                        __builtin_amdgcn_exp2f(y[e + 1] - c.m));
-    w[e] = __uint_as_float(r << 16);
-    w[e + 1] = __uint_as_float(r & 0xffff0000u);
-    c.l += w[e] + w[e + 1];
-  }
-  // The row of V that the lane points the transposed reads at.
-  const int vkey = lm < 8 ? 8 * lg + lm : 24 + 8 * lg + lm;
-  const int vswz = ((vkey >> 2) & 1) + 2 * (vkey >> 5);
-  const char* vrow = slot + kVAt + 64 * vkey;
+  for (int i = 0; i < N / 8; ++i) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    u32x4_t pb[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int e = 8 * h + 2 * i;
-        const uint32_t s0 = ((pw[h][i >> 1][(2 * i) & 3] >> (8 * g)) & 0xffu) << 23;
-        const uint32_t s1 = ((pw[h][i >> 1][(2 * i + 1) & 3] >> (8 * g)) & 0xffu) << 23;
-        pb[h][i] = perm(__float_as_uint(w[e + 1] * __uint_as_float(s1)),
-                        __float_as_uint(w[e] * __uint_as_float(s0)), kPermHiHi);
-      }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int cb = 2 * g + x;
-      typedef int v2i __attribute__((ext_vector_type(2)));
-      const v2i t = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-          (__attribute__((address_space(3))) v2i*)((__attribute__((address_space(3))) char*)(
-              vrow + 16 * (g ^ vswz) + 8 * x)));
-      c.o[cb] = mfma_bf16(dequant_fp4x8(uint32_t(t[0]), 1.f), pb[0], c.o[cb]);
-      c.o[cb] = mfma_bf16(dequant_fp4x8(uint32_t(t[1]), 1.f), pb[1], c.o[cb]);
-    }
+    for (int e = 0; e < 8; e += 2)
+      w[i][e >> 1] = pack_bf16x2_fast(
+          __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + (e >> 2)][e & 3], c2, -c.m)),
+          __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + (e >> 2)][(e & 3) + 1], c2, -c.m)));
+    c.l = mfma_bf16(ones, w[i], c.l);
   }
 }
 
+// O^T += V^T P^T over the eight keys of half h.
+__device__ __forceinline__ void weigh(const Tile& t, int h, const u32x4_t& w, Carry& c) {
+  // A power of two times a weight adds to the weight's exponent field; a sum
+  // below 0 is 0.  (A weight of 0 counts as 2^-127 there.)
+  s16x2v_t wm[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = w[i];
+    wm[i] = __builtin_bit_cast(s16x2v_t, x) - s16x2v_t{127 << 7, 127 << 7};
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    u32x4_t pb;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bytes = perm(t.v_power[h][i >> 1][(2 * i + 1) & 3],
+                                  t.v_power[h][i >> 1][(2 * i) & 3], 0x0c040c00u + 0x00010001u * g);
+      s16x2v_t x = wm[i] + __builtin_bit_cast(s16x2v_t, bytes) * s16x2v_t{128, 128};
+      x = __builtin_elementwise_max(x, s16x2v_t{0, 0});
+      pb[i] = __builtin_bit_cast(uint32_t, x);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      c.o[2 * g + x] =
+          mfma_bf16(dequant_fp4x8(uint32_t(t.v[2 * g + x][h]), 1.f), pb, c.o[2 * g + x]);
+  }
+}
+
+// A run that is NaN makes its channels NaN whatever its key weighs.
+template <int NH>
+__device__ __forceinline__ void add_nan_runs(uint32_t mine, Carry (&c)[NH]) {
+  const uint32_t inv = ~mine;  // a byte of 0 where the power is 255
+  if (__builtin_expect(
+          __builtin_amdgcn_ballot_w64(((inv - 0x01010101u) & ~inv & 0x80808080u) != 0) == 0, 1))
+    return;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const uint64_t at = __builtin_amdgcn_ballot_w64(((mine >> (8 * g)) & 255u) == 255u);
+#pragma unroll
+    for (int i = 0; i < NH; ++i)
+      if ((NH == 1 ? at : at >> (32 * i) & 0xffffffffu) != 0)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          c[i].o[2 * g + x] = f32x4_t{0.f, 0.f, 0.f, 0.f} + __uint_as_float(0x7fc00000u);
+  }
+}
+
+__device__ __forceinline__ i32x4_t scalar_rsrc(const void* base, int bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  return i32x4_t{int(uint32_t(a)), int(uint32_t(a >> 32) & 0xffffu), bytes, kBufWord3};
+}
+// Two loads of 1 KiB of codes; one of powers (of the active lanes).
+__device__ __forceinline__ void load_codes(const i32x4_t& r, int off0, int off1, int base0,
+                                           int base1, uint32_t lds) {
+  uint32_t m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %4, %5 offen nt lds\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %2, %4, %6 offen nt lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(m0)
+      : "v"(off0), "v"(off1), "s"(lds), "s"(r), "s"(base0), "s"(base1)
+      : "memory", "scc");
+}
+__device__ __forceinline__ void load_powers(const i32x4_t& r, int off, uint32_t lds) {
+  uint32_t m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %1, %3, 0 offen nt lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(m0)
+      : "v"(off), "s"(lds), "s"(r)
+      : "memory");
+}
+
+// The states of P phases, `apart` in LDS, joined: phase f makes channel blocks f, f +
+// P, .. of the lane's column.
+template <int P, class Put>
+__device__ __forceinline__ void join(const char* at, int apart, int f, int lane, const Put& put) {
+  float2 ml[P];
+  float b[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    ml[i] = reinterpret_cast<const float2*>(at + i * apart + 8192)[lane];
+  f32x4_t part[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    part[i] = *reinterpret_cast<const f32x4_t*>(at + (i % P) * apart +
+                                                (f + P * (i / P)) * 1024 + lane * 16);
+  float top = ml[0].x, l = 0.f;
+#pragma unroll
+  for (int i = 1; i < P; ++i) top = fmaxf(top, ml[i].x);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    b[i] = __builtin_amdgcn_exp2f(ml[i].x - top);
+    l += ml[i].y * b[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8 / P; ++i) {
+    f32x4_t o = part[P * i] * b[0];
+#pragma unroll
+    for (int j = 1; j < P; ++j) o += part[P * i + j] * b[j];
+    put(f + P * i, o, top, l);
+  }
+}
+
+template <int NH>
 __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p) {
+  constexpr int kKeys = kTileRows / NH;  // of a tile
   extern __shared__ __align__(1024) char smem[];
   const int lane = threadIdx.x & 63, wave = uniform(int(threadIdx.x >> 6));
   const int lm = lane & 15, lg = lane >> 4;
@@ -295,201 +520,250 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
   const int grid = gridDim.x;
   const int share = grid % 8 == 0 ? (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
   touch_kernel_args(int(sizeof(Fp4Params)));
-  const int hs = wave % p.heads_per_wg, phase = wave / p.heads_per_wg;
-  const int phases = kWaves / p.heads_per_wg;
-  const int step_keys = phases * kTile;
+  const int owners = p.heads_per_wg / NH;  // waves of one phase
+  const int own = wave % owners, phase = wave / owners;
+  const int phases = kWaves / owners;
 
-  // The share's place: row, item of the row, step of the item.
-  int row = 0, item = 0, step = 0;
+  // The share's place: row, item of the row, tile of the item.
+  int row = 0, item = 0, tile = 0, keys = 0;
   int64_t pos = 0, end = 1, size = 1;
+  float size_rcp = 1.f;
   if (p.whole) {
     row = share / p.groups;
     item = share - row * p.groups;
+    keys = keys_of(p, table_entry(p.lens, row));
   } else {
-    int64_t total = 0;
-    for (int r0 = 0; r0 < p.batch; r0 += 64) {
+    // (the first 64 rows' lengths stay in the lanes: one read of them)
+    const int keys0 = lane < p.batch ? keys_of(p, p.lens[lane]) : 0;
+    const int n0 = lane < p.batch ? tiles_of(p, keys0) : 0;
+    const int incl0 = wave_scan_add(n0);
+    int64_t rows = __builtin_amdgcn_readlane(incl0, 63);
+    for (int r0 = 64; r0 < p.batch; r0 += 64) {
       const int r = r0 + lane;
-      const int n = r < p.batch ? steps_of(keys_of(p, p.lens[r]), step_keys) : 0;
-      total += int64_t(wave_sum(n)) * p.groups;
+      rows += wave_sum(r < p.batch ? tiles_of(p, keys_of(p, p.lens[r])) : 0);
     }
-    size = max(int64_t(p.min_share), (total + grid - 1) / grid);
+    const int64_t total = rows * p.groups;
+    // total / grid, rounded up with room for the estimate's error
+    size = max(int64_t(p.min_share),
+               int64_t(float(total) * p.grid_rcp * (1.f + 0x1p-21f)) + 1);
+    if ((size - 1) * grid >= total) size = max(int64_t(p.min_share), size - 1);
+    size_rcp = __builtin_amdgcn_rcpf(float(size));
     pos = share * size;
     end = min(total, pos + size);
     if (pos >= end) return;
     int64_t before = 0;
-    for (int r0 = 0; r0 < p.batch; r0 += 64) {
-      const int r = r0 + lane;
-      const int n = r < p.batch ? steps_of(keys_of(p, p.lens[r]), step_keys) : 0;
-      const int incl = wave_scan_add(n);
+    int n = n0, incl = incl0, lens = keys0;
+    for (int r0 = 0;;) {
       const int64_t all = int64_t(__builtin_amdgcn_readlane(incl, 63)) * p.groups;
       if (pos < before + all) {
         const uint64_t past =
             __builtin_amdgcn_ballot_w64(before + int64_t(incl) * p.groups > pos);
         const int at = __builtin_ctzll(past);
         row = r0 + at;
-        const int steps = __builtin_amdgcn_readlane(n, at);
+        keys = __builtin_amdgcn_readlane(lens, at);
+        const int tiles = __builtin_amdgcn_readlane(n, at);
         const int64_t in =
-            pos - before - int64_t(__builtin_amdgcn_readlane(incl, at) - steps) * p.groups;
-        item = int(in / steps);
-        step = int(in - int64_t(item) * steps);
+            pos - before - int64_t(__builtin_amdgcn_readlane(incl, at) - tiles) * p.groups;
+        item = div_steps(in, tiles, __builtin_amdgcn_rcpf(float(tiles)));
+        tile = int(in - int64_t(item) * tiles);
         break;
       }
       before += all;
+      r0 += 64;
+      const int r = r0 + lane;
+      lens = r < p.batch ? keys_of(p, p.lens[r]) : 0;
+      n = r < p.batch ? tiles_of(p, lens) : 0;
+      incl = wave_scan_add(n);
     }
   }
 
   const uint32_t lds0 = lds_addr(smem) + wave * (kSlots * kSlotBytes);
   const char* slot0 = smem + wave * (kSlots * kSlotBytes);
-  // Offsets of the lane's 16 bytes in a tile's half of 32 keys.  K's loads fill
-  // LDS in the MFMA's row order, V's in key order; four lanes read a row, its
-  // quarters turned so that the operand reads meet no bank twice.
   const int row_bytes = p.kv_heads * kFp4RowBytes;
-  int koff[2], voff[4];
-  {
-    const int r = lane >> 2;
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      koff[x] = (8 * (r >> 2) + 4 * x + (r & 3)) * row_bytes + 16 * ((lane & 3) ^ (r >> 2));
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      voff[x] = (16 * (x & 1) + r) * row_bytes +
-                16 * ((lane & 3) ^ (((lane >> 4) & 1) + 2 * (x >> 1)));
-  }
-  const int soff = (lane & 31) * p.kv_heads * kFp4Powers;
+  // (NH = 2: the other loads' offsets differ by rows, and K's by an xor)
+  const int k0 = TileLayout<NH>::load_key(0, lane, row_bytes);
+  const int k1 = TileLayout<NH>::load_key(1, lane, row_bytes);
+  const int v0 = TileLayout<NH>::load_value(0, lane, row_bytes);
+  const int v1 = TileLayout<NH>::load_value(1, lane, row_bytes);
+  // Of power lane: key lane & 31, head lane >> 5 (NH = 2).
+  const int poff = ((lane & 31) * p.kv_heads + (NH == 2 ? lane >> 5 : 0)) * kFp4Powers;
 
   while (true) {
-    const int keys = keys_of(p, table_entry(p.lens, row));
-    const int steps = steps_of(keys, step_keys);
-    const int seg0 = step;
-    const int seg1 = p.whole ? steps : int(min(int64_t(steps), step + (end - pos)));
-    const int head = (item / p.col_blocks) * p.heads_per_wg + hs;
+    const int tiles = tiles_of(p, keys);
+    const int seg0 = tile;
+    const int seg1 = p.whole ? tiles : int(min(int64_t(tiles), tile + (end - pos)));
+    const int head = (item / p.col_blocks) * p.heads_per_wg + own * NH;
     const int col0 = (item % p.col_blocks) * 16;
     if (!p.whole && seg0 == 0 && threadIdx.x == 0)
-      p.rec[int64_t(row) * p.groups + item] = int2{share, int((pos + steps - 1) / size)};
+      p.rec[int64_t(row) * p.groups + item] = int2{share, div_steps(pos + tiles - 1, size, size_rcp)};
 
-    const int col = min(col0 + lm, p.group - 1);
-    const uint16_t* qp = p.q + row * p.q_sb + int64_t(head * p.group + col) * p.q_sh + 32 * lg;
-    u32x4_t q[4];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) q[d] = *reinterpret_cast<const u32x4_t*>(qp + 8 * d);
-    Carry c;
-#pragma unroll
-    for (int cb = 0; cb < 8; ++cb) c.o[cb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    c.m = kLowest;
-    c.l = 0.f;
-
-    // Tiles of this wave: t = seg0 phases + phase, then every phases-th.
+    // Tiles of this wave: t = seg0 + phase, then every phases-th.
     const int32_t* table = p.tables + row * p.bt_stride;
-    const int t_end = min(seg1 * phases, (keys + kTile - 1) / kTile);
-    int t = seg0 * phases + phase;
-    int pages0 = -64, pages = -1;  // the lane's table entry, of page pages0 + lane
-    auto issue = [&](int tile, uint32_t lds) {
+    const int t_end = min(seg1, (keys + kKeys - 1) / kKeys);
+    int t = seg0 + phase;
+    int pages0, pages;  // the lane's table entry, of page pages0 + lane
+    // Rows of the pool from half u (32 keys) on, times kv heads, plus the head;
+    // negative: nowhere.
+    auto place_of = [&](int u) {
+      const int pg = uniform(div_small(u, p.page_halves, p.page_halves_rcp));
+      if (pg >= pages0 + 64) {
+        pages0 = pg;
+        pages = pg + lane < p.max_blocks ? table[pg + lane] : -1;
+      }
+      const int blk = __builtin_amdgcn_readlane(pages, pg - pages0);
+      const bool there = blk >= 0 && blk < p.num_blocks;
+      return there ? (int64_t(blk) * p.page + (u - pg * p.page_halves) * 32) * p.kv_heads + head
+                   : int64_t(-1);
+    };
+    constexpr int kLoads = NH == 2 ? 10 : 12;  // of a tile
+    const int code_bytes = 31 * row_bytes + NH * kFp4RowBytes;
+    const int power_bytes = (31 * p.kv_heads + NH) * kFp4Powers;
+    auto issue = [&](int tl, uint32_t lds) {
+      if constexpr (NH == 2) {
+        const int64_t w = place_of(tl);
+        const int64_t at = max(w, int64_t(0));
+        const int there = w >= 0 ? -1 : 0;
+        load_powers(scalar_rsrc(p.ks + at * kFp4Powers, power_bytes & there), poff, lds + kKpAt);
+        load_powers(scalar_rsrc(p.vs + at * kFp4Powers, power_bytes & there), poff, lds + kVpAt);
+        const i32x4_t kr = scalar_rsrc(p.k + at * kFp4RowBytes, code_bytes & there);
+        const i32x4_t vr = scalar_rsrc(p.v + at * kFp4RowBytes, code_bytes & there);
+        const int step = 8 * row_bytes;
+        load_codes(kr, k0, k0 ^ 32, 0, step, lds);
+        load_codes(vr, v0, v0, 0, step, lds + kVAt);
+        load_codes(kr, k0 ^ 64, k0 ^ 96, 2 * step, 3 * step, lds + 2048);
+        load_codes(vr, v0, v0, 2 * step, 3 * step, lds + kVAt + 2048);
+      } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int half = 2 * tile + h;
-        const int pg = uniform(div_small(half, p.page_halves, p.page_halves_rcp));
-        if (pg >= pages0 + 64) {
-          pages0 = pg;
-          pages = pg + lane < p.max_blocks ? table[pg + lane] : -1;
-        }
-        const int blk = __builtin_amdgcn_readlane(pages, pg - pages0);
-        const bool there = half * 32 < keys && blk >= 0 && blk < p.num_blocks;
-        const int64_t at = there ? (int64_t(blk) * p.page + (half - pg * p.page_halves) * 32) *
-                                           p.kv_heads + head : 0;
-        const int codes = there ? 31 * row_bytes + kFp4RowBytes : 0;
-        const int powers = there ? (31 * p.kv_heads + 1) * kFp4Powers : 0;
-        const i32x4_t kr = raw_rsrc(p.k + at * kFp4RowBytes, codes);
-        const i32x4_t vr = raw_rsrc(p.v + at * kFp4RowBytes, codes);
-        const i32x4_t ksr = raw_rsrc(p.ks + at * kFp4Powers, powers);
-        const i32x4_t vsr = raw_rsrc(p.vs + at * kFp4Powers, powers);
-        if ((lane >> 5) == h) {
-          dma_dword(ksr, soff, lds + kKsAt);
-          dma_dword(vsr, soff, lds + kVsAt);
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          dma_to_lds(kr, koff[x], lds + 1024 * (2 * h + x));
-          dma_to_lds(vr, voff[2 * h + x], lds + kVAt + 1024 * (2 * h + x));
+        for (int h = 0; h < 2; ++h) {
+          const int64_t w = (2 * tl + h) * 32 < keys ? place_of(2 * tl + h) : int64_t(-1);
+          const int64_t at = max(w, int64_t(0));
+          const int there = w >= 0 ? -1 : 0;
+          if ((lane >> 5) == h) {
+            load_powers(scalar_rsrc(p.ks + at * kFp4Powers, power_bytes & there), poff,
+                        lds + kKpAt);
+            load_powers(scalar_rsrc(p.vs + at * kFp4Powers, power_bytes & there), poff,
+                        lds + kVpAt);
+          }
+          load_codes(scalar_rsrc(p.k + at * kFp4RowBytes, code_bytes & there), k0, k1, 0, 0,
+                     lds + 2048 * h);
+          load_codes(scalar_rsrc(p.v + at * kFp4RowBytes, code_bytes & there),
+                     v0 ^ (32 * h), v1 ^ (32 * h), 0, 0, lds + kVAt + 2048 * h);
         }
       }
     };
-    int buf = 0;
-    if (t < t_end) issue(t, lds0);
-    // The queries are waited for with the first tile on its way.
+    // Queries and table entries come in together, then two tiles go on their way
+    // and the queries are split behind them.
+    const int col = min(col0 + lm, p.group - 1);
+    QueryRow qr[NH];
 #pragma unroll
-    for (int d = 0; d < 4; ++d) asm volatile("" : "+v"(q[d]));
+    for (int i = 0; i < NH; ++i)
+      qr[i] = load_query(
+          p.q + row * p.q_sb + int64_t((head + i) * p.group + col) * p.q_sh, lg);
+    pages0 = uniform(div_small(t * (kKeys / 32), p.page_halves, p.page_halves_rcp));
+    pages = pages0 + lane < p.max_blocks ? table[pages0 + lane] : -1;
+    asm volatile("" : "+v"(pages));
+#pragma unroll
+    for (int i = 0; i < NH; ++i)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) asm volatile("" : "+v"(qr[i].x[d]));
+    if (t < t_end) issue(t, lds0);
+    if (t + phases < t_end) issue(t + phases, lds0 + kSlotBytes);
+    Query q[NH];
+    Carry c[NH];
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+      q[i] = split_query(qr[i], p.flip);
+#pragma unroll
+      for (int cb = 0; cb < 8; ++cb) c[i].o[cb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      c[i].l = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      c[i].m = kLowest;
+    }
+    int slot = 0;
     for (; t < t_end; t += phases) {
-      smem_drain();  // the other slot's reads are done
       if (t + phases < t_end) {
-        issue(t + phases, lds0 + (buf ^ 1) * kSlotBytes);
         wait_loads<kLoads>();
       } else {
         wait_loads<0>();
       }
-      attend_tile(slot0 + buf * kSlotBytes, q, c, t * kTile, keys, lm, lg, p.c2);
-      buf ^= 1;
+      Tile x;
+      read_tile<NH>(x, slot0 + slot, lane, lm, lg);
+      smem_drain();
+      if (t + 2 * phases < t_end) issue(t + 2 * phases, lds0 + slot);
+      slot ^= kSlotBytes;
+      f32x4_t s[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const Query& qi = q[NH == 2 ? i >> 1 : 0];
+        s[i] = mfma_fp4(x.k[i], qi.lo, f32x4_t{0.f, 0.f, 0.f, 0.f}, x.k_power[i], qi.lo_power);
+        s[i] = mfma_fp4(x.k[i], qi.hi, s[i], x.k_power[i], qi.hi_power);
+      }
+      if (__builtin_expect(keys - t * kKeys < kKeys, 0))
+        mask_tile<NH>(x, s, keys - t * kKeys, lane, lg);
+      u32x4_t w[2];
+#pragma unroll
+      for (int i = 0; i < NH; ++i) weights<16 / NH>(s + 2 * i, c[i], p.c2, w + i);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) weigh(x, h, w[h], c[NH == 2 ? h : 0]);
+      add_nan_runs<NH>(x.mine, c);
     }
-    c.l = rows4_sum(c.l);
 
     // Channels 16 cb .. + 15 of the wave's columns: the result, or a partial in
     // slot 2 share + 1 (the piece that begins its item), else 2 share.
-    const bool done = seg0 == 0 && seg1 == steps;
-    const int64_t part = ((int64_t(2) * share + (seg0 == 0 ? 1 : 0)) * p.heads_per_wg + hs) *
-                             p.cols + lm;
-    auto emit = [&](int cb, const f32x4_t& o, float m, float l) {
-      if (col0 + lm >= p.group) return;
+    // (Arguments of the epilogue are read again here: held through the loop, they
+    // would take registers from it.)
+    const KernelArgs* e = kernel_args();
+    const bool done = seg0 == 0 && seg1 == tiles;
+    const int64_t part =
+        (int64_t(2) * share + (seg0 == 0 ? 1 : 0)) * e->heads_per_wg * e->cols + lm;
+    auto emit = [&](int i, int cb, const f32x4_t& o, float m, float l) {
       if (done) {
         const float inv = l != 0.f ? 1.f / l : 0.f;
-        uint16_t* dst = p.out + row * p.o_sb + int64_t(head * p.group + col0 + lm) * p.o_sh +
-                        16 * cb + 4 * lg;
+        uint16_t* dst = e->out + row * e->o_sb +
+                        int64_t((head + i) * e->group + col0 + lm) * e->o_sh + 16 * cb + 4 * lg;
         *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{pack_bf16x2_fast(o[0] * inv, o[1] * inv),
                                                    pack_bf16x2_fast(o[2] * inv, o[3] * inv)};
       } else {
-        *reinterpret_cast<f32x4_t*>(p.part_o + part * kD + 16 * cb + 4 * lg) = o;
-        if (cb == 0 && lg == 0) p.part_ml[part] = float2{m, l};
+        const int64_t at = part + (own * NH + i) * e->cols;
+        *reinterpret_cast<f32x4_t*>(e->part_o + at * kD + 16 * cb + 4 * lg) = o;
+        if (cb == 0 && lg == 0) e->part_ml[at] = float2{m, l};
       }
     };
-    {
-      // Phases joined through the waves' own slots: a phase makes 8 / phases of
-      // the channel blocks of its head's columns.
-      char* own = smem + wave * (kSlots * kSlotBytes);
-      smem_drain();
+    // Phases joined through the waves' own slots, a head to a slot: each wave makes
+    // its part of its heads' channel blocks.
+    char* mine = smem + wave * (kSlots * kSlotBytes);
+    smem_drain();
+    if (col0 + lm < e->group)
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
 #pragma unroll
       for (int cb = 0; cb < 8; ++cb)
-        *reinterpret_cast<f32x4_t*>(own + cb * 1024 + lane * 16) = c.o[cb];
-      *reinterpret_cast<float2*>(own + 8192 + lane * 8) = float2{c.m, c.l};
-      pf_barrier();
-      const char* first = smem + hs * (kSlots * kSlotBytes);
-      const int apart = p.heads_per_wg * (kSlots * kSlotBytes);
-      float top = kLowest, l = 0.f;
-      for (int f = 0; f < phases; ++f)
-        top = fmaxf(top, reinterpret_cast<const float2*>(first + f * apart + 8192)[lane].x);
-      const int each = 8 / phases;
-      f32x4_t o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      for (int f = 0; f < phases; ++f) {
-        const float2 ml = reinterpret_cast<const float2*>(first + f * apart + 8192)[lane];
-        const float b = __builtin_amdgcn_exp2f(ml.x - top);
-        l += ml.y * b;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < each)
-            o[i] += *reinterpret_cast<const f32x4_t*>(first + f * apart +
-                                                      (phase * each + i) * 1024 + lane * 16) * b;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < each) emit(phase * each + i, o[i], top, l);
-      pf_barrier();
+        *reinterpret_cast<f32x4_t*>(mine + i * kSlotBytes + cb * 1024 + lane * 16) = c[i].o[cb];
+      *reinterpret_cast<float2*>(mine + i * kSlotBytes + 8192 + lane * 8) =
+          float2{c[i].m, c[i].l[0]};
     }
+    pf_barrier();
+    const char* first = smem + own * (kSlots * kSlotBytes);
+    const int apart = owners * (kSlots * kSlotBytes);
+    if (col0 + lm < e->group) {
+#pragma unroll
+      for (int i = 0; i < NH; ++i) {
+        auto put = [&](int cb, const f32x4_t& o, float top, float l) { emit(i, cb, o, top, l); };
+        if (NH == 1 || phases == 8) {
+          join<8>(first + i * kSlotBytes, apart, phase, lane, put);
+        } else {
+          join<4>(first + i * kSlotBytes, apart, phase, lane, put);
+        }
+      }
+    }
+    pf_barrier();
 
     pos += seg1 - seg0;
     if (p.whole || pos >= end) break;
-    step = 0;
+    tile = 0;
     if (++item < p.groups) continue;
     item = 0;
     ++row;
+    keys = keys_of(p, table_entry(p.lens, row));
   }
 }
 
@@ -575,6 +849,7 @@ int cu_count() {
 }
 
 struct Plan {
+  int pair;  // waves take two heads
   int heads_per_wg, col_blocks, groups, cols, grid, min_share, whole;
   size_t rec_at, ml_at, o_at, bytes;
 };
@@ -587,12 +862,10 @@ Plan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t most_keys
   pl.col_blocks = int((group + 15) / 16);
   pl.cols = int(std::min<int64_t>(group, 16));
   const int cus = cu_count();
-  const int64_t tiles = (most_keys + kTile - 1) / kTile;
   // Waves of a workgroup over kv heads, the rest over tile phases.
-  int hpw = 4;
-  while (hpw > 1 && kv_heads % hpw != 0) hpw >>= 1;
-  pl.whole = tiles <= 16;
-  if (pl.whole) hpw = 1;
+  pl.whole = most_keys <= 1024;
+  pl.pair = kv_heads % 2 == 0 && !pl.whole;
+  const int hpw = pl.pair ? (kv_heads % 4 == 0 ? 4 : 2) : 1;
   pl.heads_per_wg = hpw;
   pl.groups = int(kv_heads / hpw * pl.col_blocks);
   pl.min_share = 1;
@@ -797,11 +1070,15 @@ extern "C" int kvc_paged_decode_fp4(
   p.group = int(num_heads / num_kv_heads);
   p.col_blocks = pl.col_blocks;
   p.heads_per_wg = pl.heads_per_wg;
+  p.tile_shift = pl.pair ? 5 : 6;
+  p.grid_rcp = 1.f / float(pl.grid);
   p.groups = pl.groups;
   p.cols = pl.cols;
   p.min_share = pl.min_share;
   p.whole = pl.whole;
-  p.c2 = scale * kLog2e;
+  // (a scale of 0 stays above it: masked scores are -infinity)
+  p.c2 = std::max(std::abs(scale) * kLog2e, 1e-37f);
+  p.flip = scale < 0.f ? 0x80008000u : 0u;
   char* ws = static_cast<char*>(workspace);
   p.rec = reinterpret_cast<int2*>(ws + pl.rec_at);
   p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_at);
@@ -813,13 +1090,15 @@ extern "C" int kvc_paged_decode_fp4(
   hipError_t e = hipGetDevice(&dev);
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (e == hipSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&fp4_decode_kernel),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    for (auto kern : {fp4_decode_kernel<1>, fp4_decode_kernel<2>})
+      if (e == hipSuccess)
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e == hipSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
   }
   KVC_REQUIRE(e == hipSuccess, KVC_ERR_RUNTIME, "paged_decode_fp4: LDS limit: %s",
               hipGetErrorString(e));
-  fp4_decode_kernel<<<pl.grid, 64 * kWaves, kLds, st>>>(p);
+  (pl.pair ? fp4_decode_kernel<2> : fp4_decode_kernel<1>)<<<pl.grid, 64 * kWaves, kLds, st>>>(p);
   if (!pl.whole)
     fp4_merge_kernel<<<dim3(unsigned(items), unsigned(pl.heads_per_wg * pl.cols)), 32 * kSlices, 0,
                        st>>>(p);
