@@ -142,52 +142,97 @@ constexpr float kSlack = 2.f;
 constexpr int kStateBytes = 8 * 64 * 16 + 64 * 8;  // a wave's O and (reference, sum)
 static_assert(kStateBytes <= kSlotBytes);  // (one a head, a slot each)
 
+// An item: a block of up to 16 columns (query token x head) of one kv head group
+// and sequence.  What the merge needs of it.
+struct ItemRec {
+  int first, last;  // shares
+  int q0, sq;       // the sequence's query rows
+  int group, block;
+  int unused[2];
+};
+
 struct Fp4Params {
   const uint16_t* q;
-  int64_t q_sb, q_sh;
+  int64_t q_st, q_sh;
   uint16_t* out;
-  int64_t o_sb, o_sh;
+  int64_t o_st, o_sh;
   const uint8_t* k;
   const uint8_t* v;
   const uint8_t* ks;
   const uint8_t* vs;
   const int32_t* tables;
   int64_t bt_stride;
-  const int32_t* lens;
+  const int32_t* lens;     // of the decode rows
+  const int32_t* cu_q;     // of the chunks
+  const int32_t* cu_k;
+  int decode_rows, chunks, chunk_tokens;
   int max_blocks, num_blocks, page;
   int page_halves;         // page / 32
   float page_halves_rcp;
-  int batch, kv_heads, group;
-  int col_blocks;          // of 16 query heads, of a kv head's
+  int kv_heads, group;
+  float group_rcp;
   int heads_per_wg;        // kv heads of a workgroup
+  int head_groups;         // kv_heads / heads_per_wg
   int tile_shift;          // log2 of the keys of a wave's tile
-  int groups;              // workgroup items of a row: kv head groups x col_blocks
-  int cols;                // columns kept of a partial: min(16, group)
+  int cols;                // columns kept of a partial: min(16, columns there can be)
   int min_share;
+  int item_cost;           // of an item's setup, in tiles
   float grid_rcp;
   int whole;               // one workgroup an item, no partials
+  int row_blocks;          // blocks of a decode row
   float c2;                // |scale| log2(e)
   uint32_t flip;           // sign bits of a bf16 pair where scale is negative
-  int2* rec;               // of each item: first and last share
+  int* count;              // items
+  ItemRec* rec;            // of each item
   float* part_o;
   float2* part_ml;
 };
 
-// Keys of row b that the tables can hold; tiles of a row, 1 for a row without
-// keys: it writes zeros.
-__device__ __forceinline__ int keys_of(const Fp4Params& p, int len) {
-  const int64_t most = int64_t(p.max_blocks) * p.page;
-  return int(min(int64_t(max(len, 0)), most));
+// A sequence: a decode row or a chunk.  Query t sees the keys j < given - sq + t + 1;
+// keys counts those that its table can hold.
+struct SeqGeo {
+  int q0, sq, given, keys;
+};
+constexpr int kLongest = 1 << 29;  // of a length (tables hold fewer keys)
+__device__ __forceinline__ SeqGeo seq_geo(const Fp4Params& p, int q0, int q1, int64_t len) {
+  SeqGeo g;
+  g.q0 = q0;
+  g.sq = max(0, q1 - q0);
+  g.given = int(max(int64_t(0), min(len, int64_t(kLongest))));
+  g.keys = min(g.given, p.max_blocks * p.page);
+  return g;
 }
-__device__ __forceinline__ int tiles_of(const Fp4Params& p, int keys) {
-  return max(1, (keys + (1 << p.tile_shift) - 1) >> p.tile_shift);
+__device__ __forceinline__ SeqGeo load_row(const Fp4Params& p, int i) {  // a decode row
+  return i < p.decode_rows ? seq_geo(p, i, i + 1, p.lens[i]) : SeqGeo{0, 0, 0, 0};
+}
+template <bool kUniform>
+__device__ __forceinline__ SeqGeo load_seq(const Fp4Params& p, int i) {
+  auto at = [&](const int32_t* t, int64_t idx) {
+    if constexpr (kUniform) return table_entry(t, idx);
+    return t[idx];
+  };
+  if (i < p.decode_rows) return seq_geo(p, i, i + 1, at(p.lens, i));
+  const int c = i - p.decode_rows;
+  const int q0 = max(0, min(at(p.cu_q, c), p.chunk_tokens));
+  const int q1 = max(0, min(at(p.cu_q, c + 1), p.chunk_tokens));
+  return seq_geo(p, p.decode_rows + q0, p.decode_rows + q1,
+                 int64_t(at(p.cu_k, c + 1)) - at(p.cu_k, c));
+}
+// Its blocks, and the tiles of each: 1 at least, which writes the zeros of rows
+// without keys.
+__device__ __forceinline__ int blocks_of(const Fp4Params& p, const SeqGeo& g) {
+  return int((int64_t(g.sq) * p.group + 15) >> 4);
+}
+__device__ __forceinline__ int tiles_of(const Fp4Params& p, const SeqGeo& g) {
+  return p.whole ? 1 : max(1, (g.keys + (1 << p.tile_shift) - 1) >> p.tile_shift);
 }
 
-// floor(x / d), given rcp, 1 / d to within a few ulp, for quotients below 2^20.
-__device__ __forceinline__ int div_steps(int64_t x, int64_t d, float rcp) {
+// floor(x / d) for 0 <= x < 2^31 and quotients below 2^20, given rcp, 1 / d to
+// within a few ulp.
+__device__ __forceinline__ int div_steps(int x, int d, float rcp) {
   int q = int(float(x) * rcp);
-  q += int64_t(q + 1) * d <= x ? 1 : 0;
   q -= int64_t(q) * d > x ? 1 : 0;
+  q += x - q * d >= d ? 1 : 0;
   return uniform(q);
 }
 
@@ -352,10 +397,10 @@ __device__ __forceinline__ void read_tile(Tile& t, const char* at, int lane, int
   t.mine = *reinterpret_cast<const uint32_t*>(at + kVpAt + 4 * lane);
 }
 
-// The keys of a tile past its row's `left`: scores -infinity, no power (what lies
-// there may hold anything).
+// The keys of a tile that the lane's column, which sees `left` of them, does not:
+// scores -infinity, no power (what lies behind a sequence may hold anything).
 template <int NH>
-__device__ __forceinline__ void mask_tile(Tile& t, f32x4_t (&s)[4], int left, int lane, int lg) {
+__device__ __forceinline__ void mask_tile(Tile& t, f32x4_t (&s)[4], int left, int lg) {
   int first = 8 * lg;  // (opaque: nothing of this is worked out for every tile)
   asm volatile("" : "+v"(first));
 #pragma unroll
@@ -367,7 +412,6 @@ __device__ __forceinline__ void mask_tile(Tile& t, f32x4_t (&s)[4], int left, in
       const uint32_t word = t.v_power[h][j >> 2][j & 3];
       t.v_power[h][j >> 2][j & 3] = seen ? word : 0u;
     }
-  if ((NH == 1 ? lane : lane & 31) >= left) t.mine = 0;
 }
 
 // The weights of N scores of a column (bf16 pairs), the reference and the sum.
@@ -426,22 +470,26 @@ __device__ __forceinline__ void weigh(const Tile& t, int h, const u32x4_t& w, Ca
   }
 }
 
-// A run that is NaN makes its channels NaN whatever its key weighs.
+// A run that is NaN makes its channels NaN whatever its key weighs, for the columns
+// that see it.
 template <int NH>
-__device__ __forceinline__ void add_nan_runs(uint32_t mine, Carry (&c)[NH]) {
+__device__ __forceinline__ void add_nan_runs(uint32_t mine, int left, Carry (&c)[NH]) {
   const uint32_t inv = ~mine;  // a byte of 0 where the power is 255
   if (__builtin_expect(
           __builtin_amdgcn_ballot_w64(((inv - 0x01010101u) & ~inv & 0x80808080u) != 0) == 0, 1))
     return;
+  constexpr int kKeys = kTileRows / NH;
+  const uint64_t seen = left >= kKeys ? ~uint64_t(0) >> (64 - kKeys)
+                                      : (uint64_t(1) << max(left, 0)) - 1;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const uint64_t at = __builtin_amdgcn_ballot_w64(((mine >> (8 * g)) & 255u) == 255u);
 #pragma unroll
-    for (int i = 0; i < NH; ++i)
-      if ((NH == 1 ? at : at >> (32 * i) & 0xffffffffu) != 0)
+    for (int i = 0; i < NH; ++i) {
+      const float add = (at >> (NH == 1 ? 0 : 32 * i) & seen) != 0 ? __uint_as_float(0x7fc00000u) : 0.f;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          c[i].o[2 * g + x] = f32x4_t{0.f, 0.f, 0.f, 0.f} + __uint_as_float(0x7fc00000u);
+      for (int x = 0; x < 2; ++x) c[i].o[2 * g + x] += add;
+    }
   }
 }
 
@@ -510,7 +558,7 @@ __device__ __forceinline__ void join(const char* at, int apart, int f, int lane,
   }
 }
 
-template <int NH>
+template <int NH, bool kChunks>
 __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p) {
   constexpr int kKeys = kTileRows / NH;  // of a tile
   extern __shared__ __align__(1024) char smem[];
@@ -523,58 +571,131 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
   const int owners = p.heads_per_wg / NH;  // waves of one phase
   const int own = wave % owners, phase = wave / owners;
   const int phases = kWaves / owners;
+  const int seqs = kChunks ? p.decode_rows + p.chunks : p.decode_rows;
 
-  // The share's place: row, item of the row, tile of the item.
-  int row = 0, item = 0, tile = 0, keys = 0;
-  int64_t pos = 0, end = 1, size = 1;
+  // The share's place: sequence, head group, block, and tiles into the block, whose
+  // setup counts `cost` of them; and the number of the item.  (A cold launch pays for
+  // every line of code it runs through: decode rows have a path of their own.)
+  int seq = 0, grp = 0, blk = 0, item = 0, off = 0, cost = 0;
+  int pos = 0, end = 1, size = 1;
   float size_rcp = 1.f;
-  if (p.whole) {
-    row = share / p.groups;
-    item = share - row * p.groups;
-    keys = keys_of(p, table_entry(p.lens, row));
-  } else {
-    // (the first 64 rows' lengths stay in the lanes: one read of them)
-    const int keys0 = lane < p.batch ? keys_of(p, p.lens[lane]) : 0;
-    const int n0 = lane < p.batch ? tiles_of(p, keys0) : 0;
-    const int incl0 = wave_scan_add(n0);
-    int64_t rows = __builtin_amdgcn_readlane(incl0, 63);
-    for (int r0 = 64; r0 < p.batch; r0 += 64) {
-      const int r = r0 + lane;
-      rows += wave_sum(r < p.batch ? tiles_of(p, keys_of(p, p.lens[r])) : 0);
-    }
-    const int64_t total = rows * p.groups;
-    // total / grid, rounded up with room for the estimate's error
-    size = max(int64_t(p.min_share),
-               int64_t(float(total) * p.grid_rcp * (1.f + 0x1p-21f)) + 1);
-    if ((size - 1) * grid >= total) size = max(int64_t(p.min_share), size - 1);
+  SeqGeo g;
+  // total units over the grid, rounded up with room for the estimate's error
+  auto cut = [&](int total) {
+    size = int(float(total) * p.grid_rcp * (1.f + 0x1p-21f)) + 1;
+    size -= int64_t(size - 1) * grid >= total ? 1 : 0;
+    size = max(p.min_share, size);
     size_rcp = __builtin_amdgcn_rcpf(float(size));
-    pos = share * size;
-    end = min(total, pos + size);
-    if (pos >= end) return;
-    int64_t before = 0;
-    int n = n0, incl = incl0, lens = keys0;
-    for (int r0 = 0;;) {
-      const int64_t all = int64_t(__builtin_amdgcn_readlane(incl, 63)) * p.groups;
-      if (pos < before + all) {
-        const uint64_t past =
-            __builtin_amdgcn_ballot_w64(before + int64_t(incl) * p.groups > pos);
-        const int at = __builtin_ctzll(past);
-        row = r0 + at;
-        keys = __builtin_amdgcn_readlane(lens, at);
-        const int tiles = __builtin_amdgcn_readlane(n, at);
-        const int64_t in =
-            pos - before - int64_t(__builtin_amdgcn_readlane(incl, at) - tiles) * p.groups;
-        item = div_steps(in, tiles, __builtin_amdgcn_rcpf(float(tiles)));
-        tile = int(in - int64_t(item) * tiles);
-        break;
+    const int64_t at = int64_t(share) * size;
+    pos = int(min(at, int64_t(total)));
+    end = int(min(at + size, int64_t(total)));
+  };
+  if (!kChunks && p.whole) {
+    const int per_row = p.head_groups * p.row_blocks;
+    seq = share / per_row;
+    grp = (share - seq * per_row) / p.row_blocks;
+    blk = share - seq * per_row - grp * p.row_blocks;
+    g = load_seq<true>(p, seq);
+  } else if (!kChunks) {
+    const int per_row = p.head_groups * p.row_blocks, rows = p.decode_rows;
+    // (the first 64 rows' sizes stay in the lanes: one read of them)
+    SeqGeo gl = load_row(p, lane);
+    int tiles = lane < rows ? tiles_of(p, gl) : 0;
+    int incl = wave_scan_add(tiles);
+    int sum = __builtin_amdgcn_readlane(incl, 63);
+    cost = p.item_cost;
+    if (__builtin_expect(rows > 64, 0)) {
+      for (int r0 = 64; r0 < rows; r0 += 64) {
+        const int r = r0 + lane;
+        sum += wave_sum(r < rows ? tiles_of(p, load_row(p, r)) : 0);
       }
-      before += all;
-      r0 += 64;
-      const int r = r0 + lane;
-      lens = r < p.batch ? keys_of(p, p.lens[r]) : 0;
-      n = r < p.batch ? tiles_of(p, lens) : 0;
-      incl = wave_scan_add(n);
+    } else {
+      // Items of one length that the shares cut without remainder begin where
+      // shares do: no share has more than one, and the setup is everybody's.
+      const int one = __builtin_amdgcn_readfirstlane(tiles);
+      cut(sum * per_row);
+      if (__builtin_amdgcn_ballot_w64(lane < rows && tiles != one) == 0 &&
+          div_steps(one, size, size_rcp) * size == one)
+        cost = 0;
     }
+    cut((sum + cost * rows) * per_row);
+    if (share == 0 && threadIdx.x == 0) *p.count = rows * per_row;
+    if (pos >= end) return;
+    int before = 0;  // units of the rows ahead of r0
+    int r0 = 0;
+    uint64_t past;
+    while ((past = __builtin_amdgcn_ballot_w64(
+                before + (incl + cost * (lane + 1)) * per_row > pos && r0 + lane < rows)) == 0) {
+      before += (__builtin_amdgcn_readlane(incl, 63) + cost * 64) * per_row;
+      r0 += 64;
+      gl = load_row(p, r0 + lane);
+      tiles = r0 + lane < rows ? tiles_of(p, gl) : 0;
+      incl = wave_scan_add(tiles);
+    }
+    const int at = __builtin_ctzll(past);
+    const int each = __builtin_amdgcn_readlane(tiles, at) + cost;
+    const int in =
+        pos - before - (__builtin_amdgcn_readlane(incl, at) - each + cost * (at + 1)) * per_row;
+    const int nth = div_steps(in, each, __builtin_amdgcn_rcpf(float(each)));
+    off = in - nth * each;
+    seq = r0 + at;
+    item = seq * per_row + nth;
+    grp = p.row_blocks == 1 ? nth : nth / p.row_blocks;
+    blk = nth - grp * p.row_blocks;
+    g = SeqGeo{seq, 1, __builtin_amdgcn_readlane(gl.given, at),
+               __builtin_amdgcn_readlane(gl.keys, at)};
+  } else {
+    cost = p.whole ? 0 : p.item_cost;
+    auto load_lane = [&](int r0, SeqGeo& gl, int& blocks, int& units) {
+      gl = SeqGeo{0, 0, 0, 0};
+      if (r0 + lane < seqs) gl = load_seq<false>(p, r0 + lane);
+      blocks = blocks_of(p, gl);
+      units = blocks * (tiles_of(p, gl) + cost);
+    };
+    SeqGeo gl;
+    int blocks, units;
+    load_lane(0, gl, blocks, units);
+    int incl = wave_scan_add(units), incl_blocks = wave_scan_add(blocks);
+    int sum = __builtin_amdgcn_readlane(incl, 63);
+    int all_blocks = __builtin_amdgcn_readlane(incl_blocks, 63);
+    for (int r0 = 64; r0 < seqs; r0 += 64) {
+      SeqGeo other;
+      int b, u;
+      load_lane(r0, other, b, u);
+      sum += wave_sum(u);
+      all_blocks += wave_sum(b);
+    }
+    if (p.whole) {
+      pos = min(share, sum * p.head_groups);
+      end = min(share + 1, sum * p.head_groups);
+    } else {
+      if (share == 0 && threadIdx.x == 0) *p.count = all_blocks * p.head_groups;
+      cut(sum * p.head_groups);
+    }
+    if (pos >= end) return;
+    int before = 0, items = 0, r0 = 0;
+    uint64_t past;
+    while ((past = __builtin_amdgcn_ballot_w64(before + incl * p.head_groups > pos)) == 0) {
+      before += __builtin_amdgcn_readlane(incl, 63) * p.head_groups;
+      items += __builtin_amdgcn_readlane(incl_blocks, 63);
+      r0 += 64;
+      load_lane(r0, gl, blocks, units);
+      incl = wave_scan_add(units);
+      incl_blocks = wave_scan_add(blocks);
+    }
+    const int at = __builtin_ctzll(past);
+    seq = r0 + at;
+    g = SeqGeo{__builtin_amdgcn_readlane(gl.q0, at), __builtin_amdgcn_readlane(gl.sq, at),
+               __builtin_amdgcn_readlane(gl.given, at), __builtin_amdgcn_readlane(gl.keys, at)};
+    const int u = __builtin_amdgcn_readlane(units, at);
+    const int nb = __builtin_amdgcn_readlane(blocks, at);
+    const int each = tiles_of(p, g) + cost;
+    const int in = pos - before - (__builtin_amdgcn_readlane(incl, at) - u) * p.head_groups;
+    grp = div_steps(in, u, __builtin_amdgcn_rcpf(float(u)));
+    blk = div_steps(in - grp * u, each, __builtin_amdgcn_rcpf(float(each)));
+    off = in - grp * u - blk * each;
+    item = (items + __builtin_amdgcn_readlane(incl_blocks, at) - nb) * p.head_groups + grp * nb +
+           blk;
   }
 
   const uint32_t lds0 = lds_addr(smem) + wave * (kSlots * kSlotBytes);
@@ -589,17 +710,29 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
   const int poff = ((lane & 31) * p.kv_heads + (NH == 2 ? lane >> 5 : 0)) * kFp4Powers;
 
   while (true) {
-    const int tiles = tiles_of(p, keys);
-    const int seg0 = tile;
-    const int seg1 = p.whole ? tiles : int(min(int64_t(tiles), tile + (end - pos)));
-    const int head = (item / p.col_blocks) * p.heads_per_wg + own * NH;
-    const int col0 = (item % p.col_blocks) * 16;
+    const int tiles = p.whole ? 1 << 30 : tiles_of(p, g);
+    const int seg0 = max(0, off - cost);
+    const int seg1 = p.whole ? tiles : min(tiles, off - cost + (end - pos));
+    if (seg1 <= seg0) break;  // (the share ends within the setup)
+    const int head = grp * p.heads_per_wg + own * NH;
     if (!p.whole && seg0 == 0 && threadIdx.x == 0)
-      p.rec[int64_t(row) * p.groups + item] = int2{share, div_steps(pos + tiles - 1, size, size_rcp)};
+      p.rec[item] = ItemRec{share, div_steps(pos - off + cost + tiles - 1, size, size_rcp), g.q0, g.sq, grp,
+                            blk, {0, 0}};
 
+    // The lane's column: its query row, head and how many keys it sees; the most
+    // and the fewest that a column of the block sees.
+    const int col0 = blk * 16, last_col = g.sq * p.group - 1;
+    const int col = min(col0 + lm, last_col);
+    const int token = div_small(col, p.group, p.group_rcp);
+    const int limit = min(g.keys, g.given - g.sq + token + 1);
+    const int most = uniform(
+        min(g.keys, g.given - g.sq + 1 +
+                        div_small(min(col0 + 15, last_col), p.group, p.group_rcp)));
+    const int least =
+        uniform(min(g.keys, g.given - g.sq + 1 + div_small(col0, p.group, p.group_rcp)));
     // Tiles of this wave: t = seg0 + phase, then every phases-th.
-    const int32_t* table = p.tables + row * p.bt_stride;
-    const int t_end = min(seg1, (keys + kKeys - 1) / kKeys);
+    const int32_t* table = p.tables + seq * p.bt_stride;
+    const int t_end = min(seg1, (max(most, 0) + kKeys - 1) / kKeys);
     int t = seg0 + phase;
     int pages0, pages;  // the lane's table entry, of page pages0 + lane
     // Rows of the pool from half u (32 keys) on, times kv heads, plus the head;
@@ -635,7 +768,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int64_t w = (2 * tl + h) * 32 < keys ? place_of(2 * tl + h) : int64_t(-1);
+          const int64_t w = (2 * tl + h) * 32 < g.keys ? place_of(2 * tl + h) : int64_t(-1);
           const int64_t at = max(w, int64_t(0));
           const int there = w >= 0 ? -1 : 0;
           if ((lane >> 5) == h) {
@@ -653,12 +786,12 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     };
     // Queries and table entries come in together, then two tiles go on their way
     // and the queries are split behind them.
-    const int col = min(col0 + lm, p.group - 1);
     QueryRow qr[NH];
 #pragma unroll
     for (int i = 0; i < NH; ++i)
-      qr[i] = load_query(
-          p.q + row * p.q_sb + int64_t((head + i) * p.group + col) * p.q_sh, lg);
+      qr[i] = load_query(p.q + int64_t(g.q0 + token) * p.q_st +
+                             int64_t((head + i) * p.group + col - token * p.group) * p.q_sh,
+                         lg);
     pages0 = uniform(div_small(t * (kKeys / 32), p.page_halves, p.page_halves_rcp));
     pages = pages0 + lane < p.max_blocks ? table[pages0 + lane] : -1;
     asm volatile("" : "+v"(pages));
@@ -697,14 +830,14 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
         s[i] = mfma_fp4(x.k[i], qi.lo, f32x4_t{0.f, 0.f, 0.f, 0.f}, x.k_power[i], qi.lo_power);
         s[i] = mfma_fp4(x.k[i], qi.hi, s[i], x.k_power[i], qi.hi_power);
       }
-      if (__builtin_expect(keys - t * kKeys < kKeys, 0))
-        mask_tile<NH>(x, s, keys - t * kKeys, lane, lg);
+      if (__builtin_expect(least < (t + 1) * kKeys, 0))
+        mask_tile<NH>(x, s, limit - t * kKeys, lg);
       u32x4_t w[2];
 #pragma unroll
       for (int i = 0; i < NH; ++i) weights<16 / NH>(s + 2 * i, c[i], p.c2, w + i);
 #pragma unroll
       for (int h = 0; h < 2; ++h) weigh(x, h, w[h], c[NH == 2 ? h : 0]);
-      add_nan_runs<NH>(x.mine, c);
+      add_nan_runs<NH>(x.mine, limit - t * kKeys, c);
     }
 
     // Channels 16 cb .. + 15 of the wave's columns: the result, or a partial in
@@ -713,13 +846,15 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     // would take registers from it.)
     const KernelArgs* e = kernel_args();
     const bool done = seg0 == 0 && seg1 == tiles;
+    const bool mine_too = col0 + lm <= last_col;  // (else the last column again)
     const int64_t part =
         (int64_t(2) * share + (seg0 == 0 ? 1 : 0)) * e->heads_per_wg * e->cols + lm;
     auto emit = [&](int i, int cb, const f32x4_t& o, float m, float l) {
       if (done) {
         const float inv = l != 0.f ? 1.f / l : 0.f;
-        uint16_t* dst = e->out + row * e->o_sb +
-                        int64_t((head + i) * e->group + col0 + lm) * e->o_sh + 16 * cb + 4 * lg;
+        uint16_t* dst = e->out + int64_t(g.q0 + token) * e->o_st +
+                        int64_t((head + i) * e->group + col - token * e->group) * e->o_sh +
+                        16 * cb + 4 * lg;
         *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{pack_bf16x2_fast(o[0] * inv, o[1] * inv),
                                                    pack_bf16x2_fast(o[2] * inv, o[3] * inv)};
       } else {
@@ -732,7 +867,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     // its part of its heads' channel blocks.
     char* mine = smem + wave * (kSlots * kSlotBytes);
     smem_drain();
-    if (col0 + lm < e->group)
+    if (mine_too)
 #pragma unroll
     for (int i = 0; i < NH; ++i) {
 #pragma unroll
@@ -744,7 +879,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     pf_barrier();
     const char* first = smem + own * (kSlots * kSlotBytes);
     const int apart = owners * (kSlots * kSlotBytes);
-    if (col0 + lm < e->group) {
+    if (mine_too) {
 #pragma unroll
       for (int i = 0; i < NH; ++i) {
         auto put = [&](int cb, const f32x4_t& o, float top, float l) { emit(i, cb, o, top, l); };
@@ -757,50 +892,61 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     }
     pf_barrier();
 
-    pos += seg1 - seg0;
-    if (p.whole || pos >= end) break;
-    tile = 0;
-    if (++item < p.groups) continue;
-    item = 0;
-    ++row;
-    keys = keys_of(p, table_entry(p.lens, row));
+    if (p.whole) break;
+    pos += cost + tiles - off;
+    if (pos >= end) break;
+    off = 0;
+    ++item;
+    if (++blk < blocks_of(p, g)) continue;
+    blk = 0;
+    if (++grp < p.head_groups) continue;
+    grp = 0;
+    do {  // (pos < end: there is one)
+      g = load_seq<true>(p, ++seq);
+    } while (kChunks && g.sq == 0);
   }
 }
 
 // ---------------------------------------------------------------------------
-// Join the partials of items cut between shares: a workgroup per item and
-// column, eight slices of 32 lanes over its pieces.
+// Join the partials of items cut between shares: 32 lanes a column and slice of its
+// pieces, kGroups of them a workgroup, which takes kGroups / S columns of an item in S
+// slices each (by how many pieces an item has: 1 item in 256 pieces 4.6 us, 64 items
+// in 5 pieces each 4).
 // ---------------------------------------------------------------------------
-constexpr int kSlices = 8;
-constexpr int kAhead = 4;  // pieces of a slice whose loads are in flight together
-__global__ void __launch_bounds__(32 * kSlices) fp4_merge_kernel(Fp4Params p) {
-  __shared__ f32x4_t so[kSlices][32];
-  __shared__ float2 sml[kSlices];
-  const int item = blockIdx.x;
-  const int2 r = p.rec[item];
+constexpr int kGroups = 16;
+constexpr int kAhead = 8;  // pieces of a slice whose loads are in flight together
+template <int S>
+__global__ void __launch_bounds__(32 * kGroups) fp4_merge_kernel(Fp4Params p) {
+  __shared__ f32x4_t so[kGroups][32];
+  __shared__ float2 sml[kGroups];
+  if (int(blockIdx.x) >= *p.count) return;
+  const ItemRec rec = p.rec[blockIdx.x];
+  const int2 r = {rec.first, rec.last};
   if (r.x >= r.y) return;
-  const int row = item / p.groups, in = item - row * p.groups;
-  const int hs = blockIdx.y / p.cols, col = blockIdx.y - hs * p.cols;
-  const int head = (in / p.col_blocks) * p.heads_per_wg + hs;
-  const int qh = (in % p.col_blocks) * 16 + col;
-  if (qh >= p.group) return;
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int64_t at = int64_t(hs) * p.cols + col, cols = int64_t(p.heads_per_wg) * p.cols;
+  const int lane = threadIdx.x & 31, at_group = threadIdx.x >> 5, slice = at_group % S;
+  // The workgroup's at_group / S-th column: of a head of the item's, one of its block's.
+  const int nth = blockIdx.y * (kGroups / S) + at_group / S;
+  const int hs = nth / p.cols, in = nth - hs * p.cols;
+  const int col = rec.block * 16 + in;
+  const bool live = hs < p.heads_per_wg && col < rec.sq * p.group;
+  const int token = div_small(col, p.group, p.group_rcp);
+  const int head = (rec.group * p.heads_per_wg + hs) * p.group + col - token * p.group;
+  const int64_t cols = int64_t(p.heads_per_wg) * p.cols;
   float top = kLowest, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = r.x + slice; s0 <= r.y; s0 += kSlices * kAhead) {
+  for (int s0 = live ? r.x + slice : r.y + 1; s0 <= r.y; s0 += S * kAhead) {
     float2 ml[kAhead];
     f32x4_t part[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int s = min(s0 + kSlices * i, r.y);
-      const int64_t c = (int64_t(2) * s + (s == r.x)) * cols + at;
+      const int s = min(s0 + S * i, r.y);
+      const int64_t c = (int64_t(2) * s + (s == r.x)) * cols + nth;
       ml[i] = p.part_ml[c];
       part[i] = reinterpret_cast<const f32x4_t*>(p.part_o + c * kD)[lane];
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (s0 + kSlices * i > r.y) continue;
+      if (s0 + S * i > r.y) continue;
       const float next = fmaxf(top, ml[i].x);
       const float a = __builtin_amdgcn_exp2f(top - next);
       const float b = __builtin_amdgcn_exp2f(ml[i].x - next);
@@ -809,22 +955,25 @@ __global__ void __launch_bounds__(32 * kSlices) fp4_merge_kernel(Fp4Params p) {
       o = o * a + part[i] * b;
     }
   }
-  so[slice][lane] = o;
-  if (lane == 0) sml[slice] = float2{top, l};
-  __syncthreads();
-  if (slice != 0) return;
+  if constexpr (S > 1) {
+    so[at_group][lane] = o;
+    if (lane == 0) sml[at_group] = float2{top, l};
+    __syncthreads();
+    if (slice != 0) return;
 #pragma unroll
-  for (int i = 1; i < kSlices; ++i) top = fmaxf(top, sml[i].x);
-  l = 0.f;
-  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 1; i < S; ++i) top = fmaxf(top, sml[at_group + i].x);
+    l = 0.f;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < kSlices; ++i) {
-    const float b = __builtin_amdgcn_exp2f(sml[i].x - top);
-    l += sml[i].y * b;
-    o += so[i][lane] * b;
+    for (int i = 0; i < S; ++i) {
+      const float b = __builtin_amdgcn_exp2f(sml[at_group + i].x - top);
+      l += sml[at_group + i].y * b;
+      o += so[at_group + i][lane] * b;
+    }
   }
+  if (!live) return;
   const float inv = l != 0.f ? 1.f / l : 0.f;
-  uint16_t* dst = p.out + row * p.o_sb + int64_t(head * p.group + qh) * p.o_sh + 4 * lane;
+  uint16_t* dst = p.out + int64_t(rec.q0 + token) * p.o_st + head * p.o_sh + 4 * lane;
   *reinterpret_cast<u32x2_t*>(dst) =
       u32x2_t{pack_bf16x2_fast(o[0] * inv, o[1] * inv), pack_bf16x2_fast(o[2] * inv, o[3] * inv)};
 }
@@ -850,33 +999,63 @@ int cu_count() {
 
 struct Plan {
   int pair;  // waves take two heads
-  int heads_per_wg, col_blocks, groups, cols, grid, min_share, whole;
+  int heads_per_wg, head_groups, cols, grid, min_share, item_cost, whole;
+  int64_t items;  // at most
   size_t rec_at, ml_at, o_at, bytes;
 };
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-Plan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t most_keys) {
+// Three ways to cut the work.  Whole: a workgroup takes an item alone, eight tiles at a
+// time, of one head (64 keys each) or of two (32), and there is one launch.  Cut: two
+// heads a wave, the tiles of all items in equal shares, one a CU, and a second launch
+// joins the pieces.  Estimates in us, from decode batches of 1 to 128 rows and chunks
+// of 4 to 256 tokens over 300 to 32768 keys (kv heads 2, 4, 8):
+//   whole  the longer of ceil(items / CUs) (6 + 2.6 a round of 8 tiles) and 7 + the
+//          keys' bytes at 4.6 TB/s (one head: half lines) or 5.6 (two)
+//   cut    12, 6 more as the items get to 128 (more of them in a share), and the
+//          longer of the keys' bytes at 6.6 TB/s and 1.1 ns for every 64 keys of a
+//          head and block
+// Measured, cut / whole / whole by two heads (4 kv heads; rows x keys): 1 x 333 11.6 /
+// 7.6 / 10.5, 1 x 4096 13.2 / 27.8 / 38.4, 64 x 2048 26.9 / 22.0 / 25.1, 64 x 4096 39.7
+// / 36.3 / 40.0, 128 x 500 to 1500 29.9 / 30.6 / 22.8, 48 x 1025 to 8007 36.5 / 50.8 /
+// 66.5, 128 x 4096 62.7 / 70.5 / 54.3, 16 x 32768 62 / 182 / 246.
+Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t heads,
+               int64_t kv_heads, int64_t most_keys) {
   Plan pl{};
   const int64_t group = heads / kv_heads;
-  pl.col_blocks = int((group + 15) / 16);
-  pl.cols = int(std::min<int64_t>(group, 16));
   const int cus = cu_count();
-  // Waves of a workgroup over kv heads, the rest over tile phases.
-  pl.whole = most_keys <= 1024;
-  pl.pair = kv_heads % 2 == 0 && !pl.whole;
-  const int hpw = pl.pair ? (kv_heads % 4 == 0 ? 4 : 2) : 1;
-  pl.heads_per_wg = hpw;
-  pl.groups = int(kv_heads / hpw * pl.col_blocks);
-  pl.min_share = 1;
-  const int64_t items = batch * pl.groups;
-  pl.grid = int(pl.whole ? items : cus);
+  pl.cols = int(chunks > 0 ? 16 : std::min<int64_t>(group, 16));
+  const int64_t blocks =
+      decode_rows * ((group + 15) / 16) + chunk_tokens * group / 16 + chunks;
+  const double heads_of = double(blocks) * double(kv_heads), keys = double(most_keys);
+  const double bytes = double(decode_rows + chunks) * double(kv_heads) * keys *
+                       (2 * (kFp4RowBytes + kFp4Powers));
+  auto alone = [&](double items, double keys_a_round, double bytes_a_us) {
+    return std::max(std::ceil(items / cus) * (6 + 2.6 * keys / keys_a_round),
+                    7 + bytes / bytes_a_us);
+  };
+  const double whole = alone(heads_of, 512, 4.6e6);
+  const double whole2 = kv_heads % 2 == 0 ? alone(heads_of / 2, 256, 5.6e6) : 1e30;
+  const double cut = 12 + 6 * std::min(1., heads_of / 128) +
+                     std::max(bytes / 6.6e6, heads_of * keys / 64 * 1.1e-3);
+  pl.whole = std::min(whole, whole2) <= cut;
+  pl.pair = kv_heads % 2 == 0 && (!pl.whole || whole2 < whole);
+  // Few items are cut finer between two heads a workgroup (16 rows of 4096 keys 19.9
+  // against 21.9, one row of 4096 13.5 against 15.7); many share a workgroup better
+  // among four (128 rows of 500 to 1500 keys 39.0 against 41.5).
+  pl.heads_per_wg = !pl.pair ? 1 : kv_heads % 4 == 0 && blocks * kv_heads > 128 && !pl.whole ? 4 : 2;
+  pl.head_groups = int(kv_heads / pl.heads_per_wg);
+  pl.min_share = 2;
+  pl.item_cost = pl.pair ? 16 : 8;
+  pl.items = blocks * pl.head_groups;
+  pl.grid = int(pl.whole ? std::min<int64_t>(pl.items, 1 << 30) : cus);
   size_t at = 0;
   if (!pl.whole) {
-    pl.rec_at = 0;
-    at = up256(size_t(items) * sizeof(int2));
+    pl.rec_at = 256;  // (the count of items comes first)
+    at = up256(pl.rec_at + size_t(pl.items) * sizeof(ItemRec));
     pl.ml_at = at;
-    const size_t cols = size_t(2) * pl.grid * hpw * pl.cols;
+    const size_t cols = size_t(2) * pl.grid * pl.heads_per_wg * pl.cols;
     at = up256(at + cols * sizeof(float2));
     pl.o_at = at;
     at = up256(at + cols * kD * sizeof(float));
@@ -1001,11 +1180,128 @@ extern "C" int kvc_gather_kv_fp4(const uint8_t* k_cache, const uint8_t* v_cache,
   return check_launch("gather_kv_fp4");
 }
 
+namespace {
+int run_rows(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_t heads,
+             const uint8_t* k_cache, const uint8_t* v_cache, const uint8_t* k_scale,
+             const uint8_t* v_scale, int64_t blocks, int64_t page, int64_t kv_heads,
+             int64_t head_dim, const int32_t* tables, int64_t bt_stride, int64_t max_blocks,
+             int64_t decode_rows, const int32_t* lens, int64_t chunks, int64_t chunk_tokens,
+             const int32_t* cu_q, const int32_t* cu_k, float scale, void* out, int64_t o_st,
+             int64_t o_sh, void* workspace, size_t workspace_bytes, kvc_stream_t stream) {
+  KVC_REQUIRE(head_dim == kD, KVC_ERR_VALUE, "%s: head_dim must be 128 (got %lld)", what,
+              (long long)head_dim);
+  KVC_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, KVC_ERR_VALUE,
+              "%s: num_heads must be a multiple of num_kv_heads", what);
+  KVC_REQUIRE(page > 0 && page % 32 == 0, KVC_ERR_VALUE,
+              "%s: page_size must be a multiple of 32 (got %lld)", what, (long long)page);
+  // (offsets inside a tile and key counts are 32-bit; div_small's range)
+  KVC_REQUIRE(kv_heads <= 4096 && heads <= 65536 && max_blocks >= 0 && blocks >= 0 &&
+                  blocks < (int64_t(1) << 31) && page <= (1 << 20) &&
+                  page * max_blocks <= (int64_t(1) << 26),
+              KVC_ERR_VALUE, "%s: shape out of range (tables of up to 2^26 keys)", what);
+  KVC_REQUIRE(decode_rows >= 0 && chunks >= 0 && chunk_tokens >= 0 &&
+                  decode_rows + chunks + chunk_tokens < (int64_t(1) << 24) &&
+                  chunk_tokens * (heads / kv_heads) < (int64_t(1) << 24),
+              KVC_ERR_VALUE, "%s: too many rows", what);
+  if (decode_rows + chunk_tokens == 0 || decode_rows + chunks == 0) return KVC_OK;
+  const int rc = check_pool(what, k_cache, v_cache, k_scale, v_scale);
+  if (rc != KVC_OK) return rc;
+  KVC_REQUIRE(q != nullptr && out != nullptr && (lens != nullptr || decode_rows == 0) &&
+                  ((cu_q != nullptr && cu_k != nullptr) || chunks == 0) &&
+                  (tables != nullptr || max_blocks == 0),
+              KVC_ERR_VALUE, "%s: null pointer", what);
+  KVC_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_st % 8 == 0 && q_sh % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(out) % 16 == 0 && o_st % 8 == 0 && o_sh % 8 == 0,
+              KVC_ERR_ASSERT, "%s: q/out rows must be 16-byte aligned", what);
+  const Plan pl = make_plan(decode_rows, chunks, chunk_tokens, heads, kv_heads, page * max_blocks);
+  // (units of the cut are 32-bit)
+  KVC_REQUIRE(pl.items * (page * max_blocks / 32 + 64) < (int64_t(1) << 31), KVC_ERR_VALUE,
+              "%s: too many rows for tables of this width", what);
+  KVC_REQUIRE(pl.bytes == 0 || (workspace != nullptr && workspace_bytes >= pl.bytes),
+              KVC_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, pl.bytes);
+  KVC_REQUIRE(pl.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KVC_ERR_ASSERT,
+              "%s: workspace must be 16-byte aligned", what);
+  Fp4Params p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_st = q_st;
+  p.q_sh = q_sh;
+  p.out = static_cast<uint16_t*>(out);
+  p.o_st = o_st;
+  p.o_sh = o_sh;
+  p.k = k_cache;
+  p.v = v_cache;
+  p.ks = k_scale;
+  p.vs = v_scale;
+  p.tables = tables;
+  p.bt_stride = bt_stride;
+  p.lens = lens;
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.decode_rows = int(decode_rows);
+  p.chunks = int(chunks);
+  p.chunk_tokens = int(chunk_tokens);
+  p.max_blocks = int(max_blocks);
+  p.num_blocks = int(blocks);
+  p.page = int(page);
+  p.page_halves = int(page / 32);
+  p.page_halves_rcp = 1.f / float(p.page_halves);
+  p.kv_heads = int(kv_heads);
+  p.group = int(heads / kv_heads);
+  p.group_rcp = 1.f / float(p.group);
+  p.heads_per_wg = pl.heads_per_wg;
+  p.head_groups = pl.head_groups;
+  p.tile_shift = pl.pair ? 5 : 6;
+  p.cols = pl.cols;
+  p.min_share = pl.min_share;
+  p.item_cost = pl.item_cost;
+  p.grid_rcp = 1.f / float(pl.grid);
+  p.whole = pl.whole;
+  p.row_blocks = (p.group + 15) / 16;
+  // (a scale of 0 stays above it: masked scores are -infinity)
+  p.c2 = std::max(std::abs(scale) * kLog2e, 1e-37f);
+  p.flip = scale < 0.f ? 0x80008000u : 0u;
+  char* ws = static_cast<char*>(workspace);
+  p.count = reinterpret_cast<int*>(ws);
+  p.rec = reinterpret_cast<ItemRec*>(ws + pl.rec_at);
+  p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_at);
+  p.part_o = reinterpret_cast<float*>(ws + pl.o_at);
+  constexpr int kLds = kWaves * kSlots * kSlotBytes;
+  hipStream_t st = as_stream(stream);
+  static std::atomic<uint64_t> ready{0};  // devices whose LDS limit is set
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (e == hipSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
+    for (auto kern : {fp4_decode_kernel<1, false>, fp4_decode_kernel<2, false>,
+                      fp4_decode_kernel<1, true>, fp4_decode_kernel<2, true>})
+      if (e == hipSuccess)
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e == hipSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  KVC_REQUIRE(e == hipSuccess, KVC_ERR_RUNTIME, "%s: LDS limit: %s", what, hipGetErrorString(e));
+  auto kern = chunks > 0 ? (pl.pair ? fp4_decode_kernel<2, true> : fp4_decode_kernel<1, true>)
+                         : (pl.pair ? fp4_decode_kernel<2, false> : fp4_decode_kernel<1, false>);
+  kern<<<pl.grid, 64 * kWaves, kLds, st>>>(p);
+  if (!pl.whole) {
+    const int64_t pieces = pl.grid / std::max<int64_t>(pl.items, 1) + 2;  // of an item
+    const int slices = pieces <= kAhead ? 1 : pieces <= 4 * kAhead ? 4 : kGroups;
+    auto merge = slices == 1   ? fp4_merge_kernel<1>
+                 : slices == 4 ? fp4_merge_kernel<4>
+                               : fp4_merge_kernel<kGroups>;
+    const int per_wg = kGroups / slices;
+    merge<<<dim3(unsigned(pl.items), unsigned((pl.heads_per_wg * pl.cols + per_wg - 1) / per_wg)),
+            32 * kGroups, 0, st>>>(p);
+  }
+  return check_launch(what);
+}
+}  // namespace
+
 extern "C" size_t kvc_paged_decode_fp4_workspace_bytes(int64_t batch, int64_t num_heads,
                                                        int64_t num_kv_heads, int64_t page_size,
                                                        int64_t max_blocks_per_seq) {
   if (batch <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
-  return make_plan(batch, num_heads, num_kv_heads, page_size * max_blocks_per_seq).bytes;
+  return make_plan(batch, 0, 0, num_heads, num_kv_heads, page_size * max_blocks_per_seq).bytes;
 }
 
 extern "C" int kvc_paged_decode_fp4(
@@ -1017,90 +1313,41 @@ extern "C" int kvc_paged_decode_fp4(
     int64_t out_stride_b, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
     kvc_stream_t stream) {
   clear_error();
-  KVC_REQUIRE(head_dim == kD, KVC_ERR_VALUE, "paged_decode_fp4: head_dim must be 128 (got %lld)",
-              (long long)head_dim);
-  KVC_REQUIRE(batch >= 0 && num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0,
-              KVC_ERR_VALUE, "paged_decode_fp4: num_heads must be a multiple of num_kv_heads");
-  KVC_REQUIRE(page_size > 0 && page_size % 32 == 0, KVC_ERR_VALUE,
-              "paged_decode_fp4: page_size must be a multiple of 32 (got %lld)",
-              (long long)page_size);
-  // (row offsets inside a half tile and key counts are 32-bit; div_small's range)
-  KVC_REQUIRE(num_kv_heads <= 4096 && num_heads <= 65536 && max_blocks_per_seq >= 0 &&
-                  num_cache_blocks >= 0 && num_cache_blocks < (int64_t(1) << 31) &&
-                  page_size <= (1 << 20) && page_size * max_blocks_per_seq <= (int64_t(1) << 26),
-              KVC_ERR_VALUE, "paged_decode_fp4: shape out of range (tables of up to 2^26 keys)");
-  if (batch == 0) return KVC_OK;
-  const int rc = check_pool("paged_decode_fp4", k_cache, v_cache, k_scale, v_scale);
-  if (rc != KVC_OK) return rc;
-  KVC_REQUIRE(q != nullptr && out != nullptr && context_lens != nullptr &&
-                  (block_tables != nullptr || max_blocks_per_seq == 0),
-              KVC_ERR_VALUE, "paged_decode_fp4: null pointer");
-  KVC_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride_b % 8 == 0 &&
-                  q_stride_h % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
-                  out_stride_b % 8 == 0 && out_stride_h % 8 == 0,
-              KVC_ERR_ASSERT, "paged_decode_fp4: q/out rows must be 16-byte aligned");
-  const Plan pl = make_plan(batch, num_heads, num_kv_heads, page_size * max_blocks_per_seq);
-  const int64_t items = batch * pl.groups;
-  KVC_REQUIRE(items < (int64_t(1) << 30), KVC_ERR_VALUE, "paged_decode_fp4: batch too large");
-  KVC_REQUIRE(pl.bytes == 0 || (workspace != nullptr && workspace_bytes >= pl.bytes),
-              KVC_ERR_WORKSPACE, "paged_decode_fp4: workspace of %zu bytes needed", pl.bytes);
-  KVC_REQUIRE(pl.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KVC_ERR_ASSERT,
-              "paged_decode_fp4: workspace must be 16-byte aligned");
-  Fp4Params p{};
-  p.q = static_cast<const uint16_t*>(q);
-  p.q_sb = q_stride_b;
-  p.q_sh = q_stride_h;
-  p.out = static_cast<uint16_t*>(out);
-  p.o_sb = out_stride_b;
-  p.o_sh = out_stride_h;
-  p.k = k_cache;
-  p.v = v_cache;
-  p.ks = k_scale;
-  p.vs = v_scale;
-  p.tables = block_tables;
-  p.bt_stride = bt_stride;
-  p.lens = context_lens;
-  p.max_blocks = int(max_blocks_per_seq);
-  p.num_blocks = int(num_cache_blocks);
-  p.page = int(page_size);
-  p.page_halves = int(page_size / 32);
-  p.page_halves_rcp = 1.f / float(p.page_halves);
-  p.batch = int(batch);
-  p.kv_heads = int(num_kv_heads);
-  p.group = int(num_heads / num_kv_heads);
-  p.col_blocks = pl.col_blocks;
-  p.heads_per_wg = pl.heads_per_wg;
-  p.tile_shift = pl.pair ? 5 : 6;
-  p.grid_rcp = 1.f / float(pl.grid);
-  p.groups = pl.groups;
-  p.cols = pl.cols;
-  p.min_share = pl.min_share;
-  p.whole = pl.whole;
-  // (a scale of 0 stays above it: masked scores are -infinity)
-  p.c2 = std::max(std::abs(scale) * kLog2e, 1e-37f);
-  p.flip = scale < 0.f ? 0x80008000u : 0u;
-  char* ws = static_cast<char*>(workspace);
-  p.rec = reinterpret_cast<int2*>(ws + pl.rec_at);
-  p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_at);
-  p.part_o = reinterpret_cast<float*>(ws + pl.o_at);
-  constexpr int kLds = kWaves * kSlots * kSlotBytes;
-  hipStream_t st = as_stream(stream);
-  static std::atomic<uint64_t> ready{0};  // devices whose LDS limit is set
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  const uint64_t bit = uint64_t(1) << (dev & 63);
-  if (e == hipSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
-    for (auto kern : {fp4_decode_kernel<1>, fp4_decode_kernel<2>})
-      if (e == hipSuccess)
-        e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-    if (e == hipSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
-  }
-  KVC_REQUIRE(e == hipSuccess, KVC_ERR_RUNTIME, "paged_decode_fp4: LDS limit: %s",
-              hipGetErrorString(e));
-  (pl.pair ? fp4_decode_kernel<2> : fp4_decode_kernel<1>)<<<pl.grid, 64 * kWaves, kLds, st>>>(p);
-  if (!pl.whole)
-    fp4_merge_kernel<<<dim3(unsigned(items), unsigned(pl.heads_per_wg * pl.cols)), 32 * kSlices, 0,
-                       st>>>(p);
-  return check_launch("paged_decode_fp4");
+  return run_rows("paged_decode_fp4", q, q_stride_b, q_stride_h, num_heads, k_cache, v_cache,
+                  k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim,
+                  block_tables, bt_stride, max_blocks_per_seq, batch, context_lens, 0, 0, nullptr,
+                  nullptr, scale, out, out_stride_b, out_stride_h, workspace, workspace_bytes,
+                  stream);
+}
+
+extern "C" size_t kvc_varlen_fp4_workspace_bytes(int64_t num_q_tokens, int64_t num_heads,
+                                                 int64_t num_kv_heads, int64_t page_size,
+                                                 int64_t max_blocks_per_seq,
+                                                 int64_t num_decode_rows, int64_t num_prefill) {
+  if (num_q_tokens <= 0 || num_decode_rows < 0 || num_prefill < 0 ||
+      num_decode_rows > num_q_tokens || num_kv_heads <= 0 || num_heads <= 0 ||
+      num_heads % num_kv_heads != 0)
+    return 0;
+  return make_plan(num_decode_rows, num_prefill, num_q_tokens - num_decode_rows, num_heads,
+                   num_kv_heads, page_size * max_blocks_per_seq)
+      .bytes;
+}
+
+extern "C" int kvc_varlen_fp4(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_q_tokens,
+    int64_t num_heads, const uint8_t* k_cache, const uint8_t* v_cache, const uint8_t* k_scale,
+    const uint8_t* v_scale, int64_t num_cache_blocks, int64_t page_size, int64_t num_kv_heads,
+    int64_t head_dim, const int32_t* block_tables, int64_t bt_stride, int64_t max_blocks_per_seq,
+    int64_t num_decode_rows, const int32_t* decode_context_lens, int64_t num_prefill,
+    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, float scale, void* out,
+    int64_t out_stride_t, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
+    kvc_stream_t stream) {
+  clear_error();
+  KVC_REQUIRE(num_decode_rows >= 0 && num_decode_rows <= num_q_tokens, KVC_ERR_VALUE,
+              "varlen_fp4: more decode rows than query rows");
+  return run_rows("varlen_fp4", q, q_stride_t, q_stride_h, num_heads, k_cache, v_cache, k_scale,
+                  v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim, block_tables,
+                  bt_stride, max_blocks_per_seq, num_decode_rows, decode_context_lens,
+                  num_prefill, num_q_tokens - num_decode_rows, cu_seqlens_q, cu_seqlens_k, scale,
+                  out, out_stride_t, out_stride_h, workspace, workspace_bytes, stream);
 }

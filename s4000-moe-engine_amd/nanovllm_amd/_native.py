@@ -131,6 +131,10 @@ SIGNATURES = {
     "kvc_paged_decode_fp4": (_INT, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P,
                                     _I64, _I64, _P, _I64, _I64, _F32, _P, _I64, _I64, _P, _SZ,
                                     _P]),
+    "kvc_varlen_fp4_workspace_bytes": (_SZ, [_I64] * 7),
+    "kvc_varlen_fp4": (_INT, [_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
+                              _P, _I64, _I64, _I64, _P, _I64, _P, _P, _F32, _P, _I64, _I64, _P,
+                              _SZ, _P]),
     "kvc_step_tables": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I64,
                                _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "kvc_stage_decode": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,

@@ -163,6 +163,38 @@ def paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, contex
     return out
 
 
+def varlen_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, num_decode_rows,
+               decode_context_lens, cu_seqlens_q, cu_seqlens_k, scale, out):
+    """varlen_attention's rows over a 4-bit pool read as it is
+    (kvc_varlen_fp4), into out; arguments as varlen_attention checked and
+    converted them, int32 offsets on q's device."""
+    num_prefill = cu_seqlens_q.numel() - 1
+    _one_device(k_cache, q=q, block_tables=block_tables, cu_seqlens_q=cu_seqlens_q,
+                cu_seqlens_k=cu_seqlens_k)
+    if num_decode_rows:
+        _one_device(k_cache, decode_context_lens=decode_context_lens)
+    if block_tables.size(0) < num_decode_rows + num_prefill:
+        raise ValueError("block_tables has fewer rows than the call has sequences")
+    if not _rows16(q):
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+    tokens, num_heads, _ = q.shape
+    page_size, kvh, max_blocks = k_cache.size(1), k_cache.size(2), block_tables.size(1)
+    need = nat.query("kvc_varlen_fp4_workspace_bytes", tokens, num_heads, kvh, page_size,
+                     max_blocks, num_decode_rows, num_prefill)
+    ws = nat.workspace(need, q.device)
+    nat.call_on(
+        k_cache, "kvc_varlen_fp4", q.data_ptr(), q.stride(0), q.stride(1), tokens, num_heads,
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        k_cache.size(0), page_size, kvh, 128, block_tables.data_ptr(), block_tables.stride(0),
+        max_blocks, num_decode_rows,
+        decode_context_lens.data_ptr() if num_decode_rows else None, num_prefill,
+        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), float(scale), out.data_ptr(),
+        out.stride(0), out.stride(1), nat.ptr(ws), need, nat.stream_of(q))
+    return out
+
+
 def paged_decode_append_fp4(q, key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping,
                             block_tables, context_lens, scale, out=None):
     """The decode step over a 4-bit pool: store_kvcache_fp4 of the new tokens,

@@ -17,7 +17,7 @@ import numpy as np
 import torch
 
 from .. import _native as nat
-from .kv_fp4 import check_fp4_pool, gather_kv_fp4, paged_decode_fp4
+from .kv_fp4 import check_fp4_pool, gather_kv_fp4, paged_decode_fp4, varlen_fp4
 from .paged_attention import _kv_encoding
 
 
@@ -222,6 +222,10 @@ def _paged_rows(c, q, nd, k_cache, v_cache, scale, k_scale, v_scale, side_k, sid
     )
 
 
+def _read_in_place(c) -> bool:
+    return False
+
+
 def varlen_attention(q, k_cache, v_cache, *, scale, block_tables=None,
                      num_decode_rows=0, decode_context_lens=None,
                      cu_seqlens_q=None, cu_seqlens_k=None,
@@ -246,6 +250,10 @@ def varlen_attention(q, k_cache, v_cache, *, scale, block_tables=None,
     enc, fresh, q = c.enc, c.fresh, c.q
     if enc == nat.KVC_KV_FP4:
         check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
+        if c.num_prefill and _read_in_place(c):
+            return varlen_fp4(q, k_cache, v_cache, k_scale, v_scale, c.block_tables,
+                              num_decode_rows, c.decode_context_lens, c.cu_seqlens_q,
+                              c.cu_seqlens_k, scale, c.out)
     gathered = (enc != nat.KVC_KV_BF16 and not fresh and c.num_prefill
                 and (enc == nat.KVC_KV_FP4 or os.environ.get("KVC_PREFILL_SK", "1") != "0"))
     has_side = enc == nat.KVC_KV_INT8_CHAN and side_k is not None and head_n_out is not None
