@@ -737,23 +737,35 @@ int kvc_paged_decode_fp4(const void* q, int64_t q_stride_b, int64_t q_stride_h,
  * num_prefill chunks, chunk i's queries at rows num_decode_rows +
  * cu_seqlens_q[i] .. and its cu_seqlens_k[i + 1] - cu_seqlens_k[i] keys in table
  * row num_decode_rows + i; its t-th of n queries sees all but the last n - t - 1
- * keys.  Every 16 columns (query tokens x the query heads of a kv head) read the
- * keys once, so it is for chunks of few tokens (drafts to verify, the ends of
- * prompts); long ones are faster gathered (kvc_gather_kv_fp4).  Lengths are read
- * on the device; rows of no sequence are not written. */
+ * keys.  Every 16 columns (query tokens x the query heads of a kv head: a block)
+ * read the keys once, so it is for chunks of few tokens (drafts to verify, the
+ * ends of prompts); long ones are faster gathered (kvc_gather_kv_fp4).
+ * chunk_blocks: the chunks' blocks, sum of ceil(tokens x query heads per kv head /
+ * 16), as the host knows it (fewer than there are would leave rows out), or 0;
+ * the workspace query takes the same.  Lengths are read on the device; rows of no
+ * sequence are not written. */
 size_t kvc_varlen_fp4_workspace_bytes(int64_t num_q_tokens, int64_t num_heads,
                                       int64_t num_kv_heads, int64_t page_size,
                                       int64_t max_blocks_per_seq, int64_t num_decode_rows,
-                                      int64_t num_prefill);
+                                      int64_t num_prefill, int64_t chunk_blocks);
 int kvc_varlen_fp4(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_q_tokens,
                    int64_t num_heads, const uint8_t* k_cache, const uint8_t* v_cache,
                    const uint8_t* k_scale, const uint8_t* v_scale, int64_t num_cache_blocks,
                    int64_t page_size, int64_t num_kv_heads, int64_t head_dim,
                    const int32_t* block_tables, int64_t bt_stride, int64_t max_blocks_per_seq,
                    int64_t num_decode_rows, const int32_t* decode_context_lens,
-                   int64_t num_prefill, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                   float scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
-                   void* workspace, size_t workspace_bytes, kvc_stream_t stream);
+                   int64_t num_prefill, int64_t chunk_blocks, const int32_t* cu_seqlens_q,
+                   const int32_t* cu_seqlens_k, float scale, void* out, int64_t out_stride_t,
+                   int64_t out_stride_h, void* workspace, size_t workspace_bytes,
+                   kvc_stream_t stream);
+
+/* Host only: the chunks' blocks (chunk_blocks above) where reading the pool in
+ * place is estimated to be no slower than gathering it, else 0.  cu_seqlens_* are
+ * in HOST memory. */
+int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
+                              const int32_t* cu_seqlens_k_host, int64_t num_prefill,
+                              int64_t num_heads, int64_t num_kv_heads, int64_t page_size,
+                              int64_t max_blocks_per_seq, int64_t num_decode_rows);
 
 /* ---------------------------------------------------------------------------
  * A step's tables from its requests' lengths, on the device.

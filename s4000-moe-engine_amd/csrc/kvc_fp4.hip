@@ -1020,14 +1020,15 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // 7.6 / 10.5, 1 x 4096 13.2 / 27.8 / 38.4, 64 x 2048 26.9 / 22.0 / 25.1, 64 x 4096 39.7
 // / 36.3 / 40.0, 128 x 500 to 1500 29.9 / 30.6 / 22.8, 48 x 1025 to 8007 36.5 / 50.8 /
 // 66.5, 128 x 4096 62.7 / 70.5 / 54.3, 16 x 32768 62 / 182 / 246.
-Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t heads,
-               int64_t kv_heads, int64_t most_keys) {
+Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t chunk_blocks,
+               int64_t heads, int64_t kv_heads, int64_t most_keys) {
   Plan pl{};
   const int64_t group = heads / kv_heads;
   const int cus = cu_count();
   pl.cols = int(chunks > 0 ? 16 : std::min<int64_t>(group, 16));
-  const int64_t blocks =
-      decode_rows * ((group + 15) / 16) + chunk_tokens * group / 16 + chunks;
+  // (of the chunks at most, where the caller does not know)
+  if (chunk_blocks <= 0) chunk_blocks = (chunk_tokens * group + 15 * chunks) / 16;
+  const int64_t blocks = decode_rows * ((group + 15) / 16) + chunk_blocks;
   const double heads_of = double(blocks) * double(kv_heads), keys = double(most_keys);
   const double bytes = double(decode_rows + chunks) * double(kv_heads) * keys *
                        (2 * (kFp4RowBytes + kFp4Powers));
@@ -1186,7 +1187,7 @@ int run_rows(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_
              const uint8_t* v_scale, int64_t blocks, int64_t page, int64_t kv_heads,
              int64_t head_dim, const int32_t* tables, int64_t bt_stride, int64_t max_blocks,
              int64_t decode_rows, const int32_t* lens, int64_t chunks, int64_t chunk_tokens,
-             const int32_t* cu_q, const int32_t* cu_k, float scale, void* out, int64_t o_st,
+             int64_t chunk_blocks, const int32_t* cu_q, const int32_t* cu_k, float scale, void* out, int64_t o_st,
              int64_t o_sh, void* workspace, size_t workspace_bytes, kvc_stream_t stream) {
   KVC_REQUIRE(head_dim == kD, KVC_ERR_VALUE, "%s: head_dim must be 128 (got %lld)", what,
               (long long)head_dim);
@@ -1213,7 +1214,8 @@ int run_rows(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_
   KVC_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_st % 8 == 0 && q_sh % 8 == 0 &&
                   reinterpret_cast<uintptr_t>(out) % 16 == 0 && o_st % 8 == 0 && o_sh % 8 == 0,
               KVC_ERR_ASSERT, "%s: q/out rows must be 16-byte aligned", what);
-  const Plan pl = make_plan(decode_rows, chunks, chunk_tokens, heads, kv_heads, page * max_blocks);
+  const Plan pl = make_plan(decode_rows, chunks, chunk_tokens, chunk_blocks, heads, kv_heads,
+                            page * max_blocks);
   // (units of the cut are 32-bit)
   KVC_REQUIRE(pl.items * (page * max_blocks / 32 + 64) < (int64_t(1) << 31), KVC_ERR_VALUE,
               "%s: too many rows for tables of this width", what);
@@ -1301,7 +1303,7 @@ extern "C" size_t kvc_paged_decode_fp4_workspace_bytes(int64_t batch, int64_t nu
                                                        int64_t num_kv_heads, int64_t page_size,
                                                        int64_t max_blocks_per_seq) {
   if (batch <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
-  return make_plan(batch, 0, 0, num_heads, num_kv_heads, page_size * max_blocks_per_seq).bytes;
+  return make_plan(batch, 0, 0, 0, num_heads, num_kv_heads, page_size * max_blocks_per_seq).bytes;
 }
 
 extern "C" int kvc_paged_decode_fp4(
@@ -1315,21 +1317,22 @@ extern "C" int kvc_paged_decode_fp4(
   clear_error();
   return run_rows("paged_decode_fp4", q, q_stride_b, q_stride_h, num_heads, k_cache, v_cache,
                   k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim,
-                  block_tables, bt_stride, max_blocks_per_seq, batch, context_lens, 0, 0, nullptr,
-                  nullptr, scale, out, out_stride_b, out_stride_h, workspace, workspace_bytes,
+                  block_tables, bt_stride, max_blocks_per_seq, batch, context_lens, 0, 0, 0,
+                  nullptr, nullptr, scale, out, out_stride_b, out_stride_h, workspace, workspace_bytes,
                   stream);
 }
 
 extern "C" size_t kvc_varlen_fp4_workspace_bytes(int64_t num_q_tokens, int64_t num_heads,
                                                  int64_t num_kv_heads, int64_t page_size,
                                                  int64_t max_blocks_per_seq,
-                                                 int64_t num_decode_rows, int64_t num_prefill) {
+                                                 int64_t num_decode_rows, int64_t num_prefill,
+                                                 int64_t chunk_blocks) {
   if (num_q_tokens <= 0 || num_decode_rows < 0 || num_prefill < 0 ||
       num_decode_rows > num_q_tokens || num_kv_heads <= 0 || num_heads <= 0 ||
       num_heads % num_kv_heads != 0)
     return 0;
-  return make_plan(num_decode_rows, num_prefill, num_q_tokens - num_decode_rows, num_heads,
-                   num_kv_heads, page_size * max_blocks_per_seq)
+  return make_plan(num_decode_rows, num_prefill, num_q_tokens - num_decode_rows, chunk_blocks,
+                   num_heads, num_kv_heads, page_size * max_blocks_per_seq)
       .bytes;
 }
 
@@ -1339,7 +1342,8 @@ extern "C" int kvc_varlen_fp4(
     const uint8_t* v_scale, int64_t num_cache_blocks, int64_t page_size, int64_t num_kv_heads,
     int64_t head_dim, const int32_t* block_tables, int64_t bt_stride, int64_t max_blocks_per_seq,
     int64_t num_decode_rows, const int32_t* decode_context_lens, int64_t num_prefill,
-    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, float scale, void* out,
+    int64_t chunk_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, float scale,
+    void* out,
     int64_t out_stride_t, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
     kvc_stream_t stream) {
   clear_error();
@@ -1348,6 +1352,42 @@ extern "C" int kvc_varlen_fp4(
   return run_rows("varlen_fp4", q, q_stride_t, q_stride_h, num_heads, k_cache, v_cache, k_scale,
                   v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim, block_tables,
                   bt_stride, max_blocks_per_seq, num_decode_rows, decode_context_lens,
-                  num_prefill, num_q_tokens - num_decode_rows, cu_seqlens_q, cu_seqlens_k, scale,
+                  num_prefill, num_q_tokens - num_decode_rows, chunk_blocks, cu_seqlens_q,
+                  cu_seqlens_k, scale,
                   out, out_stride_t, out_stride_h, workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
+                                         const int32_t* cu_seqlens_k_host, int64_t num_prefill,
+                                         int64_t num_heads, int64_t num_kv_heads,
+                                         int64_t page_size, int64_t max_blocks_per_seq,
+                                         int64_t num_decode_rows) {
+  if (num_prefill <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      cu_seqlens_q_host == nullptr || cu_seqlens_k_host == nullptr)
+    return 0;
+  const int64_t group = num_heads / num_kv_heads;
+  int64_t blocks = 0, longest = 0;
+  double products = 0, all_keys = 0, pairs = 0;
+  for (int64_t i = 0; i < num_prefill; ++i) {
+    const int64_t n = std::max<int64_t>(0, int64_t(cu_seqlens_q_host[i + 1]) - cu_seqlens_q_host[i]);
+    const int64_t m = std::max<int64_t>(0, int64_t(cu_seqlens_k_host[i + 1]) - cu_seqlens_k_host[i]);
+    const int64_t b = (n * group + 15) / 16;
+    blocks += b;
+    longest = std::max(longest, m);
+    products += double(b) * double(m);
+    all_keys += double(m);
+    pairs += double(n) * double(std::max<int64_t>(0, m - n)) + double(n) * double(n) / 2;
+  }
+  if (blocks == 0) return 0;
+  const Plan pl = make_plan(num_decode_rows, num_prefill, cu_seqlens_q_host[num_prefill], blocks,
+                            num_heads, num_kv_heads, page_size * max_blocks_per_seq);
+  const double items = double(blocks) * double(num_kv_heads) / (pl.whole && pl.pair ? 2 : 1);
+  const double here =
+      pl.whole ? std::ceil(items / cu_count()) * (6.5 + 2.6 * double(longest) / (pl.pair ? 256 : 512))
+               : 12 + 6 * std::min(1., items / 128) + products * double(num_kv_heads) / 64 * 1.1e-3;
+  // Gathered: three launches, the keys written and read once more, the products at the
+  // long chunks' rate; and the decode rows in a call of their own.
+  const double gathered = (longest <= 64 ? 13 : 22) + 3e-4 * all_keys * double(num_kv_heads) +
+                          0.38e-6 * pairs * double(num_heads) + (num_decode_rows > 0 ? 12 : 0);
+  return here <= gathered ? blocks : 0;
 }

@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <cstdlib>
 #include <cstring>
+#include <vector>
 
 #include "kvc.h"
 
@@ -37,6 +38,12 @@ decltype(&kvc_tree_workspace_bytes) p_tree_workspace;
 decltype(&kvc_tree_attention) p_tree;
 decltype(&kvc_qk_norm_mrope_store) p_mrope;
 decltype(&kvc_commit_rows) p_commit;
+decltype(&kvc_store_fp4) p_store_fp4;
+decltype(&kvc_gather_kv_fp4) p_gather_fp4;
+decltype(&kvc_varlen_fp4_workspace_bytes) p_varlen_fp4_workspace;
+decltype(&kvc_varlen_fp4_blocks) p_varlen_fp4_blocks;
+decltype(&kvc_varlen_fp4) p_varlen_fp4;
+decltype(&kvc_step_tables) p_step_tables;
 
 // The tensor behind an exact torch.Tensor / Parameter, else null.
 const at::Tensor* tensor(PyObject* o) {
@@ -655,6 +662,328 @@ PyObject* commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_TRUE;
 }
 
+// A 4-bit pool: codes [pages, page, kv heads, 64] and powers [.., 4], on like's GPU.
+struct Fp4Pool {
+  uint8_t *k = nullptr, *v = nullptr, *ks = nullptr, *vs = nullptr;
+  int64_t pages = 0, page = 0, kvh = 0;
+};
+bool fp4_pool(PyObject* const* a, const at::Tensor& like, Fp4Pool& p) {
+  const at::Tensor* t[4];
+  for (int i = 0; i < 4; ++i) {
+    t[i] = tensor(a[i]);
+    if (!plain(t[i], at::kByte, 4, like) || !t[i]->is_contiguous()) return false;
+  }
+  p.pages = t[0]->size(0), p.page = t[0]->size(1), p.kvh = t[0]->size(2);
+  if (t[0]->size(3) != 64 || t[1]->sizes() != t[0]->sizes() || p.kvh == 0 || p.page == 0)
+    return false;
+  for (int i = 2; i < 4; ++i)
+    if (t[i]->size(0) != p.pages || t[i]->size(1) != p.page || t[i]->size(2) != p.kvh ||
+        t[i]->size(3) != 4)
+      return false;
+  p.k = static_cast<uint8_t*>(address(t[0])), p.v = static_cast<uint8_t*>(address(t[1]));
+  p.ks = static_cast<uint8_t*>(address(t[2])), p.vs = static_cast<uint8_t*>(address(t[3]));
+  return true;
+}
+
+// The append's rows and slots.
+struct Fp4Append {
+  Rows k, v;
+  void* slots = nullptr;
+  int64_t n = 0;
+  int sb = 4;
+};
+bool fp4_append(PyObject* key, PyObject* value, PyObject* slot_mapping, const Fp4Pool& p,
+                const at::Tensor& like, Fp4Append& r) {
+  const at::Tensor *k = tensor(key), *v = tensor(value), *slots = tensor(slot_mapping);
+  if (!plain(k, at::kBFloat16, 3, like) || !plain(v, at::kBFloat16, 3, like) ||
+      k->sizes() != v->sizes() || k->size(0) == 0 || k->size(1) != p.kvh || k->size(2) != 128 ||
+      k->stride(1) != 128 || v->stride(1) != 128 || !rows16(*k) || !rows16(*v) ||
+      !is_index(slots, k->size(0), like, &r.sb))
+    return false;
+  r.n = k->size(0);
+  r.k = rows(k), r.v = rows(v), r.slots = address(slots);
+  return true;
+}
+int fp4_store_call(const Fp4Append& r, const Fp4Pool& p, void* stream) {
+  return p_store_fp4(r.k.p, r.k.s0, r.k.s1, r.v.p, r.v.s0, r.v.s1, p.k, p.v, p.ks, p.vs,
+                     p.pages * p.page, r.slots, r.sb, r.n, p.kvh, 128, stream);
+}
+
+// fp4_store(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, stream):
+// True, or None.
+PyObject* fp4_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8) {
+    PyErr_SetString(PyExc_TypeError, "fp4_store takes 8 arguments");
+    return nullptr;
+  }
+  Fp4Pool pool;
+  Fp4Append rows_;
+  void* stream;
+  try {
+    const at::Tensor* key = tensor(a[0]);
+    if (key == nullptr || !key->defined() || !key->is_cuda() || !fp4_pool(a + 2, *key, pool) ||
+        !fp4_append(a[0], a[1], a[6], pool, *key, rows_))
+      Py_RETURN_NONE;
+    stream = PyLong_AsVoidPtr(a[7]);
+    if (PyErr_Occurred()) return nullptr;
+  } catch (const std::exception&) {
+    return declined();
+  }
+  int rc;
+  {
+    Unlocked unlocked;
+    rc = fp4_store_call(rows_, pool, stream);
+  }
+  if (rc != KVC_OK) return fail(rc, "kvc_store_fp4");
+  Py_RETURN_TRUE;
+}
+
+// fp4_rows(out or None, q, k_cache, v_cache, k_scale, v_scale, block_tables,
+//          num_decode_rows, decode_context_lens, cu_seqlens_q or None, cu_seqlens_k,
+//          cu_seqlens_q_list or None, cu_seqlens_k_list, scale, stream, key or None,
+//          value, slot_mapping): decode rows and chunks that are read in place
+// (chunks without their host lists, or that are better gathered, are declined), after
+// the append of their tokens if there is a key.
+PyObject* fp4_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 18) {
+    PyErr_SetString(PyExc_TypeError, "fp4_rows takes 18 arguments");
+    return nullptr;
+  }
+  at::Tensor out, ws;
+  Rows q_r, out_r;
+  Fp4Pool pool;
+  Fp4Append append;
+  void *bt_p, *lens_p, *cuq_p, *cuk_p, *ws_p, *stream;
+  int64_t tokens, heads, decode_rows, prefill = 0, bt_stride, blocks, chunk_blocks = 0;
+  size_t bytes;
+  float scale;
+  try {
+    const at::Tensor *q = tensor(a[1]), *bt = tensor(a[6]);
+    if (q == nullptr || !q->defined() || !plain(q, at::kBFloat16, 3, *q) ||
+        !fp4_pool(a + 2, *q, pool) || !plain(bt, at::kInt, 2, *q) || bt->stride(1) != 1 ||
+        !PyLong_CheckExact(a[7]) || !PyFloat_CheckExact(a[13]))
+      Py_RETURN_NONE;
+    tokens = q->size(0), heads = q->size(1);
+    decode_rows = PyLong_AsLongLong(a[7]);
+    if (decode_rows < 0 || decode_rows > tokens) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    if (tokens == 0 || heads == 0 || q->size(2) != 128 || !rows16(*q) || heads % pool.kvh != 0 ||
+        pool.page % 32 != 0)
+      Py_RETURN_NONE;
+    const at::Tensor *lens = nullptr, *cu_q = nullptr, *cu_k = nullptr;
+    if (decode_rows > 0 && !ints(lens = tensor(a[8]), decode_rows, *q)) Py_RETURN_NONE;
+    bt_stride = bt->stride(0), blocks = bt->size(1);
+    if (a[9] != Py_None || decode_rows < tokens) {
+      if (!PyList_CheckExact(a[11]) || !PyList_CheckExact(a[12]) || PyList_GET_SIZE(a[11]) < 1 ||
+          PyList_GET_SIZE(a[11]) != PyList_GET_SIZE(a[12]))
+        Py_RETURN_NONE;
+      prefill = PyList_GET_SIZE(a[11]) - 1;
+      std::vector<int32_t> hq(prefill + 1), hk(prefill + 1);
+      int64_t last_q = 0, last_k = 0;
+      for (int64_t i = 0; i <= prefill; ++i) {
+        int64_t cq, ck;
+        if (!item(a[11], i, &cq) || !item(a[12], i, &ck) || cq < last_q || ck < last_k ||
+            (i == 0 && (cq != 0 || ck != 0)) || (cq > last_q && ck - last_k < cq - last_q) ||
+            ck >= (int64_t(1) << 31))
+          Py_RETURN_NONE;
+        hq[i] = int32_t(cq), hk[i] = int32_t(ck);
+        last_q = cq, last_k = ck;
+      }
+      if (decode_rows + last_q != tokens) Py_RETURN_NONE;
+      if (prefill > 0) {
+        if (!ints(cu_q = tensor(a[9]), prefill + 1, *q) ||
+            !ints(cu_k = tensor(a[10]), prefill + 1, *q))
+          Py_RETURN_NONE;
+        chunk_blocks = p_varlen_fp4_blocks(hq.data(), hk.data(), prefill, heads, pool.kvh,
+                                           pool.page, blocks, decode_rows);
+        if (chunk_blocks == 0) Py_RETURN_NONE;
+      }
+    }
+    if (bt->size(0) < decode_rows + prefill) Py_RETURN_NONE;
+    if (a[15] != Py_None &&
+        (!fp4_append(a[15], a[16], a[17], pool, *q, append) || append.n != tokens))
+      Py_RETURN_NONE;
+    if (a[0] != Py_None) {
+      const at::Tensor* given = tensor(a[0]);
+      if (!plain(given, at::kBFloat16, 3, *q) || given->sizes() != q->sizes() || !rows16(*given))
+        Py_RETURN_NONE;
+      out = *given;
+    } else {
+      out = at::empty({tokens, heads, 128}, q->options());
+    }
+    stream = PyLong_AsVoidPtr(a[14]);
+    if (PyErr_Occurred()) return nullptr;
+    scale = float(PyFloat_AS_DOUBLE(a[13]));
+    bytes = p_varlen_fp4_workspace(tokens, heads, pool.kvh, pool.page, blocks, decode_rows,
+                                   prefill, chunk_blocks);
+    if (bytes > 0) ws = at::empty({int64_t(bytes)}, q->options().dtype(at::kByte));
+    ws_p = bytes > 0 ? ws.data_ptr() : nullptr;
+    q_r = rows(q), out_r = rows(&out);
+    bt_p = address(bt), lens_p = address(lens), cuq_p = address(cu_q), cuk_p = address(cu_k);
+  } catch (const std::exception&) {
+    return declined();
+  }
+  int rc = KVC_OK;
+  {
+    Unlocked unlocked;
+    if (append.n > 0) rc = fp4_store_call(append, pool, stream);
+    if (rc == KVC_OK)
+      rc = p_varlen_fp4(q_r.p, q_r.s0, q_r.s1, tokens, heads, pool.k, pool.v, pool.ks, pool.vs,
+                        pool.pages, pool.page, pool.kvh, 128, static_cast<int32_t*>(bt_p),
+                        bt_stride, blocks, decode_rows, static_cast<int32_t*>(lens_p), prefill,
+                        chunk_blocks, static_cast<int32_t*>(cuq_p), static_cast<int32_t*>(cuk_p),
+                        scale, out_r.p, out_r.s0, out_r.s1, ws_p, bytes, stream);
+  }
+  if (rc != KVC_OK) return fail(rc, "kvc_varlen_fp4");
+  if (a[0] != Py_None) {
+    Py_INCREF(a[0]);
+    return a[0];
+  }
+  return wrap(std::move(out));
+}
+
+PyObject* pair(at::Tensor&& first, at::Tensor&& second) {
+  PyObject* r = PyTuple_New(2);
+  if (r == nullptr) return nullptr;
+  PyObject* x = wrap(std::move(first));
+  PyObject* y = wrap(std::move(second));
+  PyTuple_SET_ITEM(r, 0, x);
+  PyTuple_SET_ITEM(r, 1, y);
+  if (x != nullptr && y != nullptr) return r;
+  Py_DECREF(r);
+  return nullptr;
+}
+
+// fp4_gather(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_k, row0,
+//            chunks, total, stream): (K, V), or None.
+PyObject* fp4_gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10) {
+    PyErr_SetString(PyExc_TypeError, "fp4_gather takes 10 arguments");
+    return nullptr;
+  }
+  at::Tensor k, v;
+  Fp4Pool pool;
+  void *bt_p, *cuk_p, *k_p, *v_p, *stream;
+  int64_t bt_stride, blocks, v_[3];
+  try {
+    const at::Tensor *kc = tensor(a[0]), *bt = tensor(a[4]), *cu_k = tensor(a[5]);
+    if (kc == nullptr || !kc->defined() || !kc->is_cuda() || !fp4_pool(a, *kc, pool) ||
+        !plain(bt, at::kInt, 2, *kc) || bt->stride(1) != 1)
+      Py_RETURN_NONE;
+    for (int i = 0; i < 3; ++i) {
+      if (!PyLong_CheckExact(a[6 + i])) Py_RETURN_NONE;
+      v_[i] = PyLong_AsLongLong(a[6 + i]);
+      if (v_[i] < 0) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+      }
+    }
+    if (v_[1] == 0 || v_[2] == 0 || bt->size(0) < v_[0] + v_[1] || !ints(cu_k, v_[1] + 1, *kc))
+      Py_RETURN_NONE;
+    bt_stride = bt->stride(0), blocks = bt->size(1);
+    stream = PyLong_AsVoidPtr(a[9]);
+    if (PyErr_Occurred()) return nullptr;
+    const auto options = kc->options().dtype(at::kBFloat16);
+    k = at::empty({v_[2], pool.kvh, 128}, options);
+    v = at::empty({v_[2], pool.kvh, 128}, options);
+    bt_p = address(bt), cuk_p = address(cu_k), k_p = k.data_ptr(), v_p = v.data_ptr();
+  } catch (const std::exception&) {
+    return declined();
+  }
+  int rc;
+  {
+    Unlocked unlocked;
+    rc = p_gather_fp4(pool.k, pool.v, pool.ks, pool.vs, pool.pages, pool.page, pool.kvh, 128,
+                      static_cast<int32_t*>(bt_p), bt_stride, blocks, v_[0], v_[1],
+                      static_cast<int32_t*>(cuk_p), v_[2], k_p, v_p, stream);
+  }
+  if (rc != KVC_OK) return fail(rc, "kvc_gather_kv_fp4");
+  return pair(std::move(k), std::move(v));
+}
+
+// step_tables(context_lens, query_lens, block_tables, num_blocks, free_blocks,
+//             num_free, page_size, max_tokens, tokens_per_row, finished or None,
+//             pad_slot, stream): the nine tensors of new outputs as a tuple, or None.
+PyObject* step_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 12) {
+    PyErr_SetString(PyExc_TypeError, "step_tables takes 12 arguments");
+    return nullptr;
+  }
+  at::Tensor out[9], ints_;
+  void *p[9], *lens_p, *new_p, *bt_p, *held_p, *free_p, *num_p, *gone_p = nullptr, *stream;
+  int64_t batch, width, bt_stride, free_size, page, tokens, per_row, pad;
+  try {
+    const at::Tensor *lens = tensor(a[0]), *fresh = tensor(a[1]), *bt = tensor(a[2]),
+                     *held = tensor(a[3]), *free_ = tensor(a[4]), *num = tensor(a[5]);
+    if (bt == nullptr || !bt->defined() || !plain(bt, at::kInt, 2, *bt)) Py_RETURN_NONE;
+    batch = bt->size(0), width = bt->size(1), bt_stride = bt->stride(0);
+    int64_t v_[4];
+    PyObject* from[4] = {a[6], a[7], a[8], a[10]};
+    for (int i = 0; i < 4; ++i) {
+      if (!PyLong_CheckExact(from[i])) Py_RETURN_NONE;
+      v_[i] = PyLong_AsLongLong(from[i]);
+      if (v_[i] == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+      }
+    }
+    page = v_[0], tokens = v_[1], per_row = v_[2], pad = v_[3];
+    if (batch == 0 || width == 0 || bt->stride(1) != 1 || (batch > 1 && bt_stride < width) ||
+        !ints(lens, batch, *bt) || !ints(fresh, batch, *bt) || !ints(held, batch, *bt) ||
+        !ints(num, 1, *bt) || free_ == nullptr || !free_->defined() ||
+        !ints(free_, free_->numel(), *bt) || page <= 0 || tokens <= 0 || per_row < 0 ||
+        (per_row > 0 && tokens != batch * per_row) || tokens >= (1 << 24) ||
+        pad < -(int64_t(1) << 31) || pad >= (int64_t(1) << 31))
+      Py_RETURN_NONE;
+    if (a[9] != Py_None) {
+      const at::Tensor* gone = tensor(a[9]);
+      if (gone == nullptr || !gone->defined() || gone->dim() != 1 || gone->numel() != batch ||
+          !gone->is_contiguous() ||
+          !plain(gone, gone->scalar_type() == at::kBool ? at::kBool : at::kByte, 1, *bt))
+        Py_RETURN_NONE;
+      gone_p = address(gone);
+    }
+    stream = PyLong_AsVoidPtr(a[11]);
+    if (PyErr_Occurred()) return nullptr;
+    free_size = free_->numel();
+    // slots, positions, query, seq and context lengths, offsets of both, pages held,
+    // pages free
+    out[0] = at::empty({tokens}, bt->options());
+    out[1] = at::empty({tokens}, bt->options().dtype(at::kLong));
+    const int64_t sizes[7] = {batch, batch, batch, batch + 1, batch + 1, batch, 1};
+    for (int i = 0; i < 7; ++i) out[2 + i] = at::empty({sizes[i]}, bt->options());
+    for (int i = 0; i < 9; ++i) p[i] = out[i].data_ptr();
+    lens_p = address(lens), new_p = address(fresh), bt_p = address(bt), held_p = address(held);
+    free_p = address(free_), num_p = address(num);
+  } catch (const std::exception&) {
+    return declined();
+  }
+  int rc;
+  {
+    Unlocked unlocked;
+    auto i32 = [](void* x) { return static_cast<int32_t*>(x); };
+    rc = p_step_tables(i32(lens_p), i32(new_p), static_cast<uint8_t*>(gone_p), i32(bt_p),
+                       bt_stride, width, batch, i32(held_p), i32(free_p), free_size, i32(num_p),
+                       page, tokens, per_row, int32_t(pad), i32(p[0]),
+                       static_cast<int64_t*>(p[1]), i32(p[2]), i32(p[3]), i32(p[4]), i32(p[7]),
+                       i32(p[8]), i32(p[5]), i32(p[6]), stream);
+  }
+  if (rc != KVC_OK) return fail(rc, "kvc_step_tables");
+  PyObject* r = PyTuple_New(9);
+  if (r == nullptr) return nullptr;
+  for (int i = 0; i < 9; ++i) {
+    PyObject* t = wrap(std::move(out[i]));
+    if (t == nullptr) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i, t);
+  }
+  return r;
+}
+
 template <typename F>
 bool resolve(void* lib, const char* name, F& fn) {
   fn = reinterpret_cast<F>(dlsym(lib, name));
@@ -681,7 +1010,13 @@ PyObject* bind(PyObject*, PyObject* path) {
       !resolve(lib, "kvc_tree_workspace_bytes", p_tree_workspace) ||
       !resolve(lib, "kvc_tree_attention", p_tree) ||
       !resolve(lib, "kvc_qk_norm_mrope_store", p_mrope) ||
-      !resolve(lib, "kvc_commit_rows", p_commit))
+      !resolve(lib, "kvc_commit_rows", p_commit) ||
+      !resolve(lib, "kvc_store_fp4", p_store_fp4) ||
+      !resolve(lib, "kvc_gather_kv_fp4", p_gather_fp4) ||
+      !resolve(lib, "kvc_varlen_fp4_workspace_bytes", p_varlen_fp4_workspace) ||
+      !resolve(lib, "kvc_varlen_fp4_blocks", p_varlen_fp4_blocks) ||
+      !resolve(lib, "kvc_varlen_fp4", p_varlen_fp4) ||
+      !resolve(lib, "kvc_step_tables", p_step_tables))
     return nullptr;
   Py_RETURN_NONE;
 }
@@ -700,6 +1035,14 @@ PyMethodDef methods[] = {
      "the fused norm, multi-axis rotary and append, or None"},
     {"commit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(commit)), METH_FASTCALL,
      "accepted tree paths moved, or None"},
+    {"fp4_store", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp4_store)),
+     METH_FASTCALL, "the append into a 4-bit pool, or None"},
+    {"fp4_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp4_rows)),
+     METH_FASTCALL, "decode rows and short chunks over a 4-bit pool, or None"},
+    {"fp4_gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp4_gather)),
+     METH_FASTCALL, "a 4-bit pool's rows as bf16, or None"},
+    {"step_tables", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(step_tables)),
+     METH_FASTCALL, "a step's tables, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvc_host", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

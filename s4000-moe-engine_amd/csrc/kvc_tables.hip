@@ -271,9 +271,20 @@ extern "C" int kvc_step_tables(const int32_t* context_lens, const int32_t* query
                   (free_size == 0 || free_blocks != nullptr) &&
                   (max_tokens == 0 || (slot_mapping != nullptr && positions != nullptr)),
               KVC_ERR_VALUE, "step_tables: null pointer");
-  KVC_REQUIRE(query_lens_out != context_lens && seq_lens_out != context_lens &&
-                  seq_lens_out != query_lens && context_lens_out != query_lens,
-              KVC_ERR_VALUE, "step_tables: an output over another input");
+  // An output may be the input of its own name, and nothing else of the call's.
+  const void* ins[] = {query_lens, context_lens, num_blocks, num_free, block_tables, free_blocks,
+                       finished};
+  const void* outs[] = {query_lens_out, context_lens_out, num_blocks_out, num_free_out,
+                        seq_lens_out,   cu_seqlens_q,     cu_seqlens_k,   slot_mapping,
+                        positions};
+  for (int i = 0; i < 9 && batch > 0; ++i) {
+    for (int j = 0; j < 7; ++j)
+      KVC_REQUIRE(outs[i] == nullptr || outs[i] != ins[j] || (i == j && i < 4), KVC_ERR_VALUE,
+                  "step_tables: an output over another input");
+    for (int j = 0; j < i; ++j)
+      KVC_REQUIRE(outs[i] == nullptr || outs[i] != outs[j], KVC_ERR_VALUE,
+                  "step_tables: two outputs in one place");
+  }
   TablesArgs a{};
   a.context_lens = context_lens;
   a.query_lens = query_lens;

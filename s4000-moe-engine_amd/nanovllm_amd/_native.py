@@ -131,10 +131,11 @@ SIGNATURES = {
     "kvc_paged_decode_fp4": (_INT, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P,
                                     _I64, _I64, _P, _I64, _I64, _F32, _P, _I64, _I64, _P, _SZ,
                                     _P]),
-    "kvc_varlen_fp4_workspace_bytes": (_SZ, [_I64] * 7),
+    "kvc_varlen_fp4_workspace_bytes": (_SZ, [_I64] * 8),
+    "kvc_varlen_fp4_blocks": (_I64, [_P, _P] + [_I64] * 6),
     "kvc_varlen_fp4": (_INT, [_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
-                              _P, _I64, _I64, _I64, _P, _I64, _P, _P, _F32, _P, _I64, _I64, _P,
-                              _SZ, _P]),
+                              _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _F32, _P, _I64, _I64,
+                              _P, _SZ, _P]),
     "kvc_step_tables": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I64,
                                _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "kvc_stage_decode": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,
@@ -178,6 +179,10 @@ class _NoHostPath:
     tree = staticmethod(lambda *_: None)
     mrope = staticmethod(lambda *_: None)
     commit = staticmethod(lambda *_: None)
+    fp4_store = staticmethod(lambda *_: None)
+    fp4_rows = staticmethod(lambda *_: None)
+    fp4_gather = staticmethod(lambda *_: None)
+    step_tables = staticmethod(lambda *_: None)
 
 
 _host = None

@@ -31,6 +31,7 @@ from __future__ import annotations
 import torch
 
 from .. import _native as nat
+from ..kernels.kv_fp4 import check_fp4_pool, paged_decode_append_fp4
 from ..kernels.paged_attention import decode_append_into
 from ..kernels.scored import check_scores, scored_attention
 from ..layers.attention import store_kvcache
@@ -73,10 +74,14 @@ class DecodeGraphRunner:
 
     score_shapes: scored_attention's softcap, alibi_slopes and window as a dict,
     for all layers or one per layer (None or an empty dict: plain scores).
-    from_kv_runner takes the bound layers' own unless it is given some."""
+    from_kv_runner takes the bound layers' own unless it is given some.
+
+    k_scales / v_scales: the per-layer scales of pools of 4-bit floats
+    (kernels/kv_fp4.py), whose layers append in a launch of their own."""
 
     def __init__(self, k_caches, v_caches, num_heads: int, max_bs: int, max_blocks_per_seq: int,
-                 scale: float, buckets: list[int] | None = None, fence=None, score_shapes=None):
+                 scale: float, buckets: list[int] | None = None, fence=None, score_shapes=None,
+                 k_scales=None, v_scales=None):
         assert len(k_caches) == len(v_caches) and len(k_caches) > 0
         self.fence = fence
         self.k_caches, self.v_caches = list(k_caches), list(v_caches)
@@ -84,7 +89,15 @@ class DecodeGraphRunner:
         self.num_layers = len(self.k_caches)
         self.page = kc.size(1)
         self.num_kv_heads = kc.size(2)
-        self.head_dim = kc.size(3)
+        self.k_scales = list(k_scales) if k_scales is not None else None
+        self.v_scales = list(v_scales) if v_scales is not None else None
+        fp4 = kc.dtype == torch.uint8
+        if fp4:
+            for args in zip(self.k_caches, self.v_caches, self.k_scales or [None],
+                            self.v_scales or [None]):
+                check_fp4_pool(*args)
+            assert len(self.k_scales) == len(self.v_scales) == self.num_layers
+        self.head_dim = 128 if fp4 else kc.size(3)
         self.num_heads = num_heads
         self.scratch_block_id = kc.size(0) - 1
         self.scratch_slot = self.scratch_block_id * self.page
@@ -92,7 +105,7 @@ class DecodeGraphRunner:
         self.scale = scale
         self.buckets = buckets or default_buckets(max_bs)
         assert max(self.buckets) <= max_bs
-        dev, dt = kc.device, kc.dtype
+        dev, dt = kc.device, torch.bfloat16 if fp4 else kc.dtype
         L, D = self.num_layers, self.head_dim
         self.q = torch.zeros(L, max_bs, num_heads, D, dtype=dt, device=dev)
         self.k = torch.zeros(L, max_bs, self.num_kv_heads, D, dtype=dt, device=dev)
@@ -112,6 +125,8 @@ class DecodeGraphRunner:
         for s in self.score_shapes:
             if not set(s) <= {"softcap", "alibi_slopes", "window"}:
                 raise ValueError(f"a score shape has softcap, alibi_slopes and window (got {set(s)})")
+            if s and fp4:
+                raise ValueError("shaped scores need a bf16 pool")
             if s:
                 check_scores(scale, s.get("softcap"), s.get("alibi_slopes"), s.get("window"),
                              num_heads, dev)
@@ -120,25 +135,35 @@ class DecodeGraphRunner:
     def from_kv_runner(cls, kv_runner, num_heads: int, max_bs: int, max_blocks_per_seq: int,
                        scale: float, buckets: list[int] | None = None,
                        score_shapes=None) -> "DecodeGraphRunner":
-        """A runner over every layer of a KVCacheRunner's bf16 pool, fenced by
+        """A runner over every layer of a KVCacheRunner's bf16 or 4-bit pool, fenced by
         that runner (its asynchronous offload copies, if any, are ordered
         before each capture and replay).  score_shapes: None for what the
         layers bound to that runner shape their scores with (bind them
         first), else as in the constructor ({}: plain scores)."""
         if kv_runner.kv_int8 is not None:
-            raise ValueError("the captured decode step runs on a bf16 pool")
+            raise ValueError("the captured decode step runs on a bf16 or 4-bit pool")
         if score_shapes is None:
             score_shapes = kv_runner.score_shapes()
         k_caches = [kv_runner.kv_cache[0, i] for i in range(kv_runner.num_layers)]
         v_caches = [kv_runner.kv_cache[1, i] for i in range(kv_runner.num_layers)]
+        scales = {}
+        if kv_runner.kv_fp4:
+            scales = {name: [kv_runner.kv_scales[side, i] for i in range(kv_runner.num_layers)]
+                      for side, name in enumerate(("k_scales", "v_scales"))}
         return cls(k_caches, v_caches, num_heads, max_bs, max_blocks_per_seq, scale, buckets,
-                   fence=kv_runner.fence, score_shapes=score_shapes)
+                   fence=kv_runner.fence, score_shapes=score_shapes, **scales)
 
     def _step(self, bs: int) -> None:
         sm, cl, bt = self.slot_mapping[:bs], self.context_lens[:bs], self.block_tables[:bs]
         for layer in range(self.num_layers):
             kc, vc = self.k_caches[layer], self.v_caches[layer]
             shape = self.score_shapes[layer]
+            if self.k_scales is not None:
+                paged_decode_append_fp4(
+                    self.q[layer, :bs], self.k[layer, :bs], self.v[layer, :bs], kc, vc,
+                    self.k_scales[layer], self.v_scales[layer], sm, bt, cl, self.scale,
+                    out=self.out[layer, :bs])
+                continue
             if shape:
                 store_kvcache(self.k[layer, :bs], self.v[layer, :bs], kc, vc, sm)
                 scored_attention(self.q[layer, :bs], kc, vc, scale=self.scale, block_tables=bt,

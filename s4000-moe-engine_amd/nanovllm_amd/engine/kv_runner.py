@@ -24,6 +24,7 @@ import numpy as np
 import torch
 
 from .. import _native as nat
+from ..kernels.kv_fp4 import POWERS, ROW_BYTES
 from ..utils.context import set_context
 
 
@@ -199,28 +200,42 @@ class BlockMover:
 
 class KVCacheRunner:
     """The runner's KV duties for one rank: the pool, its per-layer views, and
-    the offload executor protocol the BlockManager drives through call()."""
+    the offload executor protocol the BlockManager drives through call().
+    kv_fp4: a pool of 4-bit floats (kernels/kv_fp4.py), 3.8 times as many tokens
+    in the same memory."""
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int,
                  head_dim: int, dtype=torch.bfloat16, device="cuda", kv_int8: str | None = None,
                  kv_offload_host_blocks: int = 0, n_out_max: int = 8,
-                 async_offload_groups: int = 0, async_copy_engine: str = "kernel"):
+                 async_offload_groups: int = 0, async_copy_engine: str = "kernel",
+                 kv_fp4: bool = False):
+        if kv_fp4 and (kv_int8 is not None or head_dim != 128):
+            raise ValueError("kv_fp4 is for head_dim 128 and excludes kv_int8")
         if kv_offload_host_blocks:
             # nanovllm/config.py:75-78: a block's int8 codes would travel
             # without their scales and side pool
-            assert kv_int8 is None, (
+            assert kv_int8 is None and not kv_fp4, (
                 "KV offload requires the bf16 KV cache (int8 carries side-channel scales)")
             assert kv_offload_host_blocks >= 0
         self.block_size = block_size
         self.num_layers = num_layers
         self.num_kvcache_blocks = num_blocks
         self.kv_int8 = kv_int8
+        self.kv_fp4 = bool(kv_fp4)
         # one extra block the BlockManager never sees (graph-padding scratch)
         shape = (2, num_layers, num_blocks + 1, block_size, num_kv_heads, head_dim)
-        self.kv_cache = torch.empty(shape, dtype=torch.int8 if kv_int8 else dtype, device=device)
+        if self.kv_fp4:
+            shape = shape[:5] + (ROW_BYTES,)
+        self.kv_cache = torch.empty(shape, dtype=torch.uint8 if self.kv_fp4 else
+                                    torch.int8 if kv_int8 else dtype, device=device)
         self.kv_scales = self.kv_dscales = self.kv_side = None
         self.kv_out_idx2d = self.kv_head_n_out = None
-        if kv_int8 == "tokhead":
+        if self.kv_fp4:
+            # (every run 0 x 1: what a padded row reads of the scratch block)
+            self.kv_cache.zero_()
+            self.kv_scales = torch.full(shape[:5] + (POWERS,), 127, dtype=torch.uint8,
+                                        device=device)
+        elif kv_int8 == "tokhead":
             self.kv_scales = torch.ones(shape[:5], dtype=torch.float32, device=device)
         elif kv_int8 == "chan":
             self.kv_scales = torch.ones(2, num_layers, num_kv_heads, head_dim,
@@ -237,6 +252,7 @@ class KVCacheRunner:
         self.scratch_block_id = num_blocks
         self.scratch_slot = num_blocks * block_size
         self.mover = BlockMover(self.kv_cache)
+        self._scale_mover = BlockMover(self.kv_scales) if self.kv_fp4 else None
         self.kv_offload_host_blocks = kv_offload_host_blocks
         self.kv_offloader = None
         # async_offload_groups > 0: offload moves run on copy streams
@@ -260,7 +276,7 @@ class KVCacheRunner:
             self._layers.append(m)
             m.k_cache = self.kv_cache[0, layer]
             m.v_cache = self.kv_cache[1, layer]
-            if self.kv_int8 == "tokhead":
+            if self.kv_int8 == "tokhead" or self.kv_fp4:
                 m.k_scale = self.kv_scales[0, layer]
                 m.v_scale = self.kv_scales[1, layer]
             elif self.kv_int8 == "chan":
@@ -394,14 +410,16 @@ class KVCacheRunner:
     def compact(self, src_ids, dst_ids) -> None:
         self.fence()
         self.mover.copy(src_ids, dst_ids)
+        if self._scale_mover is not None:
+            self._scale_mover.copy(src_ids, dst_ids)
 
     def commit_tree(self, block_tables, context_lens, paths, path_lens) -> None:
-        """commit_tree_path on the pool and, for an int8 pool, on what travels
-        with its rows (per-token-head scales, side rows)."""
+        """commit_tree_path on the pool and, for an int8 or 4-bit pool, on what
+        travels with its rows (scales, side rows)."""
         from ..kernels.tree import commit_tree_path
         self.fence()
         rows = [self.kv_cache, self.kv_side]
-        if self.kv_int8 == "tokhead":
+        if self.kv_int8 == "tokhead" or self.kv_fp4:
             rows.append(self.kv_scales)
         for pool in rows:
             if pool is not None:
@@ -433,6 +451,30 @@ class KVCacheRunner:
                     context_lens=self._h2d(lens, torch.int32),
                     block_tables=self.prepare_block_tables(seqs), max_context_len=max(lens))
         return self._h2d(input_ids, torch.int64), self._h2d(positions, torch.int64)
+
+    def device_tables(self, max_rows: int, max_blocks_per_seq: int, blocks=None):
+        """DeviceBlockTables over this pool's blocks (all of them, or the given
+        ids; a BlockManager must not hand out the same ones), padded tokens
+        appended at the scratch slot."""
+        from .device_tables import DeviceBlockTables
+        return DeviceBlockTables(max_rows, max_blocks_per_seq, self.block_size,
+                                 self.num_kvcache_blocks if blocks is None else blocks,
+                                 self.device, self.scratch_slot)
+
+    def prepare_decode_device(self, tables, query_lens=None, finished=None, out=None):
+        """prepare_decode from lengths that live on the device: one token for every
+        row of `tables` (DeviceBlockTables; query_lens 0 where there is none), its
+        page taken there, with no host read.  Sets the Context and returns the
+        StepTables (positions among them); a row that waits for a page attends
+        nothing and appends at the scratch slot."""
+        if query_lens is None:
+            query_lens = torch.ones(tables.max_rows, dtype=torch.int32, device=tables.device)
+        step = tables.step(query_lens, tables.max_rows, tokens_per_row=1, finished=finished,
+                           out=out)
+        set_context(False, slot_mapping=step.slot_mapping, context_lens=step.seq_lens,
+                    block_tables=tables.block_tables,
+                    max_context_len=tables.block_tables.size(1) * self.block_size)
+        return step
 
     def prepare_prefill(self, seqs):
         return self._prepare_rows(seqs, mixed=False)

@@ -51,6 +51,9 @@ def store_kvcache_fp4(key, value, k_cache, v_cache, k_scale, v_scale, slot_mappi
     """store_kvcache into a 4-bit pool: key / value [N, KVH, 128] bf16 rows
     quantised at slot_mapping (int32 or int64 [N]; a negative slot counts from
     the pool's end, one outside the pool is skipped).  One launch, capturable."""
+    if nat.is_current(key) and nat.host().fp4_store(key, value, k_cache, v_cache, k_scale,
+                                                    v_scale, slot_mapping, nat.stream_of(key)):
+        return
     check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
     if key.ndim != 3 or value.shape != key.shape or key.shape[1:] != (k_cache.size(2), 128):
         raise ValueError("expected key/value=[tokens,kv_heads,128]")
@@ -88,6 +91,12 @@ def dequant_fp4(codes, scale):
 def gather_kv_fp4(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_k, total, row0,
                   num_prefill):
     """gather_kv's launch over a 4-bit pool (arguments as gather_kv made them)."""
+    if nat.is_current(k_cache):
+        done = nat.host().fp4_gather(k_cache, v_cache, k_scale, v_scale, block_tables,
+                                     cu_seqlens_k, row0, num_prefill, total,
+                                     nat.stream_of(k_cache))
+        if done is not None:
+            return done
     check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
     _one_device(k_cache, block_tables=block_tables, cu_seqlens_k=cu_seqlens_k)
     if block_tables.size(0) < row0 + num_prefill:
@@ -115,6 +124,12 @@ def paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, contex
                      out=None):
     """paged_decode_attention over a 4-bit pool, written to `out` if given.  A
     row with context_lens[b] <= 0 gives zeros."""
+    if nat.is_current(q):
+        done = nat.host().fp4_rows(out, q, k_cache, v_cache, k_scale, v_scale, block_tables,
+                                   q.size(0) if q.ndim else 0, context_lens, None, None, None,
+                                   None, scale, nat.stream_of(q), None, None, None)
+        if done is not None:
+            return done
     check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
     if q.ndim != 3:
         raise ValueError("expected q=[batch,heads,dim], kv=[pages,page,kv_heads,64]")
@@ -164,7 +179,7 @@ def paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, contex
 
 
 def varlen_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, num_decode_rows,
-               decode_context_lens, cu_seqlens_q, cu_seqlens_k, scale, out):
+               decode_context_lens, chunk_blocks, cu_seqlens_q, cu_seqlens_k, scale, out):
     """varlen_attention's rows over a 4-bit pool read as it is
     (kvc_varlen_fp4), into out; arguments as varlen_attention checked and
     converted them, int32 offsets on q's device."""
@@ -182,14 +197,14 @@ def varlen_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, num_decode_r
     tokens, num_heads, _ = q.shape
     page_size, kvh, max_blocks = k_cache.size(1), k_cache.size(2), block_tables.size(1)
     need = nat.query("kvc_varlen_fp4_workspace_bytes", tokens, num_heads, kvh, page_size,
-                     max_blocks, num_decode_rows, num_prefill)
+                     max_blocks, num_decode_rows, num_prefill, chunk_blocks)
     ws = nat.workspace(need, q.device)
     nat.call_on(
         k_cache, "kvc_varlen_fp4", q.data_ptr(), q.stride(0), q.stride(1), tokens, num_heads,
         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
         k_cache.size(0), page_size, kvh, 128, block_tables.data_ptr(), block_tables.stride(0),
         max_blocks, num_decode_rows,
-        decode_context_lens.data_ptr() if num_decode_rows else None, num_prefill,
+        decode_context_lens.data_ptr() if num_decode_rows else None, num_prefill, chunk_blocks,
         cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), float(scale), out.data_ptr(),
         out.stride(0), out.stride(1), nat.ptr(ws), need, nat.stream_of(q))
     return out
@@ -199,6 +214,12 @@ def paged_decode_append_fp4(q, key, value, k_cache, v_cache, k_scale, v_scale, s
                             block_tables, context_lens, scale, out=None):
     """The decode step over a 4-bit pool: store_kvcache_fp4 of the new tokens,
     then paged_decode_fp4 over context_lens (which count them)."""
+    if nat.is_current(q):
+        done = nat.host().fp4_rows(out, q, k_cache, v_cache, k_scale, v_scale, block_tables,
+                                   q.size(0) if q.ndim else 0, context_lens, None, None, None,
+                                   None, scale, nat.stream_of(q), key, value, slot_mapping)
+        if done is not None:
+            return done
     store_kvcache_fp4(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
     return paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
                             scale, out)

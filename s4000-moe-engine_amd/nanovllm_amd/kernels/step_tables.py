@@ -72,6 +72,13 @@ def build_step_tables(context_lens, query_lens, block_tables, num_blocks, free_b
     tokens_per_row); entries without a token hold pad_slot and position 0.  out:
     a StepTables to write; its num_blocks, num_free, context_lens and query_lens
     may be the given ones."""
+    if out is None and nat.is_current(block_tables):
+        done = nat.host().step_tables(context_lens, query_lens, block_tables, num_blocks,
+                                      free_blocks, num_free, page_size, max_tokens,
+                                      tokens_per_row, finished, pad_slot,
+                                      nat.stream_of(block_tables))
+        if done is not None:
+            return StepTables(*done)
     if block_tables.ndim != 2 or block_tables.dtype != torch.int32 \
             or (block_tables.size(1) > 1 and block_tables.stride(1) != 1):
         raise ValueError("block_tables must be int32 [batch, pages] with dense rows")
@@ -97,10 +104,7 @@ def build_step_tables(context_lens, query_lens, block_tables, num_blocks, free_b
                                  or finished.numel() != batch or not finished.is_contiguous()
                                  or finished.device != dev):
         raise ValueError(f"finished must be bool [{batch}] on the tables' device")
-    nat.require_device(block_tables)
-    if out is None:
-        out = new_step_tables(batch, max_tokens, dev)
-    else:
+    if out is not None:
         if out.positions.dtype != torch.int64 or out.positions.numel() != max_tokens \
                 or not out.positions.is_contiguous() or out.positions.device != dev:
             raise ValueError(f"out.positions must be int64 [{max_tokens}]")
@@ -108,6 +112,9 @@ def build_step_tables(context_lens, query_lens, block_tables, num_blocks, free_b
                         ("context_lens", batch), ("cu_seqlens_q", batch + 1),
                         ("cu_seqlens_k", batch + 1), ("num_blocks", batch), ("num_free", 1)):
             _vector(getattr(out, name), n, f"out.{name}", dev)
+    nat.require_device(block_tables)
+    if out is None:
+        out = new_step_tables(batch, max_tokens, dev)
     nat.call_on(
         block_tables, "kvc_step_tables", context_lens.data_ptr(), query_lens.data_ptr(),
         nat.ptr(finished), block_tables.data_ptr(), block_tables.stride(0), width, batch,

@@ -95,6 +95,7 @@ def _prepare(q, k_cache, v_cache, block_tables, num_decode_rows, decode_context_
     c.cu_k_list = cu_k
     cu_q_np = np.asarray(cu_q, dtype=np.int32)
     cu_k_np = np.asarray(cu_k, dtype=np.int32)
+    c.cu_q_np, c.cu_k_np = cu_q_np, cu_k_np
     c.pre_units = nat.query("kvc_varlen_prefill_units", cu_q_np.ctypes.data, cu_k_np.ctypes.data,
                             c.num_prefill, num_heads, c.num_kv_heads, c.max_seqlen_k)
     if c.num_prefill:
@@ -222,10 +223,6 @@ def _paged_rows(c, q, nd, k_cache, v_cache, scale, k_scale, v_scale, side_k, sid
     )
 
 
-def _read_in_place(c) -> bool:
-    return False
-
-
 def varlen_attention(q, k_cache, v_cache, *, scale, block_tables=None,
                      num_decode_rows=0, decode_context_lens=None,
                      cu_seqlens_q=None, cu_seqlens_k=None,
@@ -242,6 +239,13 @@ def varlen_attention(q, k_cache, v_cache, *, scale, block_tables=None,
     (optional; with them a mixed call over a bf16 pool sizes its CU split to
     the work of both sides).
     Returns out [T, H, D] bf16."""
+    if block_tables is not None and k_cache.dtype == torch.uint8 and nat.is_current(q):
+        done = nat.host().fp4_rows(None, q, k_cache, v_cache, k_scale, v_scale, block_tables,
+                                   num_decode_rows, decode_context_lens, cu_seqlens_q,
+                                   cu_seqlens_k, cu_seqlens_q_list, cu_seqlens_k_list, scale,
+                                   nat.stream_of(q), None, None, None)
+        if done is not None:
+            return done
     c = _prepare(q, k_cache, v_cache, block_tables, num_decode_rows, decode_context_lens,
                  decode_context_lens_list, cu_seqlens_q, cu_seqlens_k, cu_seqlens_q_list,
                  cu_seqlens_k_list, k, v, k_scale)
@@ -250,9 +254,13 @@ def varlen_attention(q, k_cache, v_cache, *, scale, block_tables=None,
     enc, fresh, q = c.enc, c.fresh, c.q
     if enc == nat.KVC_KV_FP4:
         check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
-        if c.num_prefill and _read_in_place(c):
+        # Chunks of few tokens read the pool as it is, with the decode rows.
+        blocks = nat.query("kvc_varlen_fp4_blocks", c.cu_q_np.ctypes.data, c.cu_k_np.ctypes.data,
+                           c.num_prefill, c.num_heads, c.num_kv_heads, c.page_size, c.max_blocks,
+                           num_decode_rows)
+        if blocks:
             return varlen_fp4(q, k_cache, v_cache, k_scale, v_scale, c.block_tables,
-                              num_decode_rows, c.decode_context_lens, c.cu_seqlens_q,
+                              num_decode_rows, c.decode_context_lens, blocks, c.cu_seqlens_q,
                               c.cu_seqlens_k, scale, c.out)
     gathered = (enc != nat.KVC_KV_BF16 and not fresh and c.num_prefill
                 and (enc == nat.KVC_KV_FP4 or os.environ.get("KVC_PREFILL_SK", "1") != "0"))

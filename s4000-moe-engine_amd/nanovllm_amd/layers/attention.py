@@ -15,6 +15,9 @@ change.  What changes is underneath:
 * prefill and mixed batches are ONE varlen launch instead of a Python loop
   over sequences plus torch.cat (attention.py:146-166, :179-213).
 
+A pool of 4-bit floats (uint8 k_cache with its k_scale / v_scale) appends in a
+launch of its own and is read by the same calls.
+
 A layer whose scores are shaped (softcap, alibi_slopes, window) or a step with
 a two-way prefix or drafted trees (Context.prefix_lens, Context.tree_mask)
 appends, then attends through scored_attention / tree_attention.
@@ -27,6 +30,7 @@ import torch
 from torch import nn
 
 from .. import _native as nat
+from ..kernels.kv_fp4 import paged_decode_append_fp4, store_kvcache_fp4
 from ..kernels.kv_int8 import store_kvcache_int8
 from ..kernels.paged_attention import (paged_decode_append, paged_decode_append_int8_chan,
                                        paged_decode_append_int8_tokhead,
@@ -89,7 +93,7 @@ class Attention(nn.Module):
         self.window = window
         self.block_size = None
         self.k_cache = self.v_cache = torch.tensor([])
-        self.k_scale = self.v_scale = None      # int8 store scales
+        self.k_scale = self.v_scale = None      # int8 store scales, 4-bit runs' powers
         self.k_dscale = self.v_dscale = None    # int8 per-channel read scales
         self.side_k = self.side_v = None        # bf16 outlier side pools
         self.out_idx2d = None
@@ -121,6 +125,10 @@ class Attention(nn.Module):
             return nullcontext()
         return self.profiler.range(name, layer=self.layer_id)
 
+    def _fp4(self) -> bool:
+        """The bound pool is one of 4-bit floats."""
+        return self.k_cache.dtype == torch.uint8
+
     def _int8_tokhead(self) -> bool:
         return self.kv_cache_is_int8 and self.k_scale is not None and self.k_scale.dim() == 3
 
@@ -134,6 +142,8 @@ class Attention(nn.Module):
     def _read_scales(self):
         """Scales the read path needs: per-slot scales (per-token-head) or the
         per-channel read scales (0 at outlier dims)."""
+        if self._fp4():
+            return self.k_scale, self.v_scale
         if not self.kv_cache_is_int8:
             return None, None
         if self._int8_tokhead():
@@ -158,7 +168,8 @@ class Attention(nn.Module):
         k3 = k.view(N, self.num_kv_heads, self.head_dim)
         v3 = v.view(N, self.num_kv_heads, self.head_dim)
         k_cache, v_cache = self.k_cache, self.v_cache
-        bf16_pool = bool(k_cache.numel() and v_cache.numel()) and not self.kv_cache_is_int8
+        bf16_pool = (bool(k_cache.numel() and v_cache.numel()) and not self.kv_cache_is_int8
+                     and not self._fp4())
         need_k = not bf16_pool or context.block_tables is None
         with self._profile("attention.qk_norm_rope_store"):
             pool = (k_cache, v_cache, context.slot_mapping) if bf16_pool else (None, None, None)
@@ -180,7 +191,7 @@ class Attention(nn.Module):
 
     def _forward_shaped(self, context, q, k, v, kv_stored):
         """The append, then attention with shaped scores or masks."""
-        if self.kv_cache_is_int8:
+        if self.kv_cache_is_int8 or self._fp4():
             raise ValueError("shaped scores, two-way prefixes and drafted trees need a bf16 pool")
         q = q.view(-1, self.num_heads, self.head_dim)
         k = k.view(-1, self.num_kv_heads, self.head_dim)
@@ -236,7 +247,7 @@ class Attention(nn.Module):
         varlen_append = (not kv_stored and (context.is_mixed or context.is_prefill)
                          and context.block_tables is not None
                          and bool(k_cache.numel() and v_cache.numel())
-                         and not self.kv_cache_is_int8)
+                         and not self.kv_cache_is_int8 and not self._fp4())
         if varlen_append:
             with self._profile("attention.mixed" if context.is_mixed else "attention.prefill"):
                 return varlen_attention_append(
@@ -253,7 +264,11 @@ class Attention(nn.Module):
                                               if context.is_mixed else None))
         if k_cache.numel() and v_cache.numel() and not kv_stored and not fuse_append:
             with self._profile("attention.kv_store"):
-                if self.kv_cache_is_int8:
+                if self._fp4():
+                    store_kvcache_fp4(k.view(-1, self.num_kv_heads, self.head_dim),
+                                      v.view(-1, self.num_kv_heads, self.head_dim), k_cache,
+                                      v_cache, self.k_scale, self.v_scale, context.slot_mapping)
+                elif self.kv_cache_is_int8:
                     store_kvcache_int8(k, v, k_cache, v_cache, self.k_scale, self.v_scale,
                                        self.side_k, self.side_v, self.out_idx2d,
                                        self.head_n_out, context.slot_mapping)
@@ -298,6 +313,14 @@ class Attention(nn.Module):
                     k.view(-1, self.num_kv_heads, self.head_dim),
                     v.view(-1, self.num_kv_heads, self.head_dim), k_cache, v_cache,
                     self.k_scale, self.v_scale, context.slot_mapping, context.block_tables,
+                    context.context_lens, self.scale)
+        if fuse_append and self._fp4():
+            with self._profile("attention.paged_decode"):
+                return paged_decode_append_fp4(
+                    q.view(-1, self.num_heads, self.head_dim),
+                    k.view(-1, self.num_kv_heads, self.head_dim),
+                    v.view(-1, self.num_kv_heads, self.head_dim), k_cache, v_cache, self.k_scale,
+                    self.v_scale, context.slot_mapping, context.block_tables,
                     context.context_lens, self.scale)
         if fuse_append:
             with self._profile("attention.paged_decode"):

@@ -1,0 +1,264 @@
+"""The 4-bit pool under the layer, the runner and the captured step, and with the
+device-built tables: the parts run together, as a serving loop uses them."""
+import pytest
+import torch
+
+from nanovllm_amd.engine.graph_runner import DecodeGraphRunner
+from nanovllm_amd.engine.kv_runner import KVCacheRunner
+from nanovllm_amd.engine.sequence import Sequence
+from nanovllm_amd.kernels.kv_fp4 import dequant_fp4, paged_decode_append_fp4
+from nanovllm_amd.layers.attention import Attention
+from nanovllm_amd.layers.rotary import build_cos_sin_cache
+from nanovllm_amd.utils.context import get_context, reset_context, set_context
+from tests import fp4_oracle as fo
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+SCALE = 128 ** -0.5
+HEADS, KVH, PAGE = 8, 2, 32
+
+
+@pytest.fixture(autouse=True)
+def _context(monkeypatch):
+    monkeypatch.setattr(Sequence, "block_size", PAGE)
+    yield
+    reset_context()
+
+
+def _runner(layers=1, blocks=24):
+    runner = KVCacheRunner(layers, blocks, PAGE, KVH, 128, kv_fp4=True)
+    modules = [Attention(HEADS, 128, SCALE, KVH) for _ in range(layers)]
+    assert runner.bind(modules) == layers
+    return runner, modules
+
+
+def _rows(gen, n):
+    q = torch.randn(n, HEADS, 128, generator=gen).to(BF)
+    k, v = (torch.randn(n, KVH, 128, generator=gen).to(BF) for _ in range(2))
+    return q, k, v
+
+
+def _stored(x):
+    return fo.values(*fo.encode(x))
+
+
+def test_pool_of_the_runner():
+    runner, (layer,) = _runner()
+    assert runner.kv_cache.shape == (2, 1, 25, PAGE, KVH, 64)
+    assert runner.kv_cache.dtype == torch.uint8 and runner.kv_scales.shape[-1] == 4
+    assert layer.k_cache.data_ptr() == runner.kv_cache[0, 0].data_ptr()
+    assert layer.v_scale.data_ptr() == runner.kv_scales[1, 0].data_ptr()
+    assert not layer.kv_cache_is_int8
+    bf16 = KVCacheRunner(1, 24, PAGE, KVH, 128)
+    per_token = 2 * KVH * 128 * 2 / (2 * KVH * (64 + 4))
+    assert bf16.kv_cache.nbytes / (runner.kv_cache.nbytes + runner.kv_scales.nbytes) == per_token
+
+
+def _seq(ids, blocks, cached, new, prefill):
+    s = Sequence(list(ids))
+    s.block_table = list(blocks)
+    s.num_cached_tokens = cached
+    s.num_scheduled_tokens = new
+    s.is_prefill = prefill
+    return s
+
+
+def test_prefill_decode_and_mixed_steps():
+    """Through the runner's own producers: a prompt without a cache (attends its fresh
+    keys), a chunk behind it, a decode step and a mixed step."""
+    runner, (layer,) = _runner()
+    gen = torch.Generator().manual_seed(1)
+    hist = {}
+
+    def run(seqs, spans, mixed=None):
+        n = sum(b - a for _, a, b in spans)
+        q, k, v = _rows(gen, n)
+        at = 0
+        for name, a, b in spans:
+            old = hist.get(name, (torch.zeros(0, KVH, 128, dtype=torch.float64),) * 2)
+            assert old[0].size(0) == a
+            hist[name] = tuple(torch.cat((o, _stored(x[at:at + b - a])))
+                               for o, x in zip(old, (k, v)))
+            at += b - a
+        got = layer(q.cuda().flatten(1), k.cuda().flatten(1), v.cuda().flatten(1))
+        return q, k, v, got.view(n, HEADS, 128)
+
+    a = _seq(range(40), [3, 7], 0, 40, True)
+    runner.prepare_prefill([a])
+    q, k, v, got = run([a], [("a", 0, 40)])
+    want, bound = fo.attend(q, k.double(), v.double(), fo.causal(40, 40), SCALE)
+    fo.check(got, want, bound, "fresh prompt")
+
+    a = _seq(range(75), [3, 7, 1], 40, 35, True)
+    runner.prepare_prefill([a])
+    assert get_context().block_tables is not None
+    q, k, v, got = run([a], [("a", 40, 75)])
+    want, bound = fo.attend(q, *hist["a"], fo.causal(35, 75), SCALE)
+    fo.check(got, want, bound, "chunk behind a prefix")
+
+    a = _seq(range(76), [3, 7, 1], 75, 1, False)
+    runner.prepare_decode([a])
+    q, k, v, got = run([a], [("a", 75, 76)])
+    want, bound = fo.attend(q, *hist["a"], fo.causal(1, 76), SCALE)
+    fo.check(got, want, bound, "decode")
+
+    a = _seq(range(77), [3, 7, 1], 76, 1, False)
+    b = _seq(range(50), [5, 9], 0, 50, True)
+    runner.prepare_mixed([a, b])
+    q, k, v, got = run([a, b], [("a", 76, 77), ("b", 0, 50)])
+    for rows, name, n, m in ((slice(0, 1), "a", 1, 77), (slice(1, 51), "b", 50, 50)):
+        want, bound = fo.attend(q[rows], *hist[name], fo.causal(n, m), SCALE)
+        fo.check(got[rows], want, bound, f"mixed, {name}")
+
+
+def test_forward_fused_equals_its_parts():
+    """The rotation runs alone and the quantising append follows, as on an int8 pool."""
+    gen = torch.Generator().manual_seed(2)
+    n = 5
+    qkv = torch.randn(n, (HEADS + 2 * KVH) * 128, generator=gen).to(BF).cuda()
+    q, k, v = qkv.split((HEADS * 128, KVH * 128, KVH * 128), dim=-1)
+    cos_sin = build_cos_sin_cache(128, 64, 1e6, "cuda")
+    w = [(1 + 0.1 * torch.randn(128, generator=gen)).to(BF).cuda() for _ in range(2)]
+    positions = torch.tensor([3, 9, 0, 31, 40]).cuda()
+    tables = torch.arange(10, dtype=torch.int32).view(5, 2).cuda()
+    lens = (positions + 1).to(torch.int32)
+    slots = (tables.gather(1, (positions // PAGE)[:, None]).squeeze(1) * PAGE + positions % PAGE)
+    outs = []
+    for fused in (True, False):
+        runner, (layer,) = _runner()
+        set_context(False, slot_mapping=slots.to(torch.int32), context_lens=lens,
+                    block_tables=tables)
+        if fused:
+            out = layer.forward_fused(positions, q, k, v, cos_sin, *w, 1e-6)
+        else:
+            from nanovllm_amd.layers.rotary import qk_norm_rope_store
+            qr, kr = qk_norm_rope_store(q.view(n, HEADS, 128), k.view(n, KVH, 128), None,
+                                        positions, cos_sin, *w, 1e-6)
+            out = layer(qr, kr, v.view(n, KVH, 128))
+        outs.append((out, runner.kv_cache.clone(), runner.kv_scales.clone()))
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+
+
+def test_moves_take_codes_and_powers():
+    """compact and commit_tree on a 4-bit pool."""
+    runner, _ = _runner(layers=2, blocks=6)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for t in (runner.kv_cache, runner.kv_scales):
+        t.copy_(torch.randint(0, 255, t.shape, generator=gen, device="cuda", dtype=torch.uint8))
+    before = [t.clone() for t in (runner.kv_cache, runner.kv_scales)]
+    runner.compact([4, 5], [0, 1])
+    for t, b in zip((runner.kv_cache, runner.kv_scales), before):
+        b[:, :, [0, 1]] = b[:, :, [4, 5]]
+        assert torch.equal(t, b)
+    tables = torch.tensor([[2, 3]], dtype=torch.int32, device="cuda")
+    runner.commit_tree(tables, torch.tensor([30], dtype=torch.int32, device="cuda"),
+                       torch.tensor([[0, 2, 5]], dtype=torch.int32, device="cuda"),
+                       torch.tensor([3], dtype=torch.int32, device="cuda"))
+    for t, b in zip((runner.kv_cache, runner.kv_scales), before):
+        rows = b[:, :, [2, 3]].flatten(2, 3)
+        rows[:, :, 30:33] = rows[:, :, [30, 32, 35]]
+        b[:, :, [2, 3]] = rows.view(b[:, :, [2, 3]].shape)
+        assert torch.equal(t, b)
+
+
+@pytest.mark.parametrize("layers,max_bs", [(1, 5), (2, 3)])
+def test_captured_decode_step(layers, max_bs):
+    """DecodeGraphRunner over a 4-bit pool equals the eager calls, outputs and pool
+    bytes, over steps of different batches."""
+    runner, _ = _runner(layers=layers, blocks=20)
+    runner.kv_scales[:, :, :20] = 255            # nothing unwritten may be read
+    eager = KVCacheRunner(layers, 20, PAGE, KVH, 128, kv_fp4=True)
+    eager.kv_cache.copy_(runner.kv_cache), eager.kv_scales.copy_(runner.kv_scales)
+    graphs = DecodeGraphRunner.from_kv_runner(runner, HEADS, max_bs, 3, SCALE, [max_bs - 2, max_bs])
+    graphs.capture()
+    gen = torch.Generator().manual_seed(4)
+    tables = torch.randperm(18, generator=gen)[:max_bs * 3].view(max_bs, 3).to(torch.int32).cuda()
+    lens = [0] * max_bs
+    for step in range(40):
+        bs = max_bs - step % 2 * (max_bs > 1)
+        pos = lens[:bs]
+        for b in range(bs):
+            lens[b] += 1
+        q = torch.randn(layers, bs, HEADS, 128, generator=gen).to(BF).cuda()
+        k, v = (torch.randn(layers, bs, KVH, 128, generator=gen).to(BF).cuda() for _ in range(2))
+        slots = torch.tensor([int(tables[b, p // PAGE]) * PAGE + p % PAGE
+                              for b, p in enumerate(pos)], dtype=torch.int32).cuda()
+        cl = torch.tensor(lens[:bs], dtype=torch.int32).cuda()
+        got = graphs.run(q, k, v, slots, cl, tables[:bs])
+        for i in range(layers):
+            want = paged_decode_append_fp4(
+                q[i], k[i], v[i], eager.kv_cache[0, i], eager.kv_cache[1, i],
+                eager.kv_scales[0, i], eager.kv_scales[1, i], slots, tables[:bs], cl, SCALE)
+            assert torch.equal(got[i], want), (step, i)
+    torch.cuda.synchronize()
+    assert torch.equal(runner.kv_cache[:, :, :20], eager.kv_cache[:, :, :20])
+    assert torch.equal(runner.kv_scales[:, :, :20], eager.kv_scales[:, :, :20])
+
+
+@pytest.mark.parametrize("capture", [False, True])
+def test_serving_loop_without_the_host(capture):
+    """Tables, append and attention of a decode loop whose lengths live on the device,
+    eager and as one graph that is replayed; a request ends, another takes its row, and
+    with the pool full a row waits."""
+    rows = 3
+    runner, (layer,) = _runner(blocks=4)
+    tables = runner.device_tables(rows, 3)
+    gen = torch.Generator().manual_seed(5)
+    q = torch.zeros(rows, HEADS, 128, dtype=BF, device="cuda")
+    k, v = (torch.zeros(rows, KVH, 128, dtype=BF, device="cuda") for _ in range(2))
+    new = torch.ones(rows, dtype=torch.int32, device="cuda")
+    finished = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    out = tables.outputs(rows)
+    result = torch.zeros_like(q)
+
+    def step():
+        runner.prepare_decode_device(tables, new, finished, out)
+        result.copy_(layer(q, k, v).view(rows, HEADS, 128))
+
+    graph = None
+    if capture:
+        state = [tables.context_lens, tables.num_blocks, tables.block_tables, tables.free_blocks,
+                 tables.num_free]
+        saved = [x.clone() for x in state]
+        step()
+        torch.cuda.synchronize()
+        for x, s in zip(state, saved):
+            x.copy_(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+    none = torch.zeros(0, KVH, 128, dtype=torch.float64)
+    hist = [(none, none)] * rows
+    waited = 0
+    for i in range(75):
+        gone = [i == 50 and b == 1 for b in range(rows)]
+        finished.copy_(torch.tensor(gone))
+        nq, nk, nv = _rows(gen, rows)
+        q.copy_(nq), k.copy_(nk), v.copy_(nv)
+        if graph is not None:
+            graph.replay()
+        else:
+            step()
+        torch.cuda.synchronize()
+        granted = out.query_lens.tolist()
+        for b in range(rows):
+            if gone[b]:
+                hist[b] = (none, none)
+            if granted[b]:
+                hist[b] = (torch.cat((hist[b][0], _stored(nk[b:b + 1]))),
+                           torch.cat((hist[b][1], _stored(nv[b:b + 1]))))
+            else:
+                waited += 1
+                assert not result[b].any()
+            assert int(tables.context_lens[b]) == len(hist[b][0])
+            if granted[b] and i % 6 == 0:
+                want, bound = fo.attend(nq[b:b + 1], *hist[b], fo.causal(1, len(hist[b][0])),
+                                        SCALE)
+                fo.check(result[b:b + 1], want, bound, f"step {i}, row {b}")
+    assert waited > 0                              # 4 pages for three rows of 2 and more
+    # what the pool holds of row 0 is what was appended
+    n = len(hist[0][0])
+    pos = torch.arange(n)
+    slot = (tables.block_tables[0].cpu()[pos // PAGE].long() * PAGE + pos % PAGE).cuda()
+    got = dequant_fp4(layer.k_cache.flatten(0, 1)[slot], layer.k_scale.flatten(0, 1)[slot])
+    assert torch.equal(got.cpu(), hist[0][0].to(BF))
