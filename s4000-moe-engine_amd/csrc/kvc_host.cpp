@@ -10,7 +10,9 @@
 // kept between calls.  Measured: one row of 333 tokens through norm, rotary,
 // append and attention (16 q / 8 kv heads) 30 -> 16-18 us a pass, a decode
 // step of 11 rows of 97-1501 tokens 20.0 -> 14.7 us (both now GPU-bound).  The
-// same holds for the shaped-score, tree, multi-axis rotary and commit calls.
+// same holds for the shaped-score, tree, multi-axis rotary and commit calls, for
+// those of a 4-bit pool (an append and a read 11 -> 9.5 us) and for a step's
+// tables (19 -> 6.5).
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -903,6 +905,15 @@ PyObject* fp4_gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return pair(std::move(k), std::move(v));
 }
 
+// `n` elements of `type` at byte `from` of base's storage (a multiple of their size).
+at::Tensor slice(const at::Tensor& base, at::ScalarType type, int64_t from, int64_t n) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+      c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  t.unsafeGetTensorImpl()->set_storage_offset(from / int64_t(c10::elementSize(type)));
+  return t;
+}
+
 // step_tables(context_lens, query_lens, block_tables, num_blocks, free_blocks,
 //             num_free, page_size, max_tokens, tokens_per_row, finished or None,
 //             pad_slot, stream): the nine tensors of new outputs as a tuple, or None.
@@ -911,7 +922,7 @@ PyObject* step_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyErr_SetString(PyExc_TypeError, "step_tables takes 12 arguments");
     return nullptr;
   }
-  at::Tensor out[9], ints_;
+  at::Tensor out[9];
   void *p[9], *lens_p, *new_p, *bt_p, *held_p, *free_p, *num_p, *gone_p = nullptr, *stream;
   int64_t batch, width, bt_stride, free_size, page, tokens, per_row, pad;
   try {
@@ -948,13 +959,20 @@ PyObject* step_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     stream = PyLong_AsVoidPtr(a[11]);
     if (PyErr_Occurred()) return nullptr;
     free_size = free_->numel();
-    // slots, positions, query, seq and context lengths, offsets of both, pages held,
-    // pages free
-    out[0] = at::empty({tokens}, bt->options());
-    out[1] = at::empty({tokens}, bt->options().dtype(at::kLong));
-    const int64_t sizes[7] = {batch, batch, batch, batch + 1, batch + 1, batch, 1};
-    for (int i = 0; i < 7; ++i) out[2 + i] = at::empty({sizes[i]}, bt->options());
-    for (int i = 0; i < 9; ++i) p[i] = out[i].data_ptr();
+    // Slots, positions, query, seq and context lengths, offsets of both, pages held,
+    // pages free: one allocation (nine took half of the call's 10 us).
+    const int64_t sizes[9] = {tokens, tokens, batch, batch, batch, batch + 1, batch + 1, batch, 1};
+    int64_t at_byte[9], all = 0;
+    for (int i = 0; i < 9; ++i) {
+      at_byte[i] = all;
+      all += (sizes[i] * (i == 1 ? 8 : 4) + 63) / 64 * 64;
+    }
+    const at::Tensor base = at::empty({all}, bt->options().dtype(at::kByte));
+    for (int i = 0; i < 9; ++i) {
+      const at::ScalarType type = i == 1 ? at::kLong : at::kInt;
+      out[i] = slice(base, type, at_byte[i], sizes[i]);
+      p[i] = out[i].data_ptr();
+    }
     lens_p = address(lens), new_p = address(fresh), bt_p = address(bt), held_p = address(held);
     free_p = address(free_), num_p = address(num);
   } catch (const std::exception&) {

@@ -88,9 +88,10 @@ def dequant_fp4(codes, scale):
     return out
 
 
-def gather_kv_fp4(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_k, total, row0,
-                  num_prefill):
-    """gather_kv's launch over a 4-bit pool (arguments as gather_kv made them)."""
+def gather_kv_fp4(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_k,
+                  cu_seqlens_k_list, row0=0):
+    """gather_kv over a 4-bit pool."""
+    num_prefill, total = len(cu_seqlens_k_list) - 1, cu_seqlens_k_list[-1]
     if nat.is_current(k_cache):
         done = nat.host().fp4_gather(k_cache, v_cache, k_scale, v_scale, block_tables,
                                      cu_seqlens_k, row0, num_prefill, total,
@@ -101,7 +102,13 @@ def gather_kv_fp4(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_k
     _one_device(k_cache, block_tables=block_tables, cu_seqlens_k=cu_seqlens_k)
     if block_tables.size(0) < row0 + num_prefill:
         raise ValueError("block_tables has fewer rows than the call has sequences")
+    if cu_seqlens_k.numel() < num_prefill + 1:
+        raise ValueError("cu_seqlens_k has fewer entries than its list")
     nat.require_device(k_cache)
+    block_tables = block_tables.to(torch.int32)
+    if block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    cu_seqlens_k = cu_seqlens_k.to(torch.int32).contiguous()
     out_k = torch.empty((total, k_cache.size(2), 128), dtype=torch.bfloat16,
                         device=k_cache.device)
     out_v = torch.empty_like(out_k)

@@ -136,16 +136,12 @@ def gather_kv(k_cache, v_cache, block_tables, cu_seqlens_k, cu_seqlens_k_list, *
     block table row block_table_row0 + i and dequantised as the reference
     does for an int8 pool (or from a 4-bit one), at rows cu_seqlens_k[i] .. of
     the returned bf16 (K, V), each [cu_seqlens_k[-1], KVH, D]."""
+    if k_cache.dtype == torch.uint8:
+        return gather_kv_fp4(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_k,
+                             cu_seqlens_k_list, block_table_row0)
     enc = _kv_encoding(k_cache, k_scale)
     cu_k = list(cu_seqlens_k_list)
     total = cu_k[-1]
-    if enc == nat.KVC_KV_FP4:
-        tables = block_tables.to(torch.int32)
-        if tables.stride(1) != 1:
-            tables = tables.contiguous()
-        return gather_kv_fp4(k_cache, v_cache, k_scale, v_scale, tables,
-                             cu_seqlens_k.to(torch.int32).contiguous(), total, block_table_row0,
-                             len(cu_k) - 1)
     kvh, page = k_cache.size(2), k_cache.size(1)
     out_k = torch.empty((total, kvh, k_cache.size(3)), dtype=torch.bfloat16, device=k_cache.device)
     out_v = torch.empty_like(out_k)

@@ -113,6 +113,30 @@ def test_gather(page, kvh, lens, row0):
         assert torch.equal(g.cpu(), torch.cat(seqs[row0:]).to(BF))
 
 
+def test_gather_index_types_strides_and_both_paths(monkeypatch):
+    lens = [70, 1, 200]
+    pool, tables, k, v = fo.paged([3] + lens, 32, 4, seed=51)
+    cu = [0, 70, 71, 271]
+    scales = dict(zip(("k_scale", "v_scale"), _dev(pool)[2:]))
+    kc, vc = _dev(pool)[:2]
+    wide = torch.full((tables.size(0), 2 * tables.size(1)), -5, dtype=torch.int32)
+    wide[:, ::2] = tables
+    forms = [(tables.cuda(), torch.int32), (tables.cuda().long(), torch.int64),
+             (wide.cuda()[:, ::2], torch.int32)]
+    for path in range(2):
+        for bt, kind in forms:
+            got = gather_kv(kc, vc, bt, torch.tensor(cu, dtype=kind, device="cuda"), cu,
+                            block_table_row0=1, **scales)
+            for g, seqs in zip(got, (k, v)):
+                assert torch.equal(g.cpu(), torch.cat(seqs[1:]).to(BF)), (path, kind)
+        assert gather_kv(kc, vc, forms[0][0], torch.zeros(1, dtype=torch.int32, device="cuda"),
+                         [0], **scales)[0].shape == (0, 4, 128)
+        monkeypatch.setattr(_native, "_host", _native._NoHostPath)
+    with pytest.raises(ValueError, match="cu_seqlens_k"):
+        gather_kv(kc, vc, forms[0][0], torch.zeros(2, dtype=torch.int32, device="cuda"), cu,
+                  **scales)
+
+
 def test_gather_of_bad_pages_is_zero():
     pool, tables, k, _ = fo.paged([96, 40], 32, 2, seed=5)
     tables[0, 1], tables[1, 0] = 1 << 20, -7

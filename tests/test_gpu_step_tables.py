@@ -199,6 +199,32 @@ def test_host_and_python_paths_agree(monkeypatch):
     _compare(*[args[0], [1] * 9, *[args[2], args[1], args[3], args[4]]], 32, 9, 1)
 
 
+@pytest.mark.parametrize("native", [True, False])
+def test_outputs_are_apart(native, monkeypatch):
+    """Fields of one result may share memory with nobody: each is written over and the
+    others keep their values; they outlive the rest of the result."""
+    if not native:
+        monkeypatch.setattr(_native, "_host", _native._NoHostPath)
+    names = ("slot_mapping", "positions", "query_lens", "seq_lens", "context_lens",
+             "cu_seqlens_q", "cu_seqlens_k", "num_blocks", "num_free")
+    for batch, tokens in ((1, 1), (5, 7), (17, 33)):
+        table = torch.full((batch, 2), -1, dtype=torch.int32, device="cuda")
+        zero = torch.zeros(batch, dtype=torch.int32, device="cuda")
+        free = torch.arange(40, dtype=torch.int32, device="cuda")
+        got = build_step_tables(zero, zero + 1, table, zero, free, _i32([40]), 32, tokens)
+        before = {n: getattr(got, n).tolist() for n in names}
+        assert [getattr(got, n).numel() for n in names] == [tokens, tokens, batch, batch, batch,
+                                                            batch + 1, batch + 1, batch, 1]
+        for i, n in enumerate(names):
+            getattr(got, n).fill_(-100 - i)
+            for other in names[i + 1:]:
+                assert getattr(got, other).tolist() == before[other], (n, other)
+        keep = got.num_free
+        del got
+        torch.empty(1 << 16, dtype=torch.int32, device="cuda").fill_(3)
+        assert keep.tolist() == [-108] and keep.dtype == torch.int32
+
+
 def test_empty_shapes():
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
     num = _i32([3])
