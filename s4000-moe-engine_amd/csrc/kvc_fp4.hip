@@ -4,21 +4,24 @@
 // Decode: out[b, h] = sum_j softmax_j(scale q[b, h].k_j) v_j over the row's first
 // context_lens[b] keys, 0 for a row without keys.
 //
-// A wave attends tiles of 64 keys of one kv head, whose G query heads are the
-// columns of S^T = K Q^T.  A lane's 16 bytes of a K row are one run of 32 dims, so
-// it needs one power and converts straight to the MFMA's operand; the dims come
-// in that order, and Q's operand is read in the same.  S^T leaves a lane the 16
-// keys of its own column that P's operand of O^T = V^T P^T takes, so weights
-// never move between lanes.  V is transposed by LDS reads of 4-bit elements and
-// converted with power 1: its powers differ by key, the summed index, so they
-// multiply the weights instead, once for each run of 32 channels (a power of two
+// K's codes are the scaled MFMA's operand as they lie in the pool: S^T = K Q^T with a
+// kv head's G query heads as columns, a run of 32 dims and its power a lane.  Q comes
+// as a sum of two 8-bit operands, exact to 2^-21 of its row.  S^T leaves a lane keys
+// of its own column that P's operand of O^T = V^T P^T takes, so weights never move
+// between lanes.  V is transposed by LDS reads of 4-bit elements and converted with
+// power 1: its powers differ by key, the summed index, so they multiply the weights
+// instead, in the exponent fields, once for each run of 32 channels (a power of two
 // times a bf16 weight is exact).  Sums are formed of the rounded weights, so the
 // weights add up to the sum that divides them; logits, sums and O are fp32.
 //
-// Every wave streams its own tiles through its own LDS slots (two of 8.5 KiB,
-// direct-to-LDS loads a tile ahead, no workgroup barrier); waves differ in kv
-// head and in tile phase.  Bound by HBM reads for batches, by the chain of launch,
-// lengths, table, tiles and merge for single rows.
+// A wave's tile is 64 rows of codes: 64 keys of one kv head, or 32 keys of two, whose
+// rows make whole 128-byte lines (loads alone 5.1 against 6.1 TB/s).  Every wave
+// streams its own tiles through its own two LDS slots of 8.5 KiB (direct-to-LDS loads
+// two tiles ahead, no workgroup barrier); eight waves a workgroup, one workgroup a CU,
+// waves differ in kv head and in tile phase.  Bound by HBM reads for batches: 64 rows
+// of 4096 keys (4 kv heads, 143 MB) 35 us, of 8192 51 + 5 to join, 128 of 4096 53: 7
+// TB/s for every further byte, and 12 to 16 us of launch, lengths, table, first tiles
+// and last results.  Single rows are bound by that chain: 333 keys 7.6 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -36,8 +39,10 @@ constexpr int kRowsPerBlock = kThreads / kLanesPerRow;
 
 // ---------------------------------------------------------------------------
 // Append.  A 16-lane group owns one (token, head) row of K and of V, eight dims
-// (16 bytes) a lane; four lanes share a run.  Bound by HBM for prompts, by the
-// launch and two dependent reads (slot, row) for a decode step.
+// (16 bytes) a lane; four lanes share a run.  Bound by HBM for prompts (16384 tokens
+// of 4 heads, 42 MB, 9.6 us: 4.4 TB/s with the launch in it; two or four rows a group
+// take 10.2 and 11.4), by the launch and two dependent reads (slot, row) for a decode
+// step (3 us).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t run_max(uint32_t x) {  // over four lanes
   x = max(x, uint32_t(__shfl_xor(int(x), 1, 64)));
@@ -76,7 +81,9 @@ store_fp4_kernel(const uint16_t* __restrict__ key, int64_t k_sn, int64_t k_sh,
 }
 
 // ---------------------------------------------------------------------------
-// Dequantising reads: 16 lanes a row, four bytes of codes in, 16 bytes out.
+// Dequantising reads: 16 lanes a row, four bytes of codes in, 16 bytes out.  Bound
+// like the append (16384 tokens of 4 heads 10.0 us; two or four rows a group 10.3,
+// 11.4).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ u32x4_t read_row(const uint8_t* codes, const uint8_t* powers,
                                             int64_t row, int lane16) {
@@ -180,6 +187,7 @@ struct Fp4Params {
   float grid_rcp;
   int whole;               // one workgroup an item, no partials
   int row_blocks;          // blocks of a decode row
+  int items;               // that there is room for
   float c2;                // |scale| log2(e)
   uint32_t flip;           // sign bits of a bf16 pair where scale is negative
   int* count;              // items
@@ -285,8 +293,10 @@ __device__ __forceinline__ Query split_query(const QueryRow& r, uint32_t flip) {
     h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, a), hp, false);
     h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, b), hp, true);
     const int hw = __builtin_bit_cast(int, h);
-    const f32x2v_t back0 = __builtin_bit_cast(f32x2v_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, hp, false));
-    const f32x2v_t back1 = __builtin_bit_cast(f32x2v_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, hp, true));
+    const auto back0 = __builtin_bit_cast(
+        f32x2v_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, hp, false));
+    const auto back1 = __builtin_bit_cast(
+        f32x2v_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, hp, true));
     l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_bits_to_f32(a & 0xffffu) - back0[0],
                                                  bf16_bits_to_f32(a >> 16) - back0[1], lp, false);
     l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_bits_to_f32(b & 0xffffu) - back1[0],
@@ -486,7 +496,8 @@ __device__ __forceinline__ void add_nan_runs(uint32_t mine, int left, Carry (&c)
     const uint64_t at = __builtin_amdgcn_ballot_w64(((mine >> (8 * g)) & 255u) == 255u);
 #pragma unroll
     for (int i = 0; i < NH; ++i) {
-      const float add = (at >> (NH == 1 ? 0 : 32 * i) & seen) != 0 ? __uint_as_float(0x7fc00000u) : 0.f;
+      const bool nan = (at >> (NH == 1 ? 0 : 32 * i) & seen) != 0;
+      const float add = nan ? __uint_as_float(0x7fc00000u) : 0.f;
 #pragma unroll
       for (int x = 0; x < 2; ++x) c[i].o[2 * g + x] += add;
     }
@@ -626,6 +637,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     uint64_t past;
     while ((past = __builtin_amdgcn_ballot_w64(
                 before + (incl + cost * (lane + 1)) * per_row > pos && r0 + lane < rows)) == 0) {
+      if (r0 + 64 >= rows) return;  // (lengths that changed since their sum)
       before += (__builtin_amdgcn_readlane(incl, 63) + cost * 64) * per_row;
       r0 += 64;
       gl = load_row(p, r0 + lane);
@@ -676,6 +688,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     int before = 0, items = 0, r0 = 0;
     uint64_t past;
     while ((past = __builtin_amdgcn_ballot_w64(before + incl * p.head_groups > pos)) == 0) {
+      if (r0 + 64 >= seqs) return;  // (as above)
       before += __builtin_amdgcn_readlane(incl, 63) * p.head_groups;
       items += __builtin_amdgcn_readlane(incl_blocks, 63);
       r0 += 64;
@@ -715,9 +728,10 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     const int seg1 = p.whole ? tiles : min(tiles, off - cost + (end - pos));
     if (seg1 <= seg0) break;  // (the share ends within the setup)
     const int head = grp * p.heads_per_wg + own * NH;
-    if (!p.whole && seg0 == 0 && threadIdx.x == 0)
-      p.rec[item] = ItemRec{share, div_steps(pos - off + cost + tiles - 1, size, size_rcp), g.q0, g.sq, grp,
-                            blk, {0, 0}};
+    // (more items than the host was told of have no record, and stay unjoined)
+    if (!p.whole && seg0 == 0 && threadIdx.x == 0 && item < p.items)
+      p.rec[item] = ItemRec{share, div_steps(pos - off + cost + tiles - 1, size, size_rcp),
+                            g.q0,  g.sq, grp, blk, {0, 0}};
 
     // The lane's column: its query row, head and how many keys it sees; the most
     // and the fewest that a column of the block sees.
@@ -867,14 +881,15 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     // its part of its heads' channel blocks.
     char* mine = smem + wave * (kSlots * kSlotBytes);
     smem_drain();
-    if (mine_too)
+    if (mine_too) {
 #pragma unroll
-    for (int i = 0; i < NH; ++i) {
+      for (int i = 0; i < NH; ++i) {
 #pragma unroll
-      for (int cb = 0; cb < 8; ++cb)
-        *reinterpret_cast<f32x4_t*>(mine + i * kSlotBytes + cb * 1024 + lane * 16) = c[i].o[cb];
-      *reinterpret_cast<float2*>(mine + i * kSlotBytes + 8192 + lane * 8) =
-          float2{c[i].m, c[i].l[0]};
+        for (int cb = 0; cb < 8; ++cb)
+          *reinterpret_cast<f32x4_t*>(mine + i * kSlotBytes + cb * 1024 + lane * 16) = c[i].o[cb];
+        *reinterpret_cast<float2*>(mine + i * kSlotBytes + 8192 + lane * 8) =
+            float2{c[i].m, c[i].l[0]};
+      }
     }
     pf_barrier();
     const char* first = smem + own * (kSlots * kSlotBytes);
@@ -901,8 +916,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
     blk = 0;
     if (++grp < p.head_groups) continue;
     grp = 0;
-    do {  // (pos < end: there is one)
-      g = load_seq<true>(p, ++seq);
+    do {
+      if (++seq >= seqs) return;  // (pos < end: there is one)
+      g = load_seq<true>(p, seq);
     } while (kChunks && g.sq == 0);
   }
 }
@@ -1045,7 +1061,8 @@ Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_
   // Few items are cut finer between two heads a workgroup (16 rows of 4096 keys 19.9
   // against 21.9, one row of 4096 13.5 against 15.7); many share a workgroup better
   // among four (128 rows of 500 to 1500 keys 39.0 against 41.5).
-  pl.heads_per_wg = !pl.pair ? 1 : kv_heads % 4 == 0 && blocks * kv_heads > 128 && !pl.whole ? 4 : 2;
+  const bool four = kv_heads % 4 == 0 && blocks * kv_heads > 128 && !pl.whole;
+  pl.heads_per_wg = !pl.pair ? 1 : four ? 4 : 2;
   pl.head_groups = int(kv_heads / pl.heads_per_wg);
   pl.min_share = 2;
   pl.item_cost = pl.pair ? 16 : 8;
@@ -1087,7 +1104,8 @@ int check_rows(const char* what, const void* key, int64_t k_sn, int64_t k_sh, co
 int check_pool(const char* what, const void* k, const void* v, const void* ks, const void* vs) {
   KVC_REQUIRE(k != nullptr && v != nullptr && ks != nullptr && vs != nullptr, KVC_ERR_VALUE,
               "%s: null pool", what);
-  KVC_REQUIRE(reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 &&
+  KVC_REQUIRE(reinterpret_cast<uintptr_t>(k) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(v) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(ks) % 4 == 0 &&
                   reinterpret_cast<uintptr_t>(vs) % 4 == 0,
               KVC_ERR_ASSERT, "%s: pools must be 16-byte aligned, scales 4-byte", what);
@@ -1187,8 +1205,9 @@ int run_rows(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_
              const uint8_t* v_scale, int64_t blocks, int64_t page, int64_t kv_heads,
              int64_t head_dim, const int32_t* tables, int64_t bt_stride, int64_t max_blocks,
              int64_t decode_rows, const int32_t* lens, int64_t chunks, int64_t chunk_tokens,
-             int64_t chunk_blocks, const int32_t* cu_q, const int32_t* cu_k, float scale, void* out, int64_t o_st,
-             int64_t o_sh, void* workspace, size_t workspace_bytes, kvc_stream_t stream) {
+             int64_t chunk_blocks, const int32_t* cu_q, const int32_t* cu_k, float scale,
+             void* out, int64_t o_st, int64_t o_sh, void* workspace, size_t workspace_bytes,
+             kvc_stream_t stream) {
   KVC_REQUIRE(head_dim == kD, KVC_ERR_VALUE, "%s: head_dim must be 128 (got %lld)", what,
               (long long)head_dim);
   KVC_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, KVC_ERR_VALUE,
@@ -1259,6 +1278,7 @@ int run_rows(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_
   p.grid_rcp = 1.f / float(pl.grid);
   p.whole = pl.whole;
   p.row_blocks = (p.group + 15) / 16;
+  p.items = int(pl.items);
   // (a scale of 0 stays above it: masked scores are -infinity)
   p.c2 = std::max(std::abs(scale) * kLog2e, 1e-37f);
   p.flip = scale < 0.f ? 0x80008000u : 0u;
@@ -1318,8 +1338,8 @@ extern "C" int kvc_paged_decode_fp4(
   return run_rows("paged_decode_fp4", q, q_stride_b, q_stride_h, num_heads, k_cache, v_cache,
                   k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim,
                   block_tables, bt_stride, max_blocks_per_seq, batch, context_lens, 0, 0, 0,
-                  nullptr, nullptr, scale, out, out_stride_b, out_stride_h, workspace, workspace_bytes,
-                  stream);
+                  nullptr, nullptr, scale, out, out_stride_b, out_stride_h, workspace,
+                  workspace_bytes, stream);
 }
 
 extern "C" size_t kvc_varlen_fp4_workspace_bytes(int64_t num_q_tokens, int64_t num_heads,
@@ -1343,9 +1363,8 @@ extern "C" int kvc_varlen_fp4(
     int64_t head_dim, const int32_t* block_tables, int64_t bt_stride, int64_t max_blocks_per_seq,
     int64_t num_decode_rows, const int32_t* decode_context_lens, int64_t num_prefill,
     int64_t chunk_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, float scale,
-    void* out,
-    int64_t out_stride_t, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
-    kvc_stream_t stream) {
+    void* out, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+    size_t workspace_bytes, kvc_stream_t stream) {
   clear_error();
   KVC_REQUIRE(num_decode_rows >= 0 && num_decode_rows <= num_q_tokens, KVC_ERR_VALUE,
               "varlen_fp4: more decode rows than query rows");
@@ -1353,8 +1372,7 @@ extern "C" int kvc_varlen_fp4(
                   v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim, block_tables,
                   bt_stride, max_blocks_per_seq, num_decode_rows, decode_context_lens,
                   num_prefill, num_q_tokens - num_decode_rows, chunk_blocks, cu_seqlens_q,
-                  cu_seqlens_k, scale,
-                  out, out_stride_t, out_stride_h, workspace, workspace_bytes, stream);
+                  cu_seqlens_k, scale, out, out_stride_t, out_stride_h, workspace, workspace_bytes, stream);
 }
 
 extern "C" int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
@@ -1369,8 +1387,10 @@ extern "C" int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
   int64_t blocks = 0, longest = 0;
   double products = 0, all_keys = 0, pairs = 0;
   for (int64_t i = 0; i < num_prefill; ++i) {
-    const int64_t n = std::max<int64_t>(0, int64_t(cu_seqlens_q_host[i + 1]) - cu_seqlens_q_host[i]);
-    const int64_t m = std::max<int64_t>(0, int64_t(cu_seqlens_k_host[i + 1]) - cu_seqlens_k_host[i]);
+    auto length = [&](const int32_t* cu) {
+      return std::max<int64_t>(0, int64_t(cu[i + 1]) - cu[i]);
+    };
+    const int64_t n = length(cu_seqlens_q_host), m = length(cu_seqlens_k_host);
     const int64_t b = (n * group + 15) / 16;
     blocks += b;
     longest = std::max(longest, m);
@@ -1383,7 +1403,8 @@ extern "C" int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
                             num_heads, num_kv_heads, page_size * max_blocks_per_seq);
   const double items = double(blocks) * double(num_kv_heads) / (pl.whole && pl.pair ? 2 : 1);
   const double here =
-      pl.whole ? std::ceil(items / cu_count()) * (6.5 + 2.6 * double(longest) / (pl.pair ? 256 : 512))
+      pl.whole ? std::ceil(items / cu_count()) *
+                     (6.5 + 2.6 * double(longest) / (pl.pair ? 256 : 512))
                : 12 + 6 * std::min(1., items / 128) + products * double(num_kv_heads) / 64 * 1.1e-3;
   // Gathered: three launches, the keys written and read once more, the products at the
   // long chunks' rate; and the decode rows in a call of their own.
