@@ -19,9 +19,10 @@
 // streams its own tiles through its own two LDS slots of 8.5 KiB (direct-to-LDS loads
 // two tiles ahead, no workgroup barrier); eight waves a workgroup, one workgroup a CU,
 // waves differ in kv head and in tile phase.  Bound by HBM reads for batches: 64 rows
-// of 4096 keys (4 kv heads, 143 MB) 35 us, of 8192 51 + 5 to join, 128 of 4096 53: 7
-// TB/s for every further byte, and 12 to 16 us of launch, lengths, table, first tiles
-// and last results.  Single rows are bound by that chain: 333 keys 7.6 us.
+// of 4096 keys (4 kv heads, 143 MB) 34 us, of 8192 51 + 5 to join (47 with the loads
+// alone), 128 of 4096 53: 7 TB/s for every further byte, and 12 to 16 us of launch,
+// lengths, table, first tiles and last results.  Single rows are bound by that chain:
+// 333 keys 7.4 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -508,23 +509,33 @@ __device__ __forceinline__ i32x4_t scalar_rsrc(const void* base, int bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   return i32x4_t{int(uint32_t(a)), int(uint32_t(a >> 32) & 0xffffu), bytes, kBufWord3};
 }
-// Two loads of 1 KiB of codes; one of powers (of the active lanes).
+// Two loads of 1 KiB of codes; one of powers (of the active lanes).  Whole lines are
+// read past the caches (`nt`); half lines are not: their other halves follow from the
+// next workgroups of the XCD (64 rows of 2304 keys 22.6 us with nt, 19.6 without).
+#define KVC_LOAD_CODES(HINT)                                                   \
+  asm volatile(                                                                \
+      "s_mov_b32 %0, m0\n\t"                                                   \
+      "s_mov_b32 m0, %3\n\t"                                                   \
+      "s_nop 0\n\t"                                                            \
+      "buffer_load_dwordx4 %1, %4, %5 offen" HINT " lds\n\t"                   \
+      "s_add_u32 m0, m0, 0x400\n\t"                                            \
+      "s_nop 0\n\t"                                                            \
+      "buffer_load_dwordx4 %2, %4, %6 offen" HINT " lds\n\t"                   \
+      "s_mov_b32 m0, %0"                                                       \
+      : "=&s"(m0)                                                              \
+      : "v"(off0), "v"(off1), "s"(lds), "s"(r), "s"(base0), "s"(base1)         \
+      : "memory", "scc")
+template <bool kWholeLines>
 __device__ __forceinline__ void load_codes(const i32x4_t& r, int off0, int off1, int base0,
                                            int base1, uint32_t lds) {
   uint32_t m0;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %4, %5 offen nt lds\n\t"
-      "s_add_u32 m0, m0, 0x400\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %2, %4, %6 offen nt lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(m0)
-      : "v"(off0), "v"(off1), "s"(lds), "s"(r), "s"(base0), "s"(base1)
-      : "memory", "scc");
+  if constexpr (kWholeLines) {
+    KVC_LOAD_CODES(" nt");
+  } else {
+    KVC_LOAD_CODES("");
+  }
 }
+#undef KVC_LOAD_CODES
 __device__ __forceinline__ void load_powers(const i32x4_t& r, int off, uint32_t lds) {
   uint32_t m0;
   asm volatile(
@@ -775,10 +786,10 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
         const i32x4_t kr = scalar_rsrc(p.k + at * kFp4RowBytes, code_bytes & there);
         const i32x4_t vr = scalar_rsrc(p.v + at * kFp4RowBytes, code_bytes & there);
         const int step = 8 * row_bytes;
-        load_codes(kr, k0, k0 ^ 32, 0, step, lds);
-        load_codes(vr, v0, v0, 0, step, lds + kVAt);
-        load_codes(kr, k0 ^ 64, k0 ^ 96, 2 * step, 3 * step, lds + 2048);
-        load_codes(vr, v0, v0, 2 * step, 3 * step, lds + kVAt + 2048);
+        load_codes<true>(kr, k0, k0 ^ 32, 0, step, lds);
+        load_codes<true>(vr, v0, v0, 0, step, lds + kVAt);
+        load_codes<true>(kr, k0 ^ 64, k0 ^ 96, 2 * step, 3 * step, lds + 2048);
+        load_codes<true>(vr, v0, v0, 2 * step, 3 * step, lds + kVAt + 2048);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -791,9 +802,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
             load_powers(scalar_rsrc(p.vs + at * kFp4Powers, power_bytes & there), poff,
                         lds + kVpAt);
           }
-          load_codes(scalar_rsrc(p.k + at * kFp4RowBytes, code_bytes & there), k0, k1, 0, 0,
+          load_codes<false>(scalar_rsrc(p.k + at * kFp4RowBytes, code_bytes & there), k0, k1, 0, 0,
                      lds + 2048 * h);
-          load_codes(scalar_rsrc(p.v + at * kFp4RowBytes, code_bytes & there),
+          load_codes<false>(scalar_rsrc(p.v + at * kFp4RowBytes, code_bytes & there),
                      v0 ^ (32 * h), v1 ^ (32 * h), 0, 0, lds + kVAt + 2048 * h);
         }
       }
@@ -1032,10 +1043,12 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 //   cut    12, 6 more as the items get to 128 (more of them in a share), and the
 //          longer of the keys' bytes at 6.6 TB/s and 1.1 ns for every 64 keys of a
 //          head and block
-// Measured, cut / whole / whole by two heads (4 kv heads; rows x keys): 1 x 333 11.6 /
-// 7.6 / 10.5, 1 x 4096 13.2 / 27.8 / 38.4, 64 x 2048 26.9 / 22.0 / 25.1, 64 x 4096 39.7
-// / 36.3 / 40.0, 128 x 500 to 1500 29.9 / 30.6 / 22.8, 48 x 1025 to 8007 36.5 / 50.8 /
-// 66.5, 128 x 4096 62.7 / 70.5 / 54.3, 16 x 32768 62 / 182 / 246.
+// (A batch's keys count as its table's width, so few long rows among many look like
+// more than they are: for those the whole form's rate is set low.)  Measured, cut /
+// whole / whole by two heads (4 kv heads; rows x keys): 1 x 1000 13.7 / 10.4 / 15.5, 8
+// x 4096 17.5 / 24.4 / 36.9, 16 x 8192 26.3 / 42.6 / 66.3, 64 x 2304 27.1 / 19.4 / 26.2,
+// 64 x 4096 36.3 / 29.5 / 39.5, 64 x 8192 57.4 / 61.3 / 69.5, 48 x 1025 to 8007 33.8 /
+// 41.7 / 64.2, 128 x 1000 29.4 / 24.1 / 19.5, 128 x 4096 60.5 / 67.8 / 52.6.
 Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t chunk_blocks,
                int64_t heads, int64_t kv_heads, int64_t most_keys) {
   Plan pl{};
