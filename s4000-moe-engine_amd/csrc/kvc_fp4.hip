@@ -1047,15 +1047,16 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // of 4 to 256 tokens over 300 to 32768 keys (kv heads 2, 4, 8):
 //   whole  the longer of ceil(items / CUs) (6 + 2.6 a round of 8 tiles) and 7 + the
 //          keys' bytes at 4.6 TB/s (one head: half lines) or 5.6 (two)
-//   cut    12, 6 more as the items get to 128 (more of them in a share), and the
-//          longer of the keys' bytes at 6.6 TB/s and 1.1 ns for every 64 keys of a
+//   cut    12.5, 7 more as the items get to 128 (more of them in a share), and the
+//          longer of the keys' bytes at 6.6 TB/s and 0.9 ns for every 64 keys of a
 //          head and block
 // (A batch's keys count as its table's width, so few long rows among many look like
-// more than they are: for those the whole form's rate is set low.)  Measured, cut /
-// whole / whole by two heads (4 kv heads; rows x keys): 1 x 1000 13.7 / 10.4 / 15.5, 8
-// x 4096 17.5 / 24.4 / 36.9, 16 x 8192 26.3 / 42.6 / 66.3, 64 x 2304 27.1 / 19.4 / 26.2,
-// 64 x 4096 36.3 / 29.5 / 39.5, 64 x 8192 57.4 / 61.3 / 69.5, 48 x 1025 to 8007 33.8 /
-// 41.7 / 64.2, 128 x 1000 29.4 / 24.1 / 19.5, 128 x 4096 60.5 / 67.8 / 52.6.
+// more than they are: for those the whole form's rate is set low.)  Of 67 shapes the
+// choice loses 4 % or more in three, 10 % at worst.  Measured, cut / whole / whole by
+// two heads (4 kv heads; rows x keys): 1 x 1000 12.3 / 9.9 / 15.0, 8 x 4096 16.7 / 23.0
+// / 34.9, 16 x 8192 25.4 / 40.2 / 61.2, 64 x 2304 26.3 / 18.9 / 25.1, 64 x 4096 35.3 /
+// 28.1 / 37.4, 64 x 8192 56.3 / 60.2 / 66.4, 48 x 1025 to 8007 32.8 / 39.2 / 59.5, 128 x
+// 1000 28.2 / 22.9 / 18.8, 128 x 4096 58.4 / 66.0 / 52.1.
 Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t chunk_blocks,
                int64_t heads, int64_t kv_heads, int64_t most_keys) {
   Plan pl{};
@@ -1074,8 +1075,8 @@ Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_
   };
   const double whole = alone(heads_of, 512, 4.6e6);
   const double whole2 = kv_heads % 2 == 0 ? alone(heads_of / 2, 256, 5.6e6) : 1e30;
-  const double cut = 12 + 6 * std::min(1., heads_of / 128) +
-                     std::max(bytes / 6.6e6, heads_of * keys / 64 * 1.1e-3);
+  const double cut = 12.5 + 7 * std::min(1., heads_of / 128) +
+                     std::max(bytes / 6.6e6, heads_of * keys / 64 * 0.9e-3);
   pl.whole = std::min(whole, whole2) <= cut;
   pl.pair = kv_heads % 2 == 0 && (!pl.whole || whole2 < whole);
   // Few items are cut finer between two heads a workgroup (16 rows of 4096 keys 19.9
@@ -1424,10 +1425,12 @@ extern "C" int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
   const double items = double(blocks) * double(num_kv_heads) / (pl.whole && pl.pair ? 2 : 1);
   const double here =
       pl.whole ? std::ceil(items / cu_count()) *
-                     (6.5 + 2.6 * double(longest) / (pl.pair ? 256 : 512))
-               : 12 + 6 * std::min(1., items / 128) + products * double(num_kv_heads) / 64 * 1.1e-3;
+                     (6 + 2.2 * double(longest) / (pl.pair ? 256 : 512))
+               : 12 + 6 * std::min(1., items / 128) + products * double(num_kv_heads) / 64 * 0.9e-3;
   // Gathered: three launches, the keys written and read once more, the products at the
-  // long chunks' rate; and the decode rows in a call of their own.
+  // long chunks' rate; and the decode rows in a call of their own.  (Of 371 shapes, 1 to
+  // 8 chunks of 4 to 512 tokens over up to 32768 keys, seven take the form that is over 10 %
+  // slower, 30 % at worst.)
   const double gathered = (longest <= 64 ? 13 : 22) + 3e-4 * all_keys * double(num_kv_heads) +
                           0.38e-6 * pairs * double(num_heads) + (num_decode_rows > 0 ? 12 : 0);
   return here <= gathered ? blocks : 0;
