@@ -689,7 +689,8 @@ int kvc_stage_decode(const void* q, int64_t q_layer_stride, int64_t q_row_stride
  * smallest power of two that brings its largest magnitude to 6 or less (2^-126
  * at least, 2^125 at most: finite values stay finite); values round to the
  * nearest code, ties to the even mantissa.  A run that holds an infinity or a
- * NaN is NaN (scale 255, codes 0).  Slots as for kvc_store_kv. */
+ * NaN is NaN (scale 255, codes 0).  Slots as for kvc_store_kv, each at most once a
+ * call. */
 int kvc_store_fp4(const void* key, int64_t key_stride_n, int64_t key_stride_h, const void* value,
                   int64_t value_stride_n, int64_t value_stride_h, uint8_t* k_cache,
                   uint8_t* v_cache, uint8_t* k_scale, uint8_t* v_scale, int64_t num_slots,
@@ -741,8 +742,8 @@ int kvc_paged_decode_fp4(const void* q, int64_t q_stride_b, int64_t q_stride_h,
  * read the keys once, so it is for chunks of few tokens (drafts to verify, the
  * ends of prompts); long ones are faster gathered (kvc_gather_kv_fp4).
  * chunk_blocks: the chunks' blocks, sum of ceil(tokens x query heads per kv head /
- * 16), as the host knows it (fewer than there are would leave rows out), or 0;
- * the workspace query takes the same.  Lengths are read on the device; rows of no
+ * 16), as the host knows it, or 0 (rows of blocks past a count that is too small
+ * come out undefined); the workspace query takes the same.  Lengths are read on the device; rows of no
  * sequence are not written. */
 size_t kvc_varlen_fp4_workspace_bytes(int64_t num_q_tokens, int64_t num_heads,
                                       int64_t num_kv_heads, int64_t page_size,

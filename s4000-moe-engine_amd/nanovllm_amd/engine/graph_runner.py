@@ -97,6 +97,8 @@ class DecodeGraphRunner:
                             self.v_scales or [None]):
                 check_fp4_pool(*args)
             assert len(self.k_scales) == len(self.v_scales) == self.num_layers
+        elif k_scales is not None or v_scales is not None:
+            raise ValueError("k_scales / v_scales are those of a 4-bit pool")
         self.head_dim = 128 if fp4 else kc.size(3)
         self.num_heads = num_heads
         self.scratch_block_id = kc.size(0) - 1

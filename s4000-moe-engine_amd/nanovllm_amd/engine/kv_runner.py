@@ -465,8 +465,9 @@ class KVCacheRunner:
         """prepare_decode from lengths that live on the device: one token for every
         row of `tables` (DeviceBlockTables; query_lens 0 where there is none), its
         page taken there, with no host read.  Sets the Context and returns the
-        StepTables (positions among them); a row that waits for a page attends
-        nothing and appends at the scratch slot."""
+        StepTables (positions among them).  A row that waits for a page, or has no
+        token, attends nothing and appends nothing that is read again: its output
+        is zeros over a 4-bit pool, NaN over the others."""
         if query_lens is None:
             query_lens = torch.ones(tables.max_rows, dtype=torch.int32, device=tables.device)
         step = tables.step(query_lens, tables.max_rows, tokens_per_row=1, finished=finished,

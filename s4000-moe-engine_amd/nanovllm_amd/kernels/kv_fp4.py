@@ -50,7 +50,8 @@ def _one_device(pool, **tensors):
 def store_kvcache_fp4(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping):
     """store_kvcache into a 4-bit pool: key / value [N, KVH, 128] bf16 rows
     quantised at slot_mapping (int32 or int64 [N]; a negative slot counts from
-    the pool's end, one outside the pool is skipped).  One launch, capturable."""
+    the pool's end, one outside the pool is skipped).  One launch, capturable.
+    Two tokens of a call at one slot leave a mixture of both there."""
     if nat.is_current(key) and nat.host().fp4_store(key, value, k_cache, v_cache, k_scale,
                                                     v_scale, slot_mapping, nat.stream_of(key)):
         return

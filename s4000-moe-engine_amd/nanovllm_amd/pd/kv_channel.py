@@ -8,7 +8,9 @@ pinned buffer (no index_select temporary, no permute copy, no device-wide
 synchronise), and one scatter kernel reads it back.  The round trip is a
 bitwise copy.  Below them: LocalKVChannel, TcpKVChannel and KVFrameAssembler
 with the engine's frame format (kv_channel.py:85-220), sent from and received
-into the pinned staging rows without host copies.
+into the pinned staging rows without host copies.  A 4-bit pool's scales
+(KVCacheRunner.kv_scales) are a pool of the same layout and travel as one: the
+same calls, with a buffer or a channel of their own.
 """
 from __future__ import annotations
 

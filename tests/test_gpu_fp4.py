@@ -592,6 +592,77 @@ def test_rows_of_no_sequence_stay():
         assert (out[9:] == 3).all()
 
 
+def test_fewer_blocks_told_than_there_are():
+    """The told blocks come first; what lies behind them is not joined, and nothing
+    outside the output is written."""
+    chunks = [(24, 90), (24, 120), (24, 64)]
+    pool, tables, k, v = fo.paged([m for _, m in chunks], 32, 2, seed=24)
+    gen = torch.Generator().manual_seed(14)
+    q = torch.randn(72, 8, 128, generator=gen).to(BF)
+    want, bound = _chunk_expect(q, k, v, [], chunks)
+    kc, vc, ks, vs = _dev(pool)
+    for width in (4, 2200):
+        t = torch.full((3, width), -1, dtype=torch.int32)
+        t[:, :4] = tables
+        whole = torch.full((74, 8, 128), 3.0, dtype=BF, device="cuda")
+        varlen_fp4(q.cuda(), kc, vc, ks, vs, t.cuda(), 0, None, 6,
+                   torch.tensor([0, 24, 48, 72], dtype=torch.int32).cuda(),
+                   torch.tensor([0, 90, 210, 274], dtype=torch.int32).cuda(), SCALE, whole[1:73])
+        fo.check(whole[1:25], want[:24], bound[:24], f"told rows, width {width}")
+        assert (whole[0] == 3).all() and (whole[73] == 3).all()
+
+
+@pytest.mark.parametrize("decode,chunks,width", [
+    ([300, 1, 40], [(4, 700), (9, 9)], 4), ([300, 1, 40], [(4, 700), (9, 9)], 200),
+    ([64], [(300, 900)], 4)])
+def test_chunks_captured(decode, chunks, width):
+    """A mixed call in a graph, replayed over other pools, queries and decode lengths
+    with eager calls between: each replay is the eager call's, bit for bit."""
+    lens = decode + [m for _, m in chunks]
+    pools = [fo.paged(lens, 256, 4, seed=60 + i, spare=2) for i in range(2)]
+    kc, vc, ks, vs = state = _dev(pools[0][0])
+    tables = torch.full((len(lens), width), -1, dtype=torch.int32, device="cuda")
+    cu_q, cu_k = [0], [0]
+    for n, m in chunks:
+        cu_q.append(cu_q[-1] + n)
+        cu_k.append(cu_k[-1] + m)
+    dq, dk = (torch.tensor(x, dtype=torch.int32).cuda() for x in (cu_q, cu_k))
+    held = torch.tensor(decode, dtype=torch.int32).cuda()
+    gen = torch.Generator().manual_seed(15)
+    q = torch.zeros(len(decode) + cu_q[-1], 16, 128, dtype=BF, device="cuda")
+
+    def call():
+        return varlen_attention(q, kc, vc, scale=SCALE, block_tables=tables,
+                                num_decode_rows=len(decode), decode_context_lens=held,
+                                cu_seqlens_q=dq, cu_seqlens_k=dk, cu_seqlens_q_list=cu_q,
+                                cu_seqlens_k_list=cu_k, k_scale=ks, v_scale=vs,
+                                decode_context_lens_list=decode)
+
+    tables[:, :pools[0][1].size(1)] = pools[0][1].cuda()
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(6):
+        pool, bt, k, v = pools[i % 2]
+        for t, new in zip(state, pool):
+            t.copy_(new)
+        tables[:, :bt.size(1)] = bt.cuda()
+        now = [max(0, n - 13 * i) for n in decode]
+        held.copy_(torch.tensor(now))
+        nq = torch.randn(q.shape, generator=gen).to(BF)
+        q.copy_(nq)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(call(), got), i
+        if i % 3 == 1:
+            short = [x[:n] for x, n in zip(k, now)] + k[len(now):]
+            other = [x[:n] for x, n in zip(v, now)] + v[len(now):]
+            fo.check(got, *_chunk_expect(nq, short, other, now, chunks), f"replay {i}")
+
+
 def test_nan_runs_reach_only_the_tokens_that_see_them():
     chunks = [(6, 70)]
     pool, tables, k, v = fo.paged([70], 32, 2, seed=23)

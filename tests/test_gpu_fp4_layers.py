@@ -262,3 +262,89 @@ def test_serving_loop_without_the_host(capture):
     slot = (tables.block_tables[0].cpu()[pos // PAGE].long() * PAGE + pos % PAGE).cuda()
     got = dequant_fp4(layer.k_cache.flatten(0, 1)[slot], layer.k_scale.flatten(0, 1)[slot])
     assert torch.equal(got.cpu(), hist[0][0].to(BF))
+
+
+@pytest.mark.parametrize("kvh,capture", [(2, False), (4, False), (4, True)])
+def test_serving_loop_over_a_bf16_pool(kvh, capture):
+    """The same loop over a bf16 pool, where the append may ride in the decode launch:
+    rows that wait give NaN and leave the pool as it was."""
+    rows, heads = 3, 2 * kvh
+    runner = KVCacheRunner(1, 4, PAGE, kvh, 128)
+    runner.kv_cache.zero_()
+    layer = Attention(heads, 128, SCALE, kvh)
+    assert runner.bind([layer]) == 1
+    tables = runner.device_tables(rows, 3)
+    gen = torch.Generator().manual_seed(6)
+    q = torch.zeros(rows, heads, 128, dtype=BF, device="cuda")
+    k, v = (torch.zeros(rows, kvh, 128, dtype=BF, device="cuda") for _ in range(2))
+    out = tables.outputs(rows)
+    new = torch.ones(rows, dtype=torch.int32, device="cuda")
+    result = torch.zeros_like(q)
+
+    def step():
+        runner.prepare_decode_device(tables, new, out=out)
+        result.copy_(layer(q, k, v).view(rows, heads, 128))
+
+    graph = None
+    if capture:
+        state = [tables.context_lens, tables.num_blocks, tables.block_tables, tables.free_blocks,
+                 tables.num_free, runner.kv_cache]
+        saved = [x.clone() for x in state]
+        step()
+        torch.cuda.synchronize()
+        for x, s in zip(state, saved):
+            x.copy_(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+    none = torch.zeros(0, kvh, 128, dtype=torch.float64)
+    hist, waited = [(none, none)] * rows, 0
+    for i in range(70):
+        nq = torch.randn(rows, heads, 128, generator=gen).to(BF)
+        nk, nv = (torch.randn(rows, kvh, 128, generator=gen).to(BF) for _ in range(2))
+        q.copy_(nq), k.copy_(nk), v.copy_(nv)
+        before = runner.kv_cache[:, :, :4].clone()
+        graph.replay() if graph is not None else step()
+        torch.cuda.synchronize()
+        granted = out.query_lens.tolist()
+        changed = (runner.kv_cache[:, 0, :4] != before[:, 0]).any(-1).any(-1)
+        assert int(changed.sum()) == 2 * sum(granted)     # a token's K and V rows each
+        for b in range(rows):
+            if not granted[b]:
+                waited += 1
+                assert result[b].isnan().all()
+                continue
+            hist[b] = (torch.cat((hist[b][0], nk[b:b + 1].double())),
+                       torch.cat((hist[b][1], nv[b:b + 1].double())))
+            if i % 7 == 0:
+                want, _ = fo.attend(nq[b:b + 1], *hist[b], fo.causal(1, len(hist[b][0])), SCALE)
+                off = (result[b:b + 1].double().cpu() - want).abs()
+                # (the paged decode's bar over a bf16 pool)
+                assert float(off.max()) < 2e-2 and float(off.mean()) < 2e-3, (i, b)
+    assert waited > 0
+
+
+def test_blocks_travel_with_their_powers():
+    """Codes and powers over the wire's staging, each as a pool: 4-bit blocks come out
+    of another runner's blocks as they went in."""
+    from nanovllm_amd.pd.kv_channel import LocalKVChannel
+    here, _ = _runner(layers=2)
+    there, _ = _runner(layers=2)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    for t in (here.kv_cache, here.kv_scales):
+        t.copy_(torch.randint(0, 250, t.shape, dtype=torch.uint8, device="cuda", generator=gen))
+    src, dst = [3, 0, 17], [5, 20, 1]
+    for a, b in ((here.kv_cache, there.kv_cache), (here.kv_scales, there.kv_scales)):
+        buf = LocalKVChannel(a).send(src)
+        LocalKVChannel(b).recv(dst, buf)
+        assert torch.equal(b[:, :, dst], a[:, :, src])
+        rest = [i for i in range(25) if i not in dst]
+        assert (b[:, :, rest] == (0 if b is there.kv_cache else 127)).all()
+
+
+def test_captured_step_refuses_scales_of_another_pool():
+    pool = torch.zeros(3, PAGE, KVH, 128, dtype=BF, device="cuda")
+    scale = torch.zeros(3, PAGE, KVH, 4, dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError, match="4-bit"):
+        DecodeGraphRunner([pool], [pool.clone()], HEADS, 2, 2, SCALE, k_scales=[scale],
+                          v_scales=[scale])
