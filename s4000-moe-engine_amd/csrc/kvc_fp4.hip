@@ -953,14 +953,18 @@ template <int S>
 __global__ void __launch_bounds__(32 * kGroups) fp4_merge_kernel(Fp4Params p) {
   __shared__ f32x4_t so[kGroups][32];
   __shared__ float2 sml[kGroups];
-  if (int(blockIdx.x) >= *p.count) return;
-  const ItemRec rec = p.rec[blockIdx.x];
+  touch_kernel_args(int(sizeof(Fp4Params)));
+  // (both read at once; past the count there is room for a record but none)
+  const int count = *p.count;
+  ItemRec rec = p.rec[blockIdx.x];
+  asm volatile("" ::"s"(count), "s"(rec.first), "s"(rec.sq));
   const int2 r = {rec.first, rec.last};
-  if (r.x >= r.y) return;
+  if (int(blockIdx.x) >= count || r.x >= r.y) return;
   const int lane = threadIdx.x & 31, at_group = threadIdx.x >> 5, slice = at_group % S;
   // The workgroup's at_group / S-th column: of a head of the item's, one of its block's.
   const int nth = blockIdx.y * (kGroups / S) + at_group / S;
-  const int hs = nth / p.cols, in = nth - hs * p.cols;
+  const int hs = div_small(nth, p.cols, __builtin_amdgcn_rcpf(float(p.cols)));
+  const int in = nth - hs * p.cols;
   const int col = rec.block * 16 + in;
   const bool live = hs < p.heads_per_wg && col < rec.sq * p.group;
   const int token = div_small(col, p.group, p.group_rcp);
