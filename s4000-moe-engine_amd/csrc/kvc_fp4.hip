@@ -83,8 +83,8 @@ store_fp4_kernel(const uint16_t* __restrict__ key, int64_t k_sn, int64_t k_sh,
 
 // ---------------------------------------------------------------------------
 // Dequantising reads: 16 lanes a row, four bytes of codes in, 16 bytes out.  Bound
-// like the append (16384 tokens of 4 heads 10.0 us; two or four rows a group 10.3,
-// 11.4).
+// like the append (16384 tokens of 4 heads 9.0 us; two or four rows a group were 3 and
+// 14 % slower).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ u32x4_t read_row(const uint8_t* codes, const uint8_t* powers,
                                             int64_t row, int lane16) {
@@ -129,8 +129,9 @@ gather_fp4_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
     k = read_row(k_cache, k_scale, slot * kvh + h, lane16);
     v = read_row(v_cache, v_scale, slot * kvh + h, lane16);
   }
-  *reinterpret_cast<u32x4_t*>(out_k + row * kD + lane16 * 8) = k;
-  *reinterpret_cast<u32x4_t*>(out_v + row * kD + lane16 * 8) = v;
+  // (past the caches: 40 MB of them 10.9 -> 8.6 us)
+  __builtin_nontemporal_store(k, reinterpret_cast<u32x4_t*>(out_k + row * kD + lane16 * 8));
+  __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(out_v + row * kD + lane16 * 8));
 }
 
 // ---------------------------------------------------------------------------
