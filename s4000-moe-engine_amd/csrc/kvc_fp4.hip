@@ -919,6 +919,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
         auto put = [&](int cb, const f32x4_t& o, float top, float l) { emit(i, cb, o, top, l); };
         if (NH == 1 || phases == 8) {
           join<8>(first + i * kSlotBytes, apart, phase, lane, put);
+        } else if (phases == 2) {
+          join<2>(first + i * kSlotBytes, apart, phase, lane, put);
         } else {
           join<4>(first + i * kSlotBytes, apart, phase, lane, put);
         }
@@ -1045,23 +1047,25 @@ struct Plan {
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Three ways to cut the work.  Whole: a workgroup takes an item alone, eight tiles at a
-// time, of one head (64 keys each) or of two (32), and there is one launch.  Cut: two
-// heads a wave, the tiles of all items in equal shares, one a CU, and a second launch
-// joins the pieces.  Estimates in us, from decode batches of 1 to 128 rows and chunks
-// of 4 to 256 tokens over 300 to 32768 keys (kv heads 2, 4, 8):
-//   whole  the longer of ceil(items / CUs) (6 + 2.6 a round of 8 tiles) and 7 + the
-//          keys' bytes at 4.6 TB/s (one head: half lines) or 5.6 (two)
-//   cut    12.5, 7 more as the items get to 128 (more of them in a share), and the
-//          longer of the keys' bytes at 6.6 TB/s and 0.9 ns for every 64 keys of a
-//          head and block
+// How the work is cut.  Whole: a workgroup takes an item of one, two, four or eight kv
+// heads alone, and there is one launch; its eight waves make one tile each a round, 512
+// keys of one head (64 a wave) or 256, 128 or 64 of more (a wave takes two heads and 32
+// keys).  Cut: two heads a wave, the tiles of all items in equal shares, one a CU, and a
+// second launch joins the pieces.  Estimates in us:
+//   whole  the longer of ceil(items / CUs) (7 + 2.2 a round) and 7 + the keys' bytes at
+//          4.6 TB/s (one head: half lines), 5.6 (two) or 6.8
+//   cut    13, 6 more as the heads' blocks get to 128 and 2 more for every 256 items
+//          (more of them in a share), and the longer of the keys' bytes at 6.2 TB/s and
+//          0.9 ns for every 64 keys of a head and block
 // (A batch's keys count as its table's width, so few long rows among many look like
-// more than they are: for those the whole form's rate is set low.)  Of 67 shapes the
-// choice loses 4 % or more in three, 10 % at worst.  Measured, cut / whole / whole by
-// two heads (4 kv heads; rows x keys): 1 x 1000 12.3 / 9.9 / 15.0, 8 x 4096 16.7 / 23.0
-// / 34.9, 16 x 8192 25.4 / 40.2 / 61.2, 64 x 2304 26.3 / 18.9 / 25.1, 64 x 4096 35.3 /
-// 28.1 / 37.4, 64 x 8192 56.3 / 60.2 / 66.4, 48 x 1025 to 8007 32.8 / 39.2 / 59.5, 128 x
-// 1000 28.2 / 22.9 / 18.8, 128 x 4096 58.4 / 66.0 / 52.1.
+// more than they are: for those the one-head form's rate is set low.)  Measured, cut /
+// whole by one, two, four and eight heads (rows x keys; 4 kv heads): 1 x 1000 13.1 /
+// 10.1 / 15.1 / 21.5, 8 x 4096 17 / 23 / 35 / 60, 16 x 8192 26 / 40 / 61 / 113, 64 x 300
+// 19 / 8.3 / 10.7 / 12.9, 64 x 4096 35 / 28 / 38 / 62, 64 x 8192 56 / 60 / 66 / 114, 48 x
+// 1025 to 8007 32 / 40 / 60 / 107, 128 x 1000 28 / 23 / 19 / 23, 128 x 4096 59 / 65 / 52 /
+// 65, 192 x 1000 34 / 34 / 33 / 24, 256 x 300 to 900 34 / 36 / 30 / 23; 8 kv heads: 128 x
+// 300 to 900 34 / 37 / 31 / 24 / 35, 200 x 1000 54 / 82 / 70 / 53 / 44, 400 x 20 to 80 35
+// / 60 / 43 / 28 / 21.  Of 133 shapes the choice is over 5 % off in two, 15 % at worst.
 Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t chunk_blocks,
                int64_t heads, int64_t kv_heads, int64_t most_keys) {
   Plan pl{};
@@ -1074,21 +1078,25 @@ Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_
   const double heads_of = double(blocks) * double(kv_heads), keys = double(most_keys);
   const double bytes = double(decode_rows + chunks) * double(kv_heads) * keys *
                        (2 * (kFp4RowBytes + kFp4Powers));
-  auto alone = [&](double items, double keys_a_round, double bytes_a_us) {
-    return std::max(std::ceil(items / cus) * (6 + 2.6 * keys / keys_a_round),
-                    7 + bytes / bytes_a_us);
-  };
-  const double whole = alone(heads_of, 512, 4.6e6);
-  const double whole2 = kv_heads % 2 == 0 ? alone(heads_of / 2, 256, 5.6e6) : 1e30;
-  const double cut = 12.5 + 7 * std::min(1., heads_of / 128) +
-                     std::max(bytes / 6.6e6, heads_of * keys / 64 * 0.9e-3);
-  pl.whole = std::min(whole, whole2) <= cut;
-  pl.pair = kv_heads % 2 == 0 && (!pl.whole || whole2 < whole);
-  // Few items are cut finer between two heads a workgroup (16 rows of 4096 keys 19.9
+  int best = 1;
+  double whole = 1e30;
+  const double rate[] = {4.6e6, 5.6e6, 6.8e6, 6.8e6};  // bytes a us
+  for (int i = 0; i < 4 && kv_heads % (1 << i) == 0; ++i) {
+    const int n = 1 << i;
+    const double t = std::max(std::ceil(heads_of / n / cus) * (7 + 2.2 * keys * n / 512),
+                              7 + bytes / rate[i]);
+    if (t < whole) whole = t, best = n;
+  }
+  // Cut: few items are cut finer between two heads a workgroup (16 rows of 4096 keys 19.9
   // against 21.9, one row of 4096 13.5 against 15.7); many share a workgroup better
   // among four (128 rows of 500 to 1500 keys 39.0 against 41.5).
-  const bool four = kv_heads % 4 == 0 && blocks * kv_heads > 128 && !pl.whole;
-  pl.heads_per_wg = !pl.pair ? 1 : four ? 4 : 2;
+  const int apart = kv_heads % 2 != 0 ? 1 : kv_heads % 4 == 0 && heads_of > 128 ? 4 : 2;
+  const double cut = 13 + 6 * std::min(1., heads_of / 128) +
+                     2 * std::max(0., heads_of / apart / cus - 0.5) +
+                     std::max(bytes / 6.2e6, heads_of * keys / 64 * 0.9e-3);
+  pl.whole = whole <= cut;
+  pl.heads_per_wg = pl.whole ? best : apart;
+  pl.pair = pl.heads_per_wg > 1;
   pl.head_groups = int(kv_heads / pl.heads_per_wg);
   pl.min_share = 2;
   pl.item_cost = pl.pair ? 16 : 8;
@@ -1427,15 +1435,17 @@ extern "C" int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
   if (blocks == 0) return 0;
   const Plan pl = make_plan(num_decode_rows, num_prefill, cu_seqlens_q_host[num_prefill], blocks,
                             num_heads, num_kv_heads, page_size * max_blocks_per_seq);
-  const double items = double(blocks) * double(num_kv_heads) / (pl.whole && pl.pair ? 2 : 1);
+  const double heads_of = double(blocks) * double(num_kv_heads);
+  const double items = std::ceil(heads_of / pl.heads_per_wg);  // (of a whole plan)
   const double here =
       pl.whole ? std::ceil(items / cu_count()) *
-                     (6 + 2.2 * double(longest) / (pl.pair ? 256 : 512))
-               : 12 + 6 * std::min(1., items / 128) + products * double(num_kv_heads) / 64 * 0.9e-3;
+                     (6 + 2.2 * double(longest) * pl.heads_per_wg / 512)
+               : 12 + 6 * std::min(1., heads_of / 128) +
+                     products * double(num_kv_heads) / 64 * 0.9e-3;
   // Gathered: three launches, the keys written and read once more, the products at the
   // long chunks' rate; and the decode rows in a call of their own.  (Of 371 shapes, 1 to
-  // 8 chunks of 4 to 512 tokens over up to 32768 keys, seven take the form that is over 10 %
-  // slower, 30 % at worst.)
+  // 8 chunks of 4 to 512 tokens over up to 32768 keys, four take the form that is over 10 %
+  // slower, 27 % at worst.)
   const double gathered = (longest <= 64 ? 13 : 22) + 3e-4 * all_keys * double(num_kv_heads) +
                           0.38e-6 * pairs * double(num_heads) + (num_decode_rows > 0 ? 12 : 0);
   return here <= gathered ? blocks : 0;

@@ -206,6 +206,35 @@ def test_decode_batches(batch, lo, hi, heads, kvh):
         fo.check(got, want, bound, f"batch {batch} {lo}..{hi} {i}")
 
 
+@pytest.mark.parametrize("rows,heads,kvh,lo,hi", [(200, 8, 4, 1, 90), (300, 4, 4, 0, 300),
+                                                  (90, 16, 8, 40, 40), (210, 16, 8, 1, 200),
+                                                  (150, 48, 16, 1, 70), (260, 24, 2, 5, 40)])
+def test_decode_many_short_rows(rows, heads, kvh, lo, hi):
+    """Batches whose workgroups take several kv heads of a row whole."""
+    gen = torch.Generator().manual_seed(rows)
+    lens = torch.randint(lo, hi + 1, (rows,), generator=gen).tolist()
+    pool, tables, k, v = fo.paged(lens, 32, kvh, seed=rows + kvh)
+    q = torch.randn(rows, heads, 128, generator=gen).to(BF)
+    got = paged_decode_fp4(q.cuda(), *_dev(pool), tables.cuda(),
+                           torch.tensor(lens, dtype=torch.int32).cuda(), SCALE)
+    want, bound = _expect(q, k, v, lens)
+    fo.check(got, want, bound, f"{rows} rows of {lo} to {hi}")
+
+
+@pytest.mark.parametrize("count,kvh", [(100, 8), (210, 8), (220, 4)])
+def test_many_short_chunks_in_place(count, kvh):
+    """The same of chunks, decode rows among them."""
+    gen = torch.Generator().manual_seed(count)
+    chunks = [(int(n), int(n + m)) for n, m in zip(
+        torch.randint(0, 9, (count,), generator=gen), torch.randint(0, 60, (count,), generator=gen))]
+    decode = torch.randint(0, 60, (20,), generator=gen).tolist()
+    pool, tables, k, v = fo.paged(decode + [m for _, m in chunks], 32, kvh, seed=count + 1)
+    q = torch.randn(20 + sum(n for n, _ in chunks), 2 * kvh, 128, generator=gen).to(BF)
+    want, bound = _chunk_expect(q, k, v, decode, chunks)
+    got = _chunk_call(pool, tables, decode, chunks, q, "known")
+    fo.check(got, want, bound, f"{count} chunks")
+
+
 @pytest.mark.parametrize("scale", [0.0, -SCALE, 1.0, 1e-20])
 def test_decode_scales(scale):
     lens = [70, 200]
