@@ -1052,20 +1052,22 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // keys of one head (64 a wave) or 256, 128 or 64 of more (a wave takes two heads and 32
 // keys).  Cut: two heads a wave, the tiles of all items in equal shares, one a CU, and a
 // second launch joins the pieces.  Estimates in us:
-//   whole  the longer of ceil(items / CUs) (7 + 2.2 a round) and 7 + the keys' bytes at
-//          4.6 TB/s (one head: half lines), 5.6 (two) or 6.8
-//   cut    13, 6 more as the heads' blocks get to 128 and 2 more for every 256 items
-//          (more of them in a share), and the longer of the keys' bytes at 6.2 TB/s and
+//   whole  the longer of ceil(items / CUs) (7 + 2.2 a round of the longest row) and 7 +
+//          the keys' bytes at 4 TB/s (one head: half lines), 6 (two) or 6.4
+//   cut    13.5, 7 more as the heads' blocks get to 128 and 6 more for every 256 items
+//          (more of them in a share), and the longer of the keys' bytes at 6.6 TB/s and
 //          0.9 ns for every 64 keys of a head and block
-// (A batch's keys count as its table's width, so few long rows among many look like
-// more than they are: for those the one-head form's rate is set low.)  Measured, cut /
+// The host knows a batch's longest row by its table's width; its keys are taken as 0.8 of
+// that for every row, between batches of one length and ragged ones, and as half of it
+// where chunks join decode rows (200 rows of 300 to 2000 keys and a chunk over 4000: cut
+// 43, whole 64).  Measured, cut /
 // whole by one, two, four and eight heads (rows x keys; 4 kv heads): 1 x 1000 13.1 /
 // 10.1 / 15.1 / 21.5, 8 x 4096 17 / 23 / 35 / 60, 16 x 8192 26 / 40 / 61 / 113, 64 x 300
 // 19 / 8.3 / 10.7 / 12.9, 64 x 4096 35 / 28 / 38 / 62, 64 x 8192 56 / 60 / 66 / 114, 48 x
 // 1025 to 8007 32 / 40 / 60 / 107, 128 x 1000 28 / 23 / 19 / 23, 128 x 4096 59 / 65 / 52 /
 // 65, 192 x 1000 34 / 34 / 33 / 24, 256 x 300 to 900 34 / 36 / 30 / 23; 8 kv heads: 128 x
 // 300 to 900 34 / 37 / 31 / 24 / 35, 200 x 1000 54 / 82 / 70 / 53 / 44, 400 x 20 to 80 35
-// / 60 / 43 / 28 / 21.  Of 133 shapes the choice is over 5 % off in two, 15 % at worst.
+// / 60 / 43 / 28 / 21.  Of 190 shapes the choice is over 6 % off in four, 21 % at worst.
 Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t chunk_blocks,
                int64_t heads, int64_t kv_heads, int64_t most_keys) {
   Plan pl{};
@@ -1076,11 +1078,12 @@ Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_
   if (chunk_blocks <= 0) chunk_blocks = (chunk_tokens * group + 15 * chunks) / 16;
   const int64_t blocks = decode_rows * ((group + 15) / 16) + chunk_blocks;
   const double heads_of = double(blocks) * double(kv_heads), keys = double(most_keys);
-  const double bytes = double(decode_rows + chunks) * double(kv_heads) * keys *
+  const double part = decode_rows > 0 && chunks > 0 ? 0.5 : 0.8;
+  const double bytes = part * double(decode_rows + chunks) * double(kv_heads) * keys *
                        (2 * (kFp4RowBytes + kFp4Powers));
   int best = 1;
   double whole = 1e30;
-  const double rate[] = {4.6e6, 5.6e6, 6.8e6, 6.8e6};  // bytes a us
+  const double rate[] = {4e6, 6e6, 6.4e6, 6.4e6};  // bytes a us
   for (int i = 0; i < 4 && kv_heads % (1 << i) == 0; ++i) {
     const int n = 1 << i;
     const double t = std::max(std::ceil(heads_of / n / cus) * (7 + 2.2 * keys * n / 512),
@@ -1091,9 +1094,9 @@ Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_
   // against 21.9, one row of 4096 13.5 against 15.7); many share a workgroup better
   // among four (128 rows of 500 to 1500 keys 39.0 against 41.5).
   const int apart = kv_heads % 2 != 0 ? 1 : kv_heads % 4 == 0 && heads_of > 128 ? 4 : 2;
-  const double cut = 13 + 6 * std::min(1., heads_of / 128) +
-                     2 * std::max(0., heads_of / apart / cus - 0.5) +
-                     std::max(bytes / 6.2e6, heads_of * keys / 64 * 0.9e-3);
+  const double cut = 13.5 + 7 * std::min(1., heads_of / 128) +
+                     6 * std::max(0., heads_of / apart / cus - 0.5) +
+                     std::max(bytes / 6.6e6, part * heads_of * keys / 64 * 0.9e-3);
   pl.whole = whole <= cut;
   pl.heads_per_wg = pl.whole ? best : apart;
   pl.pair = pl.heads_per_wg > 1;
@@ -1444,8 +1447,8 @@ extern "C" int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
                      products * double(num_kv_heads) / 64 * 0.9e-3;
   // Gathered: three launches, the keys written and read once more, the products at the
   // long chunks' rate; and the decode rows in a call of their own.  (Of 371 shapes, 1 to
-  // 8 chunks of 4 to 512 tokens over up to 32768 keys, four take the form that is over 10 %
-  // slower, 27 % at worst.)
+  // 8 chunks of 4 to 512 tokens over up to 32768 keys, five take the form that is over 10 %
+  // slower, 25 % at worst.)
   const double gathered = (longest <= 64 ? 13 : 22) + 3e-4 * all_keys * double(num_kv_heads) +
                           0.38e-6 * pairs * double(num_heads) + (num_decode_rows > 0 ? 12 : 0);
   return here <= gathered ? blocks : 0;
