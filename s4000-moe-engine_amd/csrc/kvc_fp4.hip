@@ -1060,14 +1060,13 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // The host knows a batch's longest row by its table's width; its keys are taken as 0.8 of
 // that for every row, between batches of one length and ragged ones, and as half of it
 // where chunks join decode rows (200 rows of 300 to 2000 keys and a chunk over 4000: cut
-// 43, whole 64).  Measured, cut /
-// whole by one, two, four and eight heads (rows x keys; 4 kv heads): 1 x 1000 13.1 /
-// 10.1 / 15.1 / 21.5, 8 x 4096 17 / 23 / 35 / 60, 16 x 8192 26 / 40 / 61 / 113, 64 x 300
+// 43, whole 64).  Measured, cut / whole by one, two, four and eight heads (rows x keys; 4
+// kv heads): 1 x 1000 13.1 / 10.1 / 15.1 / 21.5, 8 x 4096 17 / 23 / 35 / 60, 16 x 8192 26 / 40 / 61 / 113, 64 x 300
 // 19 / 8.3 / 10.7 / 12.9, 64 x 4096 35 / 28 / 38 / 62, 64 x 8192 56 / 60 / 66 / 114, 48 x
 // 1025 to 8007 32 / 40 / 60 / 107, 128 x 1000 28 / 23 / 19 / 23, 128 x 4096 59 / 65 / 52 /
 // 65, 192 x 1000 34 / 34 / 33 / 24, 256 x 300 to 900 34 / 36 / 30 / 23; 8 kv heads: 128 x
 // 300 to 900 34 / 37 / 31 / 24 / 35, 200 x 1000 54 / 82 / 70 / 53 / 44, 400 x 20 to 80 35
-// / 60 / 43 / 28 / 21.  Of 190 shapes the choice is over 6 % off in four, 21 % at worst.
+// / 60 / 43 / 28 / 21.  Of 190 shapes the choice is over 8 % off in four, 21 % at worst.
 Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t chunk_blocks,
                int64_t heads, int64_t kv_heads, int64_t most_keys) {
   Plan pl{};
@@ -1409,7 +1408,8 @@ extern "C" int kvc_varlen_fp4(
                   v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim, block_tables,
                   bt_stride, max_blocks_per_seq, num_decode_rows, decode_context_lens,
                   num_prefill, num_q_tokens - num_decode_rows, chunk_blocks, cu_seqlens_q,
-                  cu_seqlens_k, scale, out, out_stride_t, out_stride_h, workspace, workspace_bytes, stream);
+                  cu_seqlens_k, scale, out, out_stride_t, out_stride_h, workspace,
+                  workspace_bytes, stream);
 }
 
 extern "C" int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
