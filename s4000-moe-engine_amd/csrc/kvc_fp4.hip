@@ -853,9 +853,6 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
       }
       Tile x;
       read_tile<NH>(x, slot0 + slot, lane, lm, lg);
-      smem_drain();
-      if (t + 2 * phases < t_end) issue(t + 2 * phases, lds0 + slot);
-      slot ^= kSlotBytes;
       f32x4_t s[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -868,9 +865,17 @@ __global__ void __launch_bounds__(64 * kWaves, 2) fp4_decode_kernel(Fp4Params p)
       u32x4_t w[2];
 #pragma unroll
       for (int i = 0; i < NH; ++i) weights<16 / NH>(s + 2 * i, c[i], p.c2, w + i);
+      // (a wave at its products goes ahead of one at its softmax: another 0.7 %)
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int h = 0; h < 2; ++h) weigh(x, h, w[h], c[NH == 2 ? h : 0]);
+      __builtin_amdgcn_s_setprio(0);
       add_nan_runs<NH>(x.mine, limit - t * kKeys, c);
+      // (The next loads go out here, not once the tile is read: their addresses and
+      // issue would stand ahead of the scores.  16 rows of 32768 keys 52.6 -> 51.6 us.)
+      smem_drain();
+      if (t + 2 * phases < t_end) issue(t + 2 * phases, lds0 + slot);
+      slot ^= kSlotBytes;
     }
 
     // Channels 16 cb .. + 15 of the wave's columns: the result, or a partial in
