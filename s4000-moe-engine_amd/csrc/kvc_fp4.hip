@@ -18,9 +18,9 @@
 // rows make whole 128-byte lines (loads alone 5.1 against 6.1 TB/s).  Every wave
 // streams its own tiles through its own two LDS slots of 8.5 KiB (direct-to-LDS loads
 // two tiles ahead, no workgroup barrier); eight waves a workgroup, one workgroup a CU,
-// waves differ in kv head and in tile phase.  Bound by HBM reads for batches: 64 rows
-// of 4096 keys (4 kv heads, 143 MB) 33 us, of 8192 51 + 5 to join (47 with the loads
-// alone), 128 of 4096 52: 7 TB/s for every further byte, and 12 to 16 us of launch,
+// waves differ in kv head and in tile phase and join once an item.  Bound by HBM reads for batches: 64 rows
+// of 4096 keys (4 kv heads, 143 MB) 32 us, of 8192 50 + 5 to join (47 with the loads
+// alone), 128 of 4096 51: 7 TB/s for every further byte, and 12 to 16 us of launch,
 // lengths, table, first tiles and last results.  Single rows are bound by that chain:
 // 333 keys 7.1 us.
 #include <algorithm>
