@@ -225,6 +225,26 @@ def test_outputs_are_apart(native, monkeypatch):
         assert keep.tolist() == [-108] and keep.dtype == torch.int32
 
 
+def test_under_inference_mode():
+    """As a server runs: results are ordinary inference tensors, in place and as inputs
+    of the next step."""
+    with torch.inference_mode():
+        t = DeviceBlockTables(3, 4, 16, 9)
+        got = t.step(_i32([17, 1, 0]), 32)
+        again = build_step_tables(got.context_lens, _i32([1, 1, 1]), t.block_tables,
+                                  got.num_blocks, t.free_blocks, got.num_free, 16, 3,
+                                  tokens_per_row=1)
+        assert again.context_lens.tolist() == [18, 2, 1]
+        assert again.positions.tolist() == [17, 1, 0]
+        assert again.slot_mapping.is_inference() and again.positions.is_inference()
+        again.slot_mapping.add_(1)
+        kept = (again.positions + 1).clone()
+    assert kept.tolist() == [18, 2, 1]
+    again = build_step_tables(_i32([0]), _i32([1]), _i32([[-1]]), _i32([0]), _i32([5]), _i32([1]),
+                              16, 1)
+    assert not again.slot_mapping.is_inference() and again.slot_mapping.add_(1).tolist() == [81]
+
+
 def test_empty_shapes():
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
     num = _i32([3])
