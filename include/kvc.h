@@ -808,6 +808,23 @@ int kvc_step_tables(const int32_t* context_lens, const int32_t* query_lens,
                     int32_t* num_blocks_out, int32_t* num_free_out, int32_t* cu_seqlens_q,
                     int32_t* cu_seqlens_k, kvc_stream_t stream);
 
+/* kvc_step_tables, and ended_lens[b] = 0 for every row with finished[b] != 0, whether
+ * or not the row is granted tokens again; other entries are not touched.  For callers
+ * that hold num_blocks in place but write context_lens_out elsewhere (drafted tokens,
+ * of which the accepted ones are added later): with ended_lens over context_lens an
+ * ended row's state is 0 tokens in the pages it now holds.  NULL: none; over no
+ * output and no input but context_lens. */
+int kvc_step_tables_ended(const int32_t* context_lens, const int32_t* query_lens,
+                          const uint8_t* finished, int32_t* ended_lens, int32_t* block_tables,
+                          int64_t bt_stride, int64_t max_blocks_per_seq, int64_t batch,
+                          const int32_t* num_blocks, int32_t* free_blocks, int64_t free_size,
+                          const int32_t* num_free, int64_t page_size, int64_t max_tokens,
+                          int64_t tokens_per_row, int32_t pad_slot, int32_t* slot_mapping,
+                          int64_t* positions, int32_t* query_lens_out, int32_t* seq_lens_out,
+                          int32_t* context_lens_out, int32_t* num_blocks_out,
+                          int32_t* num_free_out, int32_t* cu_seqlens_q, int32_t* cu_seqlens_k,
+                          kvc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

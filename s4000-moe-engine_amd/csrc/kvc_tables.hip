@@ -32,6 +32,7 @@ struct TablesArgs {
   const int32_t* context_lens;
   const int32_t* query_lens;
   const uint8_t* finished;  // or null
+  int32_t* ended;           // lengths set to 0 where finished (context_lens itself, say), or null
   int32_t* tables;
   int64_t bt_stride;
   int width, batch;
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(kMaxThreads) step_tables_kernel(TablesArgs a, 
     const int seen = able ? ctx + got : 0;
     const int z[3] = {take, got, seen};
     const Sums<3> sg = block_sums<3>(z, lds + 2, lane, wave, waves);
+    if (gone && a.ended != nullptr) a.ended[r] = 0;
     if (live) {
       a.query_out[r] = got;
       a.seq_out[r] = seen;
@@ -238,17 +240,14 @@ __global__ void __launch_bounds__(kFillThreads) fill_tokens_kernel(TablesArgs a)
 
 using namespace kvc;
 
-extern "C" int kvc_step_tables(const int32_t* context_lens, const int32_t* query_lens,
-                               const uint8_t* finished, int32_t* block_tables, int64_t bt_stride,
-                               int64_t max_blocks_per_seq, int64_t batch,
-                               const int32_t* num_blocks, int32_t* free_blocks,
-                               int64_t free_size, const int32_t* num_free, int64_t page_size,
-                               int64_t max_tokens, int64_t tokens_per_row, int32_t pad_slot,
-                               int32_t* slot_mapping, int64_t* positions,
-                               int32_t* query_lens_out, int32_t* seq_lens_out,
-                               int32_t* context_lens_out, int32_t* num_blocks_out,
-                               int32_t* num_free_out, int32_t* cu_seqlens_q,
-                               int32_t* cu_seqlens_k, kvc_stream_t stream) {
+extern "C" int kvc_step_tables_ended(
+    const int32_t* context_lens, const int32_t* query_lens, const uint8_t* finished,
+    int32_t* ended_lens, int32_t* block_tables, int64_t bt_stride, int64_t max_blocks_per_seq,
+    int64_t batch, const int32_t* num_blocks, int32_t* free_blocks, int64_t free_size,
+    const int32_t* num_free, int64_t page_size, int64_t max_tokens, int64_t tokens_per_row,
+    int32_t pad_slot, int32_t* slot_mapping, int64_t* positions, int32_t* query_lens_out,
+    int32_t* seq_lens_out, int32_t* context_lens_out, int32_t* num_blocks_out,
+    int32_t* num_free_out, int32_t* cu_seqlens_q, int32_t* cu_seqlens_k, kvc_stream_t stream) {
   clear_error();
   KVC_REQUIRE(batch >= 0 && batch < (1 << 20) && max_blocks_per_seq >= 0 &&
                   batch * max_blocks_per_seq < (int64_t(1) << 30) && free_size >= 0 &&
@@ -285,10 +284,16 @@ extern "C" int kvc_step_tables(const int32_t* context_lens, const int32_t* query
       KVC_REQUIRE(outs[i] == nullptr || outs[i] != outs[j], KVC_ERR_VALUE,
                   "step_tables: two outputs in one place");
   }
+  for (int i = 0; i < 9 && ended_lens != nullptr; ++i)
+    KVC_REQUIRE(outs[i] != ended_lens, KVC_ERR_VALUE, "step_tables: ended_lens over an output");
+  for (int j = 0; j < 7 && ended_lens != nullptr; ++j)
+    KVC_REQUIRE(j == 1 || ins[j] != ended_lens, KVC_ERR_VALUE,
+                "step_tables: ended_lens over another input");
   TablesArgs a{};
   a.context_lens = context_lens;
   a.query_lens = query_lens;
   a.finished = finished;
+  a.ended = ended_lens;
   a.tables = block_tables;
   a.bt_stride = bt_stride;
   a.width = int(max_blocks_per_seq);
@@ -321,4 +326,23 @@ extern "C" int kvc_step_tables(const int32_t* context_lens, const int32_t* query
     fill_tokens_kernel<<<unsigned((max_tokens + kFillThreads - 1) / kFillThreads), kFillThreads, 0,
                          st>>>(a);
   return check_launch("step_tables");
+}
+
+extern "C" int kvc_step_tables(const int32_t* context_lens, const int32_t* query_lens,
+                               const uint8_t* finished, int32_t* block_tables, int64_t bt_stride,
+                               int64_t max_blocks_per_seq, int64_t batch,
+                               const int32_t* num_blocks, int32_t* free_blocks,
+                               int64_t free_size, const int32_t* num_free, int64_t page_size,
+                               int64_t max_tokens, int64_t tokens_per_row, int32_t pad_slot,
+                               int32_t* slot_mapping, int64_t* positions,
+                               int32_t* query_lens_out, int32_t* seq_lens_out,
+                               int32_t* context_lens_out, int32_t* num_blocks_out,
+                               int32_t* num_free_out, int32_t* cu_seqlens_q,
+                               int32_t* cu_seqlens_k, kvc_stream_t stream) {
+  return kvc_step_tables_ended(context_lens, query_lens, finished, nullptr, block_tables,
+                               bt_stride, max_blocks_per_seq, batch, num_blocks, free_blocks,
+                               free_size, num_free, page_size, max_tokens, tokens_per_row,
+                               pad_slot, slot_mapping, positions, query_lens_out, seq_lens_out,
+                               context_lens_out, num_blocks_out, num_free_out, cu_seqlens_q,
+                               cu_seqlens_k, stream);
 }

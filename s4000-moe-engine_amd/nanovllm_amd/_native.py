@@ -138,6 +138,8 @@ SIGNATURES = {
                               _P, _SZ, _P]),
     "kvc_step_tables": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I64,
                                _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "kvc_step_tables_ended": (_INT, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64,
+                                     _I64, _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "kvc_stage_decode": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,
                                 _I64, _I64, _I64, _P, _INT, _P, _INT, _P, _I64, _I64, _P, _P, _P,
                                 _P, _P, _P, _I64, _INT, _INT, _P]),

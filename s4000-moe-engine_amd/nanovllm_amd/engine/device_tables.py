@@ -49,8 +49,8 @@ class DeviceBlockTables:
         """Tensors for step(out=): places that a captured step keeps.  The pages
         held and free are the state itself, and so are the lengths with advance;
         without, out.context_lens is a tensor of its own and the state keeps the
-        lengths from before the step (drafted tokens, of which only the accepted
-        ones will count)."""
+        lengths from before the step, 0 for rows that ended (drafted tokens, of
+        which the caller adds the accepted ones to context_lens)."""
         out = new_step_tables(self.max_rows, max_tokens, self.device)
         out.num_blocks, out.num_free = self.num_blocks, self.num_free
         if advance:
@@ -72,4 +72,5 @@ class DeviceBlockTables:
         return build_step_tables(
             self.context_lens, query_lens, self.block_tables, self.num_blocks, self.free_blocks,
             self.num_free, self.page_size, max_tokens, tokens_per_row=tokens_per_row,
-            finished=finished, pad_slot=self.pad_slot, out=out)
+            finished=finished, pad_slot=self.pad_slot, out=out,
+            clear_ended=finished is not None and not advance)

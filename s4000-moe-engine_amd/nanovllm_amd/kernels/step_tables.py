@@ -54,7 +54,7 @@ def new_step_tables(batch, max_tokens, device) -> StepTables:
 
 def build_step_tables(context_lens, query_lens, block_tables, num_blocks, free_blocks, num_free,
                       page_size, max_tokens, *, tokens_per_row=0, finished=None,
-                      pad_slot=NO_SLOT, out=None) -> StepTables:
+                      pad_slot=NO_SLOT, out=None, clear_ended=False) -> StepTables:
     """Row b of block_tables (int32 [batch, width], changed in place) holds
     num_blocks[b] pages for context_lens[b] tokens and asks for query_lens[b]
     new ones; free_blocks (int32, changed in place) is a stack of num_free[0]
@@ -71,8 +71,11 @@ def build_step_tables(context_lens, query_lens, block_tables, num_blocks, free_b
     row b's begin at b * tokens_per_row (max_tokens is then batch *
     tokens_per_row); entries without a token hold pad_slot and position 0.  out:
     a StepTables to write; its num_blocks, num_free, context_lens and query_lens
-    may be the given ones."""
-    if out is None and nat.is_current(block_tables):
+    may be the given ones.
+
+    clear_ended: set the given context_lens of finished rows to 0 (for lengths that
+    are kept while out.context_lens is another tensor; refused where it is the same)."""
+    if out is None and not clear_ended and nat.is_current(block_tables):
         done = nat.host().step_tables(context_lens, query_lens, block_tables, num_blocks,
                                       free_blocks, num_free, page_size, max_tokens,
                                       tokens_per_row, finished, pad_slot,
@@ -116,10 +119,11 @@ def build_step_tables(context_lens, query_lens, block_tables, num_blocks, free_b
     if out is None:
         out = new_step_tables(batch, max_tokens, dev)
     nat.call_on(
-        block_tables, "kvc_step_tables", context_lens.data_ptr(), query_lens.data_ptr(),
-        nat.ptr(finished), block_tables.data_ptr(), block_tables.stride(0), width, batch,
-        num_blocks.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(), num_free.data_ptr(),
-        page_size, max_tokens, tokens_per_row, pad_slot, out.slot_mapping.data_ptr(),
+        block_tables, "kvc_step_tables_ended", context_lens.data_ptr(), query_lens.data_ptr(),
+        nat.ptr(finished), context_lens.data_ptr() if clear_ended else None,
+        block_tables.data_ptr(), block_tables.stride(0), width, batch, num_blocks.data_ptr(),
+        free_blocks.data_ptr(), free_blocks.numel(), num_free.data_ptr(), page_size, max_tokens,
+        tokens_per_row, pad_slot, out.slot_mapping.data_ptr(),
         out.positions.data_ptr(), out.query_lens.data_ptr(), out.seq_lens.data_ptr(),
         out.context_lens.data_ptr(), out.num_blocks.data_ptr(), out.num_free.data_ptr(),
         out.cu_seqlens_q.data_ptr(), out.cu_seqlens_k.data_ptr(), nat.stream_of(block_tables))

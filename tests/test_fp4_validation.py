@@ -279,6 +279,22 @@ def test_c_step_tables_refuse():
         assert call(**bad) == -1, bad
 
 
+def test_c_step_tables_ended_refuse():
+    """The lengths of ended rows go over context_lens or a place of their own."""
+    lib = _native.load()
+    bufs = [np.zeros(64, dtype=np.int64) for _ in range(17)]
+    p = [_ptr(b) for b in bufs]
+
+    def call(ended):
+        return lib.kvc_step_tables_ended(p[0], p[1], p[6], ended, p[2], 2, 2, 2, p[3], p[4], 4,
+                                         p[5], 32, 4, 0, 0, p[10], p[11], p[7], p[8], p[9], p[12],
+                                         p[13], p[14], p[15], None)
+
+    for i in list(range(1, 16)):
+        assert call(p[i]) == -1, i
+        assert b"ended_lens" in lib.kvc_last_error()
+
+
 def test_device_tables_refuse():
     for bad in ((0, 4, 32, 8), (3, 0, 32, 8), (3, 4, 0, 8), (3, 4, 32, [1, 1]), (3, 4, 32, [-1]),
                 (3, 4, 256, [1 << 23])):

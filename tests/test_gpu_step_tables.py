@@ -327,3 +327,76 @@ def test_captured(tokens):
             assert getattr(out, name).tolist() == w, (i, name)
         assert t.block_tables.tolist() == table and t.free_blocks.tolist() == free
         lens, held, num = want["context_lens"], want["num_blocks"], want["num_free"][0]
+
+
+@pytest.mark.parametrize("capture", [False, True])
+@pytest.mark.parametrize("marks", [torch.bool, torch.uint8])
+def test_drafted_tokens_and_requests_that_end(capture, marks):
+    """advance=False: a step grants drafts, of which some are accepted and added to the
+    state by the caller.  A row whose request ended starts empty in the state too,
+    whether or not a new one takes it in the same step."""
+    rng = random.Random(21)
+    rows, width, page, pages, tokens = 5, 6, 16, 24, 64
+    t = DeviceBlockTables(rows, width, page, pages)
+    new = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    finished = torch.zeros(rows, dtype=marks, device="cuda")
+    out = t.outputs(tokens, advance=False) if capture else None
+
+    def step():
+        return t.step(new, tokens, finished=finished, advance=False, out=out)
+
+    graph = None
+    if capture:
+        state = [t.context_lens, t.num_blocks, t.block_tables, t.free_blocks, t.num_free]
+        saved = [x.clone() for x in state]
+        step()
+        torch.cuda.synchronize()
+        for x, s in zip(state, saved):
+            x.copy_(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+    lens, held = [0] * rows, [0] * rows
+    table, free, num = [[-1] * width for _ in range(rows)], list(range(pages)), pages
+    ended = 0
+    for i in range(40):
+        gone = [rng.random() < 0.15 for _ in range(rows)]
+        ended += sum(g and n > 0 for g, n in zip(gone, lens))
+        asked = [rng.choice([0, 1, 4, 30]) for _ in range(rows)]
+        new.copy_(_i32(asked))
+        finished.copy_(torch.tensor(gone))
+        if graph is None or i % 4 == 3:
+            got = step()
+        else:
+            graph.replay()
+            got = out
+        torch.cuda.synchronize()
+        want = model(lens, asked, table, held, free, num, page, tokens, 0, gone, NO_SLOT)
+        for name, w in want.items():
+            assert getattr(got, name).tolist() == w, (i, name)
+        assert t.block_tables.tolist() == table and t.free_blocks.tolist() == free
+        lens = [0 if g else n for g, n in zip(gone, lens)]
+        assert t.context_lens.tolist() == lens, i
+        held, num = want["num_blocks"], want["num_free"][0]
+        accepted = [rng.randint(0, g) for g in want["query_lens"]]
+        t.context_lens.add_(_i32(accepted))
+        lens = [n + a for n, a in zip(lens, accepted)]
+    assert ended > 5
+
+
+def test_ended_lengths_of_the_state_alone():
+    """clear_ended touches the lengths of rows that ended, and without it none."""
+    for clear in (False, True):
+        lens = _i32([40, 20, 7])
+        build_step_tables(lens, _i32([1, 0, 1]), _i32([[0, 1], [2, 3], [4, -1]]), _i32([2, 2, 1]),
+                          _i32([0] * 8), _i32([0]), 32, 4,
+                          finished=torch.tensor([True, True, False]).cuda(),
+                          clear_ended=clear)
+        assert lens.tolist() == ([0, 0, 7] if clear else [40, 20, 7])
+    lens = _i32([40])
+    with pytest.raises(ValueError, match="ended"):
+        out = new_step_tables(1, 4, "cuda")
+        out.context_lens = lens
+        build_step_tables(lens, _i32([1]), _i32([[0, 1]]), _i32([2]), _i32([0] * 4), _i32([0]), 32,
+                          4, finished=torch.tensor([True]).cuda(), clear_ended=True, out=out)
+    assert lens.tolist() == [40]
