@@ -187,11 +187,19 @@ def paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, contex
 
 
 def varlen_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, num_decode_rows,
-               decode_context_lens, chunk_blocks, cu_seqlens_q, cu_seqlens_k, scale, out):
+               decode_context_lens, chunk_blocks, cu_seqlens_q, cu_seqlens_k, scale, out,
+               num_prefill=None):
     """varlen_attention's rows over a 4-bit pool read as it is
     (kvc_varlen_fp4), into out; arguments as varlen_attention checked and
-    converted them, int32 offsets on q's device."""
-    num_prefill = cu_seqlens_q.numel() - 1
+    converted them, int32 offsets on q's device.  num_prefill: the chunks, whose
+    offsets come first in tensors that may be longer (by default all of
+    cu_seqlens_q)."""
+    if num_prefill is None:
+        num_prefill = cu_seqlens_q.numel() - 1
+    if min(cu_seqlens_q.numel(), cu_seqlens_k.numel()) < num_prefill + 1:
+        raise ValueError("cu_seqlens_q / cu_seqlens_k have fewer entries than the call has chunks")
+    if num_decode_rows and decode_context_lens.numel() < num_decode_rows:
+        raise ValueError("decode_context_lens has fewer entries than the call has decode rows")
     _one_device(k_cache, q=q, block_tables=block_tables, cu_seqlens_q=cu_seqlens_q,
                 cu_seqlens_k=cu_seqlens_k)
     if num_decode_rows:

@@ -103,6 +103,8 @@ def _prepare(q, k_cache, v_cache, block_tables, num_decode_rows, decode_context_
             cu_seqlens_q = torch.from_numpy(cu_q_np).to(q.device, non_blocking=True)
         if cu_seqlens_k is None or cu_seqlens_k.device != q.device:
             cu_seqlens_k = torch.from_numpy(cu_k_np).to(q.device, non_blocking=True)
+        if min(cu_seqlens_q.numel(), cu_seqlens_k.numel()) < c.num_prefill + 1:
+            raise ValueError("cu_seqlens_q / cu_seqlens_k have fewer entries than their lists")
         cu_seqlens_q = cu_seqlens_q.to(torch.int32).contiguous()
         cu_seqlens_k = cu_seqlens_k.to(torch.int32).contiguous()
     c.cu_seqlens_q, c.cu_seqlens_k = cu_seqlens_q, cu_seqlens_k
@@ -120,6 +122,8 @@ def _prepare(q, k_cache, v_cache, block_tables, num_decode_rows, decode_context_
         c.max_blocks = block_tables.size(1)
     c.block_tables = block_tables
     if num_decode_rows:
+        if decode_context_lens.numel() < num_decode_rows:
+            raise ValueError("decode_context_lens has fewer entries than the call has decode rows")
         decode_context_lens = decode_context_lens.to(torch.int32).contiguous()
     c.decode_context_lens = decode_context_lens
     c.ws_bytes = nat.query("kvc_varlen_workspace_bytes", T, num_heads, c.num_kv_heads, head_dim,
@@ -202,7 +206,7 @@ def _paged_rows(c, q, nd, k_cache, v_cache, scale, k_scale, v_scale, side_k, sid
     """The decode rows 0 .. nd - 1 of a mixed call alone (no prefill chunks)."""
     if c.enc == nat.KVC_KV_FP4:
         paged_decode_fp4(q[:nd], k_cache, v_cache, k_scale, v_scale, c.block_tables[:nd],
-                         c.decode_context_lens, scale, c.out[:nd])
+                         c.decode_context_lens.view(-1)[:nd], scale, c.out[:nd])
         return
     nat.call(
         "kvc_varlen_attention",
@@ -257,7 +261,7 @@ def varlen_attention(q, k_cache, v_cache, *, scale, block_tables=None,
         if blocks:
             return varlen_fp4(q, k_cache, v_cache, k_scale, v_scale, c.block_tables,
                               num_decode_rows, c.decode_context_lens, blocks, c.cu_seqlens_q,
-                              c.cu_seqlens_k, scale, c.out)
+                              c.cu_seqlens_k, scale, c.out, num_prefill=c.num_prefill)
     gathered = (enc != nat.KVC_KV_BF16 and not fresh and c.num_prefill
                 and (enc == nat.KVC_KV_FP4 or os.environ.get("KVC_PREFILL_SK", "1") != "0"))
     has_side = enc == nat.KVC_KV_INT8_CHAN and side_k is not None and head_n_out is not None

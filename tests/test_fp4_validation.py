@@ -23,6 +23,10 @@ U8 = torch.uint8
 BF = torch.bfloat16
 
 
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
 def _pool(blocks=4, page=32, kvh=2, **kw):
     p = dict(k_cache=torch.zeros(blocks, page, kvh, 64, dtype=U8),
              v_cache=torch.zeros(blocks, page, kvh, 64, dtype=U8),
@@ -139,6 +143,66 @@ def test_varlen_needs_scales():
                          cu_seqlens_q_list=[0, 3], cu_seqlens_k_list=[0, 3])
 
 
+@pytest.fixture
+def recorded(monkeypatch):
+    """Device calls recorded instead of made: what the checks let through, on the CPU."""
+    calls = []
+    monkeypatch.setattr(_native, "require_device", lambda *_: None)
+    monkeypatch.setattr(_native, "stream_of", lambda *_: 0)
+    monkeypatch.setattr(_native, "call_on", lambda t, name, *args: calls.append((name, args)))
+    monkeypatch.setattr(_native, "call", lambda name, *args: calls.append((name, args)))
+    return calls
+
+
+def _varlen(cu_q, cu_k, list_q, list_k, tables=1, decode=0, lens=None, width=1):
+    p = _pool()
+    q = torch.zeros(decode + list_q[-1], 8, 128, dtype=BF)
+    varlen_attention(q, p["k_cache"], p["v_cache"], scale=0.1,
+                     block_tables=torch.zeros(tables, width, dtype=torch.int32),
+                     num_decode_rows=decode, decode_context_lens=lens, cu_seqlens_q=cu_q,
+                     cu_seqlens_k=cu_k, cu_seqlens_q_list=list_q, cu_seqlens_k_list=list_k,
+                     k_scale=p["k_scale"], v_scale=p["v_scale"])
+
+
+def test_varlen_sequences_are_those_of_the_host_lists(recorded):
+    """Offsets and lengths in tensors longer than the call's: what lies behind is not
+    the call's, and needs no table rows."""
+    long_q, long_k = _i32(0, 3, 5, 9), _i32(0, 20, 31, 40)
+    _varlen(long_q, long_k, [0, 3], [0, 20])
+    (name, args), = recorded
+    assert name == "kvc_varlen_fp4" and args[18] == 1
+    recorded.clear()
+    _varlen(long_q, long_k, [0, 3], [0, 20], tables=3, decode=2, lens=_i32(4, 5, 6, 7))
+    (name, args), = recorded
+    assert name == "kvc_varlen_fp4" and args[16] == 2 and args[18] == 1
+    recorded.clear()
+    # decode rows alone
+    _varlen(long_q, long_k, [0], [0], tables=2, decode=2, lens=_i32(4, 5, 6, 7))
+    (name, args), = recorded
+    assert name == "kvc_paged_decode_fp4"
+
+
+@pytest.mark.parametrize("kw", [
+    dict(cu_q=_i32(0, 3)), dict(cu_k=_i32(0, 20)), dict(cu_k=_i32()), dict(lens=_i32(4)),
+])
+def test_varlen_refuses_short_offsets_and_lengths(recorded, kw):
+    args = dict(cu_q=_i32(0, 3, 5), cu_k=_i32(0, 20, 31), list_q=[0, 3, 5], list_k=[0, 20, 31],
+                tables=4, decode=2, lens=_i32(4, 5))
+    _varlen(**args)
+    assert len(recorded) == 1
+    recorded.clear()
+    with pytest.raises(ValueError, match="fewer"):
+        _varlen(**{**args, **kw})
+    assert not recorded
+    long = dict(list_q=[0, 500, 512], list_k=[0, 20000, 30000])       # gathered
+    _varlen(**{**args, **long})
+    assert [n for n, _ in recorded][:2] == ["kvc_paged_decode_fp4", "kvc_gather_kv_fp4"]
+    recorded.clear()
+    with pytest.raises(ValueError, match="fewer"):
+        _varlen(**{**args, **long, **kw})
+    assert not recorded
+
+
 # --- the C entries ----------------------------------------------------------------
 
 def _ptr(a):
@@ -221,10 +285,6 @@ def test_in_place_rule_is_host_only_and_monotone():
 
 
 # --- step tables ------------------------------------------------------------------
-
-def _i32(*v):
-    return torch.tensor(v, dtype=torch.int32)
-
 
 def _tables_args(batch=3, width=4, **kw):
     a = dict(context_lens=torch.zeros(batch, dtype=torch.int32),

@@ -739,3 +739,34 @@ def test_library_refuses_bad_device_calls():
     lib = _native.load()
     buf = np.zeros(64, dtype=np.uint8)
     assert lib.kvc_dequant_fp4(buf.ctypes.data, buf.ctypes.data, 1, 64, buf.ctypes.data, None) == -1
+
+
+@pytest.mark.parametrize("decode,chunks,width", [
+    ([40, 3], [(5, 700), (2, 65)], None), ([40, 3], [(5, 700), (2, 65)], 2200), ([], [(9, 90)], 2200),
+    ([90, 70], [(300, 900)], None), ([33, 50], [], None)])
+@pytest.mark.parametrize("native", [True, False])
+def test_offsets_in_longer_tensors(decode, chunks, width, native, monkeypatch):
+    """Offsets and lengths at the head of longer buffers, with table rows of others
+    behind the call's: read in place whole and cut, and gathered."""
+    if not native:
+        monkeypatch.setattr(_native, "_host", _native._NoHostPath)
+    lens = decode + [m for _, m in chunks]
+    pool, tables, k, v = fo.paged(lens + [60, 80], 32, 2, seed=70 + len(lens))
+    gen = torch.Generator().manual_seed(30)
+    q = torch.randn(len(decode) + sum(n for n, _ in chunks), 8, 128, generator=gen).to(BF)
+    cu_q, cu_k = [0], [0]
+    for n, m in chunks:
+        cu_q.append(cu_q[-1] + n)
+        cu_k.append(cu_k[-1] + m)
+    kc, vc, ks, vs = _dev(pool)
+    t = torch.full((tables.size(0), width or tables.size(1)), -1, dtype=torch.int32)
+    t[:, :tables.size(1)] = tables
+    behind_q, behind_k = [cu_q[-1] + 1, 2], [cu_k[-1] + 60, cu_k[-1] + 140]
+    got = varlen_attention(
+        q.cuda(), kc, vc, scale=SCALE, block_tables=t.cuda(), num_decode_rows=len(decode),
+        decode_context_lens=torch.tensor(decode + [60, 80], dtype=torch.int32).cuda(),
+        cu_seqlens_q=torch.tensor(cu_q + behind_q, dtype=torch.int32).cuda(),
+        cu_seqlens_k=torch.tensor(cu_k + behind_k, dtype=torch.int32).cuda(),
+        cu_seqlens_q_list=cu_q, cu_seqlens_k_list=cu_k, k_scale=ks, v_scale=vs)
+    want, bound = _chunk_expect(q, k, v, decode, chunks)
+    fo.check(got, want, bound, f"{decode} {chunks} in longer tensors")
