@@ -734,6 +734,19 @@ int kvc_paged_decode_fp4(const void* q, int64_t q_stride_b, int64_t q_stride_h,
                          float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
                          void* workspace, size_t workspace_bytes, kvc_stream_t stream);
 
+/* kvc_store_fp4 of num_tokens rows, then kvc_paged_decode_fp4 (whose workspace it
+ * takes; context_lens count the new tokens): the whole call is checked before
+ * anything is stored. */
+int kvc_paged_decode_append_fp4(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* key, int64_t key_stride_n,
+    int64_t key_stride_h, const void* value, int64_t value_stride_n, int64_t value_stride_h,
+    const void* slot_mapping, int slot_index_bytes, int64_t num_tokens, uint8_t* k_cache,
+    uint8_t* v_cache, uint8_t* k_scale, uint8_t* v_scale, int64_t num_cache_blocks,
+    int64_t page_size, int64_t num_kv_heads, int64_t head_dim, const int32_t* block_tables,
+    int64_t bt_stride, int64_t max_blocks_per_seq, const int32_t* context_lens, int64_t batch,
+    int64_t num_heads, float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
+    void* workspace, size_t workspace_bytes, kvc_stream_t stream);
+
 /* kvc_varlen_attention's rows over a 4-bit pool, read as it is (nothing is
  * gathered): num_decode_rows rows of one token over decode_context_lens, then
  * num_prefill chunks, chunk i's queries at rows num_decode_rows +

@@ -1123,6 +1123,19 @@ Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_
   return pl;
 }
 
+// An append's arguments, its checks and its launch.
+struct Append {
+  const void* key;
+  int64_t k_sn, k_sh;
+  const void* value;
+  int64_t v_sn, v_sh;
+  uint8_t *k, *v, *ks, *vs;
+  int64_t num_slots;
+  const void* slots;
+  int slot_bytes;
+  int64_t tokens, kv_heads;
+};
+
 int check_rows(const char* what, const void* key, int64_t k_sn, int64_t k_sh, const void* value,
                int64_t v_sn, int64_t v_sh, int64_t num_tokens, int64_t kv_heads, int64_t head_dim,
                int slot_index_bytes) {
@@ -1153,6 +1166,27 @@ int check_pool(const char* what, const void* k, const void* v, const void* ks, c
   return KVC_OK;
 }
 
+int check_append(const char* what, const Append& a, int64_t head_dim) {
+  int rc = check_rows(what, a.key, a.k_sn, a.k_sh, a.value, a.v_sn, a.v_sh, a.tokens, a.kv_heads,
+                      head_dim, a.slot_bytes);
+  if (rc != KVC_OK || a.tokens == 0) return rc;
+  rc = check_pool(what, a.k, a.v, a.ks, a.vs);
+  if (rc != KVC_OK) return rc;
+  KVC_REQUIRE(a.key != nullptr && a.value != nullptr && a.slots != nullptr, KVC_ERR_VALUE,
+              "%s: null rows or slots", what);
+  return KVC_OK;
+}
+
+void launch_append(const Append& a, hipStream_t st) {
+  if (a.tokens == 0) return;
+  const int64_t rows = a.tokens * a.kv_heads;
+  const dim3 grid(unsigned((rows + kRowsPerBlock - 1) / kRowsPerBlock));
+  auto kern = a.slot_bytes == 8 ? store_fp4_kernel<8> : store_fp4_kernel<4>;
+  kern<<<grid, kThreads, 0, st>>>(
+      static_cast<const uint16_t*>(a.key), a.k_sn, a.k_sh, static_cast<const uint16_t*>(a.value),
+      a.v_sn, a.v_sh, a.k, a.v, a.ks, a.vs, a.num_slots, a.slots, a.tokens, int(a.kv_heads));
+}
+
 }  // namespace
 }  // namespace kvc
 
@@ -1165,21 +1199,12 @@ extern "C" int kvc_store_fp4(const void* key, int64_t key_stride_n, int64_t key_
                              int slot_index_bytes, int64_t num_tokens, int64_t num_kv_heads,
                              int64_t head_dim, kvc_stream_t stream) {
   clear_error();
-  int rc = check_rows("store_fp4", key, key_stride_n, key_stride_h, value, value_stride_n,
-                      value_stride_h, num_tokens, num_kv_heads, head_dim, slot_index_bytes);
-  if (rc != KVC_OK) return rc;
-  if (num_tokens == 0) return KVC_OK;
-  rc = check_pool("store_fp4", k_cache, v_cache, k_scale, v_scale);
-  if (rc != KVC_OK) return rc;
-  KVC_REQUIRE(key != nullptr && value != nullptr && slot_mapping != nullptr, KVC_ERR_VALUE,
-              "store_fp4: null rows or slots");
-  const int64_t rows = num_tokens * num_kv_heads;
-  const dim3 grid(unsigned((rows + kRowsPerBlock - 1) / kRowsPerBlock));
-  auto kern = slot_index_bytes == 8 ? store_fp4_kernel<8> : store_fp4_kernel<4>;
-  kern<<<grid, kThreads, 0, as_stream(stream)>>>(
-      static_cast<const uint16_t*>(key), key_stride_n, key_stride_h,
-      static_cast<const uint16_t*>(value), value_stride_n, value_stride_h, k_cache, v_cache,
-      k_scale, v_scale, num_slots, slot_mapping, num_tokens, int(num_kv_heads));
+  const Append a{key,     key_stride_n, key_stride_h, value,   value_stride_n,
+                 value_stride_h, k_cache, v_cache, k_scale, v_scale,
+                 num_slots, slot_mapping, slot_index_bytes, num_tokens, num_kv_heads};
+  const int rc = check_append("store_fp4", a, head_dim);
+  if (rc != KVC_OK || num_tokens == 0) return rc;
+  launch_append(a, as_stream(stream));
   return check_launch("store_fp4");
 }
 
@@ -1241,7 +1266,8 @@ extern "C" int kvc_gather_kv_fp4(const uint8_t* k_cache, const uint8_t* v_cache,
 }
 
 namespace {
-int run_rows(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_t heads,
+// append (or null): launched ahead of the rows, once the whole call has been checked.
+int run_rows(const char* what, const Append* append, const void* q, int64_t q_st, int64_t q_sh, int64_t heads,
              const uint8_t* k_cache, const uint8_t* v_cache, const uint8_t* k_scale,
              const uint8_t* v_scale, int64_t blocks, int64_t page, int64_t kv_heads,
              int64_t head_dim, const int32_t* tables, int64_t bt_stride, int64_t max_blocks,
@@ -1264,7 +1290,11 @@ int run_rows(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_
                   decode_rows + chunks + chunk_tokens < (int64_t(1) << 24) &&
                   chunk_tokens * (heads / kv_heads) < (int64_t(1) << 24),
               KVC_ERR_VALUE, "%s: too many rows", what);
-  if (decode_rows + chunk_tokens == 0 || decode_rows + chunks == 0) return KVC_OK;
+  if (decode_rows + chunk_tokens == 0 || decode_rows + chunks == 0) {
+    if (append == nullptr || append->tokens == 0) return KVC_OK;
+    launch_append(*append, as_stream(stream));
+    return check_launch(what);
+  }
   const int rc = check_pool(what, k_cache, v_cache, k_scale, v_scale);
   if (rc != KVC_OK) return rc;
   KVC_REQUIRE(q != nullptr && out != nullptr && (lens != nullptr || decode_rows == 0) &&
@@ -1345,6 +1375,7 @@ int run_rows(const char* what, const void* q, int64_t q_st, int64_t q_sh, int64_
   KVC_REQUIRE(e == hipSuccess, KVC_ERR_RUNTIME, "%s: LDS limit: %s", what, hipGetErrorString(e));
   auto kern = chunks > 0 ? (pl.pair ? fp4_decode_kernel<2, true> : fp4_decode_kernel<1, true>)
                          : (pl.pair ? fp4_decode_kernel<2, false> : fp4_decode_kernel<1, false>);
+  if (append != nullptr) launch_append(*append, st);
   kern<<<pl.grid, 64 * kWaves, kLds, st>>>(p);
   if (!pl.whole) {
     const int64_t pieces = pl.grid / std::max<int64_t>(pl.items, 1) + 2;  // of an item
@@ -1376,8 +1407,31 @@ extern "C" int kvc_paged_decode_fp4(
     int64_t out_stride_b, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
     kvc_stream_t stream) {
   clear_error();
-  return run_rows("paged_decode_fp4", q, q_stride_b, q_stride_h, num_heads, k_cache, v_cache,
+  return run_rows("paged_decode_fp4", nullptr, q, q_stride_b, q_stride_h, num_heads, k_cache, v_cache,
                   k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim,
+                  block_tables, bt_stride, max_blocks_per_seq, batch, context_lens, 0, 0, 0,
+                  nullptr, nullptr, scale, out, out_stride_b, out_stride_h, workspace,
+                  workspace_bytes, stream);
+}
+
+extern "C" int kvc_paged_decode_append_fp4(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* key, int64_t key_stride_n,
+    int64_t key_stride_h, const void* value, int64_t value_stride_n, int64_t value_stride_h,
+    const void* slot_mapping, int slot_index_bytes, int64_t num_tokens, uint8_t* k_cache,
+    uint8_t* v_cache, uint8_t* k_scale, uint8_t* v_scale, int64_t num_cache_blocks,
+    int64_t page_size, int64_t num_kv_heads, int64_t head_dim, const int32_t* block_tables,
+    int64_t bt_stride, int64_t max_blocks_per_seq, const int32_t* context_lens, int64_t batch,
+    int64_t num_heads, float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
+    void* workspace, size_t workspace_bytes, kvc_stream_t stream) {
+  clear_error();
+  const Append a{key,       key_stride_n, key_stride_h, value,   value_stride_n,
+                 value_stride_h, k_cache, v_cache, k_scale, v_scale,
+                 num_cache_blocks * page_size, slot_mapping, slot_index_bytes, num_tokens,
+                 num_kv_heads};
+  const int rc = check_append("paged_decode_append_fp4", a, head_dim);
+  if (rc != KVC_OK) return rc;
+  return run_rows("paged_decode_append_fp4", &a, q, q_stride_b, q_stride_h, num_heads, k_cache,
+                  v_cache, k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim,
                   block_tables, bt_stride, max_blocks_per_seq, batch, context_lens, 0, 0, 0,
                   nullptr, nullptr, scale, out, out_stride_b, out_stride_h, workspace,
                   workspace_bytes, stream);
@@ -1409,8 +1463,8 @@ extern "C" int kvc_varlen_fp4(
   clear_error();
   KVC_REQUIRE(num_decode_rows >= 0 && num_decode_rows <= num_q_tokens, KVC_ERR_VALUE,
               "varlen_fp4: more decode rows than query rows");
-  return run_rows("varlen_fp4", q, q_stride_t, q_stride_h, num_heads, k_cache, v_cache, k_scale,
-                  v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim, block_tables,
+  return run_rows("varlen_fp4", nullptr, q, q_stride_t, q_stride_h, num_heads, k_cache, v_cache,
+                  k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim, block_tables,
                   bt_stride, max_blocks_per_seq, num_decode_rows, decode_context_lens,
                   num_prefill, num_q_tokens - num_decode_rows, chunk_blocks, cu_seqlens_q,
                   cu_seqlens_k, scale, out, out_stride_t, out_stride_h, workspace,

@@ -45,6 +45,7 @@ decltype(&kvc_gather_kv_fp4) p_gather_fp4;
 decltype(&kvc_varlen_fp4_workspace_bytes) p_varlen_fp4_workspace;
 decltype(&kvc_varlen_fp4_blocks) p_varlen_fp4_blocks;
 decltype(&kvc_varlen_fp4) p_varlen_fp4;
+decltype(&kvc_paged_decode_append_fp4) p_append_fp4;
 decltype(&kvc_step_tables) p_step_tables;
 
 // The tensor behind an exact torch.Tensor / Parameter, else null.
@@ -706,10 +707,6 @@ bool fp4_append(PyObject* key, PyObject* value, PyObject* slot_mapping, const Fp
   r.k = rows(k), r.v = rows(v), r.slots = address(slots);
   return true;
 }
-int fp4_store_call(const Fp4Append& r, const Fp4Pool& p, void* stream) {
-  return p_store_fp4(r.k.p, r.k.s0, r.k.s1, r.v.p, r.v.s0, r.v.s1, p.k, p.v, p.ks, p.vs,
-                     p.pages * p.page, r.slots, r.sb, r.n, p.kvh, 128, stream);
-}
 
 // fp4_store(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, stream):
 // True, or None.
@@ -734,7 +731,9 @@ PyObject* fp4_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int rc;
   {
     Unlocked unlocked;
-    rc = fp4_store_call(rows_, pool, stream);
+    rc = p_store_fp4(rows_.k.p, rows_.k.s0, rows_.k.s1, rows_.v.p, rows_.v.s0, rows_.v.s1, pool.k,
+                     pool.v, pool.ks, pool.vs, pool.pages * pool.page, rows_.slots, rows_.sb,
+                     rows_.n, pool.kvh, 128, stream);
   }
   if (rc != KVC_OK) return fail(rc, "kvc_store_fp4");
   Py_RETURN_TRUE;
@@ -744,8 +743,8 @@ PyObject* fp4_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
 //          num_decode_rows, decode_context_lens, cu_seqlens_q or None, cu_seqlens_k,
 //          cu_seqlens_q_list or None, cu_seqlens_k_list, scale, stream, key or None,
 //          value, slot_mapping): decode rows and chunks that are read in place
-// (chunks without their host lists, or that are better gathered, are declined), after
-// the append of their tokens if there is a key.
+// (chunks without their host lists, or that are better gathered, are declined); with
+// a key decode rows alone, after the append of their tokens.
 PyObject* fp4_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 18) {
     PyErr_SetString(PyExc_TypeError, "fp4_rows takes 18 arguments");
@@ -804,8 +803,9 @@ PyObject* fp4_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
     }
     if (bt->size(0) < decode_rows + prefill) Py_RETURN_NONE;
-    if (a[15] != Py_None &&
-        (!fp4_append(a[15], a[16], a[17], pool, *q, append) || append.n != tokens))
+    if (a[15] != Py_None && (prefill > 0 || decode_rows != tokens ||
+                             !fp4_append(a[15], a[16], a[17], pool, *q, append) ||
+                             append.n != tokens))
       Py_RETURN_NONE;
     if (a[0] != Py_None) {
       const at::Tensor* given = tensor(a[0]);
@@ -827,18 +827,25 @@ PyObject* fp4_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   } catch (const std::exception&) {
     return declined();
   }
-  int rc = KVC_OK;
+  int rc;
   {
     Unlocked unlocked;
-    if (append.n > 0) rc = fp4_store_call(append, pool, stream);
-    if (rc == KVC_OK)
+    if (append.n > 0)
+      rc = p_append_fp4(q_r.p, q_r.s0, q_r.s1, append.k.p, append.k.s0, append.k.s1, append.v.p,
+                        append.v.s0, append.v.s1, append.slots, append.sb, append.n, pool.k,
+                        pool.v, pool.ks, pool.vs, pool.pages, pool.page, pool.kvh, 128,
+                        static_cast<int32_t*>(bt_p), bt_stride, blocks,
+                        static_cast<int32_t*>(lens_p), decode_rows, heads, scale, out_r.p,
+                        out_r.s0, out_r.s1, ws_p, bytes, stream);
+    else
       rc = p_varlen_fp4(q_r.p, q_r.s0, q_r.s1, tokens, heads, pool.k, pool.v, pool.ks, pool.vs,
                         pool.pages, pool.page, pool.kvh, 128, static_cast<int32_t*>(bt_p),
                         bt_stride, blocks, decode_rows, static_cast<int32_t*>(lens_p), prefill,
                         chunk_blocks, static_cast<int32_t*>(cuq_p), static_cast<int32_t*>(cuk_p),
                         scale, out_r.p, out_r.s0, out_r.s1, ws_p, bytes, stream);
   }
-  if (rc != KVC_OK) return fail(rc, "kvc_varlen_fp4");
+  if (rc != KVC_OK)
+    return fail(rc, append.n > 0 ? "kvc_paged_decode_append_fp4" : "kvc_varlen_fp4");
   if (a[0] != Py_None) {
     Py_INCREF(a[0]);
     return a[0];
@@ -1034,6 +1041,7 @@ PyObject* bind(PyObject*, PyObject* path) {
       !resolve(lib, "kvc_varlen_fp4_workspace_bytes", p_varlen_fp4_workspace) ||
       !resolve(lib, "kvc_varlen_fp4_blocks", p_varlen_fp4_blocks) ||
       !resolve(lib, "kvc_varlen_fp4", p_varlen_fp4) ||
+      !resolve(lib, "kvc_paged_decode_append_fp4", p_append_fp4) ||
       !resolve(lib, "kvc_step_tables", p_step_tables))
     return nullptr;
   Py_RETURN_NONE;

@@ -131,6 +131,10 @@ SIGNATURES = {
     "kvc_paged_decode_fp4": (_INT, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P,
                                     _I64, _I64, _P, _I64, _I64, _F32, _P, _I64, _I64, _P, _SZ,
                                     _P]),
+    "kvc_paged_decode_append_fp4": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P,
+                                           _INT, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P,
+                                           _I64, _I64, _P, _I64, _I64, _F32, _P, _I64, _I64, _P,
+                                           _SZ, _P]),
     "kvc_varlen_fp4_workspace_bytes": (_SZ, [_I64] * 8),
     "kvc_varlen_fp4_blocks": (_I64, [_P, _P] + [_I64] * 6),
     "kvc_varlen_fp4": (_INT, [_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64,

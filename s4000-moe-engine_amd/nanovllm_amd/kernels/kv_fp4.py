@@ -47,6 +47,18 @@ def _one_device(pool, **tensors):
             raise ValueError(f"{name} must be on the pool's device")
 
 
+def _append_rows(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping):
+    """An append's arguments, checked: its slots and their bytes."""
+    check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
+    if key.ndim != 3 or value.shape != key.shape or key.shape[1:] != (k_cache.size(2), 128):
+        raise ValueError("expected key/value=[tokens,kv_heads,128]")
+    _check_rows(key, value)
+    assert slot_mapping.numel() == key.size(0)
+    _one_device(k_cache, key=key, value=value, slot_mapping=slot_mapping)
+    nat.require_device(k_cache)
+    return _slots(slot_mapping)
+
+
 def store_kvcache_fp4(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping):
     """store_kvcache into a 4-bit pool: key / value [N, KVH, 128] bf16 rows
     quantised at slot_mapping (int32 or int64 [N]; a negative slot counts from
@@ -55,20 +67,12 @@ def store_kvcache_fp4(key, value, k_cache, v_cache, k_scale, v_scale, slot_mappi
     if nat.is_current(key) and nat.host().fp4_store(key, value, k_cache, v_cache, k_scale,
                                                     v_scale, slot_mapping, nat.stream_of(key)):
         return
-    check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
-    if key.ndim != 3 or value.shape != key.shape or key.shape[1:] != (k_cache.size(2), 128):
-        raise ValueError("expected key/value=[tokens,kv_heads,128]")
-    _check_rows(key, value)
-    N, KVH, D = key.shape
-    assert slot_mapping.numel() == N
-    _one_device(k_cache, key=key, value=value, slot_mapping=slot_mapping)
-    nat.require_device(k_cache)
-    slots, sb = _slots(slot_mapping)
+    slots, sb = _append_rows(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
     nat.call_on(
         k_cache, "kvc_store_fp4", key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
         value.stride(0), value.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
         k_scale.data_ptr(), v_scale.data_ptr(), k_cache.size(0) * k_cache.size(1),
-        slots.data_ptr(), sb, N, KVH, D, nat.stream_of(k_cache))
+        slots.data_ptr(), sb, key.size(0), key.size(1), 128, nat.stream_of(k_cache))
 
 
 def dequant_fp4(codes, scale):
@@ -128,16 +132,9 @@ def _rows16(t):
             and t.data_ptr() % 16 == 0)
 
 
-def paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, scale,
-                     out=None):
-    """paged_decode_attention over a 4-bit pool, written to `out` if given.  A
-    row with context_lens[b] <= 0 gives zeros."""
-    if nat.is_current(q):
-        done = nat.host().fp4_rows(out, q, k_cache, v_cache, k_scale, v_scale, block_tables,
-                                   q.size(0) if q.ndim else 0, context_lens, None, None, None,
-                                   None, scale, nat.stream_of(q), None, None, None)
-        if done is not None:
-            return done
+def _decode_rows(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, out):
+    """A decode call's arguments, checked and in the library's form: q, block_tables,
+    context_lens, out, the bytes of its workspace."""
     check_fp4_pool(k_cache, v_cache, k_scale, v_scale)
     if q.ndim != 3:
         raise ValueError("expected q=[batch,heads,dim], kv=[pages,page,kv_heads,64]")
@@ -170,18 +167,32 @@ def paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, contex
         context_lens = context_lens.to(torch.int32).contiguous()
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if batch == 0:
-        return out
-    max_blocks = block_tables.size(1)
     need = nat.query("kvc_paged_decode_fp4_workspace_bytes", batch, num_heads, num_kv_heads,
-                     page_size, max_blocks)
+                     page_size, block_tables.size(1))
+    return q, block_tables, context_lens, out, need
+
+
+def paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, scale,
+                     out=None):
+    """paged_decode_attention over a 4-bit pool, written to `out` if given.  A
+    row with context_lens[b] <= 0 gives zeros."""
+    if nat.is_current(q):
+        done = nat.host().fp4_rows(out, q, k_cache, v_cache, k_scale, v_scale, block_tables,
+                                   q.size(0) if q.ndim else 0, context_lens, None, None, None,
+                                   None, scale, nat.stream_of(q), None, None, None)
+        if done is not None:
+            return done
+    q, block_tables, context_lens, out, need = _decode_rows(
+        q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, out)
+    if q.size(0) == 0:
+        return out
     ws = nat.workspace(need, q.device)
     nat.call_on(
         k_cache, "kvc_paged_decode_fp4", q.data_ptr(), q.stride(0), q.stride(1),
         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-        k_cache.size(0), page_size, num_kv_heads, head_dim, block_tables.data_ptr(),
-        block_tables.stride(0), max_blocks, context_lens.data_ptr(), batch, num_heads,
-        float(scale), out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(ws), need,
+        k_cache.size(0), k_cache.size(1), k_cache.size(2), 128, block_tables.data_ptr(),
+        block_tables.stride(0), block_tables.size(1), context_lens.data_ptr(), q.size(0),
+        q.size(1), float(scale), out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(ws), need,
         nat.stream_of(q))
     return out
 
@@ -229,13 +240,24 @@ def varlen_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, num_decode_r
 def paged_decode_append_fp4(q, key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping,
                             block_tables, context_lens, scale, out=None):
     """The decode step over a 4-bit pool: store_kvcache_fp4 of the new tokens,
-    then paged_decode_fp4 over context_lens (which count them)."""
+    then paged_decode_fp4 over context_lens (which count them).  A call that is
+    refused stores nothing."""
     if nat.is_current(q):
         done = nat.host().fp4_rows(out, q, k_cache, v_cache, k_scale, v_scale, block_tables,
                                    q.size(0) if q.ndim else 0, context_lens, None, None, None,
                                    None, scale, nat.stream_of(q), key, value, slot_mapping)
         if done is not None:
             return done
-    store_kvcache_fp4(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
-    return paged_decode_fp4(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
-                            scale, out)
+    q, block_tables, context_lens, out, need = _decode_rows(
+        q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, out)
+    slots, sb = _append_rows(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    ws = nat.workspace(need, q.device)
+    nat.call_on(
+        k_cache, "kvc_paged_decode_append_fp4", q.data_ptr(), q.stride(0), q.stride(1),
+        key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+        value.stride(1), slots.data_ptr(), sb, key.size(0), k_cache.data_ptr(),
+        v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_cache.size(0),
+        k_cache.size(1), k_cache.size(2), 128, block_tables.data_ptr(), block_tables.stride(0),
+        block_tables.size(1), context_lens.data_ptr(), q.size(0), q.size(1), float(scale),
+        out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(ws), need, nat.stream_of(q))
+    return out

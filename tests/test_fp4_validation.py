@@ -154,6 +154,31 @@ def recorded(monkeypatch):
     return calls
 
 
+def _append_call(**kw):
+    p = _pool(**{n: kw.pop(n) for n in ("k_scale", "page") if n in kw})
+    args = dict(q=torch.zeros(3, 8, 128, dtype=BF), key=torch.zeros(3, 2, 128, dtype=BF),
+                value=torch.zeros(3, 2, 128, dtype=BF), slot_mapping=_i32(0, 1, 2),
+                block_tables=torch.zeros(3, 1, dtype=torch.int32), context_lens=_i32(1, 1, 1))
+    args.update(kw)
+    return paged_decode_append_fp4(**args, **p, scale=0.1)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(out=torch.zeros(3, 8, 128)), dict(out=torch.zeros(2, 8, 128, dtype=BF)),
+    dict(q=torch.zeros(3, 7, 128, dtype=BF)), dict(q=torch.zeros(3, 8, 64, dtype=BF)),
+    dict(q=torch.zeros(3, 8, 128)), dict(page=48), dict(k_scale=None),
+    dict(block_tables=torch.zeros(2, 1, dtype=torch.int32)), dict(block_tables=_i32(0, 0, 0)),
+    dict(context_lens=_i32(1, 1)), dict(slot_mapping=_i32(0)),
+    dict(key=torch.zeros(3, 2, 64, dtype=BF)), dict(value=torch.zeros(3, 3, 128, dtype=BF)),
+])
+def test_append_and_attend_checks_all_before_it_stores(recorded, bad):
+    with pytest.raises((ValueError, AssertionError)):
+        _append_call(**bad)
+    assert not recorded
+    _append_call()
+    assert [name for name, _ in recorded] == ["kvc_paged_decode_append_fp4"]
+
+
 def _varlen(cu_q, cu_k, list_q, list_k, tables=1, decode=0, lens=None, width=1):
     p = _pool()
     q = torch.zeros(decode + list_q[-1], 8, 128, dtype=BF)
@@ -234,6 +259,23 @@ def test_c_entries_refuse_before_the_device():
     assert decode(max_blocks=4096, ws=None, ws_bytes=need) == -4
     assert decode(max_blocks=4096, ws=p + 8, ws_bytes=need) == -2
     assert lib.kvc_paged_decode_fp4_workspace_bytes(3, 9, 2, 32, 4096) == 0
+
+    def append(page=32, kvh=2, dim=128, heads=8, blocks=4, max_blocks=1, batch=3, n=3, q=p, k=p,
+               key=p, slots=p, sb=4, lens=p, ws=None, ws_bytes=0, stride=1024, kstride=256):
+        return lib.kvc_paged_decode_append_fp4(
+            q, stride, 128, key, kstride, 128, p, kstride, 128, slots, sb, n, k, p, p, p, blocks,
+            page, kvh, dim, p, 1, max_blocks, lens, batch, heads, ctypes.c_float(0.1), p, stride,
+            128, ws, ws_bytes, None)
+
+    assert append(batch=0, n=0) == 0
+    for bad in (dict(page=48), dict(kvh=0), dict(dim=64), dict(heads=9), dict(blocks=-1),
+                dict(max_blocks=1 << 22), dict(batch=-1), dict(n=-1), dict(sb=2), dict(q=None),
+                dict(k=None), dict(key=None), dict(slots=None), dict(lens=None)):
+        assert append(**bad) == -1, bad
+    for bad in (dict(q=p + 8), dict(key=p + 2), dict(stride=1028), dict(kstride=260),
+                dict(k=p + 4)):
+        assert append(**bad) == -2, bad
+    assert append(max_blocks=4096, ws=p, ws_bytes=need - 1) == -4
 
     def store(n=3, kvh=2, dim=128, sb=4, key=p, cache=p, slots=p, stride=256):
         return lib.kvc_store_fp4(key, stride, 128, p, stride, 128, cache, p, p, p, 128, slots, sb,

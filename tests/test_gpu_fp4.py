@@ -770,3 +770,62 @@ def test_offsets_in_longer_tensors(decode, chunks, width, native, monkeypatch):
         cu_seqlens_q_list=cu_q, cu_seqlens_k_list=cu_k, k_scale=ks, v_scale=vs)
     want, bound = _chunk_expect(q, k, v, decode, chunks)
     fo.check(got, want, bound, f"{decode} {chunks} in longer tensors")
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_refused_step_stores_nothing(native, monkeypatch):
+    """paged_decode_append_fp4 with an output, tables, lengths or a shape that the
+    attention refuses: the pool is as it was."""
+    if not native:
+        monkeypatch.setattr(_native, "_host", _native._NoHostPath)
+    pool = _empty(4, 32, 2)
+    before = [t.clone() for t in pool]
+    q = torch.ones(3, 8, 128, dtype=BF, device="cuda")
+    key = torch.ones(3, 2, 128, dtype=BF, device="cuda")
+    slots = torch.tensor([0, 40, 70], dtype=torch.int32).cuda()
+    tables = torch.tensor([[0], [1], [2]], dtype=torch.int32).cuda()
+    lens = torch.tensor([1, 9, 7], dtype=torch.int32).cuda()
+    odd = torch.zeros(3 * 8 * 128 + 1, dtype=BF, device="cuda")[1:].view(3, 8, 128)
+    base = dict(q=q, tables=tables, lens=lens, out=None)
+    for bad in (dict(out=odd), dict(out=q.float()), dict(out=q[:2]), dict(tables=tables[:2]),
+                dict(tables=tables.flatten()), dict(lens=lens[:2]), dict(q=q[:, :7]),
+                dict(q=q.float()),
+                # more keys than a table may hold, which the library alone knows
+                dict(tables=tables[:, :1].expand(3, (1 << 21) + 1).contiguous())):
+        a = {**base, **bad}
+        with pytest.raises((ValueError, AssertionError)):
+            paged_decode_append_fp4(a["q"], key, key, *pool, slots, a["tables"], a["lens"], SCALE,
+                                    out=a["out"])
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(pool, before)), bad.keys()
+    paged_decode_append_fp4(q, key, key, *pool, slots, tables, lens, SCALE)
+    assert not torch.equal(pool[0], before[0])
+
+
+def test_append_of_more_or_fewer_rows_than_are_attended(monkeypatch):
+    """The appended rows need not be the attended ones: two tokens of one row, or none."""
+    lens = [34, 5]
+    pool, tables, k, v = fo.paged([32, 5], 32, 2, seed=80)
+    wide = torch.full((2, 2), -1, dtype=torch.int32)
+    wide[:, :1] = tables
+    wide[0, 1] = next(b for b in range(pool[0].size(0)) if b not in tables.flatten().tolist())
+    gen = torch.Generator().manual_seed(31)
+    q = torch.randn(2, 8, 128, generator=gen).to(BF)
+    new = torch.randn(2, 2, 128, generator=gen).to(BF)
+    slots = torch.tensor([int(wide[0, 1]) * 32, int(wide[0, 1]) * 32 + 1])
+    for seqs in (k, v):
+        seqs[0] = torch.cat((seqs[0], fo.values(*fo.encode(new))))
+    dev = _dev(pool)
+    lens_t = torch.tensor(lens, dtype=torch.int32).cuda()
+    want, bound = _expect(q, k, v, lens)
+    got = paged_decode_append_fp4(q[:1].cuda(), new.cuda(), new.cuda(), *dev, slots.cuda(),
+                                  wide[:1].cuda(), lens_t[:1], SCALE)
+    fo.check(got, want[:1], bound[:1], "two tokens of one row")
+    none = new[:0].cuda()
+    got = paged_decode_append_fp4(q.cuda(), none, none, *dev, slots[:0].cuda(), wide.cuda(),
+                                  lens_t, SCALE)
+    fo.check(got, want, bound, "no new tokens")
+    before = [t.clone() for t in dev]
+    got = paged_decode_append_fp4(q[:0].cuda(), -new.cuda(), new.cuda(), *dev, slots.cuda(),
+                                  wide[:0].cuda(), lens_t[:0], SCALE)
+    assert got.shape == (0, 8, 128) and not torch.equal(dev[0], before[0])
