@@ -463,12 +463,22 @@ __device__ __forceinline__ void weights(const f32x4_t* s, Carry& c, float c2, u3
 // O^T += V^T P^T over the eight keys of half h.
 __device__ __forceinline__ void weigh(const Tile& t, int h, const u32x4_t& w, Carry& c) {
   // A power of two times a weight adds to the weight's exponent field; a sum
-  // below 0 is 0.  (A weight of 0 counts as 2^-127 there.)  One multiply-add and one
-  // saturating subtraction a pair: the weights as words and the factor in a register
-  // keep the compiler from taking them apart.
+  // below 0 is 0.  One multiply-add and one saturating subtraction a pair: the weights
+  // as words and the factor in a register keep the compiler from taking them apart.  A
+  // weight of 0 has no exponent to add to (its field would count as 2^-127): what is
+  // subtracted is then 65535 instead of the bias, which leaves 0 whatever the power.
   u32x4_t pw = w;
   uint32_t field = 128u * 0x10001u;
   asm volatile("" : "+s"(field));
+  u16x2v_t less[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t at = pw[i];
+    const u16x2v_t none =
+        __builtin_elementwise_sub_sat(u16x2v_t{1, 1}, __builtin_bit_cast(u16x2v_t, at));
+    less[i] = none * u16x2v_t{65535 - (127 << 7), 65535 - (127 << 7)} +
+              u16x2v_t{127 << 7, 127 << 7};
+  }
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     u32x4_t pb;
@@ -479,8 +489,7 @@ __device__ __forceinline__ void weigh(const Tile& t, int h, const u32x4_t& w, Ca
       const uint32_t at = pw[i];
       const u16x2v_t x = __builtin_bit_cast(u16x2v_t, bytes) * __builtin_bit_cast(u16x2v_t, field) +
                          __builtin_bit_cast(u16x2v_t, at);
-      pb[i] = __builtin_bit_cast(
-          uint32_t, __builtin_elementwise_sub_sat(x, u16x2v_t{127 << 7, 127 << 7}));
+      pb[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(x, less[i]));
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x)

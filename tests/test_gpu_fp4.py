@@ -829,3 +829,47 @@ def test_append_of_more_or_fewer_rows_than_are_attended(monkeypatch):
     got = paged_decode_append_fp4(q[:0].cuda(), -new.cuda(), new.cuda(), *dev, slots.cuda(),
                                   wide[:0].cuda(), lens_t[:0], SCALE)
     assert got.shape == (0, 8, 128) and not torch.equal(dev[0], before[0])
+
+
+def _far_and_near(lens, kvh, page, seed, size):
+    """Keys whose scores with a query of ones differ by hundreds of binades: the first
+    one near (score 0, values near 1), the others far below it, with positive values
+    of `size`."""
+    pool, tables, _, _ = fo.paged(lens, page, kvh, seed=seed)
+    gen = torch.Generator().manual_seed(seed)
+    kc, vc, ks, vs = pool
+    k, v = [], []
+    for i, n in enumerate(lens):
+        near = torch.arange(n) == 0
+        x = torch.where(near[:, None, None], 0.0, -6.0).expand(n, kvh, 128).to(BF)
+        y = torch.randn(n, kvh, 128, generator=gen)
+        y = torch.where(near[:, None, None], y, y.abs() * size).to(BF)
+        pos = torch.arange(n)
+        slot = tables[i, pos // page].long() * page + pos % page
+        for codes, powers, seqs, z in ((kc, ks, k, x), (vc, vs, v, y)):
+            c, p = fo.encode(z)
+            codes.flatten(0, 1)[slot], powers.flatten(0, 1)[slot] = c, p
+            seqs.append(fo.values(c, p))
+    return pool, tables, k, v
+
+
+@pytest.mark.parametrize("size", [2.0 ** 80, 2.0 ** 115])
+@pytest.mark.parametrize("heads,kvh", [(3, 3), (8, 2)])
+def test_weights_that_underflow_count_nothing(size, heads, kvh):
+    """Keys 700 binades below the row's best one, with values of up to 2^117: what they
+    add to the exact result is below 2^-500, and nothing of them may be seen in the
+    kernel's, read whole and cut, by rows and by chunks.  (Counted as 2^-127 each, 699
+    of them would add about 0.1; no sum of them passes 2^126.)"""
+    lens = [1, 64, 90, 700]
+    pool, tables, k, v = _far_and_near(lens, kvh, 32, 40 + heads, size)
+    q = torch.full((4, heads, 128), 8.0).to(BF)         # scores 0 and -543
+    want, bound = _expect(q, k, v, lens)
+    assert float(want.abs().max()) < 8 and float(bound.max()) < 0.1
+    for i, got in enumerate(_decode(pool, tables, lens, q)):
+        fo.check(got, want, bound, f"{heads}/{kvh}, values of {size}, form {i}")
+    chunks = [(1, 1), (2, 64), (3, 90), (5, 700)]
+    q = torch.full((11, heads, 128), 8.0).to(BF)
+    want, bound = _chunk_expect(q, k, v, [], chunks)
+    for width in (None, 2200):
+        fo.check(_chunk_call(pool, tables, [], chunks, q, "known", width), want, bound,
+                 f"chunks, width {width}")
