@@ -27,6 +27,7 @@ constexpr int kFillThreads = 256;
 constexpr int kLdsRows = 4096;         // offsets searched in LDS up to this many rows
 constexpr int64_t kOneLaunch = 4096;   // tokens
 constexpr int kLongest = 1 << 29;      // of a length
+constexpr int kMostWanted = 1 << 25;   // past every max_tokens
 
 struct TablesArgs {
   const int32_t* context_lens;
@@ -54,12 +55,13 @@ struct TablesArgs {
   int32_t* cu_k;
 };
 
-// The sums over all rows before a thread's, and over the block, of N values.
+// The sums over all rows before a thread's, and over the block, of N values.  A wave's
+// sum counts up to kMost where waves are added.
 template <int N>
 struct Sums {
   int before[N], all[N];
 };
-template <int N>
+template <int N, int kMost = 0x7fffffff>
 __device__ __forceinline__ Sums<N> block_sums(const int (&x)[N], int (*lds)[kMaxWaves], int lane,
                                               int wave, int waves) {
   Sums<N> s;
@@ -67,7 +69,7 @@ __device__ __forceinline__ Sums<N> block_sums(const int (&x)[N], int (*lds)[kMax
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     incl[i] = wave_scan_add(x[i]);
-    if (lane == 63) lds[i][wave] = incl[i];
+    if (lane == 63) lds[i][wave] = min(incl[i], kMost);
   }
   __syncthreads();
 #pragma unroll
@@ -168,11 +170,12 @@ __global__ void __launch_bounds__(kMaxThreads) step_tables_kernel(TablesArgs a, 
     if (a.per_row > 0) {
       able = able && want <= a.per_row;
     } else {
-      // (a wave's sum stays below 2^31: max_tokens is under 2^24)
+      // (max_tokens is under 2^24, so a wave's wants are up to 2^30 and sixteen waves'
+      // 2^34: each wave's count up to 2^25, past max_tokens like what they were)
       const int y[1] = {want};
-      const Sums<1> sw = block_sums<1>(y, lds + 1, lane, wave, waves);
+      const Sums<1> sw = block_sums<1, kMostWanted>(y, lds + 1, lane, wave, waves);
       able = able && want0 + sw.before[0] + want <= a.max_tokens;
-      want0 = min(want0 + sw.all[0], int64_t(1) << 25);
+      want0 = min(want0 + sw.all[0], int64_t(kMostWanted));
     }
     const int got = able ? asked : 0, take = able ? need : 0;
     const int seen = able ? ctx + got : 0;

@@ -400,3 +400,22 @@ def test_ended_lengths_of_the_state_alone():
         build_step_tables(lens, _i32([1]), _i32([[0, 1]]), _i32([2]), _i32([0] * 4), _i32([0]), 32,
                           4, finished=torch.tensor([True]).cuda(), clear_ended=True, out=out)
     assert lens.tolist() == [40]
+
+
+@pytest.mark.parametrize("batch", [700, 1500])
+def test_wants_whose_sum_passes_32_bits(batch):
+    """Rows that hold room for 2^22 tokens each and ask for all of it, 512 of which pass
+    2^31: rows behind them wait as those do, however small their wish."""
+    tokens = (1 << 22) - 1
+    lens = [0] * batch
+    held = [4] * batch
+    table = [[b, b + 1, b + 2, b + 3] for b in range(batch)]
+    new = [1 << 22] * batch
+    new[0], new[batch - 100:] = 7, [3] * 100
+    got = build_step_tables(_i32(lens), _i32(new), _i32(table), _i32(held), _i32([]), _i32([0]),
+                            1 << 20, tokens)
+    assert got.query_lens.tolist() == [7] + [0] * (batch - 1)
+    want = model(lens, new, table, held, [], 0, 1 << 20, tokens, 0, [False] * batch, NO_SLOT)
+    for name, w in want.items():
+        equal = getattr(got, name).tolist() == w       # (lists too long to be shown apart)
+        assert equal, name
