@@ -86,7 +86,7 @@ def build_step_tables(context_lens, query_lens, block_tables, num_blocks, free_b
             or (block_tables.size(1) > 1 and block_tables.stride(1) != 1):
         raise ValueError("block_tables must be int32 [batch, pages] with dense rows")
     batch, width = block_tables.shape
-    if batch > 1 and width > 1 and block_tables.stride(0) < width:
+    if batch > 1 and width > 0 and block_tables.stride(0) < width:
         raise ValueError("block_tables has overlapping rows")
     dev = block_tables.device
     page_size, max_tokens, tokens_per_row = int(page_size), int(max_tokens), int(tokens_per_row)

@@ -355,6 +355,22 @@ def test_step_tables_refuse(bad):
         build_step_tables(**_tables_args(**bad))
 
 
+def test_step_tables_refuse_rows_in_one_place():
+    """Tables of one page a row, all rows over the same entry."""
+    shared = torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="overlapping"):
+        build_step_tables(**_tables_args(width=1, block_tables=shared.expand(3, 1)))
+    with pytest.raises(ValueError, match="overlapping"):
+        build_step_tables(**_tables_args(block_tables=torch.zeros(7, dtype=torch.int32).as_strided(
+            (3, 4), (1, 1))))
+    for fine in (torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, 0, dtype=torch.int32),
+                 torch.zeros(3, 2, dtype=torch.int32)[:, :1],
+                 torch.zeros(1, 4, dtype=torch.int32).expand(1, 4)):
+        args = _tables_args(batch=fine.size(0), block_tables=fine)
+        with pytest.raises(RuntimeError, match="device"):
+            build_step_tables(**args)
+
+
 def test_step_tables_need_device_tensors():
     for kw in ({}, dict(out=new_step_tables(3, 8, "cpu"))):
         with pytest.raises(RuntimeError, match="device"):
