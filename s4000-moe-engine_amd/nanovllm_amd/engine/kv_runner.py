@@ -457,8 +457,14 @@ class KVCacheRunner:
         ids; a BlockManager must not hand out the same ones), padded tokens
         appended at the scratch slot."""
         from .device_tables import DeviceBlockTables
-        return DeviceBlockTables(max_rows, max_blocks_per_seq, self.block_size,
-                                 self.num_kvcache_blocks if blocks is None else blocks,
+        if blocks is None:
+            blocks = self.num_kvcache_blocks
+        elif not isinstance(blocks, int):
+            blocks = [int(b) for b in blocks]
+        if (blocks if isinstance(blocks, int) else max(blocks, default=-1) + 1) \
+                > self.num_kvcache_blocks:
+            raise ValueError(f"the pool has {self.num_kvcache_blocks} blocks")
+        return DeviceBlockTables(max_rows, max_blocks_per_seq, self.block_size, blocks,
                                  self.device, self.scratch_slot)
 
     def prepare_decode_device(self, tables, query_lens=None, finished=None, out=None):

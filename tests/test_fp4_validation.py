@@ -440,6 +440,19 @@ def test_runner_arguments():
         KVCacheRunner(1, 2, 32, 2, 128, kv_fp4=True, device="cpu", kv_offload_host_blocks=1)
 
 
+def test_runner_tables_are_of_its_blocks():
+    """Blocks behind the pool, the padding's scratch block among them, are refused:
+    appends there would be dropped or shared."""
+    runner = KVCacheRunner(1, 6, 32, 2, 128, kv_fp4=True, device="cpu")
+    assert runner.device_tables(2, 3).num_free.tolist() == [6]
+    assert runner.device_tables(2, 3, 4).free_blocks.tolist() == [0, 1, 2, 3]
+    assert runner.device_tables(2, 3, torch.tensor([5, 2])).free_blocks.tolist() == [5, 2]
+    assert runner.device_tables(2, 3, []).num_free.tolist() == [0]
+    for bad in (7, [6], [0, 9], torch.tensor([6]), range(7)):
+        with pytest.raises(ValueError, match="blocks"):
+            runner.device_tables(2, 3, bad)
+
+
 def test_graph_runner_needs_scales_and_plain_scores():
     p = _pool()
     with pytest.raises(ValueError, match="scale"):
