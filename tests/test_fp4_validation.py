@@ -443,7 +443,9 @@ def test_runner_arguments():
 def test_runner_tables_are_of_its_blocks():
     """Blocks behind the pool, the padding's scratch block among them, are refused:
     appends there would be dropped or shared."""
-    runner = KVCacheRunner(1, 6, 32, 2, 128, kv_fp4=True, device="cpu")
+    runner = KVCacheRunner.__new__(KVCacheRunner)     # (the whole of it needs a GPU)
+    runner.kv_cache = torch.zeros(2, 1, 7, 32, 2, 64, dtype=U8)
+    runner.num_kvcache_blocks, runner.block_size, runner.scratch_slot = 6, 32, 6 * 32
     assert runner.device_tables(2, 3).num_free.tolist() == [6]
     assert runner.device_tables(2, 3, 4).free_blocks.tolist() == [0, 1, 2, 3]
     assert runner.device_tables(2, 3, torch.tensor([5, 2])).free_blocks.tolist() == [5, 2]
