@@ -474,6 +474,9 @@ class KVCacheRunner:
         StepTables (positions among them).  A row that waits for a page, or has no
         token, attends nothing and appends nothing that is read again: its output
         is zeros over a 4-bit pool, NaN over the others."""
+        if tables.page_size != self.block_size or tables.device != self.device:
+            raise ValueError(f"tables of pages of {tables.page_size} on {tables.device} for a pool "
+                             f"of {self.block_size} on {self.device}")
         if query_lens is None:
             query_lens = torch.ones(tables.max_rows, dtype=torch.int32, device=tables.device)
         step = tables.step(query_lens, tables.max_rows, tokens_per_row=1, finished=finished,

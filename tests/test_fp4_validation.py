@@ -455,6 +455,18 @@ def test_runner_tables_are_of_its_blocks():
             runner.device_tables(2, 3, bad)
 
 
+def test_decode_from_tables_of_another_page_size():
+    """Slots and pages counted in other pages would be those of other tokens."""
+    runner = KVCacheRunner.__new__(KVCacheRunner)
+    runner.kv_cache, runner.block_size = torch.zeros(2, 1, 7, 32, 2, 64, dtype=U8), 32
+    with pytest.raises(ValueError, match="pages of 64"):
+        runner.prepare_decode_device(DeviceBlockTables(2, 3, 64, 6, device="cpu"))
+    with pytest.raises(ValueError, match="meta"):
+        runner.prepare_decode_device(DeviceBlockTables(2, 3, 32, 6, device="meta"))
+    with pytest.raises(RuntimeError, match="device"):
+        runner.prepare_decode_device(DeviceBlockTables(2, 3, 32, 6, device="cpu"))
+
+
 def test_graph_runner_needs_scales_and_plain_scores():
     p = _pool()
     with pytest.raises(ValueError, match="scale"):
