@@ -348,3 +348,81 @@ def test_captured_step_refuses_scales_of_another_pool():
     with pytest.raises(ValueError, match="4-bit"):
         DecodeGraphRunner([pool], [pool.clone()], HEADS, 2, 2, SCALE, k_scales=[scale],
                           v_scales=[scale])
+
+
+@pytest.mark.parametrize("kind", ["tokhead", "chan"])
+@pytest.mark.parametrize("capture", [False, True])
+def test_serving_loop_over_an_int8_pool(kind, capture):
+    """The same loop over the int8 pools: bit for bit the step whose slots, lengths and
+    tables the host wrote, rows that wait among them (NaN, and the pool as it was)."""
+    rows, kvh, heads, blocks, width = 3, 4, 8, 4, 3
+    gen = torch.Generator().manual_seed(8)
+    scales = (0.01 + 0.02 * torch.rand(kvh, 128, generator=gen)).cuda()
+    sides = []
+    for _ in range(2):
+        runner = KVCacheRunner(1, blocks, PAGE, kvh, 128, kv_int8=kind)
+        runner.kv_cache.zero_()
+        if kind == "chan":
+            runner.kv_scales.copy_(scales.expand_as(runner.kv_scales))
+            runner.kv_dscales.copy_(runner.kv_scales)
+        layer = Attention(heads, 128, SCALE, kvh)
+        assert runner.bind([layer]) == 1
+        sides.append((runner, layer))
+    (runner, layer), (other, host_layer) = sides
+    tables = runner.device_tables(rows, width)
+    q = torch.zeros(rows, heads, 128, dtype=BF, device="cuda")
+    k, v = (torch.zeros(rows, kvh, 128, dtype=BF, device="cuda") for _ in range(2))
+    new = torch.ones(rows, dtype=torch.int32, device="cuda")
+    out = tables.outputs(rows)
+    result = torch.zeros_like(q)
+
+    def step():
+        runner.prepare_decode_device(tables, new, out=out)
+        result.copy_(layer(q, k, v).view(rows, heads, 128))
+
+    graph = None
+    if capture:
+        state = [tables.context_lens, tables.num_blocks, tables.block_tables, tables.free_blocks,
+                 tables.num_free, runner.kv_cache, runner.kv_scales]
+        saved = [x.clone() for x in state]
+        step()
+        torch.cuda.synchronize()
+        for x, s in zip(state, saved):
+            x.copy_(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+    lens, mine = [0] * rows, [[] for _ in range(rows)]
+    free, waited = list(range(blocks)), 0
+    for i in range(70):
+        nq = torch.randn(rows, heads, 128, generator=gen).to(BF)
+        nk, nv = (torch.randn(rows, kvh, 128, generator=gen).to(BF) for _ in range(2))
+        q.copy_(nq), k.copy_(nk), v.copy_(nv)
+        graph.replay() if graph is not None else step()
+        torch.cuda.synchronize()
+        slots, seen = [], []
+        for b in range(rows):                   # rows in order; pages off the stack's top
+            if lens[b] == PAGE * len(mine[b]) and not free:
+                slots.append(other.scratch_slot), seen.append(0)
+                waited += 1
+                continue
+            if lens[b] == PAGE * len(mine[b]):
+                mine[b].append(free.pop())
+            slots.append(mine[b][lens[b] // PAGE] * PAGE + lens[b] % PAGE)
+            lens[b] += 1
+            seen.append(lens[b])
+        set_context(False, slot_mapping=torch.tensor(slots, dtype=torch.int32).cuda(),
+                    context_lens=torch.tensor(seen, dtype=torch.int32).cuda(),
+                    block_tables=torch.tensor([m + [-1] * (width - len(m)) for m in mine],
+                                              dtype=torch.int32).cuda(),
+                    max_context_len=width * PAGE)
+        want = host_layer(q, k, v).view(rows, heads, 128)
+        for b in range(rows):
+            if seen[b]:
+                assert torch.equal(result[b], want[b]) and torch.isfinite(want[b]).all(), (i, b)
+            else:
+                assert result[b].isnan().all(), (i, b)
+        assert torch.equal(runner.kv_cache[:, :, :blocks], other.kv_cache[:, :, :blocks]), i
+        if kind == "tokhead":
+            assert torch.equal(runner.kv_scales[:, :, :blocks], other.kv_scales[:, :, :blocks]), i
+    assert waited > 0
