@@ -810,7 +810,9 @@ int64_t kvc_varlen_fp4_blocks(const int32_t* cu_seqlens_q_host,
  * 0), else row b's at b * tokens_per_row; tokens that there are not get pad_slot
  * and position 0.  block_tables and free_blocks change in place; context_lens,
  * num_blocks, num_free and query_lens may be their own outputs (context_lens_out
- * over context_lens and so on).  Lengths count up to 2^29. */
+ * over context_lens and so on).  Lengths count up to 2^29; the keys of a step's
+ * granted rows are to sum below 2^31 (rows that share pages can pass it), or
+ * cu_seqlens_k wraps. */
 int kvc_step_tables(const int32_t* context_lens, const int32_t* query_lens,
                     const uint8_t* finished, int32_t* block_tables, int64_t bt_stride,
                     int64_t max_blocks_per_seq, int64_t batch, const int32_t* num_blocks,

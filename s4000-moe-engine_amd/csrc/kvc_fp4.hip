@@ -1080,7 +1080,11 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // 1025 to 8007 32 / 40 / 60 / 107, 128 x 1000 28 / 23 / 19 / 23, 128 x 4096 59 / 65 / 52 /
 // 65, 192 x 1000 34 / 34 / 33 / 24, 256 x 300 to 900 34 / 36 / 30 / 23; 8 kv heads: 128 x
 // 300 to 900 34 / 37 / 31 / 24 / 35, 200 x 1000 54 / 82 / 70 / 53 / 44, 400 x 20 to 80 35
-// / 60 / 43 / 28 / 21.  Of 190 shapes the choice is over 8 % off in four, 21 % at worst.
+// / 60 / 43 / 28 / 21.  Of 190 shapes the choice is over 8 % off in four, 21 % at worst:
+// all with tables as wide as the longest row, over two inputs in turn, so that pools under
+// 256 MB lay partly in the cache behind the L2s (64 x 4096 whole, one head, over three:
+// 33).  Rows far shorter than their table are taken for long ones and cut: 64 rows of 300
+// keys 7.4 us under a table of 512 keys, 16.4 under one of 32768.
 Plan make_plan(int64_t decode_rows, int64_t chunks, int64_t chunk_tokens, int64_t chunk_blocks,
                int64_t heads, int64_t kv_heads, int64_t most_keys) {
   Plan pl{};

@@ -13,7 +13,7 @@
 // together), from DPP scans and one exchange of wave sums each.  The tokens are
 // filled by the same launch up to kOneLaunch of them and else by a second one
 // over the chip.  Bound by latency throughout: a decode step of 64 rows moves
-// some 4 KB and takes 3.7 us; 512 rows with 66000 tokens 6.2 + 3.3 us (2 MB).
+// some 4 KB and takes 3.7 us; 512 rows with 66000 tokens 6.2 + 4.3 us (2 MB).
 #include <algorithm>
 
 #include "kvc_internal.h"
