@@ -720,11 +720,13 @@ size_t kvc_paged_decode_fp4_workspace_bytes(int64_t batch, int64_t num_heads,
 
 /* kvc_paged_decode over a 4-bit pool: q/out bf16 [batch, num_heads, 128], any
  * number of query heads per kv head, page_size a multiple of 32, tables of up to
- * 2^26 keys.  Scores, sums and outputs are fp32 until the one rounding to bf16;
- * weights are rounded to bf16 for the product with V (one under 2^-124 of the
- * row's largest may count 0, and so does one that its run's power of V takes
- * below 2^-126).  A row with context_lens[b] <= 0 gives zeros; a length past its table counts the table's
- * keys; keys whose table entry is bad read as zeros. */
+ * 2^26 keys.  Scores, sums and outputs are fp32 until the one rounding to bf16
+ * (sums of values times weights of up to 4, divided last: values near the top of
+ * the range overflow in them); weights are rounded to bf16 for the product with V
+ * (one under 2^-124 of the row's largest may count 0, and so does one that its
+ * run's power of V takes below 2^-126).  A row with context_lens[b] <= 0 gives
+ * zeros; a length past its table counts the table's keys; keys whose table entry
+ * is bad read as zeros. */
 int kvc_paged_decode_fp4(const void* q, int64_t q_stride_b, int64_t q_stride_h,
                          const uint8_t* k_cache, const uint8_t* v_cache, const uint8_t* k_scale,
                          const uint8_t* v_scale, int64_t num_cache_blocks, int64_t page_size,

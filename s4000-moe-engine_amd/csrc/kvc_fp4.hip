@@ -18,8 +18,8 @@
 // rows make whole 128-byte lines (loads alone 5.1 against 6.1 TB/s).  Every wave
 // streams its own tiles through its own two LDS slots of 8.5 KiB (direct-to-LDS loads
 // two tiles ahead, no workgroup barrier); eight waves a workgroup, one workgroup a CU,
-// waves differ in kv head and in tile phase and join once an item.  Bound by HBM reads for batches: 64 rows
-// of 4096 keys (4 kv heads, 143 MB) 32 us, of 8192 50 + 5 to join (47 with the loads
+// waves differ in kv head and in tile phase and join once an item.  Bound by HBM reads
+// for batches: 64 rows of 4096 keys (4 kv heads, 143 MB) 32 us, of 8192 50 + 5 to join (47 with the loads
 // alone), 128 of 4096 51: 7 TB/s for every further byte, and 12 to 16 us of launch,
 // lengths, table, first tiles and last results.  Single rows are bound by that chain:
 // 333 keys 7.1 us.
@@ -1075,8 +1075,8 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // that for every row, between batches of one length and ragged ones, and as half of it
 // where chunks join decode rows (200 rows of 300 to 2000 keys and a chunk over 4000: cut
 // 43, whole 64).  Measured, cut / whole by one, two, four and eight heads (rows x keys; 4
-// kv heads): 1 x 1000 13.1 / 10.1 / 15.1 / 21.5, 8 x 4096 17 / 23 / 35 / 60, 16 x 8192 26 / 40 / 61 / 113, 64 x 300
-// 19 / 8.3 / 10.7 / 12.9, 64 x 4096 35 / 28 / 38 / 62, 64 x 8192 56 / 60 / 66 / 114, 48 x
+// kv heads): 1 x 1000 13.1 / 10.1 / 15.1 / 21.5, 8 x 4096 17 / 23 / 35 / 60, 16 x 8192
+// 26 / 40 / 61 / 113, 64 x 300 19 / 8.3 / 10.7 / 12.9, 64 x 4096 35 / 28 / 38 / 62, 64 x 8192 56 / 60 / 66 / 114, 48 x
 // 1025 to 8007 32 / 40 / 60 / 107, 128 x 1000 28 / 23 / 19 / 23, 128 x 4096 59 / 65 / 52 /
 // 65, 192 x 1000 34 / 34 / 33 / 24, 256 x 300 to 900 34 / 36 / 30 / 23; 8 kv heads: 128 x
 // 300 to 900 34 / 37 / 31 / 24 / 35, 200 x 1000 54 / 82 / 70 / 53 / 44, 400 x 20 to 80 35
@@ -1212,9 +1212,9 @@ extern "C" int kvc_store_fp4(const void* key, int64_t key_stride_n, int64_t key_
                              int slot_index_bytes, int64_t num_tokens, int64_t num_kv_heads,
                              int64_t head_dim, kvc_stream_t stream) {
   clear_error();
-  const Append a{key,     key_stride_n, key_stride_h, value,   value_stride_n,
-                 value_stride_h, k_cache, v_cache, k_scale, v_scale,
-                 num_slots, slot_mapping, slot_index_bytes, num_tokens, num_kv_heads};
+  const Append a{key, key_stride_n, key_stride_h, value, value_stride_n, value_stride_h,
+                 k_cache, v_cache, k_scale, v_scale, num_slots,
+                 slot_mapping, slot_index_bytes, num_tokens, num_kv_heads};
   const int rc = check_append("store_fp4", a, head_dim);
   if (rc != KVC_OK || num_tokens == 0) return rc;
   launch_append(a, as_stream(stream));
@@ -1280,14 +1280,14 @@ extern "C" int kvc_gather_kv_fp4(const uint8_t* k_cache, const uint8_t* v_cache,
 
 namespace {
 // append (or null): launched ahead of the rows, once the whole call has been checked.
-int run_rows(const char* what, const Append* append, const void* q, int64_t q_st, int64_t q_sh, int64_t heads,
-             const uint8_t* k_cache, const uint8_t* v_cache, const uint8_t* k_scale,
-             const uint8_t* v_scale, int64_t blocks, int64_t page, int64_t kv_heads,
-             int64_t head_dim, const int32_t* tables, int64_t bt_stride, int64_t max_blocks,
-             int64_t decode_rows, const int32_t* lens, int64_t chunks, int64_t chunk_tokens,
-             int64_t chunk_blocks, const int32_t* cu_q, const int32_t* cu_k, float scale,
-             void* out, int64_t o_st, int64_t o_sh, void* workspace, size_t workspace_bytes,
-             kvc_stream_t stream) {
+int run_rows(const char* what, const Append* append, const void* q, int64_t q_st, int64_t q_sh,
+             int64_t heads, const uint8_t* k_cache, const uint8_t* v_cache,
+             const uint8_t* k_scale, const uint8_t* v_scale, int64_t blocks, int64_t page,
+             int64_t kv_heads, int64_t head_dim, const int32_t* tables, int64_t bt_stride,
+             int64_t max_blocks, int64_t decode_rows, const int32_t* lens, int64_t chunks,
+             int64_t chunk_tokens, int64_t chunk_blocks, const int32_t* cu_q,
+             const int32_t* cu_k, float scale, void* out, int64_t o_st, int64_t o_sh,
+             void* workspace, size_t workspace_bytes, kvc_stream_t stream) {
   KVC_REQUIRE(head_dim == kD, KVC_ERR_VALUE, "%s: head_dim must be 128 (got %lld)", what,
               (long long)head_dim);
   KVC_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, KVC_ERR_VALUE,
@@ -1420,8 +1420,8 @@ extern "C" int kvc_paged_decode_fp4(
     int64_t out_stride_b, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
     kvc_stream_t stream) {
   clear_error();
-  return run_rows("paged_decode_fp4", nullptr, q, q_stride_b, q_stride_h, num_heads, k_cache, v_cache,
-                  k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim,
+  return run_rows("paged_decode_fp4", nullptr, q, q_stride_b, q_stride_h, num_heads, k_cache,
+                  v_cache, k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim,
                   block_tables, bt_stride, max_blocks_per_seq, batch, context_lens, 0, 0, 0,
                   nullptr, nullptr, scale, out, out_stride_b, out_stride_h, workspace,
                   workspace_bytes, stream);
@@ -1437,10 +1437,9 @@ extern "C" int kvc_paged_decode_append_fp4(
     int64_t num_heads, float scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
     void* workspace, size_t workspace_bytes, kvc_stream_t stream) {
   clear_error();
-  const Append a{key,       key_stride_n, key_stride_h, value,   value_stride_n,
-                 value_stride_h, k_cache, v_cache, k_scale, v_scale,
-                 num_cache_blocks * page_size, slot_mapping, slot_index_bytes, num_tokens,
-                 num_kv_heads};
+  const Append a{key, key_stride_n, key_stride_h, value, value_stride_n, value_stride_h,
+                 k_cache, v_cache, k_scale, v_scale, num_cache_blocks * page_size,
+                 slot_mapping, slot_index_bytes, num_tokens, num_kv_heads};
   const int rc = check_append("paged_decode_append_fp4", a, head_dim);
   if (rc != KVC_OK) return rc;
   return run_rows("paged_decode_append_fp4", &a, q, q_stride_b, q_stride_h, num_heads, k_cache,
@@ -1477,10 +1476,10 @@ extern "C" int kvc_varlen_fp4(
   KVC_REQUIRE(num_decode_rows >= 0 && num_decode_rows <= num_q_tokens, KVC_ERR_VALUE,
               "varlen_fp4: more decode rows than query rows");
   return run_rows("varlen_fp4", nullptr, q, q_stride_t, q_stride_h, num_heads, k_cache, v_cache,
-                  k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim, block_tables,
-                  bt_stride, max_blocks_per_seq, num_decode_rows, decode_context_lens,
-                  num_prefill, num_q_tokens - num_decode_rows, chunk_blocks, cu_seqlens_q,
-                  cu_seqlens_k, scale, out, out_stride_t, out_stride_h, workspace,
+                  k_scale, v_scale, num_cache_blocks, page_size, num_kv_heads, head_dim,
+                  block_tables, bt_stride, max_blocks_per_seq, num_decode_rows,
+                  decode_context_lens, num_prefill, num_q_tokens - num_decode_rows, chunk_blocks,
+                  cu_seqlens_q, cu_seqlens_k, scale, out, out_stride_t, out_stride_h, workspace,
                   workspace_bytes, stream);
 }
 
