@@ -19,10 +19,10 @@
 // streams its own tiles through its own two LDS slots of 8.5 KiB (direct-to-LDS loads
 // two tiles ahead, no workgroup barrier); eight waves a workgroup, one workgroup a CU,
 // waves differ in kv head and in tile phase and join once an item.  Bound by HBM reads
-// for batches: 64 rows of 4096 keys (4 kv heads, 143 MB) 32 us, of 8192 50 + 5 to join (47 with the loads
-// alone), 128 of 4096 51: 7 TB/s for every further byte, and 12 to 16 us of launch,
-// lengths, table, first tiles and last results.  Single rows are bound by that chain:
-// 333 keys 7.1 us.
+// for batches: 64 rows of 4096 keys (4 kv heads, 143 MB) 33 us, of 8192 50 + 5 to join
+// (47 with the loads alone), 128 of 4096 51: 7 TB/s for every further byte, and 12 to 16
+// us of launch, lengths, table, first tiles and last results.  Single rows are bound by
+// that chain: 333 keys 7.3 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -1076,11 +1076,12 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // where chunks join decode rows (200 rows of 300 to 2000 keys and a chunk over 4000: cut
 // 43, whole 64).  Measured, cut / whole by one, two, four and eight heads (rows x keys; 4
 // kv heads): 1 x 1000 13.1 / 10.1 / 15.1 / 21.5, 8 x 4096 17 / 23 / 35 / 60, 16 x 8192
-// 26 / 40 / 61 / 113, 64 x 300 19 / 8.3 / 10.7 / 12.9, 64 x 4096 35 / 28 / 38 / 62, 64 x 8192 56 / 60 / 66 / 114, 48 x
-// 1025 to 8007 32 / 40 / 60 / 107, 128 x 1000 28 / 23 / 19 / 23, 128 x 4096 59 / 65 / 52 /
-// 65, 192 x 1000 34 / 34 / 33 / 24, 256 x 300 to 900 34 / 36 / 30 / 23; 8 kv heads: 128 x
-// 300 to 900 34 / 37 / 31 / 24 / 35, 200 x 1000 54 / 82 / 70 / 53 / 44, 400 x 20 to 80 35
-// / 60 / 43 / 28 / 21.  Of 190 shapes the choice is over 8 % off in four, 21 % at worst:
+// 26 / 40 / 61 / 113, 64 x 300 19 / 8.3 / 10.7 / 12.9, 64 x 4096 35 / 28 / 38 / 62, 64 x
+// 8192 56 / 60 / 66 / 114, 48 x 1025 to 8007 32 / 40 / 60 / 107, 128 x 1000 28 / 23 / 19 /
+// 23, 128 x 4096 59 / 65 / 52 / 65, 192 x 1000 34 / 34 / 33 / 24, 256 x 300 to 900 34 / 36
+// / 30 / 23; 8 kv heads: 128 x 300 to 900 34 / 37 / 31 / 24 / 35, 200 x 1000 54 / 82 / 70 /
+// 53 / 44, 400 x 20 to 80 35 / 60 / 43 / 28 / 21.  Of 190 shapes the choice is over 8 % off
+// in four, 21 % at worst:
 // all with tables as wide as the longest row, over two inputs in turn, so that pools under
 // 256 MB lay partly in the cache behind the L2s (64 x 4096 whole, one head, over three:
 // 33).  Rows far shorter than their table are taken for long ones and cut: 64 rows of 300
